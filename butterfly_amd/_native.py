@@ -108,6 +108,16 @@ SIGNATURES = {
     "bfly_add_rms_norm_q4_gemv_argmax": (_int, [_vp, _vp, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp,
                                                 _i64, _vp]),
     "bfly_greedy_advance": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
+    # include/butterfly_amd_paged.h
+    "bfly_paged_plan": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                               _i64, _vp]),
+    "bfly_paged_append": (_int, [_vp, _vp, _int, _i64, _int, _int, *[_i64] * 4, _vp, _vp, _vp, _i64, _int, *[_i64] * 6,
+                                 _vp]),
+    "bfly_paged_rope_append": (_int, [_vp, _vp, _vp, _int, _i64, _int, _int, _int, *[_i64] * 6, _vp, _vp, _f32, _vp, _vp,
+                                      _i64, _int, _vp, _vp, _vp, _vp, _vp, _i64, _int, *[_i64] * 6, _vp]),
+    "bfly_paged_attention_workspace_bytes": (_i64, [_i64, _int, _int, _int, _i64, _int, _int]),
+    "bfly_paged_attention": (_int, [_vp, _int, _i64, _int, _int, _int, _i64, _i64, _vp, _vp, _i64, _int, *[_i64] * 6, _vp,
+                                    _i64, _i64, _vp, _int, _f32, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 _lib = None

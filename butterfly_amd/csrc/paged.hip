@@ -1,0 +1,462 @@
+// Paged key-value cache on gfx950: a step's bookkeeping on the device (pages, block table, slots,
+// positions), rows into pages, and the decoder's q/k norm + RoPE on the way there.  The contracts are
+// include/butterfly_amd_paged.h's; no counterpart in the reference's own code (the layers that the swap
+// leaves dense keep the host model's cache, bna/integrations/qwen_mlx.py:1822-1846).
+#include "paged.h"
+
+namespace bfly {
+
+// --------------------------------------------------------------------------- bookkeeping
+// With P(x) = ceil(x / page), a request b that goes from old to new tokens gives back pages
+// P(new)..P(old) - 1 or takes pages P(old)..P(new) - 1.  Every request's place among the rows, the given
+// and the taken pages is an exclusive sum over the requests before it: one scan of three counts.
+//
+// plan_kernel is one workgroup: each thread sums a run of requests, one scan over the threads, then the
+// writes.  Sums saturate at 2^32 - 1 (saturating addition of counts is associative, so the scan may
+// regroup them), which is above every limit they are held against.
+struct PlanArgs {
+  int32_t* table;
+  const int32_t* lengths;
+  const int32_t* counts;
+  int32_t* free_pages;
+  const int32_t* state;
+  int32_t* lengths_out;
+  int32_t* state_out;
+  int32_t* starts;
+  int64_t* slots;
+  int64_t* positions;
+  int32_t* taken;          // [requests + 1]: pages taken by the requests before
+  int64_t table_stride, capacity;   // capacity: tokens a table row holds
+  int requests, shift, free_capacity, num_rows;
+};
+
+struct PlanSum {
+  uint32_t rows, give, take;
+};
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ __forceinline__ PlanSum operator+(PlanSum a, PlanSum b) {
+  return {add_sat(a.rows, b.rows), add_sat(a.give, b.give), add_sat(a.take, b.take)};
+}
+
+struct PlanStep {
+  int old_len, new_len, count;   // count: rows added
+  int p_old, p_new;
+  bool bad, full;
+};
+__device__ __forceinline__ PlanStep plan_step(const PlanArgs& a, int b) {
+  PlanStep s;
+  const int64_t n = a.lengths[b], c = a.counts[b], pages = ((int64_t)1 << a.shift) - 1;
+  const int64_t m = n + c > 0 ? n + c : 0;
+  s.bad = n < 0 || n > a.capacity;
+  s.full = m > a.capacity;
+  const bool ok = !s.bad && !s.full;
+  s.old_len = ok ? (int)n : 0;
+  s.new_len = ok ? (int)m : 0;
+  s.count = ok && c > 0 ? (int)c : 0;
+  s.p_old = (int)((s.old_len + pages) >> a.shift);
+  s.p_new = (int)((s.new_len + pages) >> a.shift);
+  return s;
+}
+
+// Row i of the call: the request it belongs to by binary search in `starts`, its position, and its page: one
+// the request has, or the one it takes, which the page's first row also writes to the table.
+__device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* starts, const int32_t* taken,
+                                         const int32_t* new_len, int i, bool ok, int64_t stack) {
+  int64_t slot = -1, pos = 0;
+  if (ok && i < starts[a.requests]) {
+    int lo = 0, hi = a.requests - 1;               // the first request with starts[b + 1] > i
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid + 1] > i) hi = mid;
+      else lo = mid + 1;
+    }
+    const int count = starts[lo + 1] - starts[lo], old_len = new_len[lo] - count;
+    pos = (int64_t)old_len + (i - starts[lo]);
+    const int p_old = (int)(((int64_t)old_len + (1 << a.shift) - 1) >> a.shift), j = (int)(pos >> a.shift);
+    const int off = (int)(pos & ((1 << a.shift) - 1));
+    int32_t* entry = a.table + lo * a.table_stride + j;
+    int page;
+    if (j < p_old) {
+      page = *entry;
+    } else {
+      page = a.free_pages[stack - 1 - (taken[lo] + (j - p_old))];
+      if (off == 0) *entry = page;
+    }
+    slot = ((int64_t)page << a.shift) + off;
+  }
+  a.slots[i] = slot;
+  a.positions[i] = pos;
+}
+
+constexpr int kPlanMaxThreads = 1024;
+constexpr int kPlanLds = 4096;     // requests whose sums the one-launch form keeps in LDS
+
+template <bool kRows>
+__global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
+  __shared__ PlanSum part[kPlanMaxThreads / 64];
+  __shared__ int flags;
+  __shared__ int32_t s_starts[kRows ? kPlanLds + 1 : 1], s_taken[kRows ? kPlanLds + 1 : 1], s_new[kRows ? kPlanLds : 1];
+  const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wave = t >> 6;
+  const int per = (a.requests + nt - 1) / nt;
+  const int b0 = t * per < a.requests ? t * per : a.requests;
+  const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
+  const int top = a.state[0], held = a.state[1];
+  if (t == 0) flags = 0;
+  __syncthreads();
+  PlanSum mine{0, 0, 0};
+  int bad = 0;
+  for (int b = b0; b < b1; ++b) {
+    const PlanStep s = plan_step(a, b);
+    bad |= s.bad ? 1 : s.full ? 2 : 0;
+    mine = mine + PlanSum{(uint32_t)s.count, (uint32_t)(s.p_old > s.p_new ? s.p_old - s.p_new : 0),
+                          (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
+  }
+  PlanSum up = mine;                                // inclusive over the wave
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const PlanSum v{__shfl_up(up.rows, o), __shfl_up(up.give, o), __shfl_up(up.take, o)};
+    if (lane >= o) up = up + v;
+  }
+  if (lane == 63) part[wave] = up;
+  if (bad) atomicOr(&flags, bad);
+  __syncthreads();
+  PlanSum before{0, 0, 0}, total{0, 0, 0};
+  for (int w = 0; w < nt / 64; ++w) {
+    if (w == wave) before = total;
+    total = total + part[w];
+  }
+  {
+    // the sum before this thread: its inclusive sum without its own (exact where nothing saturated;
+    // where something did, the call refuses below and the sums are not used)
+    before = before + PlanSum{up.rows - mine.rows, up.give - mine.give, up.take - mine.take};
+  }
+  const int64_t stack = (int64_t)top + total.give;
+  int err = held;
+  if (err == 0) {
+    if (flags & 1) err = BFLY_PAGED_BAD_LENGTH;
+    else if (flags & 2) err = BFLY_PAGED_TABLE_FULL;
+    else if (total.rows > (uint32_t)a.num_rows) err = BFLY_PAGED_ROWS;
+    else if (stack < (int64_t)total.take) err = BFLY_PAGED_NO_PAGES;
+    else if (top < 0 || top > a.free_capacity || stack > a.free_capacity) err = BFLY_PAGED_FREE_LIST;
+  }
+  const bool ok = err == 0;
+  // lengths may be updated in place: a thread reads its own requests before it writes them
+  PlanSum at = before;
+  for (int b = b0; b < b1; ++b) {
+    const int32_t raw = a.lengths[b];
+    const PlanStep s = plan_step(a, b);
+    a.lengths_out[b] = ok ? s.new_len : raw;
+    a.starts[b] = ok ? (int)at.rows : 0;
+    if constexpr (kRows) {
+      s_starts[b] = (int)at.rows;
+      s_taken[b] = (int)at.take;
+      s_new[b] = s.new_len;
+    } else {
+      a.taken[b] = (int)at.take;
+    }
+    if (ok) {
+      for (int j = s.p_new; j < s.p_old; ++j)
+        a.free_pages[stack - 1 - ((int64_t)at.give + (j - s.p_new))] = a.table[b * a.table_stride + j];
+      at = at + PlanSum{(uint32_t)s.count, (uint32_t)(s.p_old > s.p_new ? s.p_old - s.p_new : 0),
+                        (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
+    }
+  }
+  if (t == 0) {
+    a.starts[a.requests] = ok ? (int)total.rows : 0;
+    if constexpr (kRows) {
+      s_starts[a.requests] = (int)total.rows;
+      s_taken[a.requests] = (int)total.take;
+    } else {
+      a.taken[a.requests] = (int)total.take;
+    }
+  }
+  __syncthreads();                                  // state is read by every thread before it is written
+  if (t == 0) {
+    a.state_out[0] = ok ? (int)(stack - total.take) : top;
+    a.state_out[1] = err;
+  }
+  if constexpr (kRows)
+    for (int i = t; i < a.num_rows; i += nt) plan_row(a, s_starts, s_taken, s_new, i, ok, stack);
+}
+
+// The rows of a call with many of them, after plan_kernel<false>: a thread each.
+__global__ void __launch_bounds__(256) plan_rows_kernel(PlanArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.num_rows) return;
+  const bool ok = a.state_out[1] == 0;
+  plan_row(a, a.starts, a.taken, a.lengths_out, i, ok, (int64_t)a.state_out[0] + a.taken[a.requests]);
+}
+
+// --------------------------------------------------------------------------- rows into pages
+// 16-byte pieces, a thread each: `per` pieces make a head's row.  Bound by the rows' bytes, read once and
+// written once.
+struct AppendArgs {
+  const char* k;
+  const char* v;
+  const int64_t* slots;
+  PagePtr kp, vp;
+  int64_t k_row, k_head, v_row, v_head;   // bytes
+  int64_t limit, pieces;                  // num_pages * page_size; pieces of k (and of v)
+  int hkv, per, shift;
+};
+
+__global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool is_v = i >= a.pieces;
+  if (is_v) i -= a.pieces;
+  if (i >= a.pieces) return;
+  const int64_t item = i / a.per;
+  const int pc = (int)(i - item * a.per);
+  const int64_t row = item / a.hkv;
+  const int h = (int)(item - row * a.hkv);
+  const int64_t slot = a.slots[row];
+  if (slot < 0 || slot >= a.limit) return;
+  const char* src = is_v ? a.v + row * a.v_row + h * a.v_head : a.k + row * a.k_row + h * a.k_head;
+  const PagePtr& p = is_v ? a.vp : a.kp;
+  const uint4 x = *reinterpret_cast<const uint4*>(src + 16 * pc);
+  *reinterpret_cast<uint4*>(p.row(slot >> a.shift, h, (int)(slot & ((1 << a.shift) - 1))) + 16 * pc) = x;
+}
+
+// --------------------------------------------------------------------------- norm, RoPE, rows into pages
+// A group of LPR lanes holds one head's row of a token, E = 16 bytes of it a lane: mean square by
+// shuffles inside the group, weight, then rotate-half with the lane that holds the other half
+// (rotary / 2 elements away, whole lanes since rotary is a multiple of 16).  fp32 from the loads to the
+// one rounding of each output: y = x * rsqrt(mean x^2 + eps) * w, z = y cos + rotate_half(y) sin.
+struct RopeAppendArgs {
+  const char* q;
+  const char* k;
+  const char* v;
+  const void* qw;
+  const void* kw;
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  const int64_t* slots;
+  char* q_out;
+  PagePtr kp, vp;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes
+  int64_t limit, items, table_rows;
+  int hq, hkv, shift, rot;
+  float eps;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_rope_append_kernel(RopeAppendArgs a) {
+  constexpr int E = 16 / sizeof(T), LPR = D / E;   // lanes a row: 8 (bf16, 64) to 64 (fp32, 256)
+  typedef T vec __attribute__((ext_vector_type(E)));
+  const int gl = threadIdx.x % LPR;
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  if (item >= a.items) return;                     // whole groups
+  const int nh = a.hq + 2 * a.hkv;
+  const int64_t row = item / nh;
+  const int head = (int)(item - row * nh);
+  const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
+  const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
+  const int64_t slot = is_q ? 0 : a.slots[row];
+  if (!is_q && (slot < 0 || slot >= a.limit)) return;
+  const char* src = is_q ? a.q + row * a.q_row + h * a.q_head
+                         : is_v ? a.v + row * a.v_row + h * a.v_head : a.k + row * a.k_row + h * a.k_head;
+  char* dst = is_q ? a.q_out + ((row * a.hq + h) * D) * (int64_t)sizeof(T)
+                   : (is_v ? a.vp : a.kp).row(slot >> a.shift, h, (int)(slot & ((1 << a.shift) - 1)));
+  vec x = *reinterpret_cast<const vec*>(src + 16 * gl);
+  if (!is_v) {
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = to_f32(x[e]);
+    const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
+    if (w != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+      for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o);
+      const float r = rsqrtf(ss / (float)D + a.eps);
+      const vec wv = *reinterpret_cast<const vec*>(w + E * gl);
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = y[e] * r * to_f32(wv[e]);
+    }
+    const int64_t pos = a.positions[row];
+    const bool inside = pos >= 0 && pos < a.table_rows;
+    const int half = a.rot / 2 / E;                // lanes to the other half
+    const int lane = threadIdx.x & 63;
+    const int other = gl < half ? lane + half : gl < 2 * half ? lane - half : lane;
+    float z[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = __shfl(y[e], other);
+    if (gl < 2 * half) {
+      const int64_t at = (inside ? pos : 0) * a.rot + E * gl;
+      const float sign = gl < half ? -1.f : 1.f;
+#pragma unroll
+      for (int e4 = 0; e4 < E; e4 += 4) {
+        const f32x4 c = *reinterpret_cast<const f32x4*>(a.cos + at + e4), s = *reinterpret_cast<const f32x4*>(a.sin + at + e4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e4 + e] = y[e4 + e] * c[e] + sign * z[e4 + e] * s[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = from_f32<T>(inside ? y[e] : __builtin_nanf(""));
+  }
+  *reinterpret_cast<vec*>(dst + 16 * gl) = x;
+}
+
+static int check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, const int64_t (&st)[6]) {
+  BFLY_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+                 "%s: page_size %d must be a power of two from 16 to 1024", what, page_size);
+  BFLY_CHECK_ARG(num_pages > 0 && num_pages <= INT32_MAX, "%s: bad num_pages", what);
+  for (int i = 0; i < 6; ++i)
+    BFLY_CHECK_ARG(st[i] >= 0 && st[i] < ((int64_t)1 << 48) && (st[i] * esize) % 16 == 0,
+                   "%s: page strides must be multiples of 16 bytes", what);
+  // offsets inside a page and head are kept in 32 bits
+  BFLY_CHECK_ARG(st[2] * esize * page_size <= INT32_MAX && st[5] * esize * page_size <= INT32_MAX,
+                 "%s: row stride too large", what);
+  return BFLY_OK;
+}
+
+int paged_check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, int64_t k_page,
+                      int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head, int64_t v_row) {
+  const int64_t st[6] = {k_page, k_head, k_row, v_page, v_head, v_row};
+  return check_pages(what, num_pages, page_size, esize, st);
+}
+
+static bool strides16(std::initializer_list<int64_t> st, int64_t esize) {
+  for (int64_t s : st)
+    if (s < 0 || s >= ((int64_t)1 << 48) || (s * esize) % 16 != 0) return false;
+  return true;
+}
+
+}  // namespace bfly
+
+using namespace bfly;
+
+extern "C" int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,
+                               const int32_t* lengths, const int32_t* counts, int32_t* free_pages,
+                               int64_t free_capacity, const int32_t* state, int page_size, int64_t num_rows,
+                               int32_t* lengths_out, int32_t* state_out, int32_t* starts, int64_t* slots,
+                               int64_t* positions, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+  BFLY_CHECK_ARG(requests >= 0 && requests <= (1 << 24) && table_width >= 0 && table_width <= INT32_MAX, "bad block table shape");
+  BFLY_CHECK_ARG(requests <= 1 || table_stride >= table_width, "block table rows overlap");
+  BFLY_CHECK_ARG(num_rows >= 0 && num_rows <= INT32_MAX && free_capacity >= 0 && free_capacity <= INT32_MAX,
+                 "num_rows and the free list must stay below 2^31");
+  BFLY_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+                 "page_size %d must be a power of two from 16 to 1024", page_size);
+  BFLY_CHECK_ARG(state && state_out && starts, "null pointer");
+  BFLY_CHECK_ARG(requests == 0 || (lengths && counts && lengths_out), "null pointer");
+  BFLY_CHECK_ARG(requests * table_width == 0 || block_table, "null pointer");
+  BFLY_CHECK_ARG(free_capacity == 0 || free_pages, "null pointer");
+  BFLY_CHECK_ARG(num_rows == 0 || (slots && positions), "null pointer");
+  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 4 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+                 "workspace too small");
+  PlanArgs a{};
+  a.table = block_table; a.lengths = lengths; a.counts = counts; a.free_pages = free_pages; a.state = state;
+  a.lengths_out = lengths_out; a.state_out = state_out; a.starts = starts; a.slots = slots; a.positions = positions;
+  a.taken = static_cast<int32_t*>(workspace);
+  a.table_stride = table_stride;
+  a.shift = __builtin_ctz(page_size);
+  const int64_t cap = table_width << a.shift;
+  a.capacity = cap < INT32_MAX ? cap : INT32_MAX;
+  a.requests = (int)requests; a.free_capacity = (int)free_capacity; a.num_rows = (int)num_rows;
+  const dim3 block(requests <= 256 && num_rows <= 256 ? 256 : kPlanMaxThreads);
+  if (requests <= kPlanLds && num_rows <= 4096) {
+    hipLaunchKernelGGL(plan_kernel<true>, dim3(1), block, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL(plan_kernel<false>, dim3(1), block, 0, stream, a);
+    if (num_rows > 0)
+      hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((num_rows + 255) / 256)), dim3(256), 0, stream, a);
+  }
+  BFLY_CHECK_LAUNCH("bfly_paged_plan");
+  return BFLY_OK;
+}
+
+extern "C" int bfly_paged_append(const void* k, const void* v, int dtype, int64_t rows, int hkv, int head_dim,
+                                 int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                                 int64_t v_head_stride, const int64_t* slots, void* k_pages, void* v_pages,
+                                 int64_t num_pages, int page_size, int64_t k_page_stride, int64_t k_page_head_stride,
+                                 int64_t k_page_row_stride, int64_t v_page_stride, int64_t v_page_head_stride,
+                                 int64_t v_page_row_stride, hipStream_t stream) {
+  BFLY_CHECK_ARG(dtype == BFLY_DTYPE_F32 || dtype == BFLY_DTYPE_BF16, "unsupported dtype %d", dtype);
+  const int64_t es = dtype == BFLY_DTYPE_F32 ? 4 : 2;
+  BFLY_CHECK_ARG(rows >= 0 && hkv > 0 && head_dim > 0, "bad shape");
+  BFLY_CHECK_ARG(head_dim * es % 16 == 0, "head_dim %d is not whole 16-byte pieces", head_dim);
+  const int rc = paged_check_pages("bfly_paged_append", num_pages, page_size, es, k_page_stride, k_page_head_stride,
+                                   k_page_row_stride, v_page_stride, v_page_head_stride, v_page_row_stride);
+  if (rc != BFLY_OK) return rc;
+  BFLY_CHECK_ARG(strides16({k_row_stride, k_head_stride, v_row_stride, v_head_stride}, es),
+                 "row and head strides must be multiples of 16 bytes");
+  if (rows == 0) return BFLY_OK;
+  BFLY_CHECK_ARG(k && v && slots && k_pages && v_pages, "null pointer");
+  BFLY_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages), "pointers must be 16-byte aligned");
+  AppendArgs a{};
+  a.k = static_cast<const char*>(k); a.v = static_cast<const char*>(v); a.slots = slots;
+  a.kp = {static_cast<char*>(k_pages), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
+  a.vp = {static_cast<char*>(v_pages), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
+  a.k_row = k_row_stride * es; a.k_head = k_head_stride * es; a.v_row = v_row_stride * es; a.v_head = v_head_stride * es;
+  a.limit = num_pages * page_size; a.hkv = hkv; a.per = (int)(head_dim * es / 16); a.shift = __builtin_ctz(page_size);
+  BFLY_CHECK_ARG(rows <= INT32_MAX && hkv <= 65535 && a.per <= 65535 && rows * hkv <= INT64_MAX / 65536 / 2, "too many rows");
+  a.pieces = rows * hkv * a.per;
+  const int64_t blocks = (2 * a.pieces + 255) / 256;
+  BFLY_CHECK_ARG(blocks <= INT32_MAX, "too many rows");
+  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  BFLY_CHECK_LAUNCH("bfly_paged_append");
+  return BFLY_OK;
+}
+
+extern "C" int bfly_paged_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t rows, int hq,
+                                      int hkv, int head_dim, int64_t q_row_stride, int64_t q_head_stride,
+                                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                                      int64_t v_head_stride, const void* q_weight, const void* k_weight, float eps,
+                                      const float* cos, const float* sin, int64_t table_rows, int rotary_dim,
+                                      const int64_t* positions, const int64_t* slots, void* q_out, void* k_pages,
+                                      void* v_pages, int64_t num_pages, int page_size, int64_t k_page_stride,
+                                      int64_t k_page_head_stride, int64_t k_page_row_stride, int64_t v_page_stride,
+                                      int64_t v_page_head_stride, int64_t v_page_row_stride, hipStream_t stream) {
+  BFLY_CHECK_ARG(dtype == BFLY_DTYPE_F32 || dtype == BFLY_DTYPE_BF16, "unsupported dtype %d", dtype);
+  const int64_t es = dtype == BFLY_DTYPE_F32 ? 4 : 2;
+  BFLY_CHECK_ARG(rows >= 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "bad head counts hq=%d hkv=%d", hq, hkv);
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
+    set_error("bfly_paged_rope_append: head_dim=%d unsupported (64, 128, 256)", head_dim);
+    return BFLY_ERR_UNSUPPORTED;
+  }
+  BFLY_CHECK_ARG(rotary_dim > 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0,
+                 "rotary_dim %d must be a multiple of 16, at most head_dim", rotary_dim);
+  BFLY_CHECK_ARG(table_rows > 0, "the cos/sin tables must have rows");
+  const int rc = paged_check_pages("bfly_paged_rope_append", num_pages, page_size, es, k_page_stride,
+                                   k_page_head_stride, k_page_row_stride, v_page_stride, v_page_head_stride,
+                                   v_page_row_stride);
+  if (rc != BFLY_OK) return rc;
+  BFLY_CHECK_ARG(strides16({q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride}, es),
+                 "row and head strides must be multiples of 16 bytes");
+  if (rows == 0) return BFLY_OK;
+  BFLY_CHECK_ARG(q && k && v && cos && sin && positions && slots && q_out && k_pages && v_pages, "null pointer");
+  BFLY_CHECK_ARG((q_weight == nullptr) == (k_weight == nullptr), "both norm weights or neither");
+  BFLY_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(cos) && aligned16(sin) && aligned16(q_out) &&
+                     aligned16(k_pages) && aligned16(v_pages) && aligned16(q_weight) && aligned16(k_weight),
+                 "pointers must be 16-byte aligned");
+  RopeAppendArgs a{};
+  a.q = static_cast<const char*>(q); a.k = static_cast<const char*>(k); a.v = static_cast<const char*>(v);
+  a.qw = q_weight; a.kw = k_weight; a.cos = cos; a.sin = sin; a.positions = positions; a.slots = slots;
+  a.q_out = static_cast<char*>(q_out);
+  a.kp = {static_cast<char*>(k_pages), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
+  a.vp = {static_cast<char*>(v_pages), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
+  a.q_row = q_row_stride * es; a.q_head = q_head_stride * es; a.k_row = k_row_stride * es;
+  a.k_head = k_head_stride * es; a.v_row = v_row_stride * es; a.v_head = v_head_stride * es;
+  a.limit = num_pages * page_size; a.table_rows = table_rows; a.hq = hq; a.hkv = hkv;
+  a.shift = __builtin_ctz(page_size); a.rot = rotary_dim; a.eps = eps;
+  BFLY_CHECK_ARG(rows <= INT32_MAX && hq <= (1 << 20) && (int64_t)hq + 2 * hkv <= (1 << 22), "too many rows");
+  a.items = rows * ((int64_t)hq + 2 * hkv);
+  const int64_t lanes = head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
+  BFLY_CHECK_ARG(blocks <= INT32_MAX, "too many rows");
+  const dim3 grid((unsigned)blocks), block(256);
+#define BFLY_ROPE(T, D) hipLaunchKernelGGL((paged_rope_append_kernel<T, D>), grid, block, 0, stream, a)
+  if (dtype == BFLY_DTYPE_BF16) {
+    if (head_dim == 64) BFLY_ROPE(__bf16, 64);
+    else if (head_dim == 128) BFLY_ROPE(__bf16, 128);
+    else BFLY_ROPE(__bf16, 256);
+  } else {
+    if (head_dim == 64) BFLY_ROPE(float, 64);
+    else if (head_dim == 128) BFLY_ROPE(float, 128);
+    else BFLY_ROPE(float, 256);
+  }
+#undef BFLY_ROPE
+  BFLY_CHECK_LAUNCH("bfly_paged_rope_append");
+  return BFLY_OK;
+}
