@@ -26,6 +26,7 @@ struct PlanArgs {
   int64_t* slots;
   int64_t* positions;
   int32_t* taken;          // [requests + 1]: pages taken by the requests before
+  int32_t* given;          // [requests + 1]: pages given back by them
   int64_t table_stride, capacity;   // capacity: tokens a table row holds
   int requests, shift, free_capacity, num_rows;
 };
@@ -58,18 +59,24 @@ __device__ __forceinline__ PlanStep plan_step(const PlanArgs& a, int b) {
   return s;
 }
 
+// The b with sums[b] <= i < sums[b + 1] (0 <= i < sums[requests]).
+__device__ __forceinline__ int plan_find(const int32_t* sums, int requests, int i) {
+  int lo = 0, hi = requests - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid + 1] > i) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+
 // Row i of the call: the request it belongs to by binary search in `starts`, its position, and its page: one
 // the request has, or the one it takes, which the page's first row also writes to the table.
 __device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* starts, const int32_t* taken,
                                          const int32_t* new_len, int i, bool ok, int64_t stack) {
   int64_t slot = -1, pos = 0;
   if (ok && i < starts[a.requests]) {
-    int lo = 0, hi = a.requests - 1;               // the first request with starts[b + 1] > i
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (starts[mid + 1] > i) hi = mid;
-      else lo = mid + 1;
-    }
+    const int lo = plan_find(starts, a.requests, i);
     const int count = starts[lo + 1] - starts[lo], old_len = new_len[lo] - count;
     pos = (int64_t)old_len + (i - starts[lo]);
     const int p_old = (int)(((int64_t)old_len + (1 << a.shift) - 1) >> a.shift), j = (int)(pos >> a.shift);
@@ -89,13 +96,14 @@ __device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* start
 }
 
 constexpr int kPlanMaxThreads = 1024;
-constexpr int kPlanLds = 4096;     // requests whose sums the one-launch form keeps in LDS
+constexpr int kPlanLds = 2048;     // requests whose sums the one-launch form keeps in LDS
 
 template <bool kRows>
 __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
   __shared__ PlanSum part[kPlanMaxThreads / 64];
   __shared__ int flags;
-  __shared__ int32_t s_starts[kRows ? kPlanLds + 1 : 1], s_taken[kRows ? kPlanLds + 1 : 1], s_new[kRows ? kPlanLds : 1];
+  __shared__ int32_t s_starts[kRows ? kPlanLds + 1 : 1], s_taken[kRows ? kPlanLds + 1 : 1], s_given[kRows ? kPlanLds + 1 : 1],
+      s_new[kRows ? kPlanLds : 1];
   const int t = threadIdx.x, nt = blockDim.x, lane = t & 63, wave = t >> 6;
   const int per = (a.requests + nt - 1) / nt;
   const int b0 = t * per < a.requests ? t * per : a.requests;
@@ -140,6 +148,8 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
     else if (top < 0 || top > a.free_capacity || stack > a.free_capacity) err = BFLY_PAGED_FREE_LIST;
   }
   const bool ok = err == 0;
+  int32_t* taken = kRows ? s_taken : a.taken;
+  int32_t* given = kRows ? s_given : a.given;
   // lengths may be updated in place: a thread reads its own requests before it writes them
   PlanSum at = before;
   for (int b = b0; b < b1; ++b) {
@@ -149,31 +159,33 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
     a.starts[b] = ok ? (int)at.rows : 0;
     if constexpr (kRows) {
       s_starts[b] = (int)at.rows;
-      s_taken[b] = (int)at.take;
       s_new[b] = s.new_len;
-    } else {
-      a.taken[b] = (int)at.take;
     }
-    if (ok) {
-      for (int j = s.p_new; j < s.p_old; ++j)
-        a.free_pages[stack - 1 - ((int64_t)at.give + (j - s.p_new))] = a.table[b * a.table_stride + j];
-      at = at + PlanSum{(uint32_t)s.count, (uint32_t)(s.p_old > s.p_new ? s.p_old - s.p_new : 0),
-                        (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
-    }
+    taken[b] = (int)at.take;
+    given[b] = (int)at.give;
+    at = at + PlanSum{(uint32_t)s.count, (uint32_t)(s.p_old > s.p_new ? s.p_old - s.p_new : 0),
+                      (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
   }
   if (t == 0) {
     a.starts[a.requests] = ok ? (int)total.rows : 0;
-    if constexpr (kRows) {
-      s_starts[a.requests] = (int)total.rows;
-      s_taken[a.requests] = (int)total.take;
-    } else {
-      a.taken[a.requests] = (int)total.take;
-    }
+    if constexpr (kRows) s_starts[a.requests] = (int)total.rows;
+    taken[a.requests] = (int)total.take;
+    given[a.requests] = (int)total.give;
   }
   __syncthreads();                                  // state is read by every thread before it is written
   if (t == 0) {
     a.state_out[0] = ok ? (int)(stack - total.take) : top;
     a.state_out[1] = err;
+  }
+  if (ok && total.give != 0) {
+    // the pages that are given back, a thread each: one request may leave with thousands
+    const int32_t* len = kRows ? s_new : a.lengths_out;
+    for (int i = t; i < (int)total.give; i += nt) {
+      const int b = plan_find(given, a.requests, i);
+      const int j = (int)(((int64_t)len[b] + (1 << a.shift) - 1) >> a.shift) + i - given[b];
+      a.free_pages[stack - 1 - i] = a.table[b * a.table_stride + j];
+    }
+    __syncthreads();
   }
   if constexpr (kRows)
     for (int i = t; i < a.num_rows; i += nt) plan_row(a, s_starts, s_taken, s_new, i, ok, stack);
@@ -344,12 +356,13 @@ extern "C" int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t t
   BFLY_CHECK_ARG(requests * table_width == 0 || block_table, "null pointer");
   BFLY_CHECK_ARG(free_capacity == 0 || free_pages, "null pointer");
   BFLY_CHECK_ARG(num_rows == 0 || (slots && positions), "null pointer");
-  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 4 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 8 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
                  "workspace too small");
   PlanArgs a{};
   a.table = block_table; a.lengths = lengths; a.counts = counts; a.free_pages = free_pages; a.state = state;
   a.lengths_out = lengths_out; a.state_out = state_out; a.starts = starts; a.slots = slots; a.positions = positions;
   a.taken = static_cast<int32_t*>(workspace);
+  a.given = a.taken + requests + 1;
   a.table_stride = table_stride;
   a.shift = __builtin_ctz(page_size);
   const int64_t cap = table_width << a.shift;

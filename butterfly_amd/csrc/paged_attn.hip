@@ -1,12 +1,35 @@
 // One new token of every request over its pages (include/butterfly_amd_paged.h).
 //
 //   s_t = scale q . k_t for the positions t it sees, m = max s_t, l = sum exp(s_t - m),
-//   o = (sum exp(s_t - m) v_t) / l, with running m and l over one pass of the keys.
+//   o = (sum exp(s_t - m) v_t) / l, in one pass over the keys with a running m and l.
+//
+// Work: a request's tiles (32 keys in bf16, 16 in fp32) are split into runs of at most c tiles, c such
+// that all requests and heads together make about kTarget runs.  A workgroup takes one run of one kv head
+// for up to 16 of its query heads; every workgroup finds its run from the lengths by itself (plan_run), so
+// the grid needs no host knowledge of them.  Requests with one run write their output, the others a
+// partial (fp32 sums, m, l) that paged_merge_kernel joins.
+//
+// A wave takes every fourth tile of the run, by itself: no barrier and no LDS until its sums meet the
+// other waves'.  S^T = K Q^T and O^T += V^T P^T on the matrix cores, query heads as columns, so a
+// lane's scores are the operand of the second product as they come:
+//   * K rows go from memory into the first product's operand registers (lane = key, 16 bytes of d a load).
+//   * V rows too (16 lanes take a row, a lane 4 (or 8) keys of one piece of d): the d of an output row is
+//     chosen so that the operand is the lane's own words, which v_perm_b32 pairs up by key.
+//   * The next tile's K is requested when this one's scores are done, its V after the second product.
 #include "paged.h"
 
 namespace bfly {
 
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
+constexpr int kTargetLog = 10;        // about 2^10 runs in all
+constexpr int kMinRun = 8;            // tiles of a run at least
+// A request of several runs has more than c tiles, so fewer than 2 tiles_b / c runs; all of them together,
+// with c >= total / 2^kTargetLog, fewer than 2^(kTargetLog + 1): the partials there can be.
+constexpr int kMaxSlots = 2 << kTargetLog;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <typename T>
+constexpr int kTile = sizeof(T) == 2 ? 32 : 16;
 
 struct PagedAttnArgs {
   const char* q;
@@ -16,85 +39,537 @@ struct PagedAttnArgs {
   void* out;
   float* l;
   float* m;
+  float* part;                           // partials: [slot][rows][D], then [slot][rows] m and l
+  float* part_ml;
   int64_t q_req, q_head, table_stride;   // bytes, bytes, elements
-  int64_t capacity;
-  int num_pages, hq, hkv, shift, window;
+  int64_t capacity;                      // tokens a table row holds
+  int requests, num_pages, hq, hkv, shift, window;
+  int group, row_tiles, rows;            // query heads a kv head; 16-row parts of them; rows of a part at most
+  int units;                             // hkv * row_tiles
   float scale;
 };
 
-// A workgroup per (request, query head): wave w takes keys w, w + 4, ..., a lane D / 64 elements.
+// What a request's workgroups do, from its length.
+struct Span {
+  int lo, n;      // positions seen: [lo, n)
+  int t0, tiles;  // tiles that hold them
+  bool off;       // the length is beyond the table
+};
+template <int KT>
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int b) {
+  const int len = a.lengths[b];
+  Span s;
+  s.off = (int64_t)len > a.capacity;
+  s.n = len <= 0 || s.off ? 0 : len;
+  s.lo = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
+  s.t0 = s.lo / KT;
+  s.tiles = s.n > 0 ? (s.n - 1) / KT + 1 - s.t0 : 0;
+  return s;
+}
+
+struct Run {
+  int b;          // request, -1: none
+  int sub;        // index inside the request
+  int splits;     // runs of the request (per unit)
+  int slot;       // partials before the request's
+};
+
+// The request that item `idx` falls into, where request b has units * splits_b items (kMerge: only
+// requests of more than one run, with `units` items each).  Every wave does it by itself: a lane sums a
+// stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
+template <int KT, bool kMerge>
+__device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
+  const int lane = threadIdx.x & 63;
+  const int per = (a.requests + 63) >> 6;
+  const int b0 = lane * per < a.requests ? lane * per : a.requests;
+  const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
+  int64_t total = 0;
+  for (int b = b0; b < b1; ++b) total += span_of<KT>(a, b).tiles;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+  total *= a.units;
+  int64_t c64 = (total + (1 << kTargetLog) - 1) >> kTargetLog;
+  const int c = c64 < kMinRun ? kMinRun : c64 > INT32_MAX ? INT32_MAX : (int)c64;
+  int64_t items = 0;
+  int slots = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int tiles = span_of<KT>(a, b).tiles;
+    const int s = tiles > c ? (tiles + c - 1) / c : 1;
+    items += kMerge ? (s > 1 ? 1 : 0) : s;
+    slots += s > 1 ? s : 0;
+  }
+  int64_t i_up = items;
+  int s_up = slots;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t vi = __shfl_up(i_up, o);
+    const int vs = __shfl_up(s_up, o);
+    if (lane >= o) {
+      i_up += vi;
+      s_up += vs;
+    }
+  }
+  const uint64_t over = __ballot(i_up * a.units > idx);
+  Run r{-1, 0, 0, 0};
+  if (over == 0) return r;
+  const int owner = __builtin_ctzll(over);
+  int64_t at = __shfl(i_up - items, owner);
+  int slot = __shfl(s_up - slots, owner);
+  for (int b = owner * per;; ++b) {               // (a request of the owner's stretch holds idx)
+    const int tiles = span_of<KT>(a, b).tiles;
+    const int s = tiles > c ? (tiles + c - 1) / c : 1;
+    const int64_t next = at + (kMerge ? (s > 1 ? 1 : 0) : s);
+    if (next * a.units > idx) {
+      r.b = b;
+      r.sub = (int)(idx - at * a.units);
+      r.splits = s;
+      r.slot = slot * a.units;
+      return r;
+    }
+    at = next;
+    slot += s > 1 ? s : 0;
+  }
+}
+
+__device__ __forceinline__ void store4(float* o, f32x4 y, float f) { *reinterpret_cast<f32x4*>(o) = y * f; }
+__device__ __forceinline__ void store4(__bf16* o, f32x4 y, float f) {
+  y *= f;
+  *reinterpret_cast<bf16x4*>(o) = __builtin_convertvector(y, bf16x4);
+}
+
+// The output and statistics of a row from its joined sums.  A row that sees nothing but scores of -inf
+// has no softmax: NaN, as exp(-inf - -inf) gives.
+template <typename T>
+__device__ __forceinline__ void finish_stats(const PagedAttnArgs& a, int64_t row, float m, float l) {
+  if (a.l == nullptr) return;
+  if (m == -INFINITY) l = __builtin_nanf("");
+  a.l[row] = l;
+  a.m[row] = l != l && fabsf(m) != INFINITY ? l : m;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+// The word without its bf16 infinities and NaN.
+__device__ __forceinline__ uint32_t finite_bf16(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+  return w;
+}
+
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+
+// One wave's sums over its tiles.  acc[i][r] of lane (n = lane & 15, g = lane >> 4): query row n, element
+// d_of(i, g, r).
+template <typename T, int D>
+struct Sweep;
+
+template <int D>
+struct Sweep<__bf16, D> {
+  static constexpr int KT = 32;
+  static constexpr int S = D / 32;                  // K pieces a subtile (and lane)
+  static constexpr int W = D == 64 ? 2 : 4;         // words of a V piece
+  static constexpr int H = D / (32 * W);            // V pieces a row (and lane): 1, or 2 for 256
+  static constexpr int N = D / 16;                  // products a tile, accumulators a lane
+  f32x4 acc[N];
+  float m, l;                                       // l: this lane's keys only
+  u32x4 q[S];
+  u32x4 k[2][S];
+  uint32_t v[8][H][W];
+
+  // element of acc[i][r]
+  static __device__ __forceinline__ int d_of(int i, int g, int r) {
+    return (i / (2 * W)) * (32 * W) + (2 * W) * (4 * g + r) + i % (2 * W);
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ void load_q(const char* row, int g) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      q[s] = row != nullptr ? *reinterpret_cast<const u32x4*>(row + 64 * s + 16 * g) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void load_k(const char* const (&base)[2], int row_bytes, int n, int g) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        k[u][s] = *reinterpret_cast<const u32x4*>(base[u] + (uint32_t)(n * row_bytes + 16 * g) + 64 * s);
+  }
+  __device__ __forceinline__ void load_v(const char* const (&base)[2], int row_bytes, int n, int g) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const char* p = base[j >> 2] + (uint32_t)((4 * g + (j & 3)) * row_bytes + 4 * W * n) + 256 * h;
+        if constexpr (W == 4) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) v[j][h][w] = x[w];
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          v[j][h][0] = x[0];
+          v[j][h][1] = x[1];
+        }
+      }
+  }
+  __device__ __forceinline__ void scores(float (&s)[8], float scale) const {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][i]), __builtin_bit_cast(bf16x8, q[i]), c,
+                                                    0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * u + i] = c[i] * scale;
+    }
+  }
+  static __device__ __forceinline__ int key(int i, int g) { return 16 * (i >> 2) + 4 * g + (i & 3); }
+  __device__ __forceinline__ void drop_v(int j) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int w = 0; w < W; ++w) v[j][h][w] = 0;
+  }
+  // The weights enter as two bf16 parts, 16 bits of them: with one part (8 bits) a weight would be off by
+  // as much as the output's own rounding.  kSafe: the second part skips V's infinities and NaN, which the
+  // first one has carried into the sums already (p * inf is inf, but the rest of p may be 0).
+  template <bool kSafe>
+  __device__ __forceinline__ void add(const float (&p)[8]) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = pack_bf16(p[2 * i], p[2 * i + 1]);
+      lo[i] = pack_bf16(p[2 * i] - __uint_as_float(hi[i] << 16), p[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
+    }
+    const bf16x8 ph = __builtin_bit_cast(bf16x8, u32x4{hi[0], hi[1], hi[2], hi[3]});
+    const bf16x8 pl = __builtin_bit_cast(bf16x8, u32x4{lo[0], lo[1], lo[2], lo[3]});
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int h = i / (2 * W), e = i % (2 * W), w = e >> 1;
+      const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+      u32x4 x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_perm(v[2 * j + 1][h][w], v[2 * j][h][w], sel);
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), ph, acc[i], 0, 0, 0);
+      if constexpr (kSafe) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = finite_bf16(x[j]);
+      }
+      acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), pl, acc[i], 0, 0, 0);
+    }
+  }
+};
+
+template <int D>
+struct Sweep<float, D> {
+  static constexpr int KT = 16;
+  static constexpr int S = D / 16;                  // K pieces a key (and lane)
+  static constexpr int H = D / 64;                  // V pieces a row (and lane)
+  static constexpr int N = D / 16;
+  f32x4 acc[N];
+  float m, l;
+  f32x4 q[S];
+  f32x4 k[S];
+  f32x4 v[4][H];
+
+  static __device__ __forceinline__ int d_of(int i, int g, int r) { return (i >> 2) * 64 + 4 * (4 * g + r) + (i & 3); }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+  }
+  __device__ __forceinline__ void load_q(const char* row, int g) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      q[s] = row != nullptr ? *reinterpret_cast<const f32x4*>(row + 64 * s + 16 * g) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void load_k(const char* const (&base)[1], int row_bytes, int n, int g) {
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      k[s] = *reinterpret_cast<const f32x4*>(base[0] + (uint32_t)(n * row_bytes + 16 * g) + 64 * s);
+  }
+  __device__ __forceinline__ void load_v(const char* const (&base)[1], int row_bytes, int n, int g) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        v[j][h] = *reinterpret_cast<const f32x4*>(base[0] + (uint32_t)((4 * g + j) * row_bytes + 16 * n) + 256 * h);
+  }
+  __device__ __forceinline__ void scores(float (&s)[4], float scale) const {
+    f32x4 c[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][e], q[i][e], c[e & 1], 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = (c[0][i] + c[1][i]) * scale;
+  }
+  static __device__ __forceinline__ int key(int i, int g) { return 4 * g + i; }
+  __device__ __forceinline__ void drop_v(int j) {
+#pragma unroll
+    for (int h = 0; h < H; ++h) v[j][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  template <bool kSafe>
+  __device__ __forceinline__ void add(const float (&p)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[j][i >> 2][i & 3], p[j], acc[i], 0, 0, 0);
+  }
+};
+
+// The pages of tile t: one base per 16 keys, with the page's and the rows' offsets.  Keys outside [lo, n)
+// share the page of the nearest key inside, so no entry behind the last page (or before the window) is read.
+template <int U>
+__device__ __forceinline__ bool tile_pages(const PagedAttnArgs& a, const int32_t* row, int first, const Span& s, int (&id)[U]) {
+  bool bad = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    unsigned t = (unsigned)first + 16 * u;
+    t = t < (unsigned)s.lo ? s.lo : t > (unsigned)s.n - 1 ? s.n - 1 : t;
+    id[u] = row[t >> a.shift];
+    if ((unsigned)id[u] >= (unsigned)a.num_pages) {
+      bad = true;
+      id[u] = 0;
+    }
+  }
+  return bad;
+}
+template <int U>
+__device__ __forceinline__ void tile_base(const PagedAttnArgs& a, const PagePtr& p, int h, int first, const int (&id)[U],
+                                          const char* (&base)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) base[u] = p.row(id[u], h, (first + 16 * u) & ((1 << a.shift) - 1));
+}
+
+// Tiles t, t + 4, ... below t_end.  Returns whether a page id was outside the pages.
+template <typename T, int D, bool kSafe>
+__device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, const int32_t* row, const Span& s, int kvh,
+                                      int t, int t_end) {
+  constexpr int KT = kTile<T>, U = KT / 16, P = KT / 4;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  w.clear();
+  if (t >= t_end) return false;
+  int id[U];
+  const char* base[U];
+  bool bad = tile_pages<U>(a, row, t * KT, s, id);
+  tile_base<U>(a, a.kp, kvh, t * KT, id, base);
+  w.load_k(base, a.kp.row_bytes, n, g);
+  tile_base<U>(a, a.vp, kvh, t * KT, id, base);
+  w.load_v(base, a.vp.row_bytes, n, g);
+  while (true) {
+    const int next = t + 4;
+    const bool more = next < t_end;
+    if (more) bad |= tile_pages<U>(a, row, next * KT, s, id);
+    float p[P];
+    w.scores(p, a.scale);
+    if (more) {
+      tile_base<U>(a, a.kp, kvh, next * KT, id, base);
+      w.load_k(base, a.kp.row_bytes, n, g);
+    }
+    const unsigned first = (unsigned)t * KT, lo = s.lo, end = s.n;
+    if (first < lo || first + KT > end) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const unsigned at = first + w.key(i, g);
+        if (at < lo || at >= end) {
+          p[i] = -INFINITY;
+          w.drop_v(i);                              // V's piece i is of the same key as score i
+        }
+      }
+    }
+    float mx = p[0];
+#pragma unroll
+    for (int i = 1; i < P; ++i) mx = fmaxf(mx, p[i]);
+    mx = col_max4(mx);
+    if (__any(mx > w.m)) {
+      const float nm = fmaxf(w.m, mx);
+      const float f = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m - nm) * kLog2e);
+      w.l *= f;
+#pragma unroll
+      for (int i = 0; i < w.N; ++i) w.acc[i] *= f;
+      w.m = nm;
+    }
+    const float ref = w.m == -INFINITY ? 0.f : w.m;
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * kLog2e);
+      sum += p[i];
+    }
+    w.l += sum;
+    w.template add<kSafe>(p);
+    if (!more) return bad;
+    tile_base<U>(a, a.vp, kvh, next * KT, id, base);
+    w.load_v(base, a.vp.row_bytes, n, g);
+    t = next;
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
-  constexpr int E = D / 64;
-  const int b = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int kvh = h / (a.hq / a.hkv);
-  const int len = a.lengths[b];
-  const bool off_table = (int64_t)len > a.capacity;
-  const int n = len <= 0 || off_table ? 0 : len;
-  const int lo = a.window > 0 && n > a.window ? n - a.window : 0;
-  float q[E], acc[E], m = -INFINITY, l = 0.f;
-  const T* qr = reinterpret_cast<const T*>(a.q + b * a.q_req + h * a.q_head);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    q[e] = to_f32(qr[lane * E + e]);
-    acc[e] = 0.f;
-  }
-  bool bad = off_table;
-  for (int t = lo + wave; t < n; t += 4) {
-    int page = a.table[b * a.table_stride + (t >> a.shift)];
-    if (page < 0 || page >= a.num_pages) {
-      bad = true;
-      page = 0;
-    }
-    const int r = t & ((1 << a.shift) - 1);
-    const T* k = reinterpret_cast<const T*>(a.kp.row(page, kvh, r));
-    const T* v = reinterpret_cast<const T*>(a.vp.row(page, kvh, r));
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f32(k[lane * E + e]), s);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
-    s *= a.scale;
-    const float nm = fmaxf(m, s);
-    const float ref = nm == -INFINITY ? 0.f : nm;
-    const float c = expf(m - ref), p = expf(s - ref);
-    l = l * c + p;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(p, to_f32(v[lane * E + e]), acc[e] * c);
-    m = nm;
-  }
-  __shared__ float sm[4], sl[4], so[4][D];
+  constexpr int KT = kTile<T>, LD = D + 4;
+  __shared__ float so[4][16 * LD];
+  __shared__ float sm[4][16], sl[4][16];
   __shared__ int sbad;
+  const Run run = plan_run<KT, false>(a, blockIdx.x);
+  if (run.b < 0) return;
+  const int b = __builtin_amdgcn_readfirstlane(run.b), splits = __builtin_amdgcn_readfirstlane(run.splits);
+  const int sub = __builtin_amdgcn_readfirstlane(run.sub), slot = __builtin_amdgcn_readfirstlane(run.slot) + sub;
+  const int unit = sub / splits, split = sub - unit * splits;
+  const int kvh = unit / a.row_tiles, part = unit - kvh * a.row_tiles;
+  const int rows = a.group - 16 * part < 16 ? a.group - 16 * part : 16;
+  const int head0 = kvh * a.group + 16 * part;
+  const Span s = span_of<KT>(a, b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int64_t row0 = (int64_t)b * a.hq + head0;
+  if (s.tiles == 0) {                               // nothing to see, or a length beyond the table
+    const float y = s.off ? __builtin_nanf("") : 0.f;
+    for (int i = threadIdx.x; i < rows * D; i += 256) static_cast<T*>(a.out)[row0 * D + i] = from_f32<T>(y);
+    if (a.l != nullptr && threadIdx.x < rows) {
+      a.l[row0 + threadIdx.x] = y;
+      a.m[row0 + threadIdx.x] = s.off ? y : kPagedNeg;
+    }
+    return;
+  }
+  const int each = s.tiles / splits, extra = s.tiles - each * splits;
+  const int t0 = s.t0 + split * each + (split < extra ? split : extra), t1 = t0 + each + (split < extra ? 1 : 0);
+  const int32_t* table = a.table + b * a.table_stride;
   if (threadIdx.x == 0) sbad = 0;
+  Sweep<T, D> w;
+  w.load_q(n < rows ? a.q + b * a.q_req + (int64_t)(head0 + n) * a.q_head : nullptr, g);
+  bool bad = sweep<T, D, false>(a, w, table, s, kvh, t0 + wave, t1);
+  if constexpr (sizeof(T) == 2) {
+    // infinities or NaN in the sums of a row whose weights are finite come from V: once more, with care
+    float big = 0.f;
+#pragma unroll
+    for (int i = 0; i < w.N; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) big = fmaxf(big, w.acc[i][r] - w.acc[i][r] == 0.f ? 0.f : 1.f);
+    if (__any(big != 0.f)) bad |= sweep<T, D, true>(a, w, table, s, kvh, t0 + wave, t1);
+  }
+  const float l = col_sum4(w.l);
   __syncthreads();
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
-    if (bad) sbad = 1;
+  if (n < rows) {
+#pragma unroll
+    for (int i = 0; i < w.N; i += 4)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(&so[wave][n * LD + w.d_of(i, g, r)]) =
+            f32x4{w.acc[i][r], w.acc[i + 1][r], w.acc[i + 2][r], w.acc[i + 3][r]};
+    if (g == 0) {
+      sm[wave][n] = w.m;
+      sl[wave][n] = l;
+    }
+  }
+  if (bad && lane == 0) sbad = 1;
+  __syncthreads();
+  const float poison = sbad ? __builtin_nanf("") : 0.f;
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+    const int r = i / (D / 4), c = 4 * (i % (D / 4));
+    const float mm = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    const float ref = mm == -INFINITY ? 0.f : mm;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    float ll = poison;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = __builtin_amdgcn_exp2f((sm[k][r] - ref) * kLog2e);
+      // a wave without tiles has no part in it (0 * its sums would do, but for a reference of +inf)
+      if (t0 + k < t1) {
+        ll += f * sl[k][r];
+        y += f * *reinterpret_cast<const f32x4*>(&so[k][r * LD + c]);
+      }
+    }
+    if (splits == 1) {
+      store4(static_cast<T*>(a.out) + (row0 + r) * D + c, y, 1.f / ll);
+      if (c == 0) finish_stats<T>(a, row0 + r, mm, ll);
+    } else {
+      const int64_t at = (int64_t)slot * a.rows + r;
+      *reinterpret_cast<f32x4*>(a.part + at * D + c) = y;
+      if (c == 0) {
+        a.part_ml[2 * at] = mm;
+        a.part_ml[2 * at + 1] = ll;
+      }
+    }
+  }
+}
+
+// Joins the partials of a request's runs: a workgroup per (request, unit, row, 64 elements).  The runs'
+// weights exp(m_i - m) are made once, in LDS; then 16 lanes across the elements, the runs dealt to 16 groups
+// of lanes, four loads under way in each.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
+  constexpr int KT = kTile<T>, G = 16;
+  __shared__ f32x4 sy[G][16];
+  __shared__ float weight[kMaxSlots], sl[4], smx[4];
+  const Run run = plan_run<KT, true>(a, blockIdx.x);
+  if (run.b < 0) return;
+  const int kvh = run.sub / a.row_tiles, part = run.sub - kvh * a.row_tiles, r = blockIdx.y;
+  if (16 * part + r >= a.group) return;
+  const int64_t slot0 = run.slot + (int64_t)run.sub * run.splits;
+  const int t = threadIdx.x, gr = t >> 4, c = 64 * blockIdx.z + 4 * (t & 15);
+  const float* ml = a.part_ml + 2 * (slot0 * a.rows + r);
+  float mm = -INFINITY;
+  for (int i = t; i < run.splits; i += 256) {
+    const float x = ml[2 * (int64_t)i * a.rows];
+    weight[i] = x;
+    mm = fmaxf(mm, x);
   }
 #pragma unroll
-  for (int e = 0; e < E; ++e) so[wave][lane * E + e] = acc[e];
+  for (int o = 1; o < 64; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+  if ((t & 63) == 0) smx[t >> 6] = mm;
   __syncthreads();
-  const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+  mm = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
   const float ref = mm == -INFINITY ? 0.f : mm;
-  float w[4], ll = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    w[i] = expf(sm[i] - ref);
-    ll += w[i] * sl[i];
+  float l = 0.f;
+  for (int i = t; i < run.splits; i += 256) {
+    const float f = __builtin_amdgcn_exp2f((weight[i] - ref) * kLog2e);
+    weight[i] = f;
+    l += f * ml[2 * (int64_t)i * a.rows + 1];
   }
-  const int64_t row = (int64_t)b * a.hq + h;
-  const bool nan = sbad != 0;
-  for (int c = threadIdx.x; c < D; c += 256) {
-    float y = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y += w[i] * so[i][c];
-    y = nan ? __builtin_nanf("") : n > lo ? y / ll : 0.f;
-    static_cast<T*>(a.out)[row * D + c] = from_f32<T>(y);
-  }
-  if (threadIdx.x == 0 && a.l != nullptr) {
-    a.l[row] = nan ? __builtin_nanf("") : n > lo ? ll : 0.f;
-    a.m[row] = nan ? __builtin_nanf("") : n > lo ? mm : kPagedNeg;
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  if ((t & 63) == 0) sl[t >> 6] = l;
+  __syncthreads();
+  l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  const float* src = a.part + (slot0 * a.rows + r) * D + c;
+  const int64_t step = (int64_t)a.rows * D;
+#pragma unroll 4
+  for (int i = gr; i < run.splits; i += G) y += weight[i] * *reinterpret_cast<const f32x4*>(src + i * step);
+  sy[gr][t & 15] = y;
+  __syncthreads();
+  if (gr != 0) return;
+#pragma unroll
+  for (int i = 1; i < G; ++i) y += sy[i][t];
+  const int64_t row = (int64_t)run.b * a.hq + kvh * a.group + 16 * part + r;
+  store4(static_cast<T*>(a.out) + row * D + c, y, 1.f / l);
+  if (c == 0) finish_stats<T>(a, row, mm, l);
+}
+
+// Whether any request can have more than one run: its table row (or the window) holds more than kMinRun tiles.
+static int64_t most_tiles(int64_t capacity, int window, int kt) {
+  const int64_t keys = window > 0 && window < capacity ? (int64_t)window + kt - 1 : capacity;
+  return (keys + kt - 1) / kt;
+}
+template <typename T, int D>
+static void launch_paged(const PagedAttnArgs& a, int64_t items, bool splits, hipStream_t stream) {
+  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(256), 0, stream, a);
+  if (splits) {
+    const int64_t pairs = (int64_t)a.requests * a.units;
+    const unsigned x = (unsigned)(pairs < (1 << kTargetLog) ? pairs : (1 << kTargetLog));
+    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(x, (unsigned)a.rows, D / 64), dim3(256), 0, stream, a);
   }
 }
 
@@ -104,8 +579,10 @@ using namespace bfly;
 
 extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim,
                                                         int64_t table_width, int page_size, int window) {
-  (void)requests; (void)hq; (void)hkv; (void)head_dim; (void)table_width; (void)page_size; (void)window;
-  return 0;
+  if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
+  if (most_tiles(table_width * page_size, window, 16) <= kMinRun) return 0;
+  const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
+  return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
 
 extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, int hq, int hkv, int head_dim,
@@ -136,6 +613,8 @@ extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, 
   BFLY_CHECK_ARG((l == nullptr) == (m == nullptr), "both l and m or neither");
   BFLY_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out), "pointers must be 16-byte aligned");
   BFLY_CHECK_ARG(requests <= 65535, "at most 65535 requests");
+  const int64_t need = bfly_paged_attention_workspace_bytes(requests, hq, hkv, head_dim, table_width, page_size, window);
+  BFLY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), "workspace too small");
   PagedAttnArgs a{};
   a.q = static_cast<const char*>(q);
   a.kp = {static_cast<char*>(const_cast<void*>(k_pages)), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
@@ -143,9 +622,20 @@ extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, 
   a.table = block_table; a.lengths = lengths; a.out = out; a.l = l; a.m = m;
   a.q_req = q_request_stride * es; a.q_head = q_head_stride * es; a.table_stride = table_stride;
   a.shift = __builtin_ctz(page_size); a.capacity = table_width << a.shift;
-  a.num_pages = (int)num_pages; a.hq = hq; a.hkv = hkv; a.window = window; a.scale = scale;
-  const dim3 grid((unsigned)hq, (unsigned)requests), block(256);
-#define BFLY_PAGED(T, D) hipLaunchKernelGGL((paged_attn_kernel<T, D>), grid, block, 0, stream, a)
+  a.requests = (int)requests; a.num_pages = (int)num_pages; a.hq = hq; a.hkv = hkv; a.window = window; a.scale = scale;
+  a.group = hq / hkv; a.row_tiles = (a.group + 15) / 16; a.rows = a.group < 16 ? a.group : 16;
+  BFLY_CHECK_ARG((int64_t)hkv * a.row_tiles <= 65535, "too many heads");
+  a.units = hkv * a.row_tiles;
+  a.part = static_cast<float*>(workspace);
+  a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * head_dim;
+  // runs: one for each (request, unit), and as many more as the splits make (kTargetLog, plan_run)
+  const int kt = dtype == BFLY_DTYPE_F32 ? kTile<float> : kTile<__bf16>;
+  const int64_t tiles = most_tiles(a.capacity, window, kt), pairs = requests * a.units;
+  const bool splits = tiles > kMinRun;
+  const int64_t most = pairs * ((tiles + kMinRun - 1) / kMinRun), some = pairs + (1 << kTargetLog);
+  const int64_t items = !splits ? pairs : most < some ? most : some;
+  BFLY_CHECK_ARG(items <= INT32_MAX, "too many requests and heads");
+#define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)
   if (dtype == BFLY_DTYPE_BF16) {
     if (head_dim == 64) BFLY_PAGED(__bf16, 64);
     else if (head_dim == 128) BFLY_PAGED(__bf16, 128);

@@ -21,16 +21,15 @@ gradients enabled they refuse tensors that require them.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
-from typing import List, Optional, Sequence, Union
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _native
-from ._device import on, stream_of
-from .attention import _check_heads, _dtype_code, _require_cuda, _scale
+from ._device import _GET_DEVICE, on, stream_of
+from .attention import _dtype_code
 
-PAGE_SIZES = tuple(1 << i for i in range(4, 11))
+PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
 
 # state[1] after a plan that did not fit (include/butterfly_amd_paged.h)
 PLAN_ERRORS = {
@@ -42,8 +41,7 @@ PLAN_ERRORS = {
 }
 
 
-@dataclass
-class PagedPlan:
+class PagedPlan(NamedTuple):
     """What :func:`paged_plan` gives: the requests' new ``lengths`` [B], ``state`` [2] (free pages, error),
     ``starts`` [B + 1] (each request's first row), ``slots`` and ``positions`` [num_rows] of the new rows."""
 
@@ -54,71 +52,90 @@ class PagedPlan:
     positions: torch.Tensor
 
 
-def _no_grad(*ts: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise ValueError("the paged operators are for inference: call them under torch.no_grad()")
+# The checks below cost a decode step's host time (these calls take 4 to 8 us on the GPU): each tests what a
+# well-formed call has in as few attribute reads as it takes, and only then, case by case, what is wrong.
+_GRAD = "the paged operators are for inference: call them under torch.no_grad()"
 
 
-def _one_device(*ts: Optional[torch.Tensor]) -> torch.device:
-    ts = [t for t in ts if t is not None]
-    _require_cuda(*ts)
-    if any(t.device != ts[0].device for t in ts):
-        raise ValueError("all tensors must be on one device")
-    return ts[0].device
+def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError("butterfly_amd operators take GPU tensors (device 'cuda')")
+    for o in others:
+        if o is not None and o.get_device() != dev:
+            raise ValueError("all tensors must be GPU tensors of one device")
+    return dev
 
 
-def _check_page_size(page_size: int) -> int:
-    if page_size not in PAGE_SIZES:
-        raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
-    return int(page_size)
+def _call(dev: int, name: str, *args) -> None:
+    if dev == _GET_DEVICE():
+        _native.call(name, *args, stream_of(dev))
+    else:
+        with on(torch.device("cuda", dev)):
+            _native.call(name, *args, stream_of(dev))
 
 
-def _ints(t: torch.Tensor, name: str, dtype: torch.dtype, n: Optional[int] = None) -> torch.Tensor:
-    if t.dim() != 1 or t.dtype != dtype or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be a 1-D {dtype} tensor" + (f" of {n}" if n is not None else ""))
-    return t
+def _check_ints(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> None:
+    if t.dim() != 1 or t.dtype != dtype or t.shape[0] != n:
+        raise ValueError(f"{name} must be a 1-D {dtype} tensor of {n}")
 
 
-def _table(t: torch.Tensor, b: int) -> int:
-    """The block table's row stride."""
-    if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != b:
+def _table_stride(t: torch.Tensor, b: int) -> int:
+    """The block table's row stride (its width where there is one row)."""
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not torch.int32 or shape[0] != b:
         raise ValueError(f"block_table must be an int32 [{b}, pages] tensor")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    stride, one = t.stride()
+    if one != 1 and shape[1] > 1:
         raise ValueError("block_table's rows must be contiguous")
-    return t.stride(0) if b > 1 else max(1, t.shape[1])
+    return stride if b > 1 else shape[1]
 
 
-def _strides(t: torch.Tensor, dims) -> List[int]:
-    """Strides of ``dims``; 0 where a dimension has a single entry."""
-    return [t.stride(i) if t.shape[i] > 1 else 0 for i in dims]
-
-
-def _rows_fit(t: torch.Tensor, dims) -> bool:
-    """Whether a kernel's 16-byte accesses take ``t`` as it lies: contiguous in its last dimension, 16-byte
-    aligned in every other (``dims``)."""
+def _lies(t: torch.Tensor, dims: int):
+    """The strides of the first ``dims`` dimensions of ``t`` where 16-byte accesses take it as it lies
+    (contiguous in the last dimension, 16-byte aligned in every other), else None."""
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)][:dims]
     es = t.element_size()
-    return (t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(s >= 0 and s * es % 16 == 0 for s in _strides(t, dims)))
+    if t.data_ptr() % 16 or t.stride(-1) != 1 or any(s * es % 16 for s in strides):
+        return None
+    return strides
 
 
-def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, written: bool) -> List[int]:
-    """The six page, head and row strides of a pair of page tensors."""
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: int, written: bool):
+    """Shape and the six page, head and row strides of a pair of page tensors."""
+    shape, dtype = k_pages.shape, k_pages.dtype
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not dtype:
         raise ValueError("k_pages and v_pages must be [num_pages, Hkv, page_size, d] of one shape and type")
-    if 0 in k_pages.shape:
+    if k_pages.get_device() != dev or v_pages.get_device() != dev:
+        raise ValueError("all tensors must be GPU tensors of one device")
+    if shape[2] not in PAGE_SIZES:
+        raise ValueError(f"page_size {shape[2]} must be a power of two from 16 to 1024")
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    kd, vd = k_pages.data_ptr(), v_pages.data_ptr()
+    if k3 == v3 == 1 and kd and vd and not ((kd | vd) & 15 or (k0 | k1 | k2 | v0 | v1 | v2) & (7 if dtype is torch.bfloat16 else 3)) \
+            and (not written or k0 and k1 and k2 and v0 and v1 and v2 and kd != vd):
+        return shape, (k0, k1, k2, v0, v1, v2)
+    if 0 in shape:
         raise ValueError("the pages hold nothing")
-    _check_page_size(k_pages.shape[2])
-    for t in (k_pages, v_pages):
-        if not _rows_fit(t, (0, 1, 2)):
-            raise ValueError("pages must be contiguous in head_dim and 16-byte aligned in every other dimension")
-        if written and any(t.shape[i] > 1 and t.stride(i) == 0 for i in range(3)):
-            raise ValueError("pages that are written must not overlap themselves")
-    return _strides(k_pages, (0, 1, 2)) + _strides(v_pages, (0, 1, 2))
+    k, v = _lies(k_pages, 3), _lies(v_pages, 3)
+    if k is None or v is None:
+        raise ValueError("pages must be contiguous in head_dim and 16-byte aligned in every other dimension")
+    if written and (kd == vd or any(s == 0 and n > 1 for s, n in zip(k + v, tuple(shape[:3]) * 2))):
+        raise ValueError("pages that are written must not overlap themselves or each other")
+    return shape, (*k, *v)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[N, H, d] rows that the kernels take as they lie, or a contiguous copy."""
-    return t if _rows_fit(t, (0, 1)) else t.clone(memory_format=torch.contiguous_format)
+def _rows(t: torch.Tensor):
+    """[N, H, d] rows and their two strides, as they lie where a kernel takes them so, else of a contiguous copy."""
+    s0, s1, s2 = t.stride()
+    if s2 == 1 and not (t.data_ptr() & 15 or (s0 | s1) & (7 if t.dtype is torch.bfloat16 else 3)):
+        return t, s0, s1
+    strides = _lies(t, 2)
+    if strides is None:
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides[0], strides[1]
 
 
 def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor,
@@ -139,40 +156,49 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     ``state[1]`` holds the code and every slot is -1, and so for every later step until the caller clears
     it: a captured loop that ran out of pages is found out by reading the state once.
     """
-    dev = _one_device(block_table, lengths, counts, free_pages, state)
-    page_size, num_rows = _check_page_size(page_size), int(num_rows)
-    b = lengths.shape[0] if lengths.dim() == 1 else -1
-    stride = _table(block_table, b)
-    if b > 1 and stride < block_table.shape[1]:
+    dev = _device_of(lengths, block_table, counts, free_pages, state)
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
+    if lengths.dim() != 1:
+        raise ValueError("lengths must be a 1-D torch.int32 tensor")
+    b, i32 = lengths.shape[0], torch.int32
+    if not lengths.dtype is counts.dtype is state.dtype is free_pages.dtype is i32 or counts.shape != lengths.shape \
+            or state.shape != (2,) or free_pages.dim() != 1:
+        raise ValueError("lengths and counts [B], free_pages and state [2] must be 1-D torch.int32 tensors")
+    stride, width = _table_stride(block_table, b), block_table.shape[1]
+    if stride < width:
         raise ValueError("block_table's rows must not overlap")
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
-    i32 = torch.int32
-    for t, name, n in ((lengths, "lengths", b), (counts, "counts", b), (free_pages, "free_pages", None), (state, "state", 2)):
-        _ints(t, name, i32, n)
-    if not free_pages.is_contiguous() or in_place and not (lengths.is_contiguous() and state.is_contiguous()):
-        raise ValueError("tensors that are updated must be contiguous")
-    lengths, counts, state = lengths.contiguous(), counts.contiguous(), state.contiguous()
-    new_lengths, new_state = (lengths, state) if in_place else (torch.empty_like(lengths), torch.empty_like(state))
-    # the row starts and, behind them, the kernel's workspace
-    starts = torch.empty(2, b + 1, dtype=i32, device=dev)
-    rows = torch.empty(2, num_rows, dtype=torch.int64, device=dev)
-    with on(dev):
-        _native.call("bfly_paged_plan", block_table.data_ptr(), b, block_table.shape[1], stride, lengths.data_ptr(),
-                     counts.data_ptr(), free_pages.data_ptr(), free_pages.numel(), state.data_ptr(), page_size, num_rows,
-                     new_lengths.data_ptr(), new_state.data_ptr(), starts.data_ptr(), rows.data_ptr(),
-                     rows.data_ptr() + 8 * num_rows, starts.data_ptr() + 4 * (b + 1), 4 * (b + 1), stream_of(dev))
-    return PagedPlan(new_lengths, new_state, starts[0], rows[0], rows[1])
+    if not (lengths.is_contiguous() and counts.is_contiguous() and state.is_contiguous() and free_pages.is_contiguous()):
+        if not free_pages.is_contiguous() or in_place and not (lengths.is_contiguous() and state.is_contiguous()):
+            raise ValueError("tensors that are updated must be contiguous")
+        lengths, counts, state = lengths.contiguous(), counts.contiguous(), state.contiguous()
+    cuda = lengths.device
+    # one allocation for the int32 results and the kernel's workspace, one for the rows
+    if in_place:
+        new_lengths, new_state = lengths, state
+        starts, ws = torch.empty(3 * b + 3, dtype=i32, device=cuda).split_with_sizes((b + 1, 2 * b + 2))
+    else:
+        new_lengths, new_state, starts, ws = torch.empty(4 * b + 5, dtype=i32, device=cuda).split_with_sizes(
+            (b, 2, b + 1, 2 * b + 2))
+    slots, positions = torch.empty(2, num_rows, dtype=torch.int64, device=cuda).unbind(0)
+    _call(dev, "bfly_paged_plan", block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(),
+          free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size, num_rows, new_lengths.data_ptr(),
+          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 8 * (b + 1))
+    return PagedPlan(new_lengths, new_state, starts, slots, positions)
 
 
-def _check_rows(k, v, k_pages, v_pages, slots):
-    if k.dim() != 3 or k.shape != v.shape:
-        raise ValueError("k and v must be [N, Hkv, d] of one shape")
-    if not k.dtype == v.dtype == k_pages.dtype:
+def _check_rows(k, v, shape, dtype, slots, dev):
+    n = k.shape
+    if len(n) != 3 or v.shape != n or n[1] != shape[1] or n[2] != shape[3]:
+        raise ValueError("k and v must be [N, Hkv, d] of the pages' heads and head_dim")
+    if not k.dtype is v.dtype is dtype:
         raise ValueError("rows and pages must have one type")
-    if k_pages.dim() == 4 and (k.shape[1], k.shape[2]) != (k_pages.shape[1], k_pages.shape[3]):
-        raise ValueError("rows and pages must have the same heads and head_dim")
-    _ints(slots, "slots", torch.int64, k.shape[0])
+    if k.get_device() != dev or v.get_device() != dev:
+        raise ValueError("all tensors must be GPU tensors of one device")
+    _check_ints(slots, "slots", torch.int64, n[0])
+    return n
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -181,21 +207,20 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     [num_pages, Hkv, page_size, d], one launch of ``bfly_paged_append``.  A row whose slot is negative or
     beyond the pages is passed over.  The slots of a call are distinct, as a plan gives them (of two rows
     with one slot it is not defined which stays).  float32 or bfloat16; ``d`` of whole 16-byte pieces."""
-    dev = _one_device(k, v, k_pages, v_pages, slots)
-    _no_grad(k, v, k_pages, v_pages)
-    strides = _pages(k_pages, v_pages, True)
-    _check_rows(k, v, k_pages, v_pages, slots)
-    n, hkv, d = k.shape
+    dev = _device_of(slots)
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise ValueError(_GRAD)
+    shape, strides = _pages(k_pages, v_pages, dev, True)
+    n, hkv, d = _check_rows(k, v, shape, k_pages.dtype, slots, dev)
     code = _dtype_code(k)
-    if d * k.element_size() % 16:
+    if d % (4 if code == _native.DTYPE_F32 else 8):
         raise ValueError("head_dim must be whole 16-byte pieces")
     if n == 0:
         return
-    k, v, slots = _rows(k), _rows(v), slots.contiguous()
-    with on(dev):
-        _native.call("bfly_paged_append", k.data_ptr(), v.data_ptr(), code, n, hkv, d, *_strides(k, (0, 1)),
-                     *_strides(v, (0, 1)), slots.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0],
-                     k_pages.shape[2], *strides, stream_of(dev))
+    (k, k0, k1), (v, v0, v1) = _rows(k), _rows(v)
+    slots = slots.contiguous()
+    _call(dev, "bfly_paged_append", k.data_ptr(), v.data_ptr(), code, n, hkv, d, k0, k1, v0, v1, slots.data_ptr(),
+          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides)
 
 
 def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -213,38 +238,45 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     Between the inputs and the outputs nothing is rounded to fewer than 32 bits (``bfly_qk_norm_rope``, whose
     rounding points are the modules', rounds after the norm as well).  head_dim 64, 128 or 256, ``r`` a multiple
     of 16."""
-    dev = _one_device(q, k, v, k_pages, v_pages, slots, positions, cos, sin, q_weight, k_weight)
-    _no_grad(q, k, v, k_pages, v_pages, cos, sin, q_weight, k_weight)
-    strides = _pages(k_pages, v_pages, True)
-    _check_rows(k, v, k_pages, v_pages, slots)
-    n, hkv, d = k.shape
-    if q.dim() != 3 or (q.shape[0], q.shape[2]) != (n, d) or q.dtype != k.dtype:
+    dev = _device_of(q, slots, positions, cos, sin, q_weight, k_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages, cos, sin, q_weight,
+                                                                                  k_weight)):
+        raise ValueError(_GRAD)
+    shape, strides = _pages(k_pages, v_pages, dev, True)
+    dtype = k_pages.dtype
+    n, hkv, d = _check_rows(k, v, shape, dtype, slots, dev)
+    sq = q.shape
+    if len(sq) != 3 or sq[0] != n or sq[2] != d or q.dtype is not dtype:
         raise ValueError("q must be [N, Hq, d] rows of k's type")
-    hq, code = q.shape[1], _dtype_code(q)
-    _check_heads(hq, hkv)
-    if hq == 0:
-        raise ValueError("q holds no heads")
-    _ints(positions, "positions", torch.int64, n)
-    if cos.dim() != 2 or cos.shape != sin.shape or not cos.dtype == sin.dtype == torch.float32 or cos.shape[0] == 0:
+    hq, code = sq[1], _dtype_code(q)
+    if hq == 0 or hq % hkv:
+        raise ValueError(f"query heads {hq} must be a multiple of kv heads {hkv}")
+    _check_ints(positions, "positions", torch.int64, n)
+    table = cos.shape
+    if len(table) != 2 or sin.shape != table or table[0] == 0 or not cos.dtype is sin.dtype is torch.float32:
         raise ValueError("cos and sin must be float32 [rows, r] tables of one shape")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("give both norm weights or neither")
-    if q_weight is not None and any(w.shape != (d,) or w.dtype != q.dtype for w in (q_weight, k_weight)):
-        raise ValueError("norm weights must be [d] of the rows' type")
-    out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+    qw = kw = None
+    if q_weight is not None:
+        if q_weight.shape != (d,) or k_weight.shape != (d,) or not q_weight.dtype is k_weight.dtype is dtype:
+            raise ValueError("norm weights must be [d] of the rows' type")
+        q_weight, k_weight = _flat(q_weight), _flat(k_weight)
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    out = torch.empty(sq, dtype=dtype, device=q.device)
     if n == 0:
         return out
-    q, k, v, slots, positions = _rows(q), _rows(k), _rows(v), slots.contiguous(), positions.contiguous()
-    cos, sin, qw, kw = (t if t is None or t.is_contiguous() and t.data_ptr() % 16 == 0
-                        else t.clone(memory_format=torch.contiguous_format) for t in (cos, sin, q_weight, k_weight))
-    with on(dev):
-        _native.call("bfly_paged_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d,
-                     *_strides(q, (0, 1)), *_strides(k, (0, 1)), *_strides(v, (0, 1)),
-                     qw.data_ptr() if qw is not None else None, kw.data_ptr() if kw is not None else None, float(eps),
-                     cos.data_ptr(), sin.data_ptr(), cos.shape[0], cos.shape[1], positions.data_ptr(), slots.data_ptr(),
-                     out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], k_pages.shape[2], *strides,
-                     stream_of(dev))
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
+    slots, positions, cos, sin = slots.contiguous(), positions.contiguous(), _flat(cos), _flat(sin)
+    _call(dev, "bfly_paged_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1,
+          qw, kw, eps, cos.data_ptr(), sin.data_ptr(), table[0], table[1], positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
+          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides)
     return out
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -262,34 +294,42 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     the empty stream ``(0, 0, -1e30)``; a length beyond its table row, or a page id outside the pages among
     those that are read, gives NaN for that request.  Rows of a page behind the request's last token are never
     part of the result, whatever they hold.  float32 or bfloat16, head_dim 64, 128 or 256."""
-    dev = _one_device(q, k_pages, v_pages, block_table, lengths)
-    _no_grad(q, k_pages, v_pages)
-    strides = _pages(k_pages, v_pages, False)
-    pages, hkv, page_size, d = k_pages.shape
-    if q.dim() != 4 or q.shape[2] != 1 or q.shape[3] != d or q.dtype != k_pages.dtype:
+    dev = _device_of(q, block_table, lengths)
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise ValueError(_GRAD)
+    shape, strides = _pages(k_pages, v_pages, dev, False)
+    pages, hkv, page_size, d = shape
+    sq, dtype = q.shape, q.dtype
+    if len(sq) != 4 or sq[2] != 1 or sq[3] != d or dtype is not k_pages.dtype:
         raise ValueError("q must be [B, Hq, 1, d] of the pages' type")
-    b, hq, code = q.shape[0], q.shape[1], _dtype_code(q)
-    _check_heads(hq, hkv)
-    if hq == 0:
-        raise ValueError("q holds no heads")
-    stride = _table(block_table, b)
-    _ints(lengths, "lengths", torch.int32, b)
-    window = int(window)
-    if window < 0 or window >= 1 << 31:
+    b, hq, code = sq[0], sq[1], _dtype_code(q)
+    if hq == 0 or hq % hkv:
+        raise ValueError(f"query heads {hq} must be a multiple of kv heads {hkv}")
+    stride, width = _table_stride(block_table, b), block_table.shape[1]
+    _check_ints(lengths, "lengths", torch.int32, b)
+    if not 0 <= window < 1 << 31:
         raise ValueError("window must be 0 (everything) or a number of tokens")
-    width = block_table.shape[1]
-    out = torch.empty(b, hq, 1, d, dtype=q.dtype, device=dev)
-    l = m = None
+    cuda = q.device
+    out = torch.empty(sq, dtype=dtype, device=cuda)
+    l = m = lp = mp = ws = None
     if return_stats:
-        l, m = torch.empty(2, b, hq, 1, 1, dtype=torch.float32, device=dev)
+        l, m = torch.empty(2, b, hq, 1, 1, dtype=torch.float32, device=cuda).unbind(0)
+        lp, mp = l.data_ptr(), m.data_ptr()
     if b:
-        q, lengths = _rows(q[:, :, 0]), lengths.contiguous()
-        with on(dev):
-            need = _native.lib().bfly_paged_attention_workspace_bytes(b, hq, hkv, d, width, page_size, window)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _native.call("bfly_paged_attention", q.data_ptr(), code, b, hq, hkv, d, *_strides(q, (0, 1)),
-                         k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, *strides, block_table.data_ptr(), width,
-                         stride, lengths.data_ptr(), window, _scale(scale, d), out.data_ptr(),
-                         l.data_ptr() if l is not None else None, m.data_ptr() if m is not None else None,
-                         ws.data_ptr() if ws is not None else None, need, stream_of(dev))
+        q0, q1, _, q3 = q.stride()
+        if q3 != 1 or q.data_ptr() & 15 or (q0 | q1) & (7 if code else 3):
+            q = q.clone(memory_format=torch.contiguous_format)
+            q0, q1, _, _ = q.stride()
+        lengths = lengths.contiguous()
+        need = _workspace_bytes(b, hq, hkv, d, width, page_size, window)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+        _call(dev, "bfly_paged_attention", q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages,
+              page_size, *strides, block_table.data_ptr(), width, stride, lengths.data_ptr(), window,
+              1.0 / math.sqrt(d) if scale is None else scale, out.data_ptr(), lp, mp, None if ws is None else ws.data_ptr(), need)
     return (out, l, m) if return_stats else out
+
+
+def _workspace_bytes(*args) -> int:
+    fn = _native._fns.get("bfly_paged_attention_workspace_bytes")
+    return (fn or _native.lib().bfly_paged_attention_workspace_bytes)(*args)

@@ -47,7 +47,7 @@ extern "C" {
  *   - When something does not fit (codes above), or state[1] is already set, nothing changes: lengths,
  *     free list and table stay, state_out keeps the count and holds the code, starts are 0 and every slot
  *     is -1.  The code stays until the caller clears it.
- *   - workspace: (requests + 1) * 4 bytes, 4-byte aligned.
+ *   - workspace: (requests + 1) * 8 bytes, 4-byte aligned.
  * The tensors do not overlap otherwise.  requests at most 2^24; num_rows and free_capacity below 2^31.
  */
 int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,

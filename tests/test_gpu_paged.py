@@ -172,7 +172,7 @@ def test_attention_infinities_and_nan_in_seen_rows(dtype, n):
     page = int(table[0, (n // 2) // 32])
     vp[page, 0, n // 2 % 32, 5] = float("inf")
     o = bf.paged_attention(q, kp, vp, table, lens)
-    assert bool(torch.isinf(o[0, :2, 0, 5]).all()) or bool(torch.isnan(o[0, :2, 0, 5]).any()) is False
+    assert bool((o[0, :2, 0, 5] == float("inf")).all())
     keep = torch.ones(64, dtype=torch.bool)
     keep[5] = False
     assert torch.equal(o[0, :2, 0][:, keep], want[0, :2, 0][:, keep])
@@ -230,7 +230,8 @@ def test_attention_stats_merge_with_another_stream():
     merged = bf.online_softmax_merge(a, b)
     (e, _, _), (bo, _, _) = _attention64(q, dense, 0, 64 ** -0.5)
     assert bool(((merged[0, :, 0].double().cpu() - e[0]).abs() <= 4 * bo[0] + 8 * U * e[0].abs()).all())
-    assert (merged[1] - b[0][1]).abs().max() == 0 and whole.shape == merged.shape
+    # beside an empty stream the merge is (l o) / l: one rounding of the product, one of the quotient, u each
+    assert bool(((merged[1] - b[0][1]).abs() <= 2.5 * U * b[0][1].abs()).all()) and whole.shape == merged.shape
 
 
 def test_attention_on_another_stream_and_two_at_once():
@@ -335,7 +336,7 @@ def test_append_rows_that_are_not_aligned_and_refusals():
     for a in [(rows.float(), rows.float(), kp, vp, slots), (rows[:, :1], rows[:, :1], kp, vp, slots), (rows, rows, kp, vp, slots.int()),
               (rows, rows, kp, vp, slots[:5]), (rows, rows[:5], kp, vp, slots), (rows, rows, kp, vp[:3], slots),
               (rows, rows, kp[..., 1:], vp[..., 1:], slots), (rows, rows, kp[:1].expand(4, 2, 16, 64), vp, slots),
-              (rows.cpu(), rows, kp, vp, slots), (rows[..., :60], rows[..., :60], kp[..., :60], vp[..., :60], slots)]:
+              (rows.cpu(), rows, kp, vp, slots), (rows, rows, kp, kp, slots), (rows[..., :60], rows[..., :60], kp[..., :60], vp[..., :60], slots)]:
         with pytest.raises(ValueError):
             bf.paged_append(*a)
 
@@ -418,7 +419,7 @@ def test_rope_append_refusals():
     p = torch.zeros(2, 1, 16, 80, dtype=BF, device="cuda")
     z = torch.ones(3, 1, 80, dtype=BF, device="cuda")
     with pytest.raises(NotImplementedError):
-        bf.paged_rope_append(z, z, z, p, p, i, i, tab, tab)
+        bf.paged_rope_append(z, z, z, p, p.clone(), i, i, tab, tab)
 
 
 # --------------------------------------------------------------------------- bookkeeping
