@@ -208,19 +208,20 @@ struct AppendArgs {
   const int64_t* slots;
   PagePtr kp, vp;
   int64_t k_row, k_head, v_row, v_head;   // bytes
-  int64_t limit, pieces;                  // num_pages * page_size; pieces of k (and of v)
-  int hkv, per, shift;
+  int64_t limit;                          // num_pages * page_size
+  unsigned pieces;                        // of k (and of v), below 2^31
+  unsigned hkv, per;
+  int shift;
 };
 
 __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
-  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  unsigned i = blockIdx.x * 256u + threadIdx.x;     // below 2^32: 2^31 pieces of each at most
   const bool is_v = i >= a.pieces;
   if (is_v) i -= a.pieces;
   if (i >= a.pieces) return;
-  const int64_t item = i / a.per;
-  const int pc = (int)(i - item * a.per);
-  const int64_t row = item / a.hkv;
-  const int h = (int)(item - row * a.hkv);
+  const unsigned item = i / a.per, pc = i - item * a.per;
+  const unsigned r = item / a.hkv, h = item - r * a.hkv;
+  const int64_t row = r;
   const int64_t slot = a.slots[row];
   if (slot < 0 || slot >= a.limit) return;
   const char* src = is_v ? a.v + row * a.v_row + h * a.v_head : a.k + row * a.k_row + h * a.k_head;
@@ -247,7 +248,8 @@ struct RopeAppendArgs {
   char* q_out;
   PagePtr kp, vp;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes
-  int64_t limit, items, table_rows;
+  int64_t limit, table_rows;
+  unsigned items;                         // rows x heads, below 2^31
   int hq, hkv, shift, rot;
   float eps;
 };
@@ -257,11 +259,11 @@ __global__ void __launch_bounds__(256) paged_rope_append_kernel(RopeAppendArgs a
   constexpr int E = 16 / sizeof(T), LPR = D / E;   // lanes a row: 8 (bf16, 64) to 64 (fp32, 256)
   typedef T vec __attribute__((ext_vector_type(E)));
   const int gl = threadIdx.x % LPR;
-  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LPR;
+  const unsigned item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
   if (item >= a.items) return;                     // whole groups
-  const int nh = a.hq + 2 * a.hkv;
-  const int64_t row = item / nh;
-  const int head = (int)(item - row * nh);
+  const unsigned nh = a.hq + 2 * a.hkv, r0 = item / nh;
+  const int64_t row = r0;
+  const int head = (int)(item - r0 * nh);
   const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
   const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
   const int64_t slot = is_q ? 0 : a.slots[row];
@@ -403,12 +405,10 @@ extern "C" int bfly_paged_append(const void* k, const void* v, int dtype, int64_
   a.kp = {static_cast<char*>(k_pages), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
   a.vp = {static_cast<char*>(v_pages), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
   a.k_row = k_row_stride * es; a.k_head = k_head_stride * es; a.v_row = v_row_stride * es; a.v_head = v_head_stride * es;
-  a.limit = num_pages * page_size; a.hkv = hkv; a.per = (int)(head_dim * es / 16); a.shift = __builtin_ctz(page_size);
-  BFLY_CHECK_ARG(rows <= INT32_MAX && hkv <= 65535 && a.per <= 65535 && rows * hkv <= INT64_MAX / 65536 / 2, "too many rows");
-  a.pieces = rows * hkv * a.per;
-  const int64_t blocks = (2 * a.pieces + 255) / 256;
-  BFLY_CHECK_ARG(blocks <= INT32_MAX, "too many rows");
-  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+  a.limit = num_pages * page_size; a.hkv = hkv; a.per = (unsigned)(head_dim * es / 16); a.shift = __builtin_ctz(page_size);
+  BFLY_CHECK_ARG(rows <= INT32_MAX && hkv <= 65535 && a.per <= 65535 && rows * hkv * a.per < ((int64_t)1 << 31) - 256, "too many rows");
+  a.pieces = (unsigned)(rows * hkv * a.per);
+  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((2 * (int64_t)a.pieces + 255) / 256)), dim3(256), 0, stream, a);
   BFLY_CHECK_LAUNCH("bfly_paged_append");
   return BFLY_OK;
 }
@@ -455,9 +455,9 @@ extern "C" int bfly_paged_rope_append(const void* q, const void* k, const void* 
   a.limit = num_pages * page_size; a.table_rows = table_rows; a.hq = hq; a.hkv = hkv;
   a.shift = __builtin_ctz(page_size); a.rot = rotary_dim; a.eps = eps;
   BFLY_CHECK_ARG(rows <= INT32_MAX && hq <= (1 << 20) && (int64_t)hq + 2 * hkv <= (1 << 22), "too many rows");
-  a.items = rows * ((int64_t)hq + 2 * hkv);
+  BFLY_CHECK_ARG(rows * ((int64_t)hq + 2 * hkv) < ((int64_t)1 << 31) - 256, "too many rows");
+  a.items = (unsigned)(rows * ((int64_t)hq + 2 * hkv));
   const int64_t lanes = head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
-  BFLY_CHECK_ARG(blocks <= INT32_MAX, "too many rows");
   const dim3 grid((unsigned)blocks), block(256);
 #define BFLY_ROPE(T, D) hipLaunchKernelGGL((paged_rope_append_kernel<T, D>), grid, block, 0, stream, a)
   if (dtype == BFLY_DTYPE_BF16) {

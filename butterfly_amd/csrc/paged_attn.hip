@@ -22,7 +22,8 @@ namespace bfly {
 
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
 constexpr int kTargetLog = 10;        // about 2^10 runs in all
-constexpr int kMinRun = 8;            // tiles of a run at least
+constexpr int kMinRun = 8;            // c at least
+constexpr int kWhole = 16;            // tiles that stay one run: a request of 512 keys is done before a join of two runs
 // A request of several runs has more than c tiles, so fewer than 2 tiles_b / c runs; all of them together,
 // with c >= total / 2^kTargetLog, fewer than 2^(kTargetLog + 1): the partials there can be.
 constexpr int kMaxSlots = 2 << kTargetLog;
@@ -30,6 +31,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 constexpr int kTile = sizeof(T) == 2 ? 32 : 16;
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 
 struct PagedAttnArgs {
   const char* q;
@@ -74,6 +77,38 @@ struct Run {
   int slot;       // partials before the request's
 };
 
+// Sums over the wave's lanes on DPP (row shifts inside 16 lanes, then the rows' last lanes broadcast): lane 63
+// of the inclusive scan holds the total.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_shift(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
+__device__ __forceinline__ int wave_scan(int x) {
+  x += dpp_shift<0x111, 0xf>(x);     // row_shr:1, 2, 4, 8
+  x += dpp_shift<0x112, 0xf>(x);
+  x += dpp_shift<0x114, 0xf>(x);
+  x += dpp_shift<0x118, 0xf>(x);
+  x += dpp_shift<0x142, 0xa>(x);     // row_bcast:15 into rows 1 and 3
+  x += dpp_shift<0x143, 0xc>(x);     // row_bcast:31 into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ float wave_total(float x) {
+  const auto step = [](float v, int w) { return v + __int_as_float(w); };
+  x = step(x, dpp_shift<0x111, 0xf>(__float_as_int(x)));
+  x = step(x, dpp_shift<0x112, 0xf>(__float_as_int(x)));
+  x = step(x, dpp_shift<0x114, 0xf>(__float_as_int(x)));
+  x = step(x, dpp_shift<0x118, 0xf>(__float_as_int(x)));
+  x = step(x, dpp_shift<0x142, 0xa>(__float_as_int(x)));
+  x = step(x, dpp_shift<0x143, 0xc>(__float_as_int(x)));
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// The largest over the wave's lanes, in every lane (col_max4 over the lanes of a row of 16, which hold the
+// same then).
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+  return col_max4(x);
+}
+
 // The request that item `idx` falls into, where request b has units * splits_b items (kMerge: only
 // requests of more than one run, with `units` items each).  Every wave does it by itself: a lane sums a
 // stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
@@ -83,45 +118,31 @@ __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
   const int per = (a.requests + 63) >> 6;
   const int b0 = lane * per < a.requests ? lane * per : a.requests;
   const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
-  int64_t total = 0;
-  for (int b = b0; b < b1; ++b) total += span_of<KT>(a, b).tiles;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-  total *= a.units;
-  int64_t c64 = (total + (1 << kTargetLog) - 1) >> kTargetLog;
-  const int c = c64 < kMinRun ? kMinRun : c64 > INT32_MAX ? INT32_MAX : (int)c64;
-  int64_t items = 0;
-  int slots = 0;
+  const int first = b0 < b1 ? span_of<KT>(a, b0).tiles : 0;
+  float total = (float)first;
+  for (int b = b0 + 1; b < b1; ++b) total += (float)span_of<KT>(a, b).tiles;
+  // (the sum of at most 65535 positive numbers, off by 1e-2 of 1 % at the most: c is above the bound all the same)
+  total = wave_total(total) * (float)a.units * (1.01f / (1 << kTargetLog));
+  const int c = __builtin_amdgcn_readfirstlane(total < (float)kMinRun ? kMinRun : total > 1e9f ? 1000000000 : (int)total + 1);
+  const auto runs = [&](int tiles) { return tiles > c && tiles > kWhole ? (int)(((unsigned)tiles + c - 1) / (unsigned)c) : 1; };
+  int items = 0, slots = 0;
   for (int b = b0; b < b1; ++b) {
-    const int tiles = span_of<KT>(a, b).tiles;
-    const int s = tiles > c ? (tiles + c - 1) / c : 1;
+    const int s = runs(b == b0 ? first : span_of<KT>(a, b).tiles);
     items += kMerge ? (s > 1 ? 1 : 0) : s;
     slots += s > 1 ? s : 0;
   }
-  int64_t i_up = items;
-  int s_up = slots;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t vi = __shfl_up(i_up, o);
-    const int vs = __shfl_up(s_up, o);
-    if (lane >= o) {
-      i_up += vi;
-      s_up += vs;
-    }
-  }
-  const uint64_t over = __ballot(i_up * a.units > idx);
+  const int i_up = wave_scan(items), s_up = wave_scan(slots);
+  const uint64_t over = __ballot((int64_t)i_up * a.units > idx);
   Run r{-1, 0, 0, 0};
   if (over == 0) return r;
   const int owner = __builtin_ctzll(over);
-  int64_t at = __shfl(i_up - items, owner);
-  int slot = __shfl(s_up - slots, owner);
+  int at = __builtin_amdgcn_readlane(i_up - items, owner), slot = __builtin_amdgcn_readlane(s_up - slots, owner);
   for (int b = owner * per;; ++b) {               // (a request of the owner's stretch holds idx)
-    const int tiles = span_of<KT>(a, b).tiles;
-    const int s = tiles > c ? (tiles + c - 1) / c : 1;
-    const int64_t next = at + (kMerge ? (s > 1 ? 1 : 0) : s);
-    if (next * a.units > idx) {
+    const int s = per == 1 ? runs(__builtin_amdgcn_readlane(first, owner)) : runs(span_of<KT>(a, b).tiles);
+    const int next = at + (kMerge ? (s > 1 ? 1 : 0) : s);
+    if ((int64_t)next * a.units > idx) {
       r.b = b;
-      r.sub = (int)(idx - at * a.units);
+      r.sub = (int)(idx - (int64_t)at * a.units);
       r.splits = s;
       r.slot = slot * a.units;
       return r;
@@ -148,7 +169,6 @@ __device__ __forceinline__ void finish_stats(const PagedAttnArgs& a, int64_t row
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  typedef __attribute__((ext_vector_type(2))) float f32x2;
   typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
@@ -498,8 +518,7 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
       const int64_t at = (int64_t)slot * a.rows + r;
       *reinterpret_cast<f32x4*>(a.part + at * D + c) = y;
       if (c == 0) {
-        a.part_ml[2 * at] = mm;
-        a.part_ml[2 * at + 1] = ll;
+        reinterpret_cast<f32x2*>(a.part_ml)[at] = f32x2{mm, ll};
       }
     }
   }
@@ -519,35 +538,43 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   if (16 * part + r >= a.group) return;
   const int64_t slot0 = run.slot + (int64_t)run.sub * run.splits;
   const int t = threadIdx.x, gr = t >> 4, c = 64 * blockIdx.z + 4 * (t & 15);
-  const float* ml = a.part_ml + 2 * (slot0 * a.rows + r);
-  float mm = -INFINITY;
-  for (int i = t; i < run.splits; i += 256) {
-    const float x = ml[2 * (int64_t)i * a.rows];
-    weight[i] = x;
-    mm = fmaxf(mm, x);
-  }
+  const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + slot0 * a.rows + r;
+  const float* src = a.part + (slot0 * a.rows + r) * D + c;
+  const int64_t step = (int64_t)a.rows * D;
+  // the first partials are requested beside the maxima that weigh them
+  constexpr int kAhead = 4;
+  f32x4 ahead[kAhead];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+  for (int j = 0; j < kAhead; ++j) {
+    const int i = gr + G * j;
+    ahead[j] = i < run.splits ? *reinterpret_cast<const f32x4*>(src + i * step) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  f32x2 mine = {-INFINITY, 0.f};
+  if (t < run.splits) mine = ml[(int64_t)t * a.rows];
+  float mm = mine[0];
+  for (int i = t + 256; i < run.splits; i += 256) mm = fmaxf(mm, ml[(int64_t)i * a.rows][0]);
+  mm = wave_max(mm);
   if ((t & 63) == 0) smx[t >> 6] = mm;
   __syncthreads();
   mm = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
   const float ref = mm == -INFINITY ? 0.f : mm;
   float l = 0.f;
   for (int i = t; i < run.splits; i += 256) {
-    const float f = __builtin_amdgcn_exp2f((weight[i] - ref) * kLog2e);
+    const f32x2 x = i == t ? mine : ml[(int64_t)i * a.rows];
+    const float f = __builtin_amdgcn_exp2f((x[0] - ref) * kLog2e);
     weight[i] = f;
-    l += f * ml[2 * (int64_t)i * a.rows + 1];
+    l += f * x[1];
   }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+  l = wave_total(l);
   if ((t & 63) == 0) sl[t >> 6] = l;
   __syncthreads();
   l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  const float* src = a.part + (slot0 * a.rows + r) * D + c;
-  const int64_t step = (int64_t)a.rows * D;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (gr + G * j < run.splits) y += weight[gr + G * j] * ahead[j];
 #pragma unroll 4
-  for (int i = gr; i < run.splits; i += G) y += weight[i] * *reinterpret_cast<const f32x4*>(src + i * step);
+  for (int i = gr + G * kAhead; i < run.splits; i += G) y += weight[i] * *reinterpret_cast<const f32x4*>(src + i * step);
   sy[gr][t & 15] = y;
   __syncthreads();
   if (gr != 0) return;
@@ -558,7 +585,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   if (c == 0) finish_stats<T>(a, row, mm, l);
 }
 
-// Whether any request can have more than one run: its table row (or the window) holds more than kMinRun tiles.
+// The tiles that a request spans at most; only one of more than kWhole can have several runs.
 static int64_t most_tiles(int64_t capacity, int window, int kt) {
   const int64_t keys = window > 0 && window < capacity ? (int64_t)window + kt - 1 : capacity;
   return (keys + kt - 1) / kt;
@@ -580,7 +607,7 @@ using namespace bfly;
 extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim,
                                                         int64_t table_width, int page_size, int window) {
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
-  if (most_tiles(table_width * page_size, window, 16) <= kMinRun) return 0;
+  if (most_tiles(table_width * page_size, window, 16) <= kWhole) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
@@ -631,7 +658,7 @@ extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, 
   // runs: one for each (request, unit), and as many more as the splits make (kTargetLog, plan_run)
   const int kt = dtype == BFLY_DTYPE_F32 ? kTile<float> : kTile<__bf16>;
   const int64_t tiles = most_tiles(a.capacity, window, kt), pairs = requests * a.units;
-  const bool splits = tiles > kMinRun;
+  const bool splits = tiles > kWhole;
   const int64_t most = pairs * ((tiles + kMinRun - 1) / kMinRun), some = pairs + (1 << kTargetLog);
   const int64_t items = !splits ? pairs : most < some ? most : some;
   BFLY_CHECK_ARG(items <= INT32_MAX, "too many requests and heads");

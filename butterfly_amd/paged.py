@@ -239,8 +239,10 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     rounding points are the modules', rounds after the norm as well).  head_dim 64, 128 or 256, ``r`` a multiple
     of 16."""
     dev = _device_of(q, slots, positions, cos, sin, q_weight, k_weight)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages, cos, sin, q_weight,
-                                                                                  k_weight)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
+                                    or v_pages.requires_grad or cos.requires_grad or sin.requires_grad
+                                    or q_weight is not None and q_weight.requires_grad
+                                    or k_weight is not None and k_weight.requires_grad):
         raise ValueError(_GRAD)
     shape, strides = _pages(k_pages, v_pages, dev, True)
     dtype = k_pages.dtype
