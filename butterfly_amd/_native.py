@@ -109,7 +109,7 @@ SIGNATURES = {
                                                 _i64, _vp]),
     "bfly_greedy_advance": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
     # include/butterfly_amd_paged.h
-    "bfly_paged_plan": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+    "bfly_paged_plan": (_int, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                                _i64, _vp]),
     "bfly_paged_append": (_int, [_vp, _vp, _int, _i64, _int, _int, *[_i64] * 4, _vp, _vp, _vp, _i64, _int, *[_i64] * 6,
                                  _vp]),

@@ -27,8 +27,10 @@ struct PlanArgs {
   int64_t* positions;
   int32_t* taken;          // [requests + 1]: pages taken by the requests before
   int32_t* given;          // [requests + 1]: pages given back by them
+  int32_t* before;         // [requests + 1]: rows added by them
   int64_t table_stride, capacity;   // capacity: tokens a table row holds
   int requests, shift, free_capacity, num_rows;
+  int fixed;               // rows that every request has (idle ones too), or 0: rows packed
 };
 
 struct PlanSum {
@@ -70,15 +72,26 @@ __device__ __forceinline__ int plan_find(const int32_t* sums, int requests, int 
   return lo;
 }
 
-// Row i of the call: the request it belongs to by binary search in `starts`, its position, and its page: one
-// the request has, or the one it takes, which the page's first row also writes to the table.
+// Row i of the call: the request it belongs to (by binary search in the sums `starts`, or, with a fixed number of
+// rows each, by division), its position, and its page: one the request has, or the one it takes, which the
+// page's first row also writes to the table.
 __device__ __forceinline__ void plan_row(const PlanArgs& a, const int32_t* starts, const int32_t* taken,
                                          const int32_t* new_len, int i, bool ok, int64_t stack) {
   int64_t slot = -1, pos = 0;
-  if (ok && i < starts[a.requests]) {
-    const int lo = plan_find(starts, a.requests, i);
+  int lo = 0, off_row = 0;                           // the row's request, and which of its rows it is
+  if (ok && a.fixed > 0) {
+    lo = i / a.fixed;                                // (num_rows = requests * fixed)
+    off_row = i - lo * a.fixed;
+    ok = off_row < starts[lo + 1] - starts[lo];
+  } else if (ok && i < starts[a.requests]) {
+    lo = plan_find(starts, a.requests, i);
+    off_row = i - starts[lo];
+  } else {
+    ok = false;
+  }
+  if (ok) {
     const int count = starts[lo + 1] - starts[lo], old_len = new_len[lo] - count;
-    pos = (int64_t)old_len + (i - starts[lo]);
+    pos = (int64_t)old_len + off_row;
     const int p_old = (int)(((int64_t)old_len + (1 << a.shift) - 1) >> a.shift), j = (int)(pos >> a.shift);
     const int off = (int)(pos & ((1 << a.shift) - 1));
     int32_t* entry = a.table + lo * a.table_stride + j;
@@ -115,7 +128,7 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
   int bad = 0;
   for (int b = b0; b < b1; ++b) {
     const PlanStep s = plan_step(a, b);
-    bad |= s.bad ? 1 : s.full ? 2 : 0;
+    bad |= s.bad ? 1 : s.full ? 2 : a.fixed > 0 && s.count > a.fixed ? 4 : 0;
     mine = mine + PlanSum{(uint32_t)s.count, (uint32_t)(s.p_old > s.p_new ? s.p_old - s.p_new : 0),
                           (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
   }
@@ -143,11 +156,12 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
   if (err == 0) {
     if (flags & 1) err = BFLY_PAGED_BAD_LENGTH;
     else if (flags & 2) err = BFLY_PAGED_TABLE_FULL;
-    else if (total.rows > (uint32_t)a.num_rows) err = BFLY_PAGED_ROWS;
+    else if (flags & 4 || total.rows > (uint32_t)a.num_rows) err = BFLY_PAGED_ROWS;
     else if (stack < (int64_t)total.take) err = BFLY_PAGED_NO_PAGES;
     else if (top < 0 || top > a.free_capacity || stack > a.free_capacity) err = BFLY_PAGED_FREE_LIST;
   }
   const bool ok = err == 0;
+  int32_t* rows = kRows ? s_starts : a.before;
   int32_t* taken = kRows ? s_taken : a.taken;
   int32_t* given = kRows ? s_given : a.given;
   // lengths may be updated in place: a thread reads its own requests before it writes them
@@ -156,9 +170,9 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
     const int32_t raw = a.lengths[b];
     const PlanStep s = plan_step(a, b);
     a.lengths_out[b] = ok ? s.new_len : raw;
-    a.starts[b] = ok ? (int)at.rows : 0;
+    a.starts[b] = ok ? (a.fixed > 0 ? b * a.fixed : (int)at.rows) : 0;
+    rows[b] = (int)at.rows;
     if constexpr (kRows) {
-      s_starts[b] = (int)at.rows;
       s_new[b] = s.new_len;
     }
     taken[b] = (int)at.take;
@@ -167,8 +181,8 @@ __global__ void __launch_bounds__(kPlanMaxThreads) plan_kernel(PlanArgs a) {
                       (uint32_t)(s.p_new > s.p_old ? s.p_new - s.p_old : 0)};
   }
   if (t == 0) {
-    a.starts[a.requests] = ok ? (int)total.rows : 0;
-    if constexpr (kRows) s_starts[a.requests] = (int)total.rows;
+    a.starts[a.requests] = ok ? (a.fixed > 0 ? a.requests * a.fixed : (int)total.rows) : 0;
+    rows[a.requests] = (int)total.rows;
     taken[a.requests] = (int)total.take;
     given[a.requests] = (int)total.give;
   }
@@ -196,7 +210,7 @@ __global__ void __launch_bounds__(256) plan_rows_kernel(PlanArgs a) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i >= a.num_rows) return;
   const bool ok = a.state_out[1] == 0;
-  plan_row(a, a.starts, a.taken, a.lengths_out, i, ok, (int64_t)a.state_out[0] + a.taken[a.requests]);
+  plan_row(a, a.before, a.taken, a.lengths_out, i, ok, (int64_t)a.state_out[0] + a.taken[a.requests]);
 }
 
 // --------------------------------------------------------------------------- rows into pages
@@ -345,7 +359,7 @@ using namespace bfly;
 extern "C" int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,
                                const int32_t* lengths, const int32_t* counts, int32_t* free_pages,
                                int64_t free_capacity, const int32_t* state, int page_size, int64_t num_rows,
-                               int32_t* lengths_out, int32_t* state_out, int32_t* starts, int64_t* slots,
+                               int64_t rows_each, int32_t* lengths_out, int32_t* state_out, int32_t* starts, int64_t* slots,
                                int64_t* positions, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   BFLY_CHECK_ARG(requests >= 0 && requests <= (1 << 24) && table_width >= 0 && table_width <= INT32_MAX, "bad block table shape");
   BFLY_CHECK_ARG(requests <= 1 || table_stride >= table_width, "block table rows overlap");
@@ -353,23 +367,27 @@ extern "C" int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t t
                  "num_rows and the free list must stay below 2^31");
   BFLY_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
                  "page_size %d must be a power of two from 16 to 1024", page_size);
+  BFLY_CHECK_ARG(rows_each >= 0 && (rows_each == 0 || num_rows == requests * rows_each),
+                 "num_rows must be the requests' rows_each");
   BFLY_CHECK_ARG(state && state_out && starts, "null pointer");
   BFLY_CHECK_ARG(requests == 0 || (lengths && counts && lengths_out), "null pointer");
   BFLY_CHECK_ARG(requests * table_width == 0 || block_table, "null pointer");
   BFLY_CHECK_ARG(free_capacity == 0 || free_pages, "null pointer");
   BFLY_CHECK_ARG(num_rows == 0 || (slots && positions), "null pointer");
-  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 8 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 12 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
                  "workspace too small");
   PlanArgs a{};
   a.table = block_table; a.lengths = lengths; a.counts = counts; a.free_pages = free_pages; a.state = state;
   a.lengths_out = lengths_out; a.state_out = state_out; a.starts = starts; a.slots = slots; a.positions = positions;
   a.taken = static_cast<int32_t*>(workspace);
   a.given = a.taken + requests + 1;
+  a.before = a.given + requests + 1;
   a.table_stride = table_stride;
   a.shift = __builtin_ctz(page_size);
   const int64_t cap = table_width << a.shift;
   a.capacity = cap < INT32_MAX ? cap : INT32_MAX;
   a.requests = (int)requests; a.free_capacity = (int)free_capacity; a.num_rows = (int)num_rows;
+  a.fixed = (int)rows_each;
   const dim3 block(requests <= 256 && num_rows <= 256 ? 256 : kPlanMaxThreads);
   if (requests <= kPlanLds && num_rows <= 4096) {
     hipLaunchKernelGGL(plan_kernel<true>, dim3(1), block, 0, stream, a);

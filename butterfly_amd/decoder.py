@@ -29,7 +29,8 @@ projection paths.  The attention exposes the attribute set the generic swapped
 module reads (``n_heads``, ``n_kv_heads``, ``head_dim``, ``scale``, the
 projections and norms), so ``QwenButterflyAttention`` itself also wraps it.  The
 stock attention that it replaces is plain causal GQA softmax attention (PyTorch
-SDPA).  Attention modules take ``(x, mask=None, cache=None, *,
+SDPA), over a list cache or, for captured and ragged decode steps, over the pages of a
+:class:`PagedKVCache` (``paged_attention``).  Attention modules take ``(x, mask=None, cache=None, *,
 position_embeddings=(cos, sin))``, the RoPE rows of the call's positions.
 """
 from __future__ import annotations
@@ -52,6 +53,7 @@ from . import _native
 from ._device import on, stream_of
 from .compressed_cache import CompressedKVCache
 from .integrations import QwenButterflyAttention, QwenButterflyConfig, register_butterfly_attention
+from .paged import PagedKVCache, PagedLayer
 
 
 @dataclass
@@ -630,9 +632,11 @@ class Attention(nn.Module):
         return self.o_proj(o.transpose(1, 2).reshape(b, t, -1))
 
     def forward(self, x: torch.Tensor, mask=None, cache=None, *, position_embeddings=None) -> torch.Tensor:
-        """``cache``: a list ``[k, v]`` of the full history (empty before the first call);
-        ``position_embeddings``: ``(cos, sin)`` rows of the call's positions (or a ``RopeTable``),
-        else computed from the cache length."""
+        """``cache``: a list ``[k, v]`` of the full history (empty before the first call), or a ``PagedLayer``
+        whose cache has begun the step; ``position_embeddings``: ``(cos, sin)`` rows of the call's positions
+        (or a ``RopeTable``), else computed from the cache length."""
+        if isinstance(cache, PagedLayer):
+            return self._forward_paged(x, cache, position_embeddings)
         positions = None
         if position_embeddings is None:
             start = int(cache[0].shape[2]) if cache else 0
@@ -643,13 +647,39 @@ class Attention(nn.Module):
                 k = torch.cat([cache[0], k], 2)
                 v = torch.cat([cache[1], v], 2)
             cache[:] = [k, v]
+        return self.output(self._dense(q, k, v))
+
+    @staticmethod
+    def _dense(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Causal GQA softmax attention of the last positions ``q`` over all keys (PyTorch SDPA)."""
         groups = q.shape[1] // k.shape[1]
         kk = k.repeat_interleave(groups, 1)
         vv = v.repeat_interleave(groups, 1)
         tq, tk = q.shape[2], kk.shape[2]
         mask = torch.ones(tq, tk, dtype=torch.bool, device=q.device).tril(tk - tq)
-        o = F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
-        return self.output(o)
+        return F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
+
+    def _forward_paged(self, x: torch.Tensor, cache: PagedLayer, rope) -> torch.Tensor:
+        """``forward`` over pages.  One token of every request (their lengths may differ): q/k norm, RoPE at the
+        plan's positions and the move into the pages in one launch, then ``paged_attention``; nothing of it
+        needs the host, so the step can be captured.  More than one: a part of prompts of one length, dense
+        attention over what the pages hold and the part itself."""
+        b, t, _ = x.shape
+        c = self.cfg
+        if t == 1 and isinstance(rope, RopeTable) and _hip(x):
+            q, k, v = self.qkv(x).view(b, -1, c.head_dim).split((c.num_heads, c.num_kv_heads, c.num_kv_heads), 1)
+            q = cache.rope_append(q, k, v, rope.cos_tab, rope.sin_tab, q_weight=self.q_norm.weight,
+                                  k_weight=self.k_norm.weight, eps=self.q_norm.eps)
+            return self.output(cache.attend(q.unsqueeze(2), scale=self.scale))
+        start = cache.cache.start
+        q, k, v = self.project(x, torch.arange(start, start + t, device=x.device), rope)
+        cache.append(k.transpose(1, 2).reshape(b * t, *k.shape[1::2]), v.transpose(1, 2).reshape(b * t, *v.shape[1::2]))
+        if t == 1:
+            return self.output(cache.attend(q, scale=self.scale))
+        if start:
+            k, v = (torch.cat(x, 2) for x in zip(cache.history(start), (k, v)))
+        return self.output(self._dense(q, k, v))
+
 
 class ButterflyAttention(QwenButterflyAttention):
     """The swapped attention of this decoder: ``QwenButterflyAttention`` over the base
@@ -860,14 +890,28 @@ class Decoder(nn.Module):
         x = F.embedding(tokens, self.embed_tokens)
         positions = torch.arange(start, start + tokens.shape[1], device=tokens.device)
         rope = self._rope(start, tokens.shape[1], tokens.device)
+        pools = self._paged_pools(caches, tokens.shape[0])
+        for pool in pools:
+            pool.begin(torch.full_like(pool.lengths, tokens.shape[1]), tokens.shape[1], start=start)
+        if pools:
+            rope = RopeTable(*self._rope_tab, positions)
         return self._last_logits(x, positions, caches, rope).float()
+
+    @staticmethod
+    def _paged_pools(caches: List, batch: int) -> List[PagedKVCache]:
+        """The paged caches behind ``caches``, each once."""
+        pools = list({id(c.cache): c.cache for c in caches if isinstance(c, PagedLayer)}.values())
+        if any(pool.max_requests != batch for pool in pools):
+            raise ValueError(f"a paged cache of {[p.max_requests for p in pools]} requests cannot take a batch of {batch}")
+        return pools
 
     @torch.no_grad()
     def greedy_graph(self, prompt: torch.Tensor, new_tokens: int, caches: List) -> torch.Tensor:
         """``greedy`` with the decode steps replayed from one captured HIP graph.
 
-        ``caches`` must be ``CompressedKVCache`` objects; the prompt is prefilled
-        eagerly, then the caches switch to device counters; the first decode step
+        ``caches`` must be ``CompressedKVCache`` objects (swapped layers) or ``PagedLayer`` objects
+        (layers that keep dense attention); the prompt is prefilled
+        eagerly, then the compressed caches switch to device counters; the first decode step
         runs eagerly and the next one (every layer, argmax, position advance) is
         captured and replayed ``new_tokens - 2`` times with no host
         synchronisation in between.
@@ -888,6 +932,8 @@ class Decoder(nn.Module):
         b = logits.shape[0]
         for i, (layer, c) in enumerate(zip(self.layers, caches)):
             attn = layer.self_attn
+            if isinstance(c, PagedLayer) and isinstance(attn, Attention) and _hip(self.embed_tokens):
+                continue
             if not isinstance(c, CompressedKVCache) or not (
                     isinstance(attn, ButterflyAttention)
                     and attn.core.device_step_fits(c, self.cfg.head_dim, self.embed_tokens.dtype)):
@@ -895,8 +941,11 @@ class Decoder(nn.Module):
                     f"greedy_graph: layer {i} cannot run its decode step as one device launch (it needs a swapped "
                     f"layer over a CompressedKVCache, an attention window of at most 64 tokens and a routed row "
                     f"of at most 16 blocks); use greedy() for this configuration")
-        for c in caches:
+        compressed = [c for c in caches if isinstance(c, CompressedKVCache)]
+        pools = self._paged_pools(caches, b)
+        for c in compressed:
             c.use_device_counters()
+        one_each = torch.ones(b, dtype=torch.int32, device=dev)
         self._rope(0, t + new_tokens + 1, dev)               # table sized before capture
         tok = logits.argmax(-1, keepdim=True)
         out = torch.empty(b, new_tokens, dtype=torch.long, device=dev)
@@ -913,6 +962,8 @@ class Decoder(nn.Module):
             greedy = GreedyState(tok, out, ctr, F.embedding(tok, self.embed_tokens).contiguous(), ws)
 
         def one_step():
+            for pool in pools:
+                pool.begin(one_each)
             if greedy is not None:
                 # the token, its output column, the counters and the next step's input row are
                 # advanced inside the launches after the lm_head
@@ -950,8 +1001,76 @@ class Decoder(nn.Module):
             if timed:
                 torch.cuda.synchronize(dev)
             self.last_graph_decode_s = time.perf_counter() - t0
-        for c in caches:
+        for c in compressed:
             c.use_device_counters(False)
+        for pool in pools:
+            pool.sync()
+        return out
+
+    @torch.no_grad()
+    def greedy_requests(self, prompts: List[torch.Tensor], new_tokens: int, cache: PagedKVCache, *,
+                        eos_token: Optional[int] = None) -> torch.Tensor:
+        """Greedy decoding of requests of different lengths together, over the dense layers' paged cache.
+
+        ``prompts``: one 1-D tensor of tokens per request (``cache.max_requests`` of them, the cache empty).
+        Each is prefilled by itself and its keys and values go into pages; then all requests decode together,
+        a step captured once in a HIP graph and replayed, each request at its own position.  Returns
+        [B, new_tokens]; after ``eos_token`` a request idles (its row repeats the token, its pages stay).
+        Every layer has stock attention (a compressed cache holds one length for its batch)."""
+        b = len(prompts)
+        dev = self.embed_tokens.device
+        if b != cache.max_requests or len(cache.layers) != len(self.layers) or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+            raise ValueError("greedy_requests takes one non-empty 1-D prompt for each request and a layer of the cache for "
+                             "each layer of the model")
+        if not _hip(self.embed_tokens) or not all(isinstance(layer.self_attn, Attention) for layer in self.layers):
+            raise ValueError("greedy_requests needs a bf16 model on the GPU whose layers all have stock attention")
+        if new_tokens <= 0:
+            return torch.empty(b, 0, dtype=torch.long, device=dev)
+        first = []
+        for r, prompt in enumerate(prompts):
+            n = prompt.numel()
+            held = [[] for _ in self.layers]
+            first.append(self.forward(prompt[None].to(dev), held, 0).argmax(-1))
+            counts = torch.zeros_like(cache.lengths)
+            counts[r] = n
+            cache.begin_packed(counts, n)
+            for layer, (k, v) in zip(cache.layers, held):
+                layer.append(k[0].transpose(0, 1), v[0].transpose(0, 1))
+        cache.sync()
+        tok = torch.stack(first)                             # [B, 1]
+        out = torch.empty(b, new_tokens, dtype=torch.long, device=dev)
+        out[:, :1] = tok
+        column = torch.ones(1, dtype=torch.long, device=dev)
+        alive = torch.ones(b, dtype=torch.int32, device=dev)
+        if eos_token is not None:
+            alive.copy_((tok[:, 0] != eos_token).int())
+        self._rope(0, max(p.numel() for p in prompts) + new_tokens + 1, dev)
+        rope = RopeTable(*self._rope_tab, None)
+
+        def one_step():
+            cache.begin(alive)
+            lg = self._last_logits(F.embedding(tok, self.embed_tokens), None, cache.layers, rope)
+            nxt = argmax_rows(lg)
+            if eos_token is not None:
+                nxt = torch.where(alive[:, None] != 0, nxt, tok)
+                alive.copy_((nxt[:, 0] != eos_token).int())
+            tok.copy_(nxt)
+            out.index_copy_(1, column, nxt)
+            column.add_(1)
+
+        if new_tokens > 1:
+            one_step()           # eager first step: every op meets its decode shapes before capture
+        if new_tokens > 2:
+            graph = torch.cuda.CUDAGraph()
+            side = torch.cuda.Stream(device=dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                with torch.cuda.graph(graph, stream=side):
+                    one_step()   # recorded, not run
+            torch.cuda.current_stream(dev).wait_stream(side)
+            for _ in range(new_tokens - 2):
+                graph.replay()
+        cache.sync()
         return out
 
     @torch.no_grad()
@@ -970,4 +1089,6 @@ class Decoder(nn.Module):
                 break
             logits = self.forward(nxt, caches, pos)
             pos += 1
+        for pool in self._paged_pools(caches, prompt.shape[0]):
+            pool.sync()
         return torch.cat(out, 1)

@@ -139,7 +139,7 @@ def _rows(t: torch.Tensor):
 
 
 def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.Tensor, free_pages: torch.Tensor,
-               state: torch.Tensor, *, page_size: int, num_rows: int, in_place: bool = False) -> PagedPlan:
+               state: torch.Tensor, *, page_size: int, num_rows: int, rows_each: int = 0, in_place: bool = False) -> PagedPlan:
     """One step's bookkeeping on the device (``bfly_paged_plan``, two launches for many rows, else one).
 
     Request ``b`` of ``B`` holds ``lengths[b]`` tokens and its pages are ``block_table[b]`` (int32
@@ -149,7 +149,9 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     pages that others need are taken from the top in request order.  All of these are int32.
 
     ``num_rows`` (known on the host) is how many rows the step has room for: row ``starts[b] + i`` is request
-    ``b``'s ``i``-th new token, rows behind the last have slot -1 and position 0.
+    ``b``'s ``i``-th new token, rows behind the last have slot -1 and position 0.  With ``rows_each`` every
+    request has that many rows of its own instead (``num_rows = B * rows_each``, ``starts[b] = b * rows_each``):
+    a batch of fixed shape in which requests may be idle, as a captured decode step needs.
 
     ``block_table`` and ``free_pages`` are updated; ``lengths`` and ``state`` too with ``in_place``, else the
     new ones are in the result only.  When something does not fit (``PLAN_ERRORS``) nothing changes,
@@ -170,6 +172,8 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
         raise ValueError("block_table's rows must not overlap")
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
+    if rows_each and num_rows != b * rows_each:
+        raise ValueError(f"num_rows must be the {b} requests' {rows_each} rows each")
     if not (lengths.is_contiguous() and counts.is_contiguous() and state.is_contiguous() and free_pages.is_contiguous()):
         if not free_pages.is_contiguous() or in_place and not (lengths.is_contiguous() and state.is_contiguous()):
             raise ValueError("tensors that are updated must be contiguous")
@@ -178,14 +182,14 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     # one allocation for the int32 results and the kernel's workspace, one for the rows
     if in_place:
         new_lengths, new_state = lengths, state
-        starts, ws = torch.empty(3 * b + 3, dtype=i32, device=cuda).split_with_sizes((b + 1, 2 * b + 2))
+        starts, ws = torch.empty(4 * b + 4, dtype=i32, device=cuda).split_with_sizes((b + 1, 3 * b + 3))
     else:
-        new_lengths, new_state, starts, ws = torch.empty(4 * b + 5, dtype=i32, device=cuda).split_with_sizes(
-            (b, 2, b + 1, 2 * b + 2))
+        new_lengths, new_state, starts, ws = torch.empty(5 * b + 6, dtype=i32, device=cuda).split_with_sizes(
+            (b, 2, b + 1, 3 * b + 3))
     slots, positions = torch.empty(2, num_rows, dtype=torch.int64, device=cuda).unbind(0)
     _call(dev, "bfly_paged_plan", block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(),
-          free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size, num_rows, new_lengths.data_ptr(),
-          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 8 * (b + 1))
+          free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size, num_rows, rows_each, new_lengths.data_ptr(),
+          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 12 * (b + 1))
     return PagedPlan(new_lengths, new_state, starts, slots, positions)
 
 
@@ -335,3 +339,104 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def _workspace_bytes(*args) -> int:
     fn = _native._fns.get("bfly_paged_attention_workspace_bytes")
     return (fn or _native.lib().bfly_paged_attention_workspace_bytes)(*args)
+
+
+class PagedLayer:
+    """One layer's pages of a :class:`PagedKVCache`: what an attention module takes as its ``cache``.  Between the
+    cache's :meth:`PagedKVCache.begin` and the next one, its rows are the step's."""
+
+    def __init__(self, cache: "PagedKVCache", k_pages: torch.Tensor, v_pages: torch.Tensor):
+        self.cache, self.k_pages, self.v_pages = cache, k_pages, v_pages
+
+    @property
+    def plan(self) -> PagedPlan:
+        if self.cache.plan is None:
+            raise RuntimeError("begin() a step of the paged cache before its layers")
+        return self.cache.plan
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's rows of keys and values [N, Hkv, d] into their slots."""
+        paged_append(k, v, self.k_pages, self.v_pages, self.plan.slots)
+
+    def rope_append(self, q, k, v, cos, sin, *, q_weight=None, k_weight=None, eps: float = 1e-6) -> torch.Tensor:
+        """The step's projection rows: :func:`paged_rope_append` at the plan's positions and slots."""
+        p = self.plan
+        return paged_rope_append(q, k, v, self.k_pages, self.v_pages, p.slots, p.positions, cos, sin, q_weight=q_weight,
+                                 k_weight=k_weight, eps=eps)
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, window: int = 0, return_stats: bool = False):
+        """:func:`paged_attention` of one new token ``q`` [B, Hq, 1, d] of every request over its pages."""
+        return paged_attention(q, self.k_pages, self.v_pages, self.cache.block_table, self.plan.lengths, scale=scale,
+                               window=window, return_stats=return_stats)
+
+    def history(self, tokens: int):
+        """The first ``tokens`` keys and values of every request as dense [B, Hkv, tokens, d] tensors (what a
+        prompt's further part attends to); every request holds that many."""
+        size = self.k_pages.shape[2]
+        ids = self.cache.block_table[:, :-(-tokens // size)].long()
+        return tuple(x[ids].transpose(1, 2).flatten(2, 3)[:, :, :tokens] for x in (self.k_pages, self.v_pages))
+
+
+class PagedKVCache:
+    """Keys and values of ``max_requests`` requests in ``num_layers`` dense layers: pages
+    ``[num_layers, num_pages, Hkv, page_size, d]`` and one block table, lengths and free list on the device,
+    which all layers share (page ``p`` of a request is page ``p`` in every layer).
+
+    ``max_tokens`` bounds a request (default: all pages).  A step is :meth:`begin` (or :meth:`begin_packed`), then
+    every layer's rows and attention through ``layers[i]``; :meth:`sync` reads the state back."""
+
+    def __init__(self, *, num_layers: int, num_pages: int, max_requests: int, num_kv_heads: int, head_dim: int,
+                 page_size: int = 128, max_tokens: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None):
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
+        if min(num_layers, num_pages, max_requests, num_kv_heads, head_dim) <= 0 or max_tokens is not None and max_tokens <= 0:
+            raise ValueError("the cache's sizes must be positive")
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+        device = torch.device("cuda" if device is None else device)
+        width = num_pages if max_tokens is None else min(num_pages, -(-max_tokens // page_size))
+        self.page_size, self.max_requests, self.max_tokens = page_size, max_requests, width * page_size
+        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+        self.k_pages, self.v_pages = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        self.layers = [PagedLayer(self, k, v) for k, v in zip(self.k_pages, self.v_pages)]
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((max_requests, width), -1, **i32)
+        self.lengths = torch.zeros(max_requests, **i32)
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
+        self.state = torch.tensor([num_pages, 0], **i32)
+        self.plan: Optional[PagedPlan] = None
+        self.start = 0                 # tokens before the step, for a part of a prompt (PagedLayer.history)
+
+    @property
+    def nbytes(self) -> int:
+        return self.k_pages.nbytes + self.v_pages.nbytes
+
+    def _begin(self, counts: torch.Tensor, num_rows: int, rows_each: int, start: int) -> PagedPlan:
+        self.plan = paged_plan(self.block_table, self.lengths, counts, self.free_pages, self.state,
+                               page_size=self.page_size, num_rows=num_rows, rows_each=rows_each, in_place=True)
+        self.start = int(start)
+        return self.plan
+
+    def begin(self, counts: torch.Tensor, rows_each: int = 1, *, start: int = 0) -> PagedPlan:
+        """A step in which request ``b`` adds ``counts[b] <= rows_each`` tokens (int32 [B], on the device; negative:
+        takes tokens back) and has ``rows_each`` rows, row ``b * rows_each + i`` its ``i``-th."""
+        return self._begin(counts, self.max_requests * rows_each, rows_each, start)
+
+    def begin_packed(self, counts: torch.Tensor, num_rows: int) -> PagedPlan:
+        """A step whose rows follow each other, request by request: ragged prompts."""
+        return self._begin(counts, num_rows, 0, 0)
+
+    def release(self, requests) -> None:
+        """The given requests (indices) leave: their pages go back to the free list."""
+        counts = torch.zeros_like(self.lengths)
+        counts[torch.as_tensor(requests, dtype=torch.long, device=counts.device)] = -(2 ** 31 - 1)
+        self._begin(counts, 0, 0, 0)
+
+    def sync(self) -> int:
+        """Waits for the device; the number of free pages.  Raises ``RuntimeError`` if a step did not fit (that
+        step and all after it changed nothing), and clears the error."""
+        free, error = self.state.tolist()
+        if error:
+            self.state[1] = 0
+            raise RuntimeError(f"paged cache: {PLAN_ERRORS.get(error, error)}")
+        return free

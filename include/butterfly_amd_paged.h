@@ -44,15 +44,18 @@ extern "C" {
  *   - starts [requests + 1]: the first row of each request among the call's rows (exclusive sums of the
  *     positive counts).  slots and positions [num_rows] int64: where row starts[b] + i of request b goes
  *     and its position lengths[b] + i; rows behind the last have slot -1 and position 0.
+ *   - rows_each > 0 (num_rows = requests * rows_each): every request has rows_each rows of its own instead,
+ *     starts[b] = b * rows_each, for a batch in which some stay idle; no count may exceed it (code
+ *     BFLY_PAGED_ROWS), and rows behind a request's count have slot -1 and position 0.
  *   - When something does not fit (codes above), or state[1] is already set, nothing changes: lengths,
  *     free list and table stay, state_out keeps the count and holds the code, starts are 0 and every slot
  *     is -1.  The code stays until the caller clears it.
- *   - workspace: (requests + 1) * 8 bytes, 4-byte aligned.
+ *   - workspace: (requests + 1) * 12 bytes, 4-byte aligned.
  * The tensors do not overlap otherwise.  requests at most 2^24; num_rows and free_capacity below 2^31.
  */
 int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,
                     const int32_t* lengths, const int32_t* counts, int32_t* free_pages, int64_t free_capacity,
-                    const int32_t* state, int page_size, int64_t num_rows, int32_t* lengths_out,
+                    const int32_t* state, int page_size, int64_t num_rows, int64_t rows_each, int32_t* lengths_out,
                     int32_t* state_out, int32_t* starts, int64_t* slots, int64_t* positions, void* workspace,
                     int64_t workspace_bytes, hipStream_t stream);
 

@@ -660,3 +660,46 @@ def test_a_chain_against_dense_attention():
         assert lens.tolist() == [x.shape[1] for x, _ in held] and int(state[1]) == 0
         q = torch.randn(b, hq, 1, d, generator=g).to(BF).cuda()
         _check_attention(q, kp, vp, table, lens, held)
+
+
+@pytest.mark.parametrize("b,each", [(5, 1), (5, 3), (700, 8), (3000, 2), (1, 5000)])
+def test_plan_with_rows_of_its_own_for_every_request(b, each):
+    """rows_each: row b * each + i is request b's, idle rows have slot -1; lengths, pages and positions are the
+    packed call's."""
+    r = random.Random(b)
+    page, width = 16, max(8, each // 16 + 6)
+    lens = [r.randint(0, 60) for _ in range(b)]
+    need = [-(-n // page) for n in lens]
+    ids = list(range(sum(need) + b * (each // page + 2)))
+    r.shuffle(ids)
+    table, at = [], 0
+    for u in need:
+        table.append(ids[at:at + u] + [-1] * (width - u))
+        at += u
+    free = _i32(ids[at:] + [-1] * at)
+    counts = [r.choice([0, 1, each, r.randint(0, each), -r.randint(0, 70)]) for _ in range(b)]
+    t, state = _i32(table), _i32([len(ids) - at, 0])
+    t2, free2 = t.clone(), free.clone()
+    rows = sum(max(0, c) for c in counts)
+    packed = bf.paged_plan(t, _i32(lens), _i32(counts), free, state, page_size=page, num_rows=rows)
+    fixed = bf.paged_plan(t2, _i32(lens), _i32(counts), free2, state, page_size=page, num_rows=b * each, rows_each=each)
+    assert torch.equal(t, t2) and torch.equal(free, free2)
+    assert torch.equal(packed.lengths, fixed.lengths) and torch.equal(packed.state, fixed.state) and int(fixed.state[1]) == 0
+    assert fixed.starts.tolist() == [each * i for i in range(b + 1)]
+    slots, pos = [-1] * (b * each), [0] * (b * each)
+    for i, (s, c) in enumerate(zip(packed.starts.tolist(), counts)):
+        for j in range(max(0, c)):
+            slots[i * each + j], pos[i * each + j] = int(packed.slots[s + j]) if b < 100 else None, None
+    if b < 100:
+        real = [s for s in slots if s >= 0]
+        assert real == packed.slots.tolist()
+        assert fixed.slots.tolist() == slots
+    live = fixed.slots >= 0
+    assert torch.equal(fixed.slots[live], packed.slots) and torch.equal(fixed.positions[live], packed.positions)
+    want = torch.tensor([[j < c for j in range(each)] for c in counts], device="cuda").view(-1)
+    assert torch.equal(live, want) and bool((fixed.positions[~live] == 0).all())
+    too_many = [each + 1] + counts[1:]
+    over = bf.paged_plan(t2, _i32(lens), _i32(too_many), free2, state, page_size=page, num_rows=b * each, rows_each=each)
+    assert over.state.tolist() == [int(state[0]), 3] and bool((over.slots == -1).all()) and torch.equal(over.lengths, _i32(lens))
+    with pytest.raises(ValueError, match="rows"):
+        bf.paged_plan(t2, _i32(lens), _i32(counts), free2, state, page_size=page, num_rows=b * each + 1, rows_each=each)

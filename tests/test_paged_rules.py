@@ -12,8 +12,8 @@ I = 4096   # stands for an aligned device pointer: never followed, the calls bel
 
 
 def _plan(**kw):
-    a = dict(table=I, requests=4, width=8, stride=8, lengths=I, counts=I, free=I, cap=32, state=I, page=64, rows=4,
-             lengths_out=I, state_out=I, starts=I, slots=I, positions=I, ws=I, ws_bytes=40, stream=None)
+    a = dict(table=I, requests=4, width=8, stride=8, lengths=I, counts=I, free=I, cap=32, state=I, page=64, rows=4, each=0,
+             lengths_out=I, state_out=I, starts=I, slots=I, positions=I, ws=I, ws_bytes=60, stream=None)
     a.update(kw)
     return list(a.values())
 
@@ -53,7 +53,9 @@ INVALID, UNSUPPORTED = _native.ERR_INVALID, _native.ERR_UNSUPPORTED
     (_plan, "bfly_paged_plan", dict(rows=-1), INVALID, b"num_rows"),
     (_plan, "bfly_paged_plan", dict(rows=1 << 31), INVALID, b"2^31"),
     (_plan, "bfly_paged_plan", dict(cap=1 << 31), INVALID, b"2^31"),
-    (_plan, "bfly_paged_plan", dict(ws_bytes=36), INVALID, b"workspace"),
+    (_plan, "bfly_paged_plan", dict(ws_bytes=56), INVALID, b"workspace"),
+    (_plan, "bfly_paged_plan", dict(each=2), INVALID, b"rows_each"),
+    (_plan, "bfly_paged_plan", dict(each=-1), INVALID, b"rows_each"),
     (_plan, "bfly_paged_plan", dict(ws=None), INVALID, b"workspace"),
     (_plan, "bfly_paged_plan", dict(slots=None), INVALID, b"null"),
     (_plan, "bfly_paged_plan", dict(state=None), INVALID, b"null"),
