@@ -249,6 +249,14 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
 // shuffles inside the group, weight, then rotate-half with the lane that holds the other half
 // (rotary / 2 elements away, whole lanes since rotary is a multiple of 16).  fp32 from the loads to the
 // one rounding of each output: y = x * rsqrt(mean x^2 + eps) * w, z = y cos + rotate_half(y) sin.
+//
+// kHeads = 1: a decode step's few rows, spread as wide as they go; what they write stays in the caches for the
+// attention that follows.  kHeads = 4, from kManyHeads heads' rows on: a group takes four heads of a token, so
+// four loads are under way over one position's cos and sin, and moves them past the caches.
+// Both sides, us (16/4 heads of d 128, bf16, whole rotation; one head / four): 32 rows 3.1 / 6.0, 1024 6.2 / 7.8, 2048
+// 9.3 / 9.4, 4096 15.1 / 14.5, 16384 52 / 47; d 256 in bf16, 16384 rows: 103 / 83.
+constexpr int64_t kManyHeads = 1 << 16;
+
 struct RopeAppendArgs {
   const char* q;
   const char* k;
@@ -263,68 +271,88 @@ struct RopeAppendArgs {
   PagePtr kp, vp;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes
   int64_t limit, table_rows;
-  unsigned items;                         // rows x heads, below 2^31
+  unsigned items;                         // rows x groups of heads, below 2^31
   int hq, hkv, shift, rot;
   float eps;
 };
 
-template <typename T, int D>
+template <typename T, int D, int kHeads>
 __global__ void __launch_bounds__(256) paged_rope_append_kernel(RopeAppendArgs a) {
   constexpr int E = 16 / sizeof(T), LPR = D / E;   // lanes a row: 8 (bf16, 64) to 64 (fp32, 256)
   typedef T vec __attribute__((ext_vector_type(E)));
   const int gl = threadIdx.x % LPR;
   const unsigned item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
   if (item >= a.items) return;                     // whole groups
-  const unsigned nh = a.hq + 2 * a.hkv, r0 = item / nh;
+  const unsigned nh = a.hq + 2 * a.hkv, chunks = (nh + kHeads - 1) / kHeads, r0 = item / chunks;
   const int64_t row = r0;
-  const int head = (int)(item - r0 * nh);
-  const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
-  const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
-  const int64_t slot = is_q ? 0 : a.slots[row];
-  if (!is_q && (slot < 0 || slot >= a.limit)) return;
-  const char* src = is_q ? a.q + row * a.q_row + h * a.q_head
-                         : is_v ? a.v + row * a.v_row + h * a.v_head : a.k + row * a.k_row + h * a.k_head;
-  char* dst = is_q ? a.q_out + ((row * a.hq + h) * D) * (int64_t)sizeof(T)
-                   : (is_v ? a.vp : a.kp).row(slot >> a.shift, h, (int)(slot & ((1 << a.shift) - 1)));
-  vec x = *reinterpret_cast<const vec*>(src + 16 * gl);
-  if (!is_v) {
-    float y[E];
+  const int head0 = (int)(item - r0 * chunks) * kHeads;
+  const int64_t slot = a.slots[row], pos = a.positions[row];
+  const bool keep = slot >= 0 && slot < a.limit, inside = pos >= 0 && pos < a.table_rows;
+  vec x[kHeads];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = to_f32(x[e]);
-    const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
-    if (w != nullptr) {
-      float ss = 0.f;
+  for (int i = 0; i < kHeads; ++i) {
+    const int head = head0 + i;
+    if (kHeads > 1 && head >= (int)nh) break;
+    const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
+    const char* src = is_q ? a.q + row * a.q_row + head * a.q_head
+                           : is_v ? a.v + row * a.v_row + (head - a.hq - a.hkv) * a.v_head : a.k + row * a.k_row + (head - a.hq) * a.k_head;
+    const vec* p = reinterpret_cast<const vec*>(src + 16 * gl);
+    x[i] = kHeads > 1 ? __builtin_nontemporal_load(p) : *p;
+  }
+  const int half = a.rot / 2 / E;                  // lanes to the other half
+  const int lane = threadIdx.x & 63;
+  const int other = gl < half ? lane + half : gl < 2 * half ? lane - half : lane;
+  const bool turned = gl < 2 * half;
+  float c[E], s[E];
+  {
+    const int64_t at = turned ? (inside ? pos : 0) * a.rot + E * gl : 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+    for (int e4 = 0; e4 < E; e4 += 4) {
+      const f32x4 cv = *reinterpret_cast<const f32x4*>(a.cos + at + (turned ? e4 : 0));
+      const f32x4 sv = *reinterpret_cast<const f32x4*>(a.sin + at + (turned ? e4 : 0));
 #pragma unroll
-      for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o);
-      const float r = rsqrtf(ss / (float)D + a.eps);
-      const vec wv = *reinterpret_cast<const vec*>(w + E * gl);
-#pragma unroll
-      for (int e = 0; e < E; ++e) y[e] = y[e] * r * to_f32(wv[e]);
-    }
-    const int64_t pos = a.positions[row];
-    const bool inside = pos >= 0 && pos < a.table_rows;
-    const int half = a.rot / 2 / E;                // lanes to the other half
-    const int lane = threadIdx.x & 63;
-    const int other = gl < half ? lane + half : gl < 2 * half ? lane - half : lane;
-    float z[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) z[e] = __shfl(y[e], other);
-    if (gl < 2 * half) {
-      const int64_t at = (inside ? pos : 0) * a.rot + E * gl;
-      const float sign = gl < half ? -1.f : 1.f;
-#pragma unroll
-      for (int e4 = 0; e4 < E; e4 += 4) {
-        const f32x4 c = *reinterpret_cast<const f32x4*>(a.cos + at + e4), s = *reinterpret_cast<const f32x4*>(a.sin + at + e4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e4 + e] = y[e4 + e] * c[e] + sign * z[e4 + e] * s[e];
+      for (int e = 0; e < 4; ++e) {
+        c[e4 + e] = turned ? cv[e] : 1.f;
+        s[e4 + e] = gl < half ? -sv[e] : sv[e];
       }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = from_f32<T>(inside ? y[e] : __builtin_nanf(""));
   }
-  *reinterpret_cast<vec*>(dst + 16 * gl) = x;
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int head = head0 + i;
+    if (kHeads > 1 && head >= (int)nh) break;
+    const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
+    if (!is_q && !keep) continue;
+    const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
+    char* dst = is_q ? a.q_out + ((row * a.hq + h) * D) * (int64_t)sizeof(T)
+                     : (is_v ? a.vp : a.kp).row(slot >> a.shift, h, (int)(slot & ((1 << a.shift) - 1)));
+    if (!is_v) {
+      float y[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) y[e] = to_f32(x[i][e]);
+      const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
+      if (w != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+        for (int o = 1; o < LPR; o <<= 1) ss += __shfl_xor(ss, o);
+        const float r = rsqrtf(ss / (float)D + a.eps);
+        const vec wv = *reinterpret_cast<const vec*>(w + E * gl);
+#pragma unroll
+        for (int e = 0; e < E; ++e) y[e] = y[e] * r * to_f32(wv[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float z = __shfl(y[e], other);
+        const float t = y[e] * c[e] + z * s[e];
+        x[i][e] = from_f32<T>(!inside ? __builtin_nanf("") : turned ? t : y[e]);
+      }
+    }
+    vec* p = reinterpret_cast<vec*>(dst + 16 * gl);
+    if constexpr (kHeads > 1) __builtin_nontemporal_store(x[i], p);
+    else *p = x[i];
+  }
 }
 
 static int check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, const int64_t (&st)[6]) {
@@ -474,10 +502,16 @@ extern "C" int bfly_paged_rope_append(const void* q, const void* k, const void* 
   a.shift = __builtin_ctz(page_size); a.rot = rotary_dim; a.eps = eps;
   BFLY_CHECK_ARG(rows <= INT32_MAX && hq <= (1 << 20) && (int64_t)hq + 2 * hkv <= (1 << 22), "too many rows");
   BFLY_CHECK_ARG(rows * ((int64_t)hq + 2 * hkv) < ((int64_t)1 << 31) - 256, "too many rows");
-  a.items = (unsigned)(rows * ((int64_t)hq + 2 * hkv));
+  const int64_t heads = (int64_t)hq + 2 * hkv;
+  const bool many = rows * heads >= kManyHeads;
+  a.items = (unsigned)(rows * (many ? (heads + 3) / 4 : heads));
   const int64_t lanes = head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
   const dim3 grid((unsigned)blocks), block(256);
-#define BFLY_ROPE(T, D) hipLaunchKernelGGL((paged_rope_append_kernel<T, D>), grid, block, 0, stream, a)
+#define BFLY_ROPE(T, D)                                                                                \
+  do {                                                                                                 \
+    if (many) hipLaunchKernelGGL((paged_rope_append_kernel<T, D, 4>), grid, block, 0, stream, a);      \
+    else hipLaunchKernelGGL((paged_rope_append_kernel<T, D, 1>), grid, block, 0, stream, a);           \
+  } while (0)
   if (dtype == BFLY_DTYPE_BF16) {
     if (head_dim == 64) BFLY_ROPE(__bf16, 64);
     else if (head_dim == 128) BFLY_ROPE(__bf16, 128);

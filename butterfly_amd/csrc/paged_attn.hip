@@ -3,11 +3,11 @@
 //   s_t = scale q . k_t for the positions t it sees, m = max s_t, l = sum exp(s_t - m),
 //   o = (sum exp(s_t - m) v_t) / l, in one pass over the keys with a running m and l.
 //
-// Work: a request's tiles (32 keys in bf16, 16 in fp32) are split into runs of at most c tiles, c such
-// that all requests and heads together make about kTarget runs.  A workgroup takes one run of one kv head
-// for up to 16 of its query heads; every workgroup finds its run from the lengths by itself (plan_run), so
-// the grid needs no host knowledge of them.  Requests with one run write their output, the others a
-// partial (fp32 sums, m, l) that paged_merge_kernel joins.
+// Work: a request's tiles (32 keys in bf16, 16 in fp32) go in rounds of four, one for each wave of a
+// workgroup, and its rounds in runs of at most c, c such that all requests and heads together make about
+// kRuns runs.  A workgroup takes one run of one kv head for up to 16 of its query heads; every workgroup finds
+// its run from the lengths by itself (plan_run), so the grid needs no host knowledge of them.  Requests with
+// one run write their output, the others a partial (fp32 sums, m, l) that paged_merge_kernel joins.
 //
 // A wave takes every fourth tile of the run, by itself: no barrier and no LDS until its sums meet the
 // other waves'.  S^T = K Q^T and O^T += V^T P^T on the matrix cores, query heads as columns, so a
@@ -21,16 +21,18 @@
 namespace bfly {
 
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
-constexpr int kTargetLog = 10;        // about 2^10 runs in all
-constexpr int kMinRun = 8;            // c at least
-constexpr int kWhole = 16;            // tiles that stay one run: a request of 512 keys is done before a join of two runs
-// A request of several runs has more than c tiles, so fewer than 2 tiles_b / c runs; all of them together,
-// with c >= total / 2^kTargetLog, fewer than 2^(kTargetLog + 1): the partials there can be.
-constexpr int kMaxSlots = 2 << kTargetLog;
+constexpr int kRuns = 256;            // runs in all, where the requests and heads leave that many: one for each CU
+constexpr int kMinRun = 1;            // c at least
+constexpr int kWhole = 4;             // rounds that stay one run: 512 keys are done before a join of two runs
+// A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
+// c >= total / kRuns, fewer than 2 kRuns: the partials there can be.  (kSlack: the total is a sum of floats.)
+constexpr int kSlack = 64;
+constexpr int kMaxSlots = 2 * kRuns + kSlack;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 constexpr int kTile = sizeof(T) == 2 ? 32 : 16;
+constexpr int kWaves = 4;             // waves of a workgroup, tiles of a round
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
@@ -49,6 +51,7 @@ struct PagedAttnArgs {
   int requests, num_pages, hq, hkv, shift, window;
   int group, row_tiles, rows;            // query heads a kv head; 16-row parts of them; rows of a part at most
   int units;                             // hkv * row_tiles
+  int whole;                             // every request is one run (its table row is that short)
   float scale;
 };
 
@@ -56,22 +59,23 @@ struct PagedAttnArgs {
 struct Span {
   int lo, n;      // positions seen: [lo, n)
   int t0, tiles;  // tiles that hold them
+  int rounds;     // four tiles each
   bool off;       // the length is beyond the table
 };
 template <int KT>
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int b) {
-  const int len = a.lengths[b];
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
   Span s;
   s.off = (int64_t)len > a.capacity;
   s.n = len <= 0 || s.off ? 0 : len;
   s.lo = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
   s.t0 = s.lo / KT;
   s.tiles = s.n > 0 ? (s.n - 1) / KT + 1 - s.t0 : 0;
+  s.rounds = (s.tiles + kWaves - 1) / kWaves;
   return s;
 }
 
 struct Run {
-  int b;          // request, -1: none
+  int b, len;     // request (-1: none) and its length
   int sub;        // index inside the request
   int splits;     // runs of the request (per unit)
   int slot;       // partials before the request's
@@ -114,34 +118,49 @@ __device__ __forceinline__ float wave_max(float x) {
 // stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
 template <int KT, bool kMerge>
 __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
+  if (a.whole) {                                    // no request can have several runs: item = (request, unit)
+    const int b = (int)idx / a.units;
+    return Run{b, a.lengths[b], (int)idx - b * a.units, 1, 0};
+  }
   const int lane = threadIdx.x & 63;
   const int per = (a.requests + 63) >> 6;
   const int b0 = lane * per < a.requests ? lane * per : a.requests;
   const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
-  const int first = b0 < b1 ? span_of<KT>(a, b0).tiles : 0;
+  const int len0 = b0 < b1 ? a.lengths[b0] : 0;
+  const int first = b0 < b1 ? span_of<KT>(a, len0).rounds : 0;
+  const auto rounds = [&](int b) { return b == b0 ? first : span_of<KT>(a, a.lengths[b]).rounds; };
   float total = (float)first;
-  for (int b = b0 + 1; b < b1; ++b) total += (float)span_of<KT>(a, b).tiles;
-  // (the sum of at most 65535 positive numbers, off by 1e-2 of 1 % at the most: c is above the bound all the same)
-  total = wave_total(total) * (float)a.units * (1.01f / (1 << kTargetLog));
-  const int c = __builtin_amdgcn_readfirstlane(total < (float)kMinRun ? kMinRun : total > 1e9f ? 1000000000 : (int)total + 1);
-  const auto runs = [&](int tiles) { return tiles > c && tiles > kWhole ? (int)(((unsigned)tiles + c - 1) / (unsigned)c) : 1; };
-  int items = 0, slots = 0;
+  for (int b = b0 + 1; b < b1; ++b) total += (float)rounds(b);
+  total = wave_total(total) * (float)a.units;
+  // c fills kRuns exactly if the requests' last, shorter runs fit among them; else room is left for one each
+  const auto over = [&](float to) { return fminf(fmaxf(ceilf(total / to), (float)kMinRun), 1e9f); };
+  int c = __builtin_amdgcn_readfirstlane((int)over((float)kRuns));
+  const auto runs = [&](int n) { return n > c && n > kWhole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
+  int items = 0;
+  for (int b = b0; b < b1; ++b) items += runs(rounds(b));
+  const int64_t pairs = (int64_t)a.requests * a.units;
+  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > kRuns && pairs < kRuns)
+    c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < kRuns / 2 ? kRuns - (int)pairs : kRuns / 2)));
+  int slots = 0;
+  items = 0;
   for (int b = b0; b < b1; ++b) {
-    const int s = runs(b == b0 ? first : span_of<KT>(a, b).tiles);
+    const int s = runs(rounds(b));
     items += kMerge ? (s > 1 ? 1 : 0) : s;
     slots += s > 1 ? s : 0;
   }
   const int i_up = wave_scan(items), s_up = wave_scan(slots);
-  const uint64_t over = __ballot((int64_t)i_up * a.units > idx);
-  Run r{-1, 0, 0, 0};
-  if (over == 0) return r;
-  const int owner = __builtin_ctzll(over);
+  const uint64_t mine = __ballot((int64_t)i_up * a.units > idx);
+  Run r{-1, 0, 0, 0, 0};
+  if (mine == 0) return r;
+  const int owner = __builtin_ctzll(mine);
   int at = __builtin_amdgcn_readlane(i_up - items, owner), slot = __builtin_amdgcn_readlane(s_up - slots, owner);
   for (int b = owner * per;; ++b) {               // (a request of the owner's stretch holds idx)
-    const int s = per == 1 ? runs(__builtin_amdgcn_readlane(first, owner)) : runs(span_of<KT>(a, b).tiles);
+    const int len = per == 1 ? __builtin_amdgcn_readlane(len0, owner) : a.lengths[b];
+    const int s = runs(span_of<KT>(a, len).rounds);
     const int next = at + (kMerge ? (s > 1 ? 1 : 0) : s);
     if ((int64_t)next * a.units > idx) {
       r.b = b;
+      r.len = len;
       r.sub = (int)(idx - (int64_t)at * a.units);
       r.splits = s;
       r.slot = slot * a.units;
@@ -372,7 +391,7 @@ __device__ __forceinline__ void tile_base(const PagedAttnArgs& a, const PagePtr&
   for (int u = 0; u < U; ++u) base[u] = p.row(id[u], h, (first + 16 * u) & ((1 << a.shift) - 1));
 }
 
-// Tiles t, t + 4, ... below t_end.  Returns whether a page id was outside the pages.
+// Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.
 template <typename T, int D, bool kSafe>
 __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, const int32_t* row, const Span& s, int kvh,
                                       int t, int t_end) {
@@ -388,7 +407,7 @@ __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, co
   tile_base<U>(a, a.vp, kvh, t * KT, id, base);
   w.load_v(base, a.vp.row_bytes, n, g);
   while (true) {
-    const int next = t + 4;
+    const int next = t + kWaves;
     const bool more = next < t_end;
     if (more) bad |= tile_pages<U>(a, row, next * KT, s, id);
     float p[P];
@@ -437,10 +456,10 @@ __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, co
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a) {
   constexpr int KT = kTile<T>, LD = D + 4;
-  __shared__ float so[4][16 * LD];
-  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float so[kWaves][16 * LD];
+  __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int sbad;
   const Run run = plan_run<KT, false>(a, blockIdx.x);
   if (run.b < 0) return;
@@ -450,21 +469,22 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
   const int kvh = unit / a.row_tiles, part = unit - kvh * a.row_tiles;
   const int rows = a.group - 16 * part < 16 ? a.group - 16 * part : 16;
   const int head0 = kvh * a.group + 16 * part;
-  const Span s = span_of<KT>(a, b);
+  const Span s = span_of<KT>(a, __builtin_amdgcn_readfirstlane(run.len));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int64_t row0 = (int64_t)b * a.hq + head0;
   if (s.tiles == 0) {                               // nothing to see, or a length beyond the table
     const float y = s.off ? __builtin_nanf("") : 0.f;
-    for (int i = threadIdx.x; i < rows * D; i += 256) static_cast<T*>(a.out)[row0 * D + i] = from_f32<T>(y);
+    for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) static_cast<T*>(a.out)[row0 * D + i] = from_f32<T>(y);
     if (a.l != nullptr && threadIdx.x < rows) {
       a.l[row0 + threadIdx.x] = y;
       a.m[row0 + threadIdx.x] = s.off ? y : kPagedNeg;
     }
     return;
   }
-  const int each = s.tiles / splits, extra = s.tiles - each * splits;
-  const int t0 = s.t0 + split * each + (split < extra ? split : extra), t1 = t0 + each + (split < extra ? 1 : 0);
+  const int each = s.rounds / splits, extra = s.rounds - each * splits;
+  const int r0 = split * each + (split < extra ? split : extra), r1 = r0 + each + (split < extra ? 1 : 0);
+  const int t0 = s.t0 + kWaves * r0, t1 = s.t0 + (kWaves * r1 < s.tiles ? kWaves * r1 : s.tiles);
   const int32_t* table = a.table + b * a.table_stride;
   if (threadIdx.x == 0) sbad = 0;
   Sweep<T, D> w;
@@ -496,14 +516,16 @@ __global__ void __launch_bounds__(256) paged_attn_kernel(PagedAttnArgs a) {
   if (bad && lane == 0) sbad = 1;
   __syncthreads();
   const float poison = sbad ? __builtin_nanf("") : 0.f;
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
+  for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * kWaves) {
     const int r = i / (D / 4), c = 4 * (i % (D / 4));
-    const float mm = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
+    float mm = sm[0][r];
+#pragma unroll
+    for (int k = 1; k < kWaves; ++k) mm = fmaxf(mm, sm[k][r]);
     const float ref = mm == -INFINITY ? 0.f : mm;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
     float ll = poison;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kWaves; ++k) {
       const float f = __builtin_amdgcn_exp2f((sm[k][r] - ref) * kLog2e);
       // a wave without tiles has no part in it (0 * its sums would do, but for a reference of +inf)
       if (t0 + k < t1) {
@@ -585,17 +607,18 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   if (c == 0) finish_stats<T>(a, row, mm, l);
 }
 
-// The tiles that a request spans at most; only one of more than kWhole can have several runs.
-static int64_t most_tiles(int64_t capacity, int window, int kt) {
+// The rounds of a request at most; only one of more than kWhole can have several runs.
+static int64_t most_rounds(int64_t capacity, int window, int esize) {
+  const int kt = esize == 2 ? kTile<__bf16> : kTile<float>;
   const int64_t keys = window > 0 && window < capacity ? (int64_t)window + kt - 1 : capacity;
-  return (keys + kt - 1) / kt;
+  return (keys + kWaves * kt - 1) / (kWaves * kt);
 }
 template <typename T, int D>
 static void launch_paged(const PagedAttnArgs& a, int64_t items, bool splits, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(64 * kWaves), 0, stream, a);
   if (splits) {
     const int64_t pairs = (int64_t)a.requests * a.units;
-    const unsigned x = (unsigned)(pairs < (1 << kTargetLog) ? pairs : (1 << kTargetLog));
+    const unsigned x = (unsigned)(pairs < kRuns ? pairs : kRuns);
     hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(x, (unsigned)a.rows, D / 64), dim3(256), 0, stream, a);
   }
 }
@@ -607,7 +630,7 @@ using namespace bfly;
 extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim,
                                                         int64_t table_width, int page_size, int window) {
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
-  if (most_tiles(table_width * page_size, window, 16) <= kWhole) return 0;
+  if (most_rounds(table_width * page_size, window, 4) <= kWhole) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
@@ -655,11 +678,11 @@ extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, 
   a.units = hkv * a.row_tiles;
   a.part = static_cast<float*>(workspace);
   a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * head_dim;
-  // runs: one for each (request, unit), and as many more as the splits make (kTargetLog, plan_run)
-  const int kt = dtype == BFLY_DTYPE_F32 ? kTile<float> : kTile<__bf16>;
-  const int64_t tiles = most_tiles(a.capacity, window, kt), pairs = requests * a.units;
-  const bool splits = tiles > kWhole;
-  const int64_t most = pairs * ((tiles + kMinRun - 1) / kMinRun), some = pairs + (1 << kTargetLog);
+  // runs: one for each (request, unit), and as many more as the splits make (plan_run)
+  const int64_t rounds = most_rounds(a.capacity, window, (int)es), pairs = requests * a.units;
+  const bool splits = rounds > kWhole;
+  a.whole = !splits;
+  const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + kRuns + kSlack;
   const int64_t items = !splits ? pairs : most < some ? most : some;
   BFLY_CHECK_ARG(items <= INT32_MAX, "too many requests and heads");
 #define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)

@@ -21,12 +21,13 @@ gradients enabled they refuse tensors that require them.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _native
-from ._device import _GET_DEVICE, on, stream_of
+from ._device import _GET_DEVICE, stream_of
 from .attention import _dtype_code
 
 PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
@@ -57,22 +58,15 @@ class PagedPlan(NamedTuple):
 _GRAD = "the paged operators are for inference: call them under torch.no_grad()"
 
 
-def _device_of(t: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+def _device_of(t: torch.Tensor) -> int:
     dev = t.get_device()
     if dev < 0:
         raise ValueError("butterfly_amd operators take GPU tensors (device 'cuda')")
-    for o in others:
-        if o is not None and o.get_device() != dev:
-            raise ValueError("all tensors must be GPU tensors of one device")
     return dev
 
 
-def _call(dev: int, name: str, *args) -> None:
-    if dev == _GET_DEVICE():
-        _native.call(name, *args, stream_of(dev))
-    else:
-        with on(torch.device("cuda", dev)):
-            _native.call(name, *args, stream_of(dev))
+def _other_device() -> None:
+    raise ValueError("all tensors must be GPU tensors of one device")
 
 
 def _check_ints(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> None:
@@ -107,7 +101,7 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: int, written: bool
     if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype is not dtype:
         raise ValueError("k_pages and v_pages must be [num_pages, Hkv, page_size, d] of one shape and type")
     if k_pages.get_device() != dev or v_pages.get_device() != dev:
-        raise ValueError("all tensors must be GPU tensors of one device")
+        _other_device()
     if shape[2] not in PAGE_SIZES:
         raise ValueError(f"page_size {shape[2]} must be a power of two from 16 to 1024")
     k0, k1, k2, k3 = k_pages.stride()
@@ -158,7 +152,13 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     ``state[1]`` holds the code and every slot is -1, and so for every later step until the caller clears
     it: a captured loop that ran out of pages is found out by reading the state once.
     """
-    dev = _device_of(lengths, block_table, counts, free_pages, state)
+    dev = _device_of(lengths)
+    if not block_table.get_device() == counts.get_device() == free_pages.get_device() == state.get_device() == dev:
+        _other_device()
+    if dev != _GET_DEVICE():
+        with torch.cuda.device(dev):
+            return paged_plan(block_table, lengths, counts, free_pages, state, page_size=page_size, num_rows=num_rows,
+                              rows_each=rows_each, in_place=in_place)
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
     if lengths.dim() != 1:
@@ -187,9 +187,9 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
         new_lengths, new_state, starts, ws = torch.empty(5 * b + 6, dtype=i32, device=cuda).split_with_sizes(
             (b, 2, b + 1, 3 * b + 3))
     slots, positions = torch.empty(2, num_rows, dtype=torch.int64, device=cuda).unbind(0)
-    _call(dev, "bfly_paged_plan", block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(),
+    _native.call("bfly_paged_plan", block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(),
           free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size, num_rows, rows_each, new_lengths.data_ptr(),
-          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 12 * (b + 1))
+          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 12 * (b + 1), stream_of(dev))
     return PagedPlan(new_lengths, new_state, starts, slots, positions)
 
 
@@ -200,7 +200,7 @@ def _check_rows(k, v, shape, dtype, slots, dev):
     if not k.dtype is v.dtype is dtype:
         raise ValueError("rows and pages must have one type")
     if k.get_device() != dev or v.get_device() != dev:
-        raise ValueError("all tensors must be GPU tensors of one device")
+        _other_device()
     _check_ints(slots, "slots", torch.int64, n[0])
     return n
 
@@ -212,6 +212,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     beyond the pages is passed over.  The slots of a call are distinct, as a plan gives them (of two rows
     with one slot it is not defined which stays).  float32 or bfloat16; ``d`` of whole 16-byte pieces."""
     dev = _device_of(slots)
+    if dev != _GET_DEVICE():
+        with torch.cuda.device(dev):
+            return paged_append(k, v, k_pages, v_pages, slots)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise ValueError(_GRAD)
     shape, strides = _pages(k_pages, v_pages, dev, True)
@@ -223,8 +226,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         return
     (k, k0, k1), (v, v0, v1) = _rows(k), _rows(v)
     slots = slots.contiguous()
-    _call(dev, "bfly_paged_append", k.data_ptr(), v.data_ptr(), code, n, hkv, d, k0, k1, v0, v1, slots.data_ptr(),
-          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides)
+    _native.call("bfly_paged_append", k.data_ptr(), v.data_ptr(), code, n, hkv, d, k0, k1, v0, v1, slots.data_ptr(),
+          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides, stream_of(dev))
 
 
 def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -242,7 +245,13 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     Between the inputs and the outputs nothing is rounded to fewer than 32 bits (``bfly_qk_norm_rope``, whose
     rounding points are the modules', rounds after the norm as well).  head_dim 64, 128 or 256, ``r`` a multiple
     of 16."""
-    dev = _device_of(q, slots, positions, cos, sin, q_weight, k_weight)
+    dev = _device_of(q)
+    if not slots.get_device() == positions.get_device() == cos.get_device() == sin.get_device() == dev:
+        _other_device()
+    if dev != _GET_DEVICE():
+        with torch.cuda.device(dev):
+            return paged_rope_append(q, k, v, k_pages, v_pages, slots, positions, cos, sin, q_weight=q_weight,
+                                     k_weight=k_weight, eps=eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad
                                     or v_pages.requires_grad or cos.requires_grad or sin.requires_grad
                                     or q_weight is not None and q_weight.requires_grad
@@ -267,6 +276,8 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     if q_weight is not None:
         if q_weight.shape != (d,) or k_weight.shape != (d,) or not q_weight.dtype is k_weight.dtype is dtype:
             raise ValueError("norm weights must be [d] of the rows' type")
+        if not q_weight.get_device() == k_weight.get_device() == dev:
+            _other_device()
         q_weight, k_weight = _flat(q_weight), _flat(k_weight)
         qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
     out = torch.empty(sq, dtype=dtype, device=q.device)
@@ -274,9 +285,9 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
         return out
     (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
     slots, positions, cos, sin = slots.contiguous(), positions.contiguous(), _flat(cos), _flat(sin)
-    _call(dev, "bfly_paged_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1,
+    _native.call("bfly_paged_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1,
           qw, kw, eps, cos.data_ptr(), sin.data_ptr(), table[0], table[1], positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
-          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides)
+          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides, stream_of(dev))
     return out
 
 
@@ -300,7 +311,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     the empty stream ``(0, 0, -1e30)``; a length beyond its table row, or a page id outside the pages among
     those that are read, gives NaN for that request.  Rows of a page behind the request's last token are never
     part of the result, whatever they hold.  float32 or bfloat16, head_dim 64, 128 or 256."""
-    dev = _device_of(q, block_table, lengths)
+    dev = _device_of(q)
+    if not block_table.get_device() == lengths.get_device() == dev:
+        _other_device()
+    if dev != _GET_DEVICE():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_pages, v_pages, block_table, lengths, scale=scale, window=window,
+                                   return_stats=return_stats)
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise ValueError(_GRAD)
     shape, strides = _pages(k_pages, v_pages, dev, False)
@@ -330,15 +347,16 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         need = _workspace_bytes(b, hq, hkv, d, width, page_size, window)
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=cuda)
-        _call(dev, "bfly_paged_attention", q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages,
+        _native.call("bfly_paged_attention", q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages,
               page_size, *strides, block_table.data_ptr(), width, stride, lengths.data_ptr(), window,
-              1.0 / math.sqrt(d) if scale is None else scale, out.data_ptr(), lp, mp, None if ws is None else ws.data_ptr(), need)
+              1.0 / math.sqrt(d) if scale is None else scale, out.data_ptr(), lp, mp, None if ws is None else ws.data_ptr(), need,
+                     stream_of(dev))
     return (out, l, m) if return_stats else out
 
 
-def _workspace_bytes(*args) -> int:
-    fn = _native._fns.get("bfly_paged_attention_workspace_bytes")
-    return (fn or _native.lib().bfly_paged_attention_workspace_bytes)(*args)
+@lru_cache(maxsize=1024)
+def _workspace_bytes(*sizes: int) -> int:
+    return _native.lib().bfly_paged_attention_workspace_bytes(*sizes)
 
 
 class PagedLayer:
