@@ -16,8 +16,17 @@ struct PagePtr {
   }
 };
 
-// The host's checks of page_size, num_pages and the six page strides (elements); BFLY_OK or an error.
-int paged_check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, int64_t k_page,
-                      int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head, int64_t v_row);
+// The host's checks of a pair of page tensors (elements of `esize` bytes); BFLY_OK or an error.
+int paged_check_pages(const char* what, const bfly_pages_t& p, int64_t esize);
+
+inline PagePtr page_ptr(void* base, int64_t page, int64_t head, int64_t row, int64_t esize) {
+  return PagePtr{static_cast<char*>(base), page * esize, head * esize, (int)(row * esize)};
+}
+inline PagePtr k_page_ptr(const bfly_pages_t& p, int64_t esize) {
+  return page_ptr(p.k, p.k_page_stride, p.k_head_stride, p.k_row_stride, esize);
+}
+inline PagePtr v_page_ptr(const bfly_pages_t& p, int64_t esize) {
+  return page_ptr(p.v, p.v_page_stride, p.v_head_stride, p.v_row_stride, esize);
+}
 
 }  // namespace bfly

@@ -355,23 +355,16 @@ __global__ void __launch_bounds__(256) paged_rope_append_kernel(RopeAppendArgs a
   }
 }
 
-static int check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, const int64_t (&st)[6]) {
-  BFLY_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
-                 "%s: page_size %d must be a power of two from 16 to 1024", what, page_size);
-  BFLY_CHECK_ARG(num_pages > 0 && num_pages <= INT32_MAX, "%s: bad num_pages", what);
-  for (int i = 0; i < 6; ++i)
-    BFLY_CHECK_ARG(st[i] >= 0 && st[i] < ((int64_t)1 << 48) && (st[i] * esize) % 16 == 0,
-                   "%s: page strides must be multiples of 16 bytes", what);
+int paged_check_pages(const char* what, const bfly_pages_t& p, int64_t esize) {
+  BFLY_CHECK_ARG(p.page_size >= 16 && p.page_size <= 1024 && (p.page_size & (p.page_size - 1)) == 0,
+                 "%s: page_size %lld must be a power of two from 16 to 1024", what, (long long)p.page_size);
+  BFLY_CHECK_ARG(p.num_pages > 0 && p.num_pages <= INT32_MAX, "%s: bad num_pages", what);
+  for (const int64_t s : {p.k_page_stride, p.k_head_stride, p.k_row_stride, p.v_page_stride, p.v_head_stride, p.v_row_stride})
+    BFLY_CHECK_ARG(s >= 0 && s < ((int64_t)1 << 48) && (s * esize) % 16 == 0, "%s: page strides must be multiples of 16 bytes", what);
   // offsets inside a page and head are kept in 32 bits
-  BFLY_CHECK_ARG(st[2] * esize * page_size <= INT32_MAX && st[5] * esize * page_size <= INT32_MAX,
+  BFLY_CHECK_ARG(p.k_row_stride * esize * p.page_size <= INT32_MAX && p.v_row_stride * esize * p.page_size <= INT32_MAX,
                  "%s: row stride too large", what);
   return BFLY_OK;
-}
-
-int paged_check_pages(const char* what, int64_t num_pages, int page_size, int64_t esize, int64_t k_page,
-                      int64_t k_head, int64_t k_row, int64_t v_page, int64_t v_head, int64_t v_row) {
-  const int64_t st[6] = {k_page, k_head, k_row, v_page, v_head, v_row};
-  return check_pages(what, num_pages, page_size, esize, st);
 }
 
 static bool strides16(std::initializer_list<int64_t> st, int64_t esize) {
@@ -384,141 +377,128 @@ static bool strides16(std::initializer_list<int64_t> st, int64_t esize) {
 
 using namespace bfly;
 
-extern "C" int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,
-                               const int32_t* lengths, const int32_t* counts, int32_t* free_pages,
-                               int64_t free_capacity, const int32_t* state, int page_size, int64_t num_rows,
-                               int64_t rows_each, int32_t* lengths_out, int32_t* state_out, int32_t* starts, int64_t* slots,
-                               int64_t* positions, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
-  BFLY_CHECK_ARG(requests >= 0 && requests <= (1 << 24) && table_width >= 0 && table_width <= INT32_MAX, "bad block table shape");
-  BFLY_CHECK_ARG(requests <= 1 || table_stride >= table_width, "block table rows overlap");
-  BFLY_CHECK_ARG(num_rows >= 0 && num_rows <= INT32_MAX && free_capacity >= 0 && free_capacity <= INT32_MAX,
+extern "C" int bfly_paged_plan(const bfly_paged_plan_args_t* args, hipStream_t stream) {
+  BFLY_CHECK_ARG(args, "null pointer");
+  const bfly_paged_plan_args_t& x = *args;
+  BFLY_CHECK_ARG(x.requests >= 0 && x.requests <= (1 << 24) && x.table_width >= 0 && x.table_width <= INT32_MAX, "bad block table shape");
+  BFLY_CHECK_ARG(x.requests <= 1 || x.table_stride >= x.table_width, "block table rows overlap");
+  BFLY_CHECK_ARG(x.num_rows >= 0 && x.num_rows <= INT32_MAX && x.free_capacity >= 0 && x.free_capacity <= INT32_MAX,
                  "num_rows and the free list must stay below 2^31");
-  BFLY_CHECK_ARG(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
-                 "page_size %d must be a power of two from 16 to 1024", page_size);
-  BFLY_CHECK_ARG(rows_each >= 0 && (rows_each == 0 || num_rows == requests * rows_each),
+  BFLY_CHECK_ARG(x.page_size >= 16 && x.page_size <= 1024 && (x.page_size & (x.page_size - 1)) == 0,
+                 "page_size %lld must be a power of two from 16 to 1024", (long long)x.page_size);
+  BFLY_CHECK_ARG(x.rows_each >= 0 && (x.rows_each == 0 || (x.rows_each <= INT32_MAX && x.num_rows == x.requests * x.rows_each)),
                  "num_rows must be the requests' rows_each");
-  BFLY_CHECK_ARG(state && state_out && starts, "null pointer");
-  BFLY_CHECK_ARG(requests == 0 || (lengths && counts && lengths_out), "null pointer");
-  BFLY_CHECK_ARG(requests * table_width == 0 || block_table, "null pointer");
-  BFLY_CHECK_ARG(free_capacity == 0 || free_pages, "null pointer");
-  BFLY_CHECK_ARG(num_rows == 0 || (slots && positions), "null pointer");
-  BFLY_CHECK_ARG(workspace && workspace_bytes >= (requests + 1) * 12 && (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+  BFLY_CHECK_ARG(x.state && x.state_out && x.starts, "null pointer");
+  BFLY_CHECK_ARG(x.requests == 0 || (x.lengths && x.counts && x.lengths_out), "null pointer");
+  BFLY_CHECK_ARG(x.requests * x.table_width == 0 || x.block_table, "null pointer");
+  BFLY_CHECK_ARG(x.free_capacity == 0 || x.free_pages, "null pointer");
+  BFLY_CHECK_ARG(x.num_rows == 0 || (x.slots && x.positions), "null pointer");
+  BFLY_CHECK_ARG(x.workspace && x.workspace_bytes >= (x.requests + 1) * 12 && (reinterpret_cast<uintptr_t>(x.workspace) & 3) == 0,
                  "workspace too small");
   PlanArgs a{};
-  a.table = block_table; a.lengths = lengths; a.counts = counts; a.free_pages = free_pages; a.state = state;
-  a.lengths_out = lengths_out; a.state_out = state_out; a.starts = starts; a.slots = slots; a.positions = positions;
-  a.taken = static_cast<int32_t*>(workspace);
-  a.given = a.taken + requests + 1;
-  a.before = a.given + requests + 1;
-  a.table_stride = table_stride;
-  a.shift = __builtin_ctz(page_size);
-  const int64_t cap = table_width << a.shift;
+  a.table = x.block_table; a.lengths = x.lengths; a.counts = x.counts; a.free_pages = x.free_pages; a.state = x.state;
+  a.lengths_out = x.lengths_out; a.state_out = x.state_out; a.starts = x.starts; a.slots = x.slots; a.positions = x.positions;
+  a.taken = static_cast<int32_t*>(x.workspace);
+  a.given = a.taken + x.requests + 1;
+  a.before = a.given + x.requests + 1;
+  a.table_stride = x.table_stride;
+  a.shift = __builtin_ctzll(x.page_size);
+  const int64_t cap = x.table_width << a.shift;
   a.capacity = cap < INT32_MAX ? cap : INT32_MAX;
-  a.requests = (int)requests; a.free_capacity = (int)free_capacity; a.num_rows = (int)num_rows;
-  a.fixed = (int)rows_each;
-  const dim3 block(requests <= 256 && num_rows <= 256 ? 256 : kPlanMaxThreads);
-  if (requests <= kPlanLds && num_rows <= 4096) {
+  a.requests = (int)x.requests; a.free_capacity = (int)x.free_capacity; a.num_rows = (int)x.num_rows;
+  a.fixed = (int)x.rows_each;
+  const dim3 block(x.requests <= 256 && x.num_rows <= 256 ? 256 : kPlanMaxThreads);
+  if (x.requests <= kPlanLds && x.num_rows <= 4096) {
     hipLaunchKernelGGL(plan_kernel<true>, dim3(1), block, 0, stream, a);
   } else {
     hipLaunchKernelGGL(plan_kernel<false>, dim3(1), block, 0, stream, a);
-    if (num_rows > 0)
-      hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((num_rows + 255) / 256)), dim3(256), 0, stream, a);
+    if (x.num_rows > 0)
+      hipLaunchKernelGGL(plan_rows_kernel, dim3((unsigned)((x.num_rows + 255) / 256)), dim3(256), 0, stream, a);
   }
   BFLY_CHECK_LAUNCH("bfly_paged_plan");
   return BFLY_OK;
 }
 
-extern "C" int bfly_paged_append(const void* k, const void* v, int dtype, int64_t rows, int hkv, int head_dim,
-                                 int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
-                                 int64_t v_head_stride, const int64_t* slots, void* k_pages, void* v_pages,
-                                 int64_t num_pages, int page_size, int64_t k_page_stride, int64_t k_page_head_stride,
-                                 int64_t k_page_row_stride, int64_t v_page_stride, int64_t v_page_head_stride,
-                                 int64_t v_page_row_stride, hipStream_t stream) {
-  BFLY_CHECK_ARG(dtype == BFLY_DTYPE_F32 || dtype == BFLY_DTYPE_BF16, "unsupported dtype %d", dtype);
-  const int64_t es = dtype == BFLY_DTYPE_F32 ? 4 : 2;
-  BFLY_CHECK_ARG(rows >= 0 && hkv > 0 && head_dim > 0, "bad shape");
-  BFLY_CHECK_ARG(head_dim * es % 16 == 0, "head_dim %d is not whole 16-byte pieces", head_dim);
-  const int rc = paged_check_pages("bfly_paged_append", num_pages, page_size, es, k_page_stride, k_page_head_stride,
-                                   k_page_row_stride, v_page_stride, v_page_head_stride, v_page_row_stride);
+extern "C" int bfly_paged_append(const bfly_paged_append_args_t* args, hipStream_t stream) {
+  BFLY_CHECK_ARG(args, "null pointer");
+  const bfly_paged_append_args_t& x = *args;
+  BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
+  const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
+  BFLY_CHECK_ARG(x.rows >= 0 && x.rows <= INT32_MAX && x.hkv > 0 && x.hkv <= 65535 && x.head_dim > 0 && x.head_dim <= 65535, "bad shape");
+  BFLY_CHECK_ARG(x.head_dim * es % 16 == 0, "head_dim %lld is not whole 16-byte pieces", (long long)x.head_dim);
+  const int rc = paged_check_pages("bfly_paged_append", x.pages, es);
   if (rc != BFLY_OK) return rc;
-  BFLY_CHECK_ARG(strides16({k_row_stride, k_head_stride, v_row_stride, v_head_stride}, es),
+  BFLY_CHECK_ARG(strides16({x.k_row_stride, x.k_head_stride, x.v_row_stride, x.v_head_stride}, es),
                  "row and head strides must be multiples of 16 bytes");
-  if (rows == 0) return BFLY_OK;
-  BFLY_CHECK_ARG(k && v && slots && k_pages && v_pages, "null pointer");
-  BFLY_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages), "pointers must be 16-byte aligned");
+  if (x.rows == 0) return BFLY_OK;
+  BFLY_CHECK_ARG(x.k && x.v && x.slots && x.pages.k && x.pages.v, "null pointer");
+  BFLY_CHECK_ARG(aligned16(x.k) && aligned16(x.v) && aligned16(x.pages.k) && aligned16(x.pages.v), "pointers must be 16-byte aligned");
   AppendArgs a{};
-  a.k = static_cast<const char*>(k); a.v = static_cast<const char*>(v); a.slots = slots;
-  a.kp = {static_cast<char*>(k_pages), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
-  a.vp = {static_cast<char*>(v_pages), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
-  a.k_row = k_row_stride * es; a.k_head = k_head_stride * es; a.v_row = v_row_stride * es; a.v_head = v_head_stride * es;
-  a.limit = num_pages * page_size; a.hkv = hkv; a.per = (unsigned)(head_dim * es / 16); a.shift = __builtin_ctz(page_size);
-  BFLY_CHECK_ARG(rows <= INT32_MAX && hkv <= 65535 && a.per <= 65535 && rows * hkv * a.per < ((int64_t)1 << 31) - 256, "too many rows");
-  a.pieces = (unsigned)(rows * hkv * a.per);
+  a.k = static_cast<const char*>(x.k); a.v = static_cast<const char*>(x.v); a.slots = x.slots;
+  a.kp = k_page_ptr(x.pages, es); a.vp = v_page_ptr(x.pages, es);
+  a.k_row = x.k_row_stride * es; a.k_head = x.k_head_stride * es; a.v_row = x.v_row_stride * es; a.v_head = x.v_head_stride * es;
+  a.limit = x.pages.num_pages * x.pages.page_size; a.hkv = (unsigned)x.hkv; a.per = (unsigned)(x.head_dim * es / 16);
+  a.shift = __builtin_ctzll(x.pages.page_size);
+  // (rows < 2^31, hkv and per < 2^16 and 2^14: no overflow)
+  BFLY_CHECK_ARG(x.rows * x.hkv * a.per < ((int64_t)1 << 31) - 256, "too many rows");
+  a.pieces = (unsigned)(x.rows * x.hkv * a.per);
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)((2 * (int64_t)a.pieces + 255) / 256)), dim3(256), 0, stream, a);
   BFLY_CHECK_LAUNCH("bfly_paged_append");
   return BFLY_OK;
 }
 
-extern "C" int bfly_paged_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t rows, int hq,
-                                      int hkv, int head_dim, int64_t q_row_stride, int64_t q_head_stride,
-                                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
-                                      int64_t v_head_stride, const void* q_weight, const void* k_weight, float eps,
-                                      const float* cos, const float* sin, int64_t table_rows, int rotary_dim,
-                                      const int64_t* positions, const int64_t* slots, void* q_out, void* k_pages,
-                                      void* v_pages, int64_t num_pages, int page_size, int64_t k_page_stride,
-                                      int64_t k_page_head_stride, int64_t k_page_row_stride, int64_t v_page_stride,
-                                      int64_t v_page_head_stride, int64_t v_page_row_stride, hipStream_t stream) {
-  BFLY_CHECK_ARG(dtype == BFLY_DTYPE_F32 || dtype == BFLY_DTYPE_BF16, "unsupported dtype %d", dtype);
-  const int64_t es = dtype == BFLY_DTYPE_F32 ? 4 : 2;
-  BFLY_CHECK_ARG(rows >= 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "bad head counts hq=%d hkv=%d", hq, hkv);
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
-    set_error("bfly_paged_rope_append: head_dim=%d unsupported (64, 128, 256)", head_dim);
+extern "C" int bfly_paged_rope_append(const bfly_paged_rope_append_args_t* args, hipStream_t stream) {
+  BFLY_CHECK_ARG(args, "null pointer");
+  const bfly_paged_rope_append_args_t& x = *args;
+  BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
+  const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
+  BFLY_CHECK_ARG(x.rows >= 0 && x.rows <= INT32_MAX, "bad shape");
+  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0, "bad head counts hq=%lld hkv=%lld",
+                 (long long)x.hq, (long long)x.hkv);
+  if (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) {
+    set_error("bfly_paged_rope_append: head_dim=%lld unsupported (64, 128, 256)", (long long)x.head_dim);
     return BFLY_ERR_UNSUPPORTED;
   }
-  BFLY_CHECK_ARG(rotary_dim > 0 && rotary_dim <= head_dim && rotary_dim % 16 == 0,
-                 "rotary_dim %d must be a multiple of 16, at most head_dim", rotary_dim);
-  BFLY_CHECK_ARG(table_rows > 0, "the cos/sin tables must have rows");
-  const int rc = paged_check_pages("bfly_paged_rope_append", num_pages, page_size, es, k_page_stride,
-                                   k_page_head_stride, k_page_row_stride, v_page_stride, v_page_head_stride,
-                                   v_page_row_stride);
+  BFLY_CHECK_ARG(x.rotary_dim > 0 && x.rotary_dim <= x.head_dim && x.rotary_dim % 16 == 0,
+                 "rotary_dim %lld must be a multiple of 16, at most head_dim", (long long)x.rotary_dim);
+  BFLY_CHECK_ARG(x.table_rows > 0, "the cos/sin tables must have rows");
+  const int rc = paged_check_pages("bfly_paged_rope_append", x.pages, es);
   if (rc != BFLY_OK) return rc;
-  BFLY_CHECK_ARG(strides16({q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride}, es),
+  BFLY_CHECK_ARG(strides16({x.q_row_stride, x.q_head_stride, x.k_row_stride, x.k_head_stride, x.v_row_stride, x.v_head_stride}, es),
                  "row and head strides must be multiples of 16 bytes");
-  if (rows == 0) return BFLY_OK;
-  BFLY_CHECK_ARG(q && k && v && cos && sin && positions && slots && q_out && k_pages && v_pages, "null pointer");
-  BFLY_CHECK_ARG((q_weight == nullptr) == (k_weight == nullptr), "both norm weights or neither");
-  BFLY_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(cos) && aligned16(sin) && aligned16(q_out) &&
-                     aligned16(k_pages) && aligned16(v_pages) && aligned16(q_weight) && aligned16(k_weight),
+  if (x.rows == 0) return BFLY_OK;
+  BFLY_CHECK_ARG(x.q && x.k && x.v && x.cos && x.sin && x.positions && x.slots && x.q_out && x.pages.k && x.pages.v, "null pointer");
+  BFLY_CHECK_ARG((x.q_weight == nullptr) == (x.k_weight == nullptr), "both norm weights or neither");
+  BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.k) && aligned16(x.v) && aligned16(x.cos) && aligned16(x.sin) && aligned16(x.q_out) &&
+                     aligned16(x.pages.k) && aligned16(x.pages.v) && aligned16(x.q_weight) && aligned16(x.k_weight),
                  "pointers must be 16-byte aligned");
   RopeAppendArgs a{};
-  a.q = static_cast<const char*>(q); a.k = static_cast<const char*>(k); a.v = static_cast<const char*>(v);
-  a.qw = q_weight; a.kw = k_weight; a.cos = cos; a.sin = sin; a.positions = positions; a.slots = slots;
-  a.q_out = static_cast<char*>(q_out);
-  a.kp = {static_cast<char*>(k_pages), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
-  a.vp = {static_cast<char*>(v_pages), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
-  a.q_row = q_row_stride * es; a.q_head = q_head_stride * es; a.k_row = k_row_stride * es;
-  a.k_head = k_head_stride * es; a.v_row = v_row_stride * es; a.v_head = v_head_stride * es;
-  a.limit = num_pages * page_size; a.table_rows = table_rows; a.hq = hq; a.hkv = hkv;
-  a.shift = __builtin_ctz(page_size); a.rot = rotary_dim; a.eps = eps;
-  BFLY_CHECK_ARG(rows <= INT32_MAX && hq <= (1 << 20) && (int64_t)hq + 2 * hkv <= (1 << 22), "too many rows");
-  BFLY_CHECK_ARG(rows * ((int64_t)hq + 2 * hkv) < ((int64_t)1 << 31) - 256, "too many rows");
-  const int64_t heads = (int64_t)hq + 2 * hkv;
-  const bool many = rows * heads >= kManyHeads;
-  a.items = (unsigned)(rows * (many ? (heads + 3) / 4 : heads));
-  const int64_t lanes = head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
+  a.q = static_cast<const char*>(x.q); a.k = static_cast<const char*>(x.k); a.v = static_cast<const char*>(x.v);
+  a.qw = x.q_weight; a.kw = x.k_weight; a.cos = x.cos; a.sin = x.sin; a.positions = x.positions; a.slots = x.slots;
+  a.q_out = static_cast<char*>(x.q_out);
+  a.kp = k_page_ptr(x.pages, es); a.vp = v_page_ptr(x.pages, es);
+  a.q_row = x.q_row_stride * es; a.q_head = x.q_head_stride * es; a.k_row = x.k_row_stride * es;
+  a.k_head = x.k_head_stride * es; a.v_row = x.v_row_stride * es; a.v_head = x.v_head_stride * es;
+  a.limit = x.pages.num_pages * x.pages.page_size; a.table_rows = x.table_rows; a.hq = (int)x.hq; a.hkv = (int)x.hkv;
+  a.shift = __builtin_ctzll(x.pages.page_size); a.rot = (int)x.rotary_dim; a.eps = (float)x.eps;
+  const int64_t heads = x.hq + 2 * x.hkv;
+  BFLY_CHECK_ARG(x.rows * heads < ((int64_t)1 << 31) - 256, "too many rows");
+  const bool many = x.rows * heads >= kManyHeads;
+  a.items = (unsigned)(x.rows * (many ? (heads + 3) / 4 : heads));
+  const int64_t lanes = x.head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
   const dim3 grid((unsigned)blocks), block(256);
 #define BFLY_ROPE(T, D)                                                                                \
   do {                                                                                                 \
     if (many) hipLaunchKernelGGL((paged_rope_append_kernel<T, D, 4>), grid, block, 0, stream, a);      \
     else hipLaunchKernelGGL((paged_rope_append_kernel<T, D, 1>), grid, block, 0, stream, a);           \
   } while (0)
-  if (dtype == BFLY_DTYPE_BF16) {
-    if (head_dim == 64) BFLY_ROPE(__bf16, 64);
-    else if (head_dim == 128) BFLY_ROPE(__bf16, 128);
+  if (x.dtype == BFLY_DTYPE_BF16) {
+    if (x.head_dim == 64) BFLY_ROPE(__bf16, 64);
+    else if (x.head_dim == 128) BFLY_ROPE(__bf16, 128);
     else BFLY_ROPE(__bf16, 256);
   } else {
-    if (head_dim == 64) BFLY_ROPE(float, 64);
-    else if (head_dim == 128) BFLY_ROPE(float, 128);
+    if (x.head_dim == 64) BFLY_ROPE(float, 64);
+    else if (x.head_dim == 128) BFLY_ROPE(float, 128);
     else BFLY_ROPE(float, 256);
   }
 #undef BFLY_ROPE

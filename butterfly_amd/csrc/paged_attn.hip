@@ -635,64 +635,60 @@ extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq
   return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
 
-extern "C" int bfly_paged_attention(const void* q, int dtype, int64_t requests, int hq, int hkv, int head_dim,
-                                    int64_t q_request_stride, int64_t q_head_stride, const void* k_pages,
-                                    const void* v_pages, int64_t num_pages, int page_size, int64_t k_page_stride,
-                                    int64_t k_page_head_stride, int64_t k_page_row_stride, int64_t v_page_stride,
-                                    int64_t v_page_head_stride, int64_t v_page_row_stride, const int32_t* block_table,
-                                    int64_t table_width, int64_t table_stride, const int32_t* lengths, int window,
-                                    float scale, void* out, float* l, float* m, void* workspace,
-                                    int64_t workspace_bytes, hipStream_t stream) {
-  BFLY_CHECK_ARG(dtype == BFLY_DTYPE_F32 || dtype == BFLY_DTYPE_BF16, "unsupported dtype %d", dtype);
-  const int64_t es = dtype == BFLY_DTYPE_F32 ? 4 : 2;
-  BFLY_CHECK_ARG(requests >= 0 && hq > 0 && hkv > 0 && hq % hkv == 0, "bad head counts hq=%d hkv=%d", hq, hkv);
-  if (head_dim != 64 && head_dim != 128 && head_dim != 256) {
-    set_error("bfly_paged_attention: head_dim=%d unsupported (64, 128, 256)", head_dim);
+extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hipStream_t stream) {
+  BFLY_CHECK_ARG(args, "null pointer");
+  const bfly_paged_attention_args_t& x = *args;
+  BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
+  const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
+  BFLY_CHECK_ARG(x.requests >= 0 && x.requests <= 65535, "bad number of requests (at most 65535)");
+  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0, "bad head counts hq=%lld hkv=%lld",
+                 (long long)x.hq, (long long)x.hkv);
+  if (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) {
+    set_error("bfly_paged_attention: head_dim=%lld unsupported (64, 128, 256)", (long long)x.head_dim);
     return BFLY_ERR_UNSUPPORTED;
   }
-  const int rc = paged_check_pages("bfly_paged_attention", num_pages, page_size, es, k_page_stride, k_page_head_stride,
-                                   k_page_row_stride, v_page_stride, v_page_head_stride, v_page_row_stride);
+  const int rc = paged_check_pages("bfly_paged_attention", x.pages, es);
   if (rc != BFLY_OK) return rc;
-  BFLY_CHECK_ARG(window >= 0, "window must not be negative");
-  BFLY_CHECK_ARG(table_width >= 0 && table_width <= INT32_MAX && (requests <= 1 || table_stride >= 0), "bad block table shape");
-  BFLY_CHECK_ARG(q_request_stride >= 0 && q_head_stride >= 0 && q_request_stride * es % 16 == 0 && q_head_stride * es % 16 == 0,
+  BFLY_CHECK_ARG(x.window >= 0 && x.window <= INT32_MAX, "bad window");
+  BFLY_CHECK_ARG(x.table_width >= 0 && x.table_width <= INT32_MAX && (x.requests <= 1 || x.table_stride >= 0), "bad block table shape");
+  BFLY_CHECK_ARG(x.q_request_stride >= 0 && x.q_head_stride >= 0 && x.q_request_stride * es % 16 == 0 && x.q_head_stride * es % 16 == 0,
                  "q strides must be multiples of 16 bytes");
-  if (requests == 0) return BFLY_OK;
-  BFLY_CHECK_ARG(q && k_pages && v_pages && lengths && out, "null pointer");
-  BFLY_CHECK_ARG(table_width == 0 || block_table, "null pointer");
-  BFLY_CHECK_ARG((l == nullptr) == (m == nullptr), "both l and m or neither");
-  BFLY_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out), "pointers must be 16-byte aligned");
-  BFLY_CHECK_ARG(requests <= 65535, "at most 65535 requests");
-  const int64_t need = bfly_paged_attention_workspace_bytes(requests, hq, hkv, head_dim, table_width, page_size, window);
-  BFLY_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)), "workspace too small");
+  if (x.requests == 0) return BFLY_OK;
+  BFLY_CHECK_ARG(x.q && x.pages.k && x.pages.v && x.lengths && x.out, "null pointer");
+  BFLY_CHECK_ARG(x.table_width == 0 || x.block_table, "null pointer");
+  BFLY_CHECK_ARG((x.l == nullptr) == (x.m == nullptr), "both l and m or neither");
+  BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.pages.k) && aligned16(x.pages.v) && aligned16(x.out), "pointers must be 16-byte aligned");
+  const int64_t need = bfly_paged_attention_workspace_bytes(x.requests, (int)x.hq, (int)x.hkv, (int)x.head_dim, x.table_width,
+                                                            (int)x.pages.page_size, (int)x.window);
+  BFLY_CHECK_ARG(need == 0 || (x.workspace && x.workspace_bytes >= need && aligned16(x.workspace)), "workspace too small");
   PagedAttnArgs a{};
-  a.q = static_cast<const char*>(q);
-  a.kp = {static_cast<char*>(const_cast<void*>(k_pages)), k_page_stride * es, k_page_head_stride * es, (int)(k_page_row_stride * es)};
-  a.vp = {static_cast<char*>(const_cast<void*>(v_pages)), v_page_stride * es, v_page_head_stride * es, (int)(v_page_row_stride * es)};
-  a.table = block_table; a.lengths = lengths; a.out = out; a.l = l; a.m = m;
-  a.q_req = q_request_stride * es; a.q_head = q_head_stride * es; a.table_stride = table_stride;
-  a.shift = __builtin_ctz(page_size); a.capacity = table_width << a.shift;
-  a.requests = (int)requests; a.num_pages = (int)num_pages; a.hq = hq; a.hkv = hkv; a.window = window; a.scale = scale;
-  a.group = hq / hkv; a.row_tiles = (a.group + 15) / 16; a.rows = a.group < 16 ? a.group : 16;
-  BFLY_CHECK_ARG((int64_t)hkv * a.row_tiles <= 65535, "too many heads");
-  a.units = hkv * a.row_tiles;
-  a.part = static_cast<float*>(workspace);
-  a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * head_dim;
+  a.q = static_cast<const char*>(x.q);
+  a.kp = k_page_ptr(x.pages, es); a.vp = v_page_ptr(x.pages, es);
+  a.table = x.block_table; a.lengths = x.lengths; a.out = x.out; a.l = x.l; a.m = x.m;
+  a.q_req = x.q_request_stride * es; a.q_head = x.q_head_stride * es; a.table_stride = x.table_stride;
+  a.shift = __builtin_ctzll(x.pages.page_size); a.capacity = x.table_width << a.shift;
+  a.requests = (int)x.requests; a.num_pages = (int)x.pages.num_pages; a.hq = (int)x.hq; a.hkv = (int)x.hkv;
+  a.window = (int)x.window; a.scale = (float)x.scale;
+  a.group = a.hq / a.hkv; a.row_tiles = (a.group + 15) / 16; a.rows = a.group < 16 ? a.group : 16;
+  BFLY_CHECK_ARG((int64_t)a.hkv * a.row_tiles <= 65535, "too many heads");
+  a.units = a.hkv * a.row_tiles;
+  a.part = static_cast<float*>(x.workspace);
+  a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * x.head_dim;
   // runs: one for each (request, unit), and as many more as the splits make (plan_run)
-  const int64_t rounds = most_rounds(a.capacity, window, (int)es), pairs = requests * a.units;
+  const int64_t rounds = most_rounds(a.capacity, a.window, (int)es), pairs = x.requests * a.units;
   const bool splits = rounds > kWhole;
   a.whole = !splits;
   const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + kRuns + kSlack;
   const int64_t items = !splits ? pairs : most < some ? most : some;
   BFLY_CHECK_ARG(items <= INT32_MAX, "too many requests and heads");
 #define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)
-  if (dtype == BFLY_DTYPE_BF16) {
-    if (head_dim == 64) BFLY_PAGED(__bf16, 64);
-    else if (head_dim == 128) BFLY_PAGED(__bf16, 128);
+  if (x.dtype == BFLY_DTYPE_BF16) {
+    if (x.head_dim == 64) BFLY_PAGED(__bf16, 64);
+    else if (x.head_dim == 128) BFLY_PAGED(__bf16, 128);
     else BFLY_PAGED(__bf16, 256);
   } else {
-    if (head_dim == 64) BFLY_PAGED(float, 64);
-    else if (head_dim == 128) BFLY_PAGED(float, 128);
+    if (x.head_dim == 64) BFLY_PAGED(float, 64);
+    else if (x.head_dim == 128) BFLY_PAGED(float, 128);
     else BFLY_PAGED(float, 256);
   }
 #undef BFLY_PAGED

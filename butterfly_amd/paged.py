@@ -30,6 +30,8 @@ from . import _native
 from ._device import _GET_DEVICE, stream_of
 from .attention import _dtype_code
 
+_PLAN, _APPEND, _ROPE, _ATTN = (_native.PAGED_STRUCTS["bfly_paged_" + x].pack
+                                for x in ("plan", "append", "rope_append", "attention"))
 PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
 
 # state[1] after a plan that did not fit (include/butterfly_amd_paged.h)
@@ -187,9 +189,10 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
         new_lengths, new_state, starts, ws = torch.empty(5 * b + 6, dtype=i32, device=cuda).split_with_sizes(
             (b, 2, b + 1, 3 * b + 3))
     slots, positions = torch.empty(2, num_rows, dtype=torch.int64, device=cuda).unbind(0)
-    _native.call("bfly_paged_plan", block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(),
-          free_pages.data_ptr(), free_pages.shape[0], state.data_ptr(), page_size, num_rows, rows_each, new_lengths.data_ptr(),
-          new_state.data_ptr(), starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 12 * (b + 1), stream_of(dev))
+    _native.call("bfly_paged_plan", _PLAN(
+        block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(), free_pages.data_ptr(),
+        free_pages.shape[0], state.data_ptr(), page_size, num_rows, rows_each, new_lengths.data_ptr(), new_state.data_ptr(),
+        starts.data_ptr(), slots.data_ptr(), positions.data_ptr(), ws.data_ptr(), 12 * (b + 1)), stream_of(dev))
     return PagedPlan(new_lengths, new_state, starts, slots, positions)
 
 
@@ -226,8 +229,9 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         return
     (k, k0, k1), (v, v0, v1) = _rows(k), _rows(v)
     slots = slots.contiguous()
-    _native.call("bfly_paged_append", k.data_ptr(), v.data_ptr(), code, n, hkv, d, k0, k1, v0, v1, slots.data_ptr(),
-          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides, stream_of(dev))
+    _native.call("bfly_paged_append", _APPEND(
+        k.data_ptr(), v.data_ptr(), code, n, hkv, d, k0, k1, v0, v1, slots.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides), stream_of(dev))
 
 
 def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -272,7 +276,7 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
         raise ValueError("cos and sin must be float32 [rows, r] tables of one shape")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("give both norm weights or neither")
-    qw = kw = None
+    qw = kw = 0
     if q_weight is not None:
         if q_weight.shape != (d,) or k_weight.shape != (d,) or not q_weight.dtype is k_weight.dtype is dtype:
             raise ValueError("norm weights must be [d] of the rows' type")
@@ -285,9 +289,10 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
         return out
     (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
     slots, positions, cos, sin = slots.contiguous(), positions.contiguous(), _flat(cos), _flat(sin)
-    _native.call("bfly_paged_rope_append", q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1,
-          qw, kw, eps, cos.data_ptr(), sin.data_ptr(), table[0], table[1], positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
-          k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides, stream_of(dev))
+    _native.call("bfly_paged_rope_append", _ROPE(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1, qw, kw, eps, cos.data_ptr(),
+        sin.data_ptr(), table[0], table[1], positions.data_ptr(), slots.data_ptr(), out.data_ptr(),
+        k_pages.data_ptr(), v_pages.data_ptr(), shape[0], shape[2], *strides), stream_of(dev))
     return out
 
 
@@ -334,7 +339,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError("window must be 0 (everything) or a number of tokens")
     cuda = q.device
     out = torch.empty(sq, dtype=dtype, device=cuda)
-    l = m = lp = mp = ws = None
+    l = m = ws = None
+    lp = mp = 0
     if return_stats:
         l, m = torch.empty(2, b, hq, 1, 1, dtype=torch.float32, device=cuda).unbind(0)
         lp, mp = l.data_ptr(), m.data_ptr()
@@ -347,10 +353,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         need = _workspace_bytes(b, hq, hkv, d, width, page_size, window)
         if need:
             ws = torch.empty(need, dtype=torch.uint8, device=cuda)
-        _native.call("bfly_paged_attention", q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages,
-              page_size, *strides, block_table.data_ptr(), width, stride, lengths.data_ptr(), window,
-              1.0 / math.sqrt(d) if scale is None else scale, out.data_ptr(), lp, mp, None if ws is None else ws.data_ptr(), need,
-                     stream_of(dev))
+        _native.call("bfly_paged_attention", _ATTN(
+            q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, *strides,
+            block_table.data_ptr(), width, stride, lengths.data_ptr(), window, 1.0 / math.sqrt(d) if scale is None else scale,
+            out.data_ptr(), lp, mp, 0 if ws is None else ws.data_ptr(), need), stream_of(dev))
     return (out, l, m) if return_stats else out
 
 

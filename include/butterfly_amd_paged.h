@@ -8,6 +8,8 @@
  *
  * Conventions are those of butterfly_amd.h (caller-owned device pointers, work enqueued on `stream`,
  * nothing allocates or synchronises, 0 or a negative BFLY_ERR_*), and:
+ *   - arguments come in one struct a call, every member eight bytes wide (a caller in another language
+ *     packs them in order).
  *   - pages are [num_pages, hkv, page_size, head_dim] with strides (in elements) of their own for page,
  *     head and row; head_dim is contiguous.  Base addresses are 16-byte aligned, strides multiples of
  *     16 bytes.  page_size is a power of two from 16 to 1024.
@@ -25,6 +27,15 @@
 #ifdef __cplusplus
 extern "C" {
 #endif
+
+typedef struct bfly_pages {
+  void* k;
+  void* v;
+  int64_t num_pages;
+  int64_t page_size;
+  int64_t k_page_stride, k_head_stride, k_row_stride;
+  int64_t v_page_stride, v_head_stride, v_row_stride;
+} bfly_pages_t;
 
 /* Error codes of state[1] (bfly_paged_plan); the lowest that applies is kept. */
 #define BFLY_PAGED_BAD_LENGTH 1 /* a length that is negative or beyond its table row */
@@ -53,23 +64,39 @@ extern "C" {
  *   - workspace: (requests + 1) * 12 bytes, 4-byte aligned.
  * The tensors do not overlap otherwise.  requests at most 2^24; num_rows and free_capacity below 2^31.
  */
-int bfly_paged_plan(int32_t* block_table, int64_t requests, int64_t table_width, int64_t table_stride,
-                    const int32_t* lengths, const int32_t* counts, int32_t* free_pages, int64_t free_capacity,
-                    const int32_t* state, int page_size, int64_t num_rows, int64_t rows_each, int32_t* lengths_out,
-                    int32_t* state_out, int32_t* starts, int64_t* slots, int64_t* positions, void* workspace,
-                    int64_t workspace_bytes, hipStream_t stream);
+typedef struct bfly_paged_plan_args {
+  int32_t* block_table;
+  int64_t requests, table_width, table_stride;
+  const int32_t* lengths;
+  const int32_t* counts;
+  int32_t* free_pages;
+  int64_t free_capacity;
+  const int32_t* state;
+  int64_t page_size, num_rows, rows_each;
+  int32_t* lengths_out;
+  int32_t* state_out;
+  int32_t* starts;
+  int64_t* slots;
+  int64_t* positions;
+  void* workspace;
+  int64_t workspace_bytes;
+} bfly_paged_plan_args_t;
+int bfly_paged_plan(const bfly_paged_plan_args_t* args, hipStream_t stream);
 
 /*
  * Device: rows k, v [rows, hkv, head_dim] (row and head strides in elements, multiples of 16 bytes) into
  * their slots.  A row whose slot is negative or beyond the pages is passed over.  Of two rows with one
  * slot it is not defined which stays, element by element.  Any head_dim of whole 16-byte pieces.
  */
-int bfly_paged_append(const void* k, const void* v, int dtype, int64_t rows, int hkv, int head_dim,
-                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                      const int64_t* slots, void* k_pages, void* v_pages, int64_t num_pages, int page_size,
-                      int64_t k_page_stride, int64_t k_page_head_stride, int64_t k_page_row_stride,
-                      int64_t v_page_stride, int64_t v_page_head_stride, int64_t v_page_row_stride,
-                      hipStream_t stream);
+typedef struct bfly_paged_append_args {
+  const void* k;
+  const void* v;
+  int64_t dtype, rows, hkv, head_dim;
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  const int64_t* slots;
+  bfly_pages_t pages;
+} bfly_paged_append_args_t;
+int bfly_paged_append(const bfly_paged_append_args_t* args, hipStream_t stream);
 
 /*
  * Device: bfly_paged_append for a decoder's projection rows, with the per-head RMSNorm of q and k (weights
@@ -79,15 +106,24 @@ int bfly_paged_append(const void* k, const void* v, int dtype, int64_t rows, int
  * the inputs to the one rounding of each output.  A position outside the table gives NaN in q_out and in k.
  * head_dim 64, 128 or 256; rotary_dim a multiple of 16, at most head_dim.
  */
-int bfly_paged_rope_append(const void* q, const void* k, const void* v, int dtype, int64_t rows, int hq, int hkv,
-                           int head_dim, int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,
-                           int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
-                           const void* q_weight, const void* k_weight, float eps, const float* cos,
-                           const float* sin, int64_t table_rows, int rotary_dim, const int64_t* positions,
-                           const int64_t* slots, void* q_out, void* k_pages, void* v_pages, int64_t num_pages,
-                           int page_size, int64_t k_page_stride, int64_t k_page_head_stride,
-                           int64_t k_page_row_stride, int64_t v_page_stride, int64_t v_page_head_stride,
-                           int64_t v_page_row_stride, hipStream_t stream);
+typedef struct bfly_paged_rope_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t dtype, rows, hq, hkv, head_dim;
+  int64_t q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  const void* q_weight;
+  const void* k_weight;
+  double eps;
+  const float* cos;
+  const float* sin;
+  int64_t table_rows, rotary_dim;
+  const int64_t* positions;
+  const int64_t* slots;
+  void* q_out;
+  bfly_pages_t pages;
+} bfly_paged_rope_append_args_t;
+int bfly_paged_rope_append(const bfly_paged_rope_append_args_t* args, hipStream_t stream);
 
 /*
  * Device: one new token of every request over its pages.  q [requests, hq, head_dim] with request and head
@@ -102,13 +138,23 @@ int bfly_paged_rope_append(const void* q, const void* k, const void* v, int dtyp
  */
 int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim, int64_t table_width,
                                              int page_size, int window);
-int bfly_paged_attention(const void* q, int dtype, int64_t requests, int hq, int hkv, int head_dim,
-                         int64_t q_request_stride, int64_t q_head_stride, const void* k_pages, const void* v_pages,
-                         int64_t num_pages, int page_size, int64_t k_page_stride, int64_t k_page_head_stride,
-                         int64_t k_page_row_stride, int64_t v_page_stride, int64_t v_page_head_stride,
-                         int64_t v_page_row_stride, const int32_t* block_table, int64_t table_width,
-                         int64_t table_stride, const int32_t* lengths, int window, float scale, void* out, float* l,
-                         float* m, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+typedef struct bfly_paged_attention_args {
+  const void* q;
+  int64_t dtype, requests, hq, hkv, head_dim;
+  int64_t q_request_stride, q_head_stride;
+  bfly_pages_t pages;
+  const int32_t* block_table;
+  int64_t table_width, table_stride;
+  const int32_t* lengths;
+  int64_t window;
+  double scale;
+  void* out;
+  float* l;
+  float* m;
+  void* workspace;
+  int64_t workspace_bytes;
+} bfly_paged_attention_args_t;
+int bfly_paged_attention(const bfly_paged_attention_args_t* args, hipStream_t stream);
 
 #ifdef __cplusplus
 }
