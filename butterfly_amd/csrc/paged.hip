@@ -486,6 +486,7 @@ extern "C" int bfly_paged_rope_append(const bfly_paged_rope_append_args_t* args,
   const bool many = x.rows * heads >= kManyHeads;
   a.items = (unsigned)(x.rows * (many ? (heads + 3) / 4 : heads));
   const int64_t lanes = x.head_dim * es / 16, blocks = (a.items * lanes + 255) / 256;
+  BFLY_CHECK_ARG(blocks < (1 << 24), "too many rows");       // a grid holds fewer than 2^32 threads
   const dim3 grid((unsigned)blocks), block(256);
 #define BFLY_ROPE(T, D)                                                                                \
   do {                                                                                                 \

@@ -6,24 +6,39 @@
 // Work: a request's tiles (32 keys in bf16, 16 in fp32) go in rounds of four, one for each wave of a
 // workgroup, and its rounds in runs of at most c, c such that all requests and heads together make about
 // kRuns runs.  A workgroup takes one run of one kv head for up to 16 of its query heads; every workgroup finds
-// its run from the lengths by itself (plan_run), so the grid needs no host knowledge of them.  Requests with
-// one run write their output, the others a partial (fp32 sums, m, l) that paged_merge_kernel joins.
+// its run from the lengths by itself (plan_run), so the grid needs no host knowledge of them and a long request
+// among short ones is split as far as a lone one.  Requests with one run write their output, the others a
+// partial (fp32 sums, m, l) that paged_merge_kernel joins.
 //
 // A wave takes every fourth tile of the run, by itself: no barrier and no LDS until its sums meet the
-// other waves'.  S^T = K Q^T and O^T += V^T P^T on the matrix cores, query heads as columns, so a
-// lane's scores are the operand of the second product as they come:
+// other waves'.  S^T = K Q^T and O^T += V^T P^T on the matrix cores (v_mfma_f32_16x16x32_bf16, or
+// v_mfma_f32_16x16x4_f32), query heads as columns, so a lane's scores are the operand of the second product as
+// they come:
 //   * K rows go from memory into the first product's operand registers (lane = key, 16 bytes of d a load).
 //   * V rows too (16 lanes take a row, a lane 4 (or 8) keys of one piece of d): the d of an output row is
 //     chosen so that the operand is the lane's own words, which v_perm_b32 pairs up by key.
-//   * The next tile's K is requested when this one's scores are done, its V after the second product.
+//   * The next tile's K is requested when this one's scores are done, its V after the second product: a wave
+//     has 8 to 32 KB under way.
+// Rows that hold no token the request sees (behind the last one, before the window) are read with their tile; their
+// scores become -inf and their V zero, whatever they hold.
+//
+// Bound by HBM: keys and values are read once (4 hq / (2 hkv size) flops a byte, 4 to 32 here, against some 250 that
+// the card's product and copy rates take).  Kernel times: 1.36 GB of 32 requests of up to 131072 tokens 209 us
+// (6.5 TB/s; a large copy on this card moves 4.96), 262144 tokens of d 256 161 us (6.7); 32768 tokens of one
+// request 15.5 us, of which some 3 us are four dependent reads (arguments, lengths, page, K) and the sums' way
+// through LDS, and 3.9 us for the join.
 #include "paged.h"
 
 namespace bfly {
 
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
+// Whole calls, us, with 256 / 512 / 1024 runs: one request of 32768 tokens 21.6 / 22.0 / 22.1, 131072 tokens x 32 247 /
+// 248 / 247, 262144 tokens of d 256 193 / 196 / 199, 64 of up to 2000 tokens with 32/8 heads 39.8 / 43.6 / 40.6.
+// c at least 1 / 2: one request of 1024 tokens 9.9 / 11.4.  Single runs of up to 4 / 8 rounds (c at least 2): 11.4 / 14.8.
+// Workgroups of 4 / 8 waves: 64 of up to 2000 tokens 39.8 / 46.9, one of 32768 21.6 / 21.6.
 constexpr int kRuns = 256;            // runs in all, where the requests and heads leave that many: one for each CU
 constexpr int kMinRun = 1;            // c at least
-constexpr int kWhole = 4;             // rounds that stay one run: 512 keys are done before a join of two runs
+constexpr int kWhole = 4;             // rounds that stay one run: 512 keys (bf16) are done before a join of two runs
 // A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
 // c >= total / kRuns, fewer than 2 kRuns: the partials there can be.  (kSlack: the total is a sum of floats.)
 constexpr int kSlack = 64;
@@ -201,6 +216,15 @@ __device__ __forceinline__ uint32_t finite_bf16(uint32_t w) {
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
+// V rows are read once, whole lines an instruction, past the caches' replacement: the K half-lines of two
+// neighbouring instructions then stay until both have been taken.  Measured, V past the caches / nothing / K and V,
+// us: 131072 tokens x 32 227 / 247 / 246, 262144 tokens of d 256 175 / 193 / 172, 64 requests of 4096 tokens 175 / 194 /
+// 177, one of 1024 (in the caches) 10.3 / 9.9 / 10.6.
+template <typename V>
+__device__ __forceinline__ V stream_load(const char* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+
 // One wave's sums over its tiles.  acc[i][r] of lane (n = lane & 15, g = lane >> 4): query row n, element
 // d_of(i, g, r).
 template <typename T, int D>
@@ -248,11 +272,11 @@ struct Sweep<__bf16, D> {
       for (int h = 0; h < H; ++h) {
         const char* p = base[j >> 2] + (uint32_t)((4 * g + (j & 3)) * row_bytes + 4 * W * n) + 256 * h;
         if constexpr (W == 4) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+          const u32x4 x = stream_load<u32x4>(p);
 #pragma unroll
           for (int w = 0; w < 4; ++w) v[j][h][w] = x[w];
         } else {
-          const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+          const u32x2 x = stream_load<u32x2>(p);
           v[j][h][0] = x[0];
           v[j][h][1] = x[1];
         }
@@ -278,7 +302,8 @@ struct Sweep<__bf16, D> {
       for (int w = 0; w < W; ++w) v[j][h][w] = 0;
   }
   // The weights enter as two bf16 parts, 16 bits of them: with one part (8 bits) a weight would be off by
-  // as much as the output's own rounding.  kSafe: the second part skips V's infinities and NaN, which the
+  // as much as the output's own rounding, and the second part hides behind the loads (131072 tokens x 32: 249 us
+  // with it, 246 without).  kSafe: the second part skips V's infinities and NaN, which the
   // first one has carried into the sums already (p * inf is inf, but the rest of p may be 0).
   template <bool kSafe>
   __device__ __forceinline__ void add(const float (&p)[8]) {
@@ -341,7 +366,7 @@ struct Sweep<float, D> {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int h = 0; h < H; ++h)
-        v[j][h] = *reinterpret_cast<const f32x4*>(base[0] + (uint32_t)((4 * g + j) * row_bytes + 16 * n) + 256 * h);
+        v[j][h] = stream_load<f32x4>(base[0] + (uint32_t)((4 * g + j) * row_bytes + 16 * n) + 256 * h);
   }
   __device__ __forceinline__ void scores(float (&s)[4], float scale) const {
     f32x4 c[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -651,7 +676,8 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   if (rc != BFLY_OK) return rc;
   BFLY_CHECK_ARG(x.window >= 0 && x.window <= INT32_MAX, "bad window");
   BFLY_CHECK_ARG(x.table_width >= 0 && x.table_width <= INT32_MAX && (x.requests <= 1 || x.table_stride >= 0), "bad block table shape");
-  BFLY_CHECK_ARG(x.q_request_stride >= 0 && x.q_head_stride >= 0 && x.q_request_stride * es % 16 == 0 && x.q_head_stride * es % 16 == 0,
+  BFLY_CHECK_ARG(x.q_request_stride >= 0 && x.q_head_stride >= 0 && x.q_request_stride < ((int64_t)1 << 48) &&
+                     x.q_head_stride < ((int64_t)1 << 48) && x.q_request_stride * es % 16 == 0 && x.q_head_stride * es % 16 == 0,
                  "q strides must be multiples of 16 bytes");
   if (x.requests == 0) return BFLY_OK;
   BFLY_CHECK_ARG(x.q && x.pages.k && x.pages.v && x.lengths && x.out, "null pointer");
@@ -680,7 +706,7 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   a.whole = !splits;
   const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + kRuns + kSlack;
   const int64_t items = !splits ? pairs : most < some ? most : some;
-  BFLY_CHECK_ARG(items <= INT32_MAX, "too many requests and heads");
+  BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads
 #define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)
   if (x.dtype == BFLY_DTYPE_BF16) {
     if (x.head_dim == 64) BFLY_PAGED(__bf16, 64);

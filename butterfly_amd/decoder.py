@@ -1024,6 +1024,8 @@ class Decoder(nn.Module):
                              "each layer of the model")
         if not _hip(self.embed_tokens) or not all(isinstance(layer.self_attn, Attention) for layer in self.layers):
             raise ValueError("greedy_requests needs a bf16 model on the GPU whose layers all have stock attention")
+        if bool(cache.lengths.any()):
+            raise ValueError("greedy_requests starts from an empty cache (release the requests it holds)")
         if new_tokens <= 0:
             return torch.empty(b, 0, dtype=torch.long, device=dev)
         first = []

@@ -22,7 +22,8 @@ from __future__ import annotations
 
 import math
 from functools import lru_cache
-from typing import NamedTuple, Optional
+from operator import index
+from typing import Iterable, NamedTuple, Optional
 
 import torch
 
@@ -174,7 +175,7 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
         raise ValueError("block_table's rows must not overlap")
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
-    if rows_each and num_rows != b * rows_each:
+    if rows_each < 0 or rows_each and num_rows != b * rows_each:
         raise ValueError(f"num_rows must be the {b} requests' {rows_each} rows each")
     if not (lengths.is_contiguous() and counts.is_contiguous() and state.is_contiguous() and free_pages.is_contiguous()):
         if not free_pages.is_contiguous() or in_place and not (lengths.is_contiguous() and state.is_contiguous()):
@@ -213,7 +214,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     """Rows ``k``, ``v`` [N, Hkv, d] (any strides) into their ``slots`` (int64 [N]) of the pages
     [num_pages, Hkv, page_size, d], one launch of ``bfly_paged_append``.  A row whose slot is negative or
     beyond the pages is passed over.  The slots of a call are distinct, as a plan gives them (of two rows
-    with one slot it is not defined which stays).  float32 or bfloat16; ``d`` of whole 16-byte pieces."""
+    with one slot it is not defined which stays), and the rows are not themselves among the slots' rows.
+    float32 or bfloat16; ``d`` of whole 16-byte pieces."""
     dev = _device_of(slots)
     if dev != _GET_DEVICE():
         with torch.cuda.device(dev):
@@ -335,6 +337,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"query heads {hq} must be a multiple of kv heads {hkv}")
     stride, width = _table_stride(block_table, b), block_table.shape[1]
     _check_ints(lengths, "lengths", torch.int32, b)
+    window = index(window)
     if not 0 <= window < 1 << 31:
         raise ValueError("window must be 0 (everything) or a number of tokens")
     cuda = q.device
@@ -397,7 +400,7 @@ class PagedLayer:
         """The first ``tokens`` keys and values of every request as dense [B, Hkv, tokens, d] tensors (what a
         prompt's further part attends to); every request holds that many."""
         size = self.k_pages.shape[2]
-        ids = self.cache.block_table[:, :-(-tokens // size)].long()
+        ids = self.cache.block_table[:, :-(-tokens // size)].long().clamp_(0, self.k_pages.shape[0] - 1)
         return tuple(x[ids].transpose(1, 2).flatten(2, 3)[:, :, :tokens] for x in (self.k_pages, self.v_pages))
 
 
@@ -450,14 +453,17 @@ class PagedKVCache:
         """A step whose rows follow each other, request by request: ragged prompts."""
         return self._begin(counts, num_rows, 0, 0)
 
-    def release(self, requests) -> None:
+    def release(self, requests: Iterable[int]) -> None:
         """The given requests (indices) leave: their pages go back to the free list."""
-        counts = torch.zeros_like(self.lengths)
-        counts[torch.as_tensor(requests, dtype=torch.long, device=counts.device)] = -(2 ** 31 - 1)
-        self._begin(counts, 0, 0, 0)
+        counts = [0] * self.max_requests
+        for r in requests:
+            if not 0 <= r < self.max_requests:
+                raise ValueError(f"request {r} is not one of {self.max_requests}")
+            counts[r] = -(2 ** 31 - 1)
+        self._begin(torch.tensor(counts, dtype=torch.int32, device=self.lengths.device), 0, 0, 0)
 
     def sync(self) -> int:
-        """Waits for the device; the number of free pages.  Raises ``RuntimeError`` if a step did not fit (that
+        """Waits for the current stream; the number of free pages.  Raises ``RuntimeError`` if a step did not fit (that
         step and all after it changed nothing), and clears the error."""
         free, error = self.state.tolist()
         if error:

@@ -282,6 +282,8 @@ def test_attention_refusals():
             bf.paged_attention(*a.values())
     with pytest.raises(ValueError):
         bf.paged_attention(q, kp, vp, table, lens, window=-1)
+    with pytest.raises(TypeError):
+        bf.paged_attention(q, kp, vp, table, lens, window=3.5)
     with pytest.raises(ValueError, match="inference"):
         bf.paged_attention(q.clone().requires_grad_(), kp, vp, table, lens)
     wide = torch.zeros(3, 2, 16, 96, dtype=BF, device="cuda")
@@ -703,3 +705,27 @@ def test_plan_with_rows_of_its_own_for_every_request(b, each):
     assert over.state.tolist() == [int(state[0]), 3] and bool((over.slots == -1).all()) and torch.equal(over.lengths, _i32(lens))
     with pytest.raises(ValueError, match="rows"):
         bf.paged_plan(t2, _i32(lens), _i32(counts), free2, state, page_size=page, num_rows=b * each + 1, rows_each=each)
+
+
+def test_two_captured_attentions_replayed_at_once():
+    """Each capture has a workspace of its own: replays on two streams at once give each its own result."""
+    q, kp, vp, table, lens, _ = _paged_case([9000, 300, 7000], 8, 2, 128, 64, BF)
+    qs = [q, q.flip(0).contiguous()]
+    want = [bf.paged_attention(x, kp, vp, table, lens) for x in qs]
+    streams, graphs, outs = [torch.cuda.Stream() for _ in qs], [], []
+    torch.cuda.synchronize()
+    for x, s in zip(qs, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s), torch.cuda.graph(g, stream=s):
+            outs.append(bf.paged_attention(x, kp, vp, table, lens))
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))

@@ -120,7 +120,13 @@ def test_requests_of_different_lengths_decode_as_each_alone(head_dim):
     pool.release([0, 2])
     assert pool.lengths.tolist() == [0, 33 + 49, 0, 64 + 49]
     assert pool.sync() == 40 - 3 - 4
-    pool.release([1, 3])
+    with pytest.raises(ValueError, match="empty"):
+        model.greedy_requests(prompts, 50, pool)
+    for bad in ([4], [-1]):
+        with pytest.raises(ValueError):
+            pool.release(bad)
+    pool.release([])
+    pool.release([1, 3, 1])
     again = model.greedy_requests(prompts, 50, pool)
     assert torch.equal(out, again)
 

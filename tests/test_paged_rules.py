@@ -71,6 +71,11 @@ INVALID, UNSUPPORTED = _native.ERR_INVALID, _native.ERR_UNSUPPORTED
     ("bfly_paged_rope_append", dict(hq=3), INVALID, b"head counts"),
     ("bfly_paged_rope_append", dict(cos=I + 4), INVALID, b"aligned"),
     ("bfly_paged_rope_append", dict(pos=None), INVALID, b"null"),
+    ("bfly_paged_rope_append", dict(rows=1 << 27), INVALID, b"too many"),
+    ("bfly_paged_append", dict(rows=1 << 27), INVALID, b"too many"),
+    ("bfly_paged_attention", dict(requests=65536), INVALID, b"65535"),
+    ("bfly_paged_attention", dict(requests=65535, hq=512, hkv=512), INVALID, b"too many"),
+    ("bfly_paged_attention", dict(ws_bytes=100, width=1000), INVALID, b"workspace"),
     ("bfly_paged_attention", dict(d=80), UNSUPPORTED, b"head_dim"),
     ("bfly_paged_attention", dict(hq=5), INVALID, b"head counts"),
     ("bfly_paged_attention", dict(window=-1), INVALID, b"window"),
