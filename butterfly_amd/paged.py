@@ -29,10 +29,10 @@ import torch
 
 from . import _native
 from ._device import _GET_DEVICE, stream_of
-from .attention import _dtype_code
 
 _PLAN, _APPEND, _ROPE, _ATTN = (_native.PAGED_STRUCTS["bfly_paged_" + x].pack
                                 for x in ("plan", "append", "rope_append", "attention"))
+_EMPTY = torch.empty_strided     # (0.95 us a call; torch.empty, which also sorts out layouts, 1.8)
 PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
 
 # state[1] after a plan that did not fit (include/butterfly_amd_paged.h)
@@ -72,8 +72,16 @@ def _other_device() -> None:
     raise ValueError("all tensors must be GPU tensors of one device")
 
 
+def _dtype_code(dtype: torch.dtype) -> int:
+    if dtype is torch.bfloat16:
+        return _native.DTYPE_BF16
+    if dtype is torch.float32:
+        return _native.DTYPE_F32
+    raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+
+
 def _check_ints(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> None:
-    if t.dim() != 1 or t.dtype != dtype or t.shape[0] != n:
+    if t.dtype is not dtype or t.shape != (n,):
         raise ValueError(f"{name} must be a 1-D {dtype} tensor of {n}")
 
 
@@ -185,11 +193,11 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     # one allocation for the int32 results and the kernel's workspace, one for the rows
     if in_place:
         new_lengths, new_state = lengths, state
-        starts, ws = torch.empty(4 * b + 4, dtype=i32, device=cuda).split_with_sizes((b + 1, 3 * b + 3))
+        starts, ws = _EMPTY((4 * b + 4,), (1,), dtype=i32, device=cuda).split_with_sizes((b + 1, 3 * b + 3))
     else:
-        new_lengths, new_state, starts, ws = torch.empty(5 * b + 6, dtype=i32, device=cuda).split_with_sizes(
+        new_lengths, new_state, starts, ws = _EMPTY((5 * b + 6,), (1,), dtype=i32, device=cuda).split_with_sizes(
             (b, 2, b + 1, 3 * b + 3))
-    slots, positions = torch.empty(2, num_rows, dtype=torch.int64, device=cuda).unbind(0)
+    slots, positions = _EMPTY((2, num_rows), (num_rows, 1), dtype=torch.int64, device=cuda).unbind(0)
     _native.call("bfly_paged_plan", _PLAN(
         block_table.data_ptr(), b, width, stride, lengths.data_ptr(), counts.data_ptr(), free_pages.data_ptr(),
         free_pages.shape[0], state.data_ptr(), page_size, num_rows, rows_each, new_lengths.data_ptr(), new_state.data_ptr(),
@@ -224,7 +232,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
         raise ValueError(_GRAD)
     shape, strides = _pages(k_pages, v_pages, dev, True)
     n, hkv, d = _check_rows(k, v, shape, k_pages.dtype, slots, dev)
-    code = _dtype_code(k)
+    code = _dtype_code(k_pages.dtype)
     if d % (4 if code == _native.DTYPE_F32 else 8):
         raise ValueError("head_dim must be whole 16-byte pieces")
     if n == 0:
@@ -269,7 +277,7 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     sq = q.shape
     if len(sq) != 3 or sq[0] != n or sq[2] != d or q.dtype is not dtype:
         raise ValueError("q must be [N, Hq, d] rows of k's type")
-    hq, code = sq[1], _dtype_code(q)
+    hq, code = sq[1], _dtype_code(dtype)
     if hq == 0 or hq % hkv:
         raise ValueError(f"query heads {hq} must be a multiple of kv heads {hkv}")
     _check_ints(positions, "positions", torch.int64, n)
@@ -286,10 +294,15 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
             _other_device()
         q_weight, k_weight = _flat(q_weight), _flat(k_weight)
         qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
-    out = torch.empty(sq, dtype=dtype, device=q.device)
+    out = _EMPTY(sq, (hq * d, d, 1), dtype=dtype, device=q.device)
     if n == 0:
         return out
-    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
+    q0, q1, q2 = q.stride()
+    k0, k1, k2 = k.stride()
+    v0, v1, v2 = v.stride()
+    if not q2 == k2 == v2 == 1 or (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 \
+            or (q0 | q1 | k0 | k1 | v0 | v1) & (7 if code else 3):
+        (q, q0, q1), (k, k0, k1), (v, v0, v1) = _rows(q), _rows(k), _rows(v)
     slots, positions, cos, sin = slots.contiguous(), positions.contiguous(), _flat(cos), _flat(sin)
     _native.call("bfly_paged_rope_append", _ROPE(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), code, n, hq, hkv, d, q0, q1, k0, k1, v0, v1, qw, kw, eps, cos.data_ptr(),
@@ -332,7 +345,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     sq, dtype = q.shape, q.dtype
     if len(sq) != 4 or sq[2] != 1 or sq[3] != d or dtype is not k_pages.dtype:
         raise ValueError("q must be [B, Hq, 1, d] of the pages' type")
-    b, hq, code = sq[0], sq[1], _dtype_code(q)
+    b, hq, code = sq[0], sq[1], _dtype_code(dtype)
     if hq == 0 or hq % hkv:
         raise ValueError(f"query heads {hq} must be a multiple of kv heads {hkv}")
     stride, width = _table_stride(block_table, b), block_table.shape[1]
@@ -341,11 +354,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if not 0 <= window < 1 << 31:
         raise ValueError("window must be 0 (everything) or a number of tokens")
     cuda = q.device
-    out = torch.empty(sq, dtype=dtype, device=cuda)
+    out = _EMPTY(sq, (hq * d, d, d, 1), dtype=dtype, device=cuda)
     l = m = ws = None
     lp = mp = 0
     if return_stats:
-        l, m = torch.empty(2, b, hq, 1, 1, dtype=torch.float32, device=cuda).unbind(0)
+        l, m = _EMPTY((2, b, hq, 1, 1), (b * hq, hq, 1, 1, 1), dtype=torch.float32, device=cuda).unbind(0)
         lp, mp = l.data_ptr(), m.data_ptr()
     if b:
         q0, q1, _, q3 = q.stride()
@@ -355,7 +368,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         lengths = lengths.contiguous()
         need = _workspace_bytes(b, hq, hkv, d, width, page_size, window)
         if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=cuda)
+            ws = _EMPTY((need,), (1,), dtype=torch.uint8, device=cuda)
         _native.call("bfly_paged_attention", _ATTN(
             q.data_ptr(), code, b, hq, hkv, d, q0, q1, k_pages.data_ptr(), v_pages.data_ptr(), pages, page_size, *strides,
             block_table.data_ptr(), width, stride, lengths.data_ptr(), window, 1.0 / math.sqrt(d) if scale is None else scale,
