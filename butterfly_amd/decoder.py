@@ -311,11 +311,11 @@ def _followed(x: torch.Tensor, weight: torch.Tensor) -> bool:
                 and any(type(m) is not DeviceContext for m in _get_current_function_mode_stack())))
 
 
-def _hooked(layer: nn.Module) -> bool:
-    """Whether calling ``layer`` runs more than ``QuantLinear.forward``: hooks of its own or of all modules, another
+def _hooked(layer: nn.Module, plain: type = QuantLinear) -> bool:
+    """Whether calling ``layer`` runs more than ``plain.forward``: hooks of its own or of all modules, another
     class or a forward set on the instance."""
     m = torch.nn.modules.module
-    return (type(layer) is not QuantLinear or "forward" in layer.__dict__
+    return (type(layer) is not plain or "forward" in layer.__dict__
             or bool(layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks
                     or layer._backward_pre_hooks or m._global_forward_hooks or m._global_forward_pre_hooks
                     or m._global_backward_hooks or m._global_backward_pre_hooks))
@@ -666,11 +666,8 @@ class Attention(nn.Module):
         attention over what the pages hold and the part itself."""
         b, t, _ = x.shape
         c = self.cfg
-        if t == 1 and isinstance(rope, RopeTable) and _hip(x):
-            q, k, v = self.qkv(x).view(b, -1, c.head_dim).split((c.num_heads, c.num_kv_heads, c.num_kv_heads), 1)
-            q = cache.rope_append(q, k, v, rope.cos_tab, rope.sin_tab, q_weight=self.q_norm.weight,
-                                  k_weight=self.k_norm.weight, eps=self.q_norm.eps)
-            return self.output(cache.attend(q.unsqueeze(2), scale=self.scale))
+        if self.takes_paged_rows(x, cache, rope):
+            return self.forward_paged_rows(self.qkv(x), cache, rope)
         start = cache.cache.start
         q, k, v = self.project(x, torch.arange(start, start + t, device=x.device), rope)
         cache.append(k.transpose(1, 2).reshape(b * t, *k.shape[1::2]), v.transpose(1, 2).reshape(b * t, *v.shape[1::2]))
@@ -679,6 +676,20 @@ class Attention(nn.Module):
         if start:
             k, v = (torch.cat(x, 2) for x in zip(cache.history(start), (k, v)))
         return self.output(self._dense(q, k, v))
+
+    @staticmethod
+    def takes_paged_rows(x: torch.Tensor, cache, rope) -> bool:
+        """Whether this call is one token of every request over pages, fed with the raw q|k|v rows."""
+        return isinstance(cache, PagedLayer) and isinstance(rope, RopeTable) and x.shape[1] == 1 and _hip(x)
+
+    def forward_paged_rows(self, qkv: torch.Tensor, cache: PagedLayer, rope: "RopeTable") -> torch.Tensor:
+        """The paged step from the fused projection's raw output rows (``takes_paged_rows`` held), through the
+        output projection."""
+        c = self.cfg
+        q, k, v = qkv.view(qkv.shape[0], -1, c.head_dim).split((c.num_heads, c.num_kv_heads, c.num_kv_heads), 1)
+        q = cache.rope_append(q, k, v, rope.cos_tab, rope.sin_tab, q_weight=self.q_norm.weight,
+                              k_weight=self.k_norm.weight, eps=self.q_norm.eps)
+        return self.output(cache.attend(q.unsqueeze(2), scale=self.scale))
 
 
 class ButterflyAttention(QwenButterflyAttention):
@@ -814,6 +825,10 @@ class DecoderLayer(nn.Module):
                 h, s = add_rms_norm_q4_gemv_silu_parts(x, parts, post.weight, post.eps, mlp.gate_up)
                 return h, mlp.down_proj(s)
             a = attn.forward_qkv_row(qkv, cache, rope)
+        elif (isinstance(cache, PagedLayer) and not _hooked(attn, Attention) and attn.takes_paged_rows(x, cache, rope)
+              and norm_q4_fits(x, attn.qkv) and not _hooked(attn.qkv)):
+            x, qkv = add_rms_norm_q4_gemv(x, pending, ln.weight, ln.eps, attn.qkv)
+            a = attn.forward_paged_rows(qkv, cache, rope)
         else:
             x, n = add_rms_norm(x, pending, ln.weight, ln.eps)
             a = attn(n, cache=cache, position_embeddings=rope)

@@ -170,3 +170,20 @@ def test_running_out_of_pages_is_reported():
     for kw in (dict(page=48), dict(pages=0), dict(max_tokens=0), dict(dtype=torch.float16)):
         with pytest.raises(ValueError):
             _cache(cfg, 2, **kw)
+
+
+def test_one_request_rides_its_norm_in_the_projection_and_hooks_are_seen():
+    """hidden 2048: the step's input norm rides in the q|k|v product's launch (bit-identical to the two); a hook on the
+    attention or its projection takes the separate calls, and runs."""
+    cfg = DecoderConfig(vocab_size=1024, hidden_size=2048, num_layers=2, num_heads=16, num_kv_heads=4, head_dim=128,
+                        intermediate_size=1024)
+    model = Decoder(cfg, seed=4)
+    prompt = torch.randint(0, cfg.vocab_size, (1, 70), generator=torch.Generator().manual_seed(3)).cuda()
+    want = model.greedy_graph(prompt, 20, _cache(cfg, 1).layers)
+    for module in (model.layers[0].self_attn, model.layers[1].self_attn.qkv):
+        seen = []
+        hook = module.register_forward_hook(lambda *a: seen.append(1))
+        got = model.greedy(prompt, 20, _cache(cfg, 1).layers)
+        hook.remove()
+        assert len(seen) == 20 and torch.equal(got, want)
+    assert torch.equal(model.greedy(prompt, 20, _cache(cfg, 1).layers), want)
