@@ -955,7 +955,7 @@ class Decoder(nn.Module):
                 raise ValueError(
                     f"greedy_graph: layer {i} cannot run its decode step as one device launch (it needs a swapped "
                     f"layer over a CompressedKVCache, an attention window of at most 64 tokens and a routed row "
-                    f"of at most 16 blocks); use greedy() for this configuration")
+                    f"of at most 16 blocks, or a dense layer over a PagedLayer); use greedy() for this configuration")
         compressed = [c for c in caches if isinstance(c, CompressedKVCache)]
         pools = self._paged_pools(caches, b)
         for c in compressed:
@@ -1034,7 +1034,8 @@ class Decoder(nn.Module):
         Every layer has stock attention (a compressed cache holds one length for its batch)."""
         b = len(prompts)
         dev = self.embed_tokens.device
-        if b != cache.max_requests or len(cache.layers) != len(self.layers) or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        if b != cache.max_requests or len(cache.layers) != len(self.layers) \
+                or any(p.dim() != 1 or p.numel() == 0 for p in prompts):
             raise ValueError("greedy_requests takes one non-empty 1-D prompt for each request and a layer of the cache for "
                              "each layer of the model")
         if not _hip(self.embed_tokens) or not all(isinstance(layer.self_attn, Attention) for layer in self.layers):
