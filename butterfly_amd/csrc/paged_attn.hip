@@ -34,11 +34,16 @@ namespace bfly {
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
 // Whole calls, us, with 256 / 512 / 1024 runs: one request of 32768 tokens 21.6 / 22.0 / 22.1, 131072 tokens x 32 247 /
 // 248 / 247, 262144 tokens of d 256 193 / 196 / 199, 64 of up to 2000 tokens with 32/8 heads 39.8 / 43.6 / 40.6.
-// c at least 1 / 2: one request of 1024 tokens 9.9 / 11.4.  Single runs of up to 4 / 8 rounds (c at least 2): 11.4 / 14.8.
+// c at least 1 / 2: one request of 1024 tokens 9.9 / 11.4.  Two tiles of a wave under way instead of one: 131072 tokens x 32
+// 227 -> 237 (334 registers), 64 of up to 2000 38.5 -> 41.2.
 // Workgroups of 4 / 8 waves: 64 of up to 2000 tokens 39.8 / 46.9, one of 32768 21.6 / 21.6.
 constexpr int kRuns = 256;            // runs in all, where the requests and heads leave that many: one for each CU
 constexpr int kMinRun = 1;            // c at least
-constexpr int kWhole = 4;             // rounds that stay one run: 512 keys (bf16) are done before a join of two runs
+// Rounds that stay one run, and without a second launch where the tables hold no more: 512 keys (bf16) are done before a
+// join of two runs, and the more pairs of request and head (x16 query heads) there are, the longer runs hide behind each
+// other.  Measured, this many / the next fewer, us: 128 pairs of 1000 tokens 18.3 / 20.9, 512 of up to 2000 87.6 / 90.7
+// (all 2000), 2048 and more of up to 3000 287 / 380; 512 of up to 4000 with 32 instead of 16: 69.6 / 63.4.
+constexpr int whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 // A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
 // c >= total / kRuns, fewer than 2 kRuns: the partials there can be.  (kSlack: the total is a sum of floats.)
 constexpr int kSlack = 64;
@@ -66,7 +71,8 @@ struct PagedAttnArgs {
   int requests, num_pages, hq, hkv, shift, window;
   int group, row_tiles, rows;            // query heads a kv head; 16-row parts of them; rows of a part at most
   int units;                             // hkv * row_tiles
-  int whole;                             // every request is one run (its table row is that short)
+  int whole;                             // rounds that stay one run
+  int direct;                            // every request is one run (its table row is that short)
   float scale;
 };
 
@@ -133,7 +139,7 @@ __device__ __forceinline__ float wave_max(float x) {
 // stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
 template <int KT, bool kMerge>
 __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
-  if (a.whole) {                                    // no request can have several runs: item = (request, unit)
+  if (a.direct) {                                   // no request can have several runs: item = (request, unit)
     const int b = (int)idx / a.units;
     return Run{b, a.lengths[b], (int)idx - b * a.units, 1, 0};
   }
@@ -141,28 +147,36 @@ __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
   const int per = (a.requests + 63) >> 6;
   const int b0 = lane * per < a.requests ? lane * per : a.requests;
   const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
+  // (up to 64 requests a lane has one, in registers)
   const int len0 = b0 < b1 ? a.lengths[b0] : 0;
-  const int first = b0 < b1 ? span_of<KT>(a, len0).rounds : 0;
-  const auto rounds = [&](int b) { return b == b0 ? first : span_of<KT>(a, a.lengths[b]).rounds; };
-  float total = (float)first;
-  for (int b = b0 + 1; b < b1; ++b) total += (float)rounds(b);
+  const int first = span_of<KT>(a, len0).rounds;
+  const auto each = [&](auto&& f) {
+    if (per == 1) {
+      if (b0 < b1) f(first);
+    } else {
+#pragma unroll 4
+      for (int b = b0; b < b1; ++b) f(span_of<KT>(a, a.lengths[b]).rounds);
+    }
+  };
+  float total = 0.f;
+  each([&](int n) { total += (float)n; });
   total = wave_total(total) * (float)a.units;
   // c fills kRuns exactly if the requests' last, shorter runs fit among them; else room is left for one each
   const auto over = [&](float to) { return fminf(fmaxf(ceilf(total / to), (float)kMinRun), 1e9f); };
   int c = __builtin_amdgcn_readfirstlane((int)over((float)kRuns));
-  const auto runs = [&](int n) { return n > c && n > kWhole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
+  const auto runs = [&](int n) { return n > c && n > a.whole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
   int items = 0;
-  for (int b = b0; b < b1; ++b) items += runs(rounds(b));
+  each([&](int n) { items += runs(n); });
   const int64_t pairs = (int64_t)a.requests * a.units;
   if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > kRuns && pairs < kRuns)
     c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < kRuns / 2 ? kRuns - (int)pairs : kRuns / 2)));
   int slots = 0;
   items = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int s = runs(rounds(b));
+  each([&](int n) {
+    const int s = runs(n);
     items += kMerge ? (s > 1 ? 1 : 0) : s;
     slots += s > 1 ? s : 0;
-  }
+  });
   const int i_up = wave_scan(items), s_up = wave_scan(slots);
   const uint64_t mine = __ballot((int64_t)i_up * a.units > idx);
   Run r{-1, 0, 0, 0, 0};
@@ -192,14 +206,15 @@ __device__ __forceinline__ void store4(__bf16* o, f32x4 y, float f) {
   *reinterpret_cast<bf16x4*>(o) = __builtin_convertvector(y, bf16x4);
 }
 
-// The output and statistics of a row from its joined sums.  A row that sees nothing but scores of -inf
-// has no softmax: NaN, as exp(-inf - -inf) gives.
+// The statistics of a row from its joined sums.  A row that sees nothing but scores of -inf has no softmax: its sum is
+// NaN, as exp(-inf - -inf) gives (its output is 0 / 0).  NaN scores make the sum NaN, and then the maximum, which
+// has passed over them (a maximum of +inf makes a NaN sum by itself).
 template <typename T>
 __device__ __forceinline__ void finish_stats(const PagedAttnArgs& a, int64_t row, float m, float l) {
   if (a.l == nullptr) return;
-  if (m == -INFINITY) l = __builtin_nanf("");
-  a.l[row] = l;
-  a.m[row] = l != l && fabsf(m) != INFINITY ? l : m;
+  const bool nan = l != l;
+  a.l[row] = m == -INFINITY ? __builtin_nanf("") : l;
+  a.m[row] = nan && m != INFINITY ? l : m;
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -632,7 +647,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   if (c == 0) finish_stats<T>(a, row, mm, l);
 }
 
-// The rounds of a request at most; only one of more than kWhole can have several runs.
+// The rounds of a request at most; only one of more than whole_rounds can have several runs.
 static int64_t most_rounds(int64_t capacity, int window, int esize) {
   const int kt = esize == 2 ? kTile<__bf16> : kTile<float>;
   const int64_t keys = window > 0 && window < capacity ? (int64_t)window + kt - 1 : capacity;
@@ -655,8 +670,8 @@ using namespace bfly;
 extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim,
                                                         int64_t table_width, int page_size, int window) {
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
-  if (most_rounds(table_width * page_size, window, 4) <= kWhole) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
+  if (most_rounds(table_width * page_size, window, 4) <= whole_rounds(requests * hkv * ((group + 15) / 16))) return 0;
   return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
 
@@ -702,8 +717,9 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * x.head_dim;
   // runs: one for each (request, unit), and as many more as the splits make (plan_run)
   const int64_t rounds = most_rounds(a.capacity, a.window, (int)es), pairs = x.requests * a.units;
-  const bool splits = rounds > kWhole;
-  a.whole = !splits;
+  a.whole = whole_rounds(pairs);
+  const bool splits = rounds > a.whole;
+  a.direct = !splits;
   const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + kRuns + kSlack;
   const int64_t items = !splits ? pairs : most < some ? most : some;
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads

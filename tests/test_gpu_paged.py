@@ -198,6 +198,15 @@ def test_attention_all_scores_minus_infinity_is_nan_and_empty_is_zero(dtype):
     o, l, m = bf.paged_attention(q, k2, vp, table, lens, return_stats=True)
     assert bool(torch.isnan(o[0]).all()) and bool(torch.isnan(o[2]).all())
     assert bool((o[1] == 0).all()) and bool((l[1] == 0).all()) and bool((m[1] == -1e30).all())
+    assert bool(torch.isnan(l[[0, 2]]).all()) and bool((m[[0, 2]] == -float("inf")).all())
+    # NaN scores: the maximum is NaN too, whether some keys or all of them have one
+    for keys in (slice(0, 1), slice(None)):
+        k3 = kp.clone()
+        k3[table[0, :1].long(), :, keys] = NAN
+        if keys == slice(None):
+            k3[table[0, 1].long()] = NAN
+        o, l, m = bf.paged_attention(q, k3, vp, table, lens, return_stats=True)
+        assert all(bool(torch.isnan(x[0]).all()) for x in (o, l, m)) and bool(torch.isfinite(m[2]).all())
 
 
 def test_attention_bad_tables_give_nan_for_their_request_only():
@@ -729,3 +738,12 @@ def test_two_captured_attentions_replayed_at_once():
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("batch,width", [(40, 8), (40, 70), (130, 20), (130, 200), (520, 12), (520, 400)])
+def test_attention_batches_on_both_sides_of_each_split_rule(dtype, batch, width):
+    """Narrow tables (one run a request, one launch) and wide ones, for few, some and many pairs of request and head."""
+    r = random.Random(batch + width)
+    lens = [r.choice([0, 1, 17, 64, r.randint(1, 32 * min(width, 60))]) for _ in range(batch)]
+    _check_attention(*_paged_case(lens, 8, 4, 64, 32, dtype, width=width if width >= 60 else None))
