@@ -113,7 +113,7 @@ SIGNATURES = {
     "bfly_paged_plan": (_int, [C.c_char_p, _vp]),
     "bfly_paged_append": (_int, [C.c_char_p, _vp]),
     "bfly_paged_rope_append": (_int, [C.c_char_p, _vp]),
-    "bfly_paged_attention_workspace_bytes": (_i64, [_i64, _int, _int, _int, _i64, _int, _int]),
+    "bfly_paged_attention_workspace_bytes": (_i64, [_int, _i64, _int, _int, _int, _i64, _int, _int]),
     "bfly_paged_attention": (_int, [C.c_char_p, _vp]),
 }
 

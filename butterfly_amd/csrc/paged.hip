@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(256) paged_rope_append_kernel(RopeAppendArgs a
     if (kHeads > 1 && head >= (int)nh) break;
     const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
     const char* src = is_q ? a.q + row * a.q_row + head * a.q_head
-                           : is_v ? a.v + row * a.v_row + (head - a.hq - a.hkv) * a.v_head : a.k + row * a.k_row + (head - a.hq) * a.k_head;
+                           : is_v ? a.v + row * a.v_row + (head - a.hq - a.hkv) * a.v_head
+                                  : a.k + row * a.k_row + (head - a.hq) * a.k_head;
     const vec* p = reinterpret_cast<const vec*>(src + 16 * gl);
     x[i] = kHeads > 1 ? __builtin_nontemporal_load(p) : *p;
   }
@@ -360,7 +361,8 @@ int paged_check_pages(const char* what, const bfly_pages_t& p, int64_t esize) {
                  "%s: page_size %lld must be a power of two from 16 to 1024", what, (long long)p.page_size);
   BFLY_CHECK_ARG(p.num_pages > 0 && p.num_pages <= INT32_MAX, "%s: bad num_pages", what);
   for (const int64_t s : {p.k_page_stride, p.k_head_stride, p.k_row_stride, p.v_page_stride, p.v_head_stride, p.v_row_stride})
-    BFLY_CHECK_ARG(s >= 0 && s < ((int64_t)1 << 48) && (s * esize) % 16 == 0, "%s: page strides must be multiples of 16 bytes", what);
+    BFLY_CHECK_ARG(s >= 0 && s < ((int64_t)1 << 48) && (s * esize) % 16 == 0,
+                   "%s: page strides must be multiples of 16 bytes", what);
   // offsets inside a page and head are kept in 32 bits
   BFLY_CHECK_ARG(p.k_row_stride * esize * p.page_size <= INT32_MAX && p.v_row_stride * esize * p.page_size <= INT32_MAX,
                  "%s: row stride too large", what);
@@ -380,7 +382,8 @@ using namespace bfly;
 extern "C" int bfly_paged_plan(const bfly_paged_plan_args_t* args, hipStream_t stream) {
   BFLY_CHECK_ARG(args, "null pointer");
   const bfly_paged_plan_args_t& x = *args;
-  BFLY_CHECK_ARG(x.requests >= 0 && x.requests <= (1 << 24) && x.table_width >= 0 && x.table_width <= INT32_MAX, "bad block table shape");
+  BFLY_CHECK_ARG(x.requests >= 0 && x.requests <= (1 << 24) && x.table_width >= 0 && x.table_width <= INT32_MAX,
+                 "bad block table shape");
   BFLY_CHECK_ARG(x.requests <= 1 || x.table_stride >= x.table_width, "block table rows overlap");
   BFLY_CHECK_ARG(x.num_rows >= 0 && x.num_rows <= INT32_MAX && x.free_capacity >= 0 && x.free_capacity <= INT32_MAX,
                  "num_rows and the free list must stay below 2^31");
@@ -424,7 +427,8 @@ extern "C" int bfly_paged_append(const bfly_paged_append_args_t* args, hipStream
   const bfly_paged_append_args_t& x = *args;
   BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
   const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
-  BFLY_CHECK_ARG(x.rows >= 0 && x.rows <= INT32_MAX && x.hkv > 0 && x.hkv <= 65535 && x.head_dim > 0 && x.head_dim <= 65535, "bad shape");
+  BFLY_CHECK_ARG(x.rows >= 0 && x.rows <= INT32_MAX && x.hkv > 0 && x.hkv <= 65535 && x.head_dim > 0 && x.head_dim <= 65535,
+                 "bad shape");
   BFLY_CHECK_ARG(x.head_dim * es % 16 == 0, "head_dim %lld is not whole 16-byte pieces", (long long)x.head_dim);
   const int rc = paged_check_pages("bfly_paged_append", x.pages, es);
   if (rc != BFLY_OK) return rc;
@@ -432,7 +436,8 @@ extern "C" int bfly_paged_append(const bfly_paged_append_args_t* args, hipStream
                  "row and head strides must be multiples of 16 bytes");
   if (x.rows == 0) return BFLY_OK;
   BFLY_CHECK_ARG(x.k && x.v && x.slots && x.pages.k && x.pages.v, "null pointer");
-  BFLY_CHECK_ARG(aligned16(x.k) && aligned16(x.v) && aligned16(x.pages.k) && aligned16(x.pages.v), "pointers must be 16-byte aligned");
+  BFLY_CHECK_ARG(aligned16(x.k) && aligned16(x.v) && aligned16(x.pages.k) && aligned16(x.pages.v),
+                 "pointers must be 16-byte aligned");
   AppendArgs a{};
   a.k = static_cast<const char*>(x.k); a.v = static_cast<const char*>(x.v); a.slots = x.slots;
   a.kp = k_page_ptr(x.pages, es); a.vp = v_page_ptr(x.pages, es);
@@ -453,8 +458,8 @@ extern "C" int bfly_paged_rope_append(const bfly_paged_rope_append_args_t* args,
   BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
   const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
   BFLY_CHECK_ARG(x.rows >= 0 && x.rows <= INT32_MAX, "bad shape");
-  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0, "bad head counts hq=%lld hkv=%lld",
-                 (long long)x.hq, (long long)x.hkv);
+  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0,
+                 "bad head counts hq=%lld hkv=%lld", (long long)x.hq, (long long)x.hkv);
   if (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) {
     set_error("bfly_paged_rope_append: head_dim=%lld unsupported (64, 128, 256)", (long long)x.head_dim);
     return BFLY_ERR_UNSUPPORTED;
@@ -464,10 +469,12 @@ extern "C" int bfly_paged_rope_append(const bfly_paged_rope_append_args_t* args,
   BFLY_CHECK_ARG(x.table_rows > 0, "the cos/sin tables must have rows");
   const int rc = paged_check_pages("bfly_paged_rope_append", x.pages, es);
   if (rc != BFLY_OK) return rc;
-  BFLY_CHECK_ARG(strides16({x.q_row_stride, x.q_head_stride, x.k_row_stride, x.k_head_stride, x.v_row_stride, x.v_head_stride}, es),
+  BFLY_CHECK_ARG(strides16({x.q_row_stride, x.q_head_stride, x.k_row_stride, x.k_head_stride, x.v_row_stride,
+                            x.v_head_stride}, es),
                  "row and head strides must be multiples of 16 bytes");
   if (x.rows == 0) return BFLY_OK;
-  BFLY_CHECK_ARG(x.q && x.k && x.v && x.cos && x.sin && x.positions && x.slots && x.q_out && x.pages.k && x.pages.v, "null pointer");
+  BFLY_CHECK_ARG(x.q && x.k && x.v && x.cos && x.sin && x.positions && x.slots && x.q_out && x.pages.k && x.pages.v,
+                 "null pointer");
   BFLY_CHECK_ARG((x.q_weight == nullptr) == (x.k_weight == nullptr), "both norm weights or neither");
   BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.k) && aligned16(x.v) && aligned16(x.cos) && aligned16(x.sin) && aligned16(x.q_out) &&
                      aligned16(x.pages.k) && aligned16(x.pages.v) && aligned16(x.q_weight) && aligned16(x.k_weight),

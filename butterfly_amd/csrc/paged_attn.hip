@@ -5,7 +5,7 @@
 //
 // Work: a request's tiles (32 keys in bf16, 16 in fp32) go in rounds of four, one for each wave of a
 // workgroup, and its rounds in runs of at most c, c such that all requests and heads together make about
-// kRuns runs.  A workgroup takes one run of one kv head for up to 16 of its query heads; every workgroup finds
+// 256 runs (512 of d 64).  A workgroup takes one run of one kv head for up to 16 of its query heads; every workgroup finds
 // its run from the lengths by itself (plan_run), so the grid needs no host knowledge of them and a long request
 // among short ones is split as far as a lone one.  Requests with one run write their output, the others a
 // partial (fp32 sums, m, l) that paged_merge_kernel joins.
@@ -37,7 +37,10 @@ constexpr float kPagedNeg = -1e30f;   // the largest score of a request without 
 // c at least 1 / 2: one request of 1024 tokens 9.9 / 11.4.  Two tiles of a wave under way instead of one: 131072 tokens x 32
 // 227 -> 237 (334 registers), 64 of up to 2000 38.5 -> 41.2.
 // Workgroups of 4 / 8 waves: 64 of up to 2000 tokens 39.8 / 46.9, one of 32768 21.6 / 21.6.
-constexpr int kRuns = 256;            // runs in all, where the requests and heads leave that many: one for each CU
+// Tiles of d 64 have half the bytes and half the registers: two runs a CU (512 / 256 runs: 8 requests of 60000 tokens
+// 86.0 / 88.0, fp32 8 of 30000 86.7 / 92.5; d 128 in fp32 166 / 161).
+constexpr int runs_for(int head_dim) { return head_dim <= 64 ? 512 : 256; }   // in all, where requests and heads leave them
+constexpr int kMaxRuns = 512;
 constexpr int kMinRun = 1;            // c at least
 // Rounds that stay one run, and without a second launch where the tables hold no more: 512 keys (bf16) are done before a
 // join of two runs, and the more pairs of request and head (x16 query heads) there are, the longer runs hide behind each
@@ -45,9 +48,9 @@ constexpr int kMinRun = 1;            // c at least
 // (all 2000), 2048 and more of up to 3000 287 / 380; 512 of up to 4000 with 32 instead of 16: 69.6 / 63.4.
 constexpr int whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 // A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
-// c >= total / kRuns, fewer than 2 kRuns: the partials there can be.  (kSlack: the total is a sum of floats.)
+// c >= total / runs_for, fewer than twice runs_for: the partials there can be.  (kSlack: the total is a sum of floats.)
 constexpr int kSlack = 64;
-constexpr int kMaxSlots = 2 * kRuns + kSlack;
+constexpr int kMaxSlots = 2 * kMaxRuns + kSlack;
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
@@ -71,6 +74,7 @@ struct PagedAttnArgs {
   int requests, num_pages, hq, hkv, shift, window;
   int group, row_tiles, rows;            // query heads a kv head; 16-row parts of them; rows of a part at most
   int units;                             // hkv * row_tiles
+  int runs;                              // runs_for(D)
   int whole;                             // rounds that stay one run
   int direct;                            // every request is one run (its table row is that short)
   float scale;
@@ -161,15 +165,15 @@ __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
   float total = 0.f;
   each([&](int n) { total += (float)n; });
   total = wave_total(total) * (float)a.units;
-  // c fills kRuns exactly if the requests' last, shorter runs fit among them; else room is left for one each
+  // c fills the runs exactly if the requests' last, shorter runs fit among them; else room is left for one each
   const auto over = [&](float to) { return fminf(fmaxf(ceilf(total / to), (float)kMinRun), 1e9f); };
-  int c = __builtin_amdgcn_readfirstlane((int)over((float)kRuns));
+  int c = __builtin_amdgcn_readfirstlane((int)over((float)a.runs));
   const auto runs = [&](int n) { return n > c && n > a.whole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
   int items = 0;
   each([&](int n) { items += runs(n); });
   const int64_t pairs = (int64_t)a.requests * a.units;
-  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > kRuns && pairs < kRuns)
-    c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < kRuns / 2 ? kRuns - (int)pairs : kRuns / 2)));
+  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs)
+    c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
   int slots = 0;
   items = 0;
   each([&](int n) {
@@ -658,7 +662,7 @@ static void launch_paged(const PagedAttnArgs& a, int64_t items, bool splits, hip
   hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(64 * kWaves), 0, stream, a);
   if (splits) {
     const int64_t pairs = (int64_t)a.requests * a.units;
-    const unsigned x = (unsigned)(pairs < kRuns ? pairs : kRuns);
+    const unsigned x = (unsigned)(pairs < a.runs ? pairs : a.runs);
     hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(x, (unsigned)a.rows, D / 64), dim3(256), 0, stream, a);
   }
 }
@@ -667,11 +671,12 @@ static void launch_paged(const PagedAttnArgs& a, int64_t items, bool splits, hip
 
 using namespace bfly;
 
-extern "C" int64_t bfly_paged_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim,
+extern "C" int64_t bfly_paged_attention_workspace_bytes(int dtype, int64_t requests, int hq, int hkv, int head_dim,
                                                         int64_t table_width, int page_size, int window) {
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
-  if (most_rounds(table_width * page_size, window, 4) <= whole_rounds(requests * hkv * ((group + 15) / 16))) return 0;
+  const int64_t pairs = requests * hkv * ((group + 15) / 16);
+  if (most_rounds(table_width * page_size, window, dtype == BFLY_DTYPE_F32 ? 4 : 2) <= whole_rounds(pairs)) return 0;
   return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
 }
 
@@ -681,8 +686,8 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   BFLY_CHECK_ARG(x.dtype == BFLY_DTYPE_F32 || x.dtype == BFLY_DTYPE_BF16, "unsupported dtype %lld", (long long)x.dtype);
   const int64_t es = x.dtype == BFLY_DTYPE_F32 ? 4 : 2;
   BFLY_CHECK_ARG(x.requests >= 0 && x.requests <= 65535, "bad number of requests (at most 65535)");
-  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0, "bad head counts hq=%lld hkv=%lld",
-                 (long long)x.hq, (long long)x.hkv);
+  BFLY_CHECK_ARG(x.hkv > 0 && x.hq > 0 && x.hq <= (1 << 20) && x.hkv <= x.hq && x.hq % x.hkv == 0,
+                 "bad head counts hq=%lld hkv=%lld", (long long)x.hq, (long long)x.hkv);
   if (x.head_dim != 64 && x.head_dim != 128 && x.head_dim != 256) {
     set_error("bfly_paged_attention: head_dim=%lld unsupported (64, 128, 256)", (long long)x.head_dim);
     return BFLY_ERR_UNSUPPORTED;
@@ -690,17 +695,20 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   const int rc = paged_check_pages("bfly_paged_attention", x.pages, es);
   if (rc != BFLY_OK) return rc;
   BFLY_CHECK_ARG(x.window >= 0 && x.window <= INT32_MAX, "bad window");
-  BFLY_CHECK_ARG(x.table_width >= 0 && x.table_width <= INT32_MAX && (x.requests <= 1 || x.table_stride >= 0), "bad block table shape");
+  BFLY_CHECK_ARG(x.table_width >= 0 && x.table_width <= INT32_MAX && (x.requests <= 1 || x.table_stride >= 0),
+                 "bad block table shape");
   BFLY_CHECK_ARG(x.q_request_stride >= 0 && x.q_head_stride >= 0 && x.q_request_stride < ((int64_t)1 << 48) &&
-                     x.q_head_stride < ((int64_t)1 << 48) && x.q_request_stride * es % 16 == 0 && x.q_head_stride * es % 16 == 0,
+                     x.q_head_stride < ((int64_t)1 << 48) && x.q_request_stride * es % 16 == 0 &&
+                     x.q_head_stride * es % 16 == 0,
                  "q strides must be multiples of 16 bytes");
   if (x.requests == 0) return BFLY_OK;
   BFLY_CHECK_ARG(x.q && x.pages.k && x.pages.v && x.lengths && x.out, "null pointer");
   BFLY_CHECK_ARG(x.table_width == 0 || x.block_table, "null pointer");
   BFLY_CHECK_ARG((x.l == nullptr) == (x.m == nullptr), "both l and m or neither");
-  BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.pages.k) && aligned16(x.pages.v) && aligned16(x.out), "pointers must be 16-byte aligned");
-  const int64_t need = bfly_paged_attention_workspace_bytes(x.requests, (int)x.hq, (int)x.hkv, (int)x.head_dim, x.table_width,
-                                                            (int)x.pages.page_size, (int)x.window);
+  BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.pages.k) && aligned16(x.pages.v) && aligned16(x.out),
+                 "pointers must be 16-byte aligned");
+  const int64_t need = bfly_paged_attention_workspace_bytes((int)x.dtype, x.requests, (int)x.hq, (int)x.hkv, (int)x.head_dim,
+                                                            x.table_width, (int)x.pages.page_size, (int)x.window);
   BFLY_CHECK_ARG(need == 0 || (x.workspace && x.workspace_bytes >= need && aligned16(x.workspace)), "workspace too small");
   PagedAttnArgs a{};
   a.q = static_cast<const char*>(x.q);
@@ -717,10 +725,11 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * x.head_dim;
   // runs: one for each (request, unit), and as many more as the splits make (plan_run)
   const int64_t rounds = most_rounds(a.capacity, a.window, (int)es), pairs = x.requests * a.units;
+  a.runs = runs_for((int)x.head_dim);
   a.whole = whole_rounds(pairs);
   const bool splits = rounds > a.whole;
   a.direct = !splits;
-  const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + kRuns + kSlack;
+  const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + a.runs + kSlack;
   const int64_t items = !splits ? pairs : most < some ? most : some;
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads
 #define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)

@@ -118,7 +118,8 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: int, written: bool
     k0, k1, k2, k3 = k_pages.stride()
     v0, v1, v2, v3 = v_pages.stride()
     kd, vd = k_pages.data_ptr(), v_pages.data_ptr()
-    if k3 == v3 == 1 and kd and vd and not ((kd | vd) & 15 or (k0 | k1 | k2 | v0 | v1 | v2) & (7 if dtype is torch.bfloat16 else 3)) \
+    if k3 == v3 == 1 and kd and vd \
+            and not ((kd | vd) & 15 or (k0 | k1 | k2 | v0 | v1 | v2) & (7 if dtype is torch.bfloat16 else 3)) \
             and (not written or k0 and k1 and k2 and v0 and v1 and v2 and kd != vd):
         return shape, (k0, k1, k2, v0, v1, v2)
     if 0 in shape:
@@ -366,7 +367,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             q = q.clone(memory_format=torch.contiguous_format)
             q0, q1, _, _ = q.stride()
         lengths = lengths.contiguous()
-        need = _workspace_bytes(b, hq, hkv, d, width, page_size, window)
+        need = _workspace_bytes(code, b, hq, hkv, d, width, page_size, window)
         if need:
             ws = _EMPTY((need,), (1,), dtype=torch.uint8, device=cuda)
         _native.call("bfly_paged_attention", _ATTN(
