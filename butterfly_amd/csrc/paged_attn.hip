@@ -69,6 +69,8 @@ struct PagedAttnArgs {
   float* m;
   float* part;                           // partials: [slot][rows][D], then [slot][rows] m and l
   float* part_ml;
+  int4* join;                            // what to join: request, unit, runs, first slot
+  int* joins;                            // how many of them
   int64_t q_req, q_head, table_stride;   // bytes, bytes, elements
   int64_t capacity;                      // tokens a table row holds
   int requests, num_pages, hq, hkv, shift, window;
@@ -104,6 +106,8 @@ struct Run {
   int sub;        // index inside the request
   int splits;     // runs of the request (per unit)
   int slot;       // partials before the request's
+  int join;       // (request, unit) pairs of several runs before the request's
+  int joins;      // and in all
 };
 
 // Sums over the wave's lanes on DPP (row shifts inside 16 lanes, then the rows' last lanes broadcast): lane 63
@@ -138,14 +142,13 @@ __device__ __forceinline__ float wave_max(float x) {
   return col_max4(x);
 }
 
-// The request that item `idx` falls into, where request b has units * splits_b items (kMerge: only
-// requests of more than one run, with `units` items each).  Every wave does it by itself: a lane sums a
-// stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
-template <int KT, bool kMerge>
+// The request that item `idx` falls into, where request b has units * splits_b items.  Every wave does it by
+// itself: a lane sums a stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
+template <int KT>
 __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
   if (a.direct) {                                   // no request can have several runs: item = (request, unit)
     const int b = (int)idx / a.units;
-    return Run{b, a.lengths[b], (int)idx - b * a.units, 1, 0};
+    return Run{b, a.lengths[b], (int)idx - b * a.units, 1, 0, 0, 0};
   }
   const int lane = threadIdx.x & 63;
   const int per = (a.requests + 63) >> 6;
@@ -174,33 +177,35 @@ __device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
   const int64_t pairs = (int64_t)a.requests * a.units;
   if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs)
     c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
-  int slots = 0;
-  items = 0;
+  int slots = 0;                                    // low half: partials; high half: requests that have them (both
+  items = 0;                                        // below kMaxSlots in all)
+  const auto parts = [](int s) { return s > 1 ? s | 0x10000 : 0; };
   each([&](int n) {
     const int s = runs(n);
-    items += kMerge ? (s > 1 ? 1 : 0) : s;
-    slots += s > 1 ? s : 0;
+    items += s;
+    slots += parts(s);
   });
   const int i_up = wave_scan(items), s_up = wave_scan(slots);
   const uint64_t mine = __ballot((int64_t)i_up * a.units > idx);
-  Run r{-1, 0, 0, 0, 0};
+  Run r{-1, 0, 0, 0, 0, 0, (__builtin_amdgcn_readlane(s_up, 63) >> 16) * a.units};
   if (mine == 0) return r;
   const int owner = __builtin_ctzll(mine);
   int at = __builtin_amdgcn_readlane(i_up - items, owner), slot = __builtin_amdgcn_readlane(s_up - slots, owner);
   for (int b = owner * per;; ++b) {               // (a request of the owner's stretch holds idx)
     const int len = per == 1 ? __builtin_amdgcn_readlane(len0, owner) : a.lengths[b];
     const int s = runs(span_of<KT>(a, len).rounds);
-    const int next = at + (kMerge ? (s > 1 ? 1 : 0) : s);
+    const int next = at + s;
     if ((int64_t)next * a.units > idx) {
       r.b = b;
       r.len = len;
       r.sub = (int)(idx - (int64_t)at * a.units);
       r.splits = s;
-      r.slot = slot * a.units;
+      r.slot = (slot & 0xffff) * a.units;
+      r.join = (slot >> 16) * a.units;
       return r;
     }
     at = next;
-    slot += s > 1 ? s : 0;
+    slot += parts(s);
   }
 }
 
@@ -505,8 +510,13 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a
   __shared__ float so[kWaves][16 * LD];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int sbad;
-  const Run run = plan_run<KT, false>(a, blockIdx.x);
+  const Run run = plan_run<KT>(a, blockIdx.x);
   if (run.b < 0) return;
+  // (every store comes after the last page id is read: a store before would take those reads off the scalar cache
+  // and into the order of the K and V loads, 131072 tokens x 32: 207 -> 280 us)
+  const auto leave = [&]() {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !a.direct) *a.joins = run.joins;
+  };
   const int b = __builtin_amdgcn_readfirstlane(run.b), splits = __builtin_amdgcn_readfirstlane(run.splits);
   const int sub = __builtin_amdgcn_readfirstlane(run.sub), slot = __builtin_amdgcn_readfirstlane(run.slot) + sub;
   const int unit = sub / splits, split = sub - unit * splits;
@@ -518,6 +528,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a
   const int n = lane & 15, g = lane >> 4;
   const int64_t row0 = (int64_t)b * a.hq + head0;
   if (s.tiles == 0) {                               // nothing to see, or a length beyond the table
+    leave();
     const float y = s.off ? __builtin_nanf("") : 0.f;
     for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) static_cast<T*>(a.out)[row0 * D + i] = from_f32<T>(y);
     if (a.l != nullptr && threadIdx.x < rows) {
@@ -559,6 +570,8 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a
   }
   if (bad && lane == 0) sbad = 1;
   __syncthreads();
+  leave();
+  if (splits > 1 && split == 0 && threadIdx.x == 0) a.join[run.join + unit] = int4{b, unit, splits, slot};
   const float poison = sbad ? __builtin_nanf("") : 0.f;
   for (int i = threadIdx.x; i < rows * (D / 4); i += 64 * kWaves) {
     const int r = i / (D / 4), c = 4 * (i % (D / 4));
@@ -590,19 +603,22 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a
   }
 }
 
-// Joins the partials of a request's runs: a workgroup per (request, unit, row, 64 elements).  The runs'
+// Joins the partials of a request's runs: a workgroup per (request, unit, row, 64 elements) of the list that the runs
+// have left.  The runs'
 // weights exp(m_i - m) are made once, in LDS; then 16 lanes across the elements, the runs dealt to 16 groups
 // of lanes, four loads under way in each.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
-  constexpr int KT = kTile<T>, G = 16;
+  constexpr int G = 16;
   __shared__ f32x4 sy[G][16];
   __shared__ float weight[kMaxSlots], sl[4], smx[4];
-  const Run run = plan_run<KT, true>(a, blockIdx.x);
-  if (run.b < 0) return;
-  const int kvh = run.sub / a.row_tiles, part = run.sub - kvh * a.row_tiles, r = blockIdx.y;
+  const int joins = *a.joins;
+  const int4 what = a.join[blockIdx.x];             // (what is there behind the last is not looked at)
+  if ((int)blockIdx.x >= joins) return;
+  const int unit = what.y, splits = what.z;
+  const int kvh = unit / a.row_tiles, part = unit - kvh * a.row_tiles, r = blockIdx.y;
   if (16 * part + r >= a.group) return;
-  const int64_t slot0 = run.slot + (int64_t)run.sub * run.splits;
+  const int64_t slot0 = what.w;
   const int t = threadIdx.x, gr = t >> 4, c = 64 * blockIdx.z + 4 * (t & 15);
   const f32x2* ml = reinterpret_cast<const f32x2*>(a.part_ml) + slot0 * a.rows + r;
   const float* src = a.part + (slot0 * a.rows + r) * D + c;
@@ -613,19 +629,19 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
 #pragma unroll
   for (int j = 0; j < kAhead; ++j) {
     const int i = gr + G * j;
-    ahead[j] = i < run.splits ? *reinterpret_cast<const f32x4*>(src + i * step) : f32x4{0.f, 0.f, 0.f, 0.f};
+    ahead[j] = i < splits ? *reinterpret_cast<const f32x4*>(src + i * step) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   f32x2 mine = {-INFINITY, 0.f};
-  if (t < run.splits) mine = ml[(int64_t)t * a.rows];
+  if (t < splits) mine = ml[(int64_t)t * a.rows];
   float mm = mine[0];
-  for (int i = t + 256; i < run.splits; i += 256) mm = fmaxf(mm, ml[(int64_t)i * a.rows][0]);
+  for (int i = t + 256; i < splits; i += 256) mm = fmaxf(mm, ml[(int64_t)i * a.rows][0]);
   mm = wave_max(mm);
   if ((t & 63) == 0) smx[t >> 6] = mm;
   __syncthreads();
   mm = fmaxf(fmaxf(smx[0], smx[1]), fmaxf(smx[2], smx[3]));
   const float ref = mm == -INFINITY ? 0.f : mm;
   float l = 0.f;
-  for (int i = t; i < run.splits; i += 256) {
+  for (int i = t; i < splits; i += 256) {
     const f32x2 x = i == t ? mine : ml[(int64_t)i * a.rows];
     const float f = __builtin_amdgcn_exp2f((x[0] - ref) * kLog2e);
     weight[i] = f;
@@ -638,15 +654,15 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < kAhead; ++j)
-    if (gr + G * j < run.splits) y += weight[gr + G * j] * ahead[j];
+    if (gr + G * j < splits) y += weight[gr + G * j] * ahead[j];
 #pragma unroll 4
-  for (int i = gr + G * kAhead; i < run.splits; i += G) y += weight[i] * *reinterpret_cast<const f32x4*>(src + i * step);
+  for (int i = gr + G * kAhead; i < splits; i += G) y += weight[i] * *reinterpret_cast<const f32x4*>(src + i * step);
   sy[gr][t & 15] = y;
   __syncthreads();
   if (gr != 0) return;
 #pragma unroll
   for (int i = 1; i < G; ++i) y += sy[i][t];
-  const int64_t row = (int64_t)run.b * a.hq + kvh * a.group + 16 * part + r;
+  const int64_t row = (int64_t)what.x * a.hq + kvh * a.group + 16 * part + r;
   store4(static_cast<T*>(a.out) + row * D + c, y, 1.f / l);
   if (c == 0) finish_stats<T>(a, row, mm, l);
 }
@@ -677,7 +693,7 @@ extern "C" int64_t bfly_paged_attention_workspace_bytes(int dtype, int64_t reque
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   const int64_t pairs = requests * hkv * ((group + 15) / 16);
   if (most_rounds(table_width * page_size, window, dtype == BFLY_DTYPE_F32 ? 4 : 2) <= whole_rounds(pairs)) return 0;
-  return (int64_t)kMaxSlots * rows * (head_dim + 2) * 4;
+  return (int64_t)kMaxSlots * (rows * (head_dim + 2) * 4 + 16) + 16;
 }
 
 extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hipStream_t stream) {
@@ -721,7 +737,9 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   a.group = a.hq / a.hkv; a.row_tiles = (a.group + 15) / 16; a.rows = a.group < 16 ? a.group : 16;
   BFLY_CHECK_ARG((int64_t)a.hkv * a.row_tiles <= 65535, "too many heads");
   a.units = a.hkv * a.row_tiles;
-  a.part = static_cast<float*>(x.workspace);
+  a.join = static_cast<int4*>(x.workspace);
+  a.joins = reinterpret_cast<int*>(a.join + kMaxSlots);
+  a.part = reinterpret_cast<float*>(a.join + kMaxSlots + 1);
   a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * x.head_dim;
   // runs: one for each (request, unit), and as many more as the splits make (plan_run)
   const int64_t rounds = most_rounds(a.capacity, a.window, (int)es), pairs = x.requests * a.units;
