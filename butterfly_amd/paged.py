@@ -163,6 +163,9 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
     new ones are in the result only.  When something does not fit (``PLAN_ERRORS``) nothing changes,
     ``state[1]`` holds the code and every slot is -1, and so for every later step until the caller clears
     it: a captured loop that ran out of pages is found out by reading the state once.
+
+    A page belongs to one request (``paged_attention`` reads tables whose rows share pages, but a plan would
+    give such a page back with each of them).
     """
     dev = _device_of(lengths)
     if not block_table.get_device() == counts.get_device() == free_pages.get_device() == state.get_device() == dev:
