@@ -542,6 +542,14 @@ class RopeTable:
     def rows(self):
         return self.cos_tab.index_select(0, self.pos), self.sin_tab.index_select(0, self.pos)
 
+    def at(self, positions: torch.Tensor):
+        """The tables' rows of ``positions`` [N]; NaN for a position outside them."""
+        n = self.cos_tab.shape[0]
+        if n == 0:
+            raise ValueError("the cos/sin tables must have rows")
+        inside, row = ((positions >= 0) & (positions < n))[:, None], positions.clamp(0, n - 1)
+        return tuple(torch.where(inside, tab.index_select(0, row), float("nan")) for tab in (self.cos_tab, self.sin_tab))
+
     def fits(self, x: torch.Tensor, d: int) -> bool:
         """Whether a kernel can read its row of the tables by itself: one int64 position, plain fp32 tables of
         ``d`` columns on ``x``'s device, ``rows`` as it stands above.  Two row selections and their launches less for each layer: a step of
@@ -634,7 +642,8 @@ class Attention(nn.Module):
     def forward(self, x: torch.Tensor, mask=None, cache=None, *, position_embeddings=None) -> torch.Tensor:
         """``cache``: a list ``[k, v]`` of the full history (empty before the first call), or a ``PagedLayer``
         whose cache has begun the step; ``position_embeddings``: ``(cos, sin)`` rows of the call's positions
-        (or a ``RopeTable``), else computed from the cache length."""
+        (or a ``RopeTable``), else computed from the cache length.  Over pages the plan has the positions: a ``RopeTable``
+        is read at those."""
         if isinstance(cache, PagedLayer):
             return self._forward_paged(x, cache, position_embeddings)
         positions = None
@@ -660,22 +669,55 @@ class Attention(nn.Module):
         return F.scaled_dot_product_attention(q, kk, vv, attn_mask=mask)
 
     def _forward_paged(self, x: torch.Tensor, cache: PagedLayer, rope) -> torch.Tensor:
-        """``forward`` over pages.  One token of every request (their lengths may differ): q/k norm, RoPE at the
-        plan's positions and the move into the pages in one launch, then ``paged_attention``; nothing of it
-        needs the host, so the step can be captured.  More than one: a part of prompts of one length, dense
-        attention over what the pages hold and the part itself."""
+        """``forward`` over pages, every row at its position of the plan.  One token of every request (their lengths
+        may differ): q/k norm, RoPE and the move into the pages in one launch, then ``paged_attention``; nothing
+        of it needs the host, so the step can be captured.  More than one: dense attention over what the pages
+        hold and the part itself, for which the lengths are read back once a step; requests of different lengths
+        one by one.  Rows without a token (idle requests, counts below the step's rows) are undefined."""
         b, t, _ = x.shape
-        c = self.cfg
         if self.takes_paged_rows(x, cache, rope):
             return self.forward_paged_rows(self.qkv(x), cache, rope)
-        start = cache.cache.start
-        q, k, v = self.project(x, torch.arange(start, start + t, device=x.device), rope)
+        held = cache.cache.held() if t > 1 else []
+        starts = sorted({n for n in held if n is not None})
+        q, k, v = self._project_paged(x, cache, rope, shared=len(starts) <= 1)
         cache.append(k.transpose(1, 2).reshape(b * t, *k.shape[1::2]), v.transpose(1, 2).reshape(b * t, *v.shape[1::2]))
         if t == 1:
             return self.output(cache.attend(q, scale=self.scale))
+        if len(starts) <= 1:
+            return self.output(self._dense_after(cache, starts[0] if starts else 0, q, k, v))
+        o = torch.zeros_like(q)
+        for r, n in enumerate(held):
+            if n is not None:
+                one = slice(r, r + 1)
+                o[one] = self._dense_after(cache, n, q[one], k[one], v[one], r)
+        return self.output(o)
+
+    def _dense_after(self, cache: PagedLayer, start: int, q, k, v, request: Optional[int] = None) -> torch.Tensor:
+        """A part's ``q``, ``k``, ``v`` behind the ``start`` tokens that the pages of all requests, or of one, hold."""
         if start:
-            k, v = (torch.cat(x, 2) for x in zip(cache.history(start), (k, v)))
-        return self.output(self._dense(q, k, v))
+            k, v = (torch.cat(x, 2) for x in zip(cache.history(start, request), (k, v)))
+        return self._dense(q, k, v)
+
+    def _project_paged(self, x: torch.Tensor, cache: PagedLayer, rope, shared: bool):
+        """``project`` at the plan's positions.  ``rope`` as rows: ``t`` that all requests have in common (``shared``:
+        their positions may be the same) or one for each of the ``b * t``."""
+        b, t, _ = x.shape
+        positions = cache.plan.positions
+        if isinstance(rope, RopeTable):
+            rope = rope.at(positions)
+        if rope is not None:
+            rope = tuple(r.reshape(-1, r.shape[-1]) for r in rope)
+            rows = rope[0].shape[0]
+            if rows not in (t, b * t) or rope[1].shape[0] != rows:
+                raise ValueError(f"{rows} rows of position_embeddings for {b} requests of {t} rows each")
+            if rows == t and not shared:
+                raise ValueError("requests of different lengths take position_embeddings of their own, one for each of "
+                                 "their rows")
+            if rows == t:
+                return self.project(x, None, rope)
+        # requests' rows as one sequence: each has its own position
+        rows = self.project(x.reshape(1, b * t, -1), positions, rope)
+        return tuple(y.view(y.shape[1], b, t, -1).transpose(0, 1).contiguous() for y in rows)
 
     @staticmethod
     def takes_paged_rows(x: torch.Tensor, cache, rope) -> bool:
@@ -901,14 +943,16 @@ class Decoder(nn.Module):
 
     @torch.no_grad()
     def forward(self, tokens: torch.Tensor, caches: List, start: int) -> torch.Tensor:
-        """tokens [B, T] at positions [start, start+T); returns logits [B, vocab] of the last position."""
+        """tokens [B, T] at positions [start, start+T); returns logits [B, vocab] of the last position.
+        A paged cache's requests hold ``start`` tokens each (several tokens: else ``ValueError``; one token: each
+        request goes on at its own length, at most ``start``)."""
         x = F.embedding(tokens, self.embed_tokens)
         positions = torch.arange(start, start + tokens.shape[1], device=tokens.device)
         rope = self._rope(start, tokens.shape[1], tokens.device)
-        pools = self._paged_pools(caches, tokens.shape[0])
+        pools, t = self._paged_pools(caches, tokens.shape[0]), tokens.shape[1]
         for pool in pools:
-            pool.begin(torch.full_like(pool.lengths, tokens.shape[1]), tokens.shape[1], start=start)
-        if pools:
+            pool.begin(torch.full_like(pool.lengths, t), t, start=start if t > 1 else None)
+        if pools and t == 1:
             rope = RopeTable(*self._rope_tab, positions)
         return self._last_logits(x, positions, caches, rope).float()
 

@@ -23,7 +23,7 @@ from __future__ import annotations
 import math
 from functools import lru_cache
 from operator import index
-from typing import Iterable, NamedTuple, Optional
+from typing import Iterable, List, NamedTuple, Optional
 
 import torch
 
@@ -413,11 +413,13 @@ class PagedLayer:
         return paged_attention(q, self.k_pages, self.v_pages, self.cache.block_table, self.plan.lengths, scale=scale,
                                window=window, return_stats=return_stats)
 
-    def history(self, tokens: int):
-        """The first ``tokens`` keys and values of every request as dense [B, Hkv, tokens, d] tensors (what a
-        prompt's further part attends to); every request holds that many."""
-        size = self.k_pages.shape[2]
-        ids = self.cache.block_table[:, :-(-tokens // size)].long().clamp_(0, self.k_pages.shape[0] - 1)
+    def history(self, tokens: int, request: Optional[int] = None):
+        """The first ``tokens`` keys and values of every request, or of one, as dense [B, Hkv, tokens, d] tensors
+        (what a prompt's further part attends to); the requests hold that many."""
+        size, table = self.k_pages.shape[2], self.cache.block_table
+        if request is not None:
+            table = table[request:request + 1]
+        ids = table[:, :-(-tokens // size)].long().clamp_(0, self.k_pages.shape[0] - 1)
         return tuple(x[ids].transpose(1, 2).flatten(2, 3)[:, :, :tokens] for x in (self.k_pages, self.v_pages))
 
 
@@ -449,26 +451,58 @@ class PagedKVCache:
         self.free_pages = torch.arange(num_pages - 1, -1, -1, **i32)
         self.state = torch.tensor([num_pages, 0], **i32)
         self.plan: Optional[PagedPlan] = None
-        self.start = 0                 # tokens before the step, for a part of a prompt (PagedLayer.history)
+        self.rows_each = 0             # the step's rows of every request; 0: packed
+        self._held: Optional[List[Optional[int]]] = None
 
     @property
     def nbytes(self) -> int:
         return self.k_pages.nbytes + self.v_pages.nbytes
 
-    def _begin(self, counts: torch.Tensor, num_rows: int, rows_each: int, start: int) -> PagedPlan:
+    def _begin(self, counts: torch.Tensor, num_rows: int, rows_each: int) -> PagedPlan:
         self.plan = paged_plan(self.block_table, self.lengths, counts, self.free_pages, self.state,
                                page_size=self.page_size, num_rows=num_rows, rows_each=rows_each, in_place=True)
-        self.start = int(start)
+        self.rows_each, self._held = rows_each, None
         return self.plan
 
-    def begin(self, counts: torch.Tensor, rows_each: int = 1, *, start: int = 0) -> PagedPlan:
+    def begin(self, counts: torch.Tensor, rows_each: int = 1, *, start: Optional[int] = None) -> PagedPlan:
         """A step in which request ``b`` adds ``counts[b] <= rows_each`` tokens (int32 [B], on the device; negative:
-        takes tokens back) and has ``rows_each`` rows, row ``b * rows_each + i`` its ``i``-th."""
-        return self._begin(counts, self.max_requests * rows_each, rows_each, start)
+        takes tokens back) and has ``rows_each`` rows, row ``b * rows_each + i`` its ``i``-th.  ``start``: every request
+        holds that many tokens before the step, else ``ValueError`` and nothing changes (the lengths are read
+        back for it)."""
+        known = start is not None and self.require(start)
+        plan = self._begin(counts, self.max_requests * rows_each, rows_each)
+        if known:
+            self._held = [int(start)] * self.max_requests
+        return plan
 
     def begin_packed(self, counts: torch.Tensor, num_rows: int) -> PagedPlan:
         """A step whose rows follow each other, request by request: ragged prompts."""
-        return self._begin(counts, num_rows, 0, 0)
+        return self._begin(counts, num_rows, 0)
+
+    def require(self, tokens: int) -> bool:
+        """``ValueError`` unless every request holds ``tokens`` tokens (waits for the current stream).  ``False`` where an
+        earlier step did not fit: lengths stand still then, until :meth:`sync` reports it."""
+        *lengths, _, error = self._read(torch.cat([self.lengths, self.state]))
+        if error:
+            return False
+        if any(n != tokens for n in lengths):
+            raise ValueError(f"the paged cache's requests hold {lengths} tokens, not {tokens} each (release() empties them)")
+        return True
+
+    def held(self) -> List[Optional[int]]:
+        """How many tokens each request held before the step (``None``: one that adds none in it), for a step of
+        ``rows_each`` rows.  Read back once a step, which waits for the current stream."""
+        if self._held is None:
+            p = self.plan
+            first = torch.where(p.slots >= 0, p.positions, -1).view(-1, self.rows_each)[:, 0]
+            self._held = [None if n < 0 else n for n in self._read(first)]
+        return self._held
+
+    @staticmethod
+    def _read(x: torch.Tensor) -> List[int]:
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a paged step that needs its lengths on the host cannot be captured (steps of one token can)")
+        return x.tolist()
 
     def release(self, requests: Iterable[int]) -> None:
         """The given requests (indices) leave: their pages go back to the free list."""
@@ -477,7 +511,7 @@ class PagedKVCache:
             if not 0 <= r < self.max_requests:
                 raise ValueError(f"request {r} is not one of {self.max_requests}")
             counts[r] = -(2 ** 31 - 1)
-        self._begin(torch.tensor(counts, dtype=torch.int32, device=self.lengths.device), 0, 0, 0)
+        self._begin(torch.tensor(counts, dtype=torch.int32, device=self.lengths.device), 0, 0)
 
     def sync(self) -> int:
         """Waits for the current stream; the number of free pages.  Raises ``RuntimeError`` if a step did not fit (that

@@ -1,0 +1,78 @@
+"""GPU: the decoder's attention over pages, given a ``PagedLayer`` by itself, against the same attention over a list
+cache for each request alone.
+
+Both round q, k, the softmax weights and the output to bf16 at places of their own, half a step of 2^-8 each, and the
+scores (at most sqrt(d) for normed heads) move by about 2^-8: 2^-5 of the largest output covers them.  A row at
+another position or behind another history differs by the output's own size."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import butterfly_amd as bf
+from butterfly_amd.decoder import Attention, DecoderConfig, RopeTable, rope_cos_sin
+
+pytestmark = pytest.mark.gpu
+
+
+def _config(head_dim):
+    return DecoderConfig(vocab_size=64, hidden_size=512, num_layers=1, num_heads=4, num_kv_heads=2, head_dim=head_dim,
+                         intermediate_size=512)
+
+
+def _cache(cfg, requests, pages=40, page=16):
+    return bf.PagedKVCache(num_layers=1, num_pages=pages, max_requests=requests, num_kv_heads=cfg.num_kv_heads,
+                           head_dim=cfg.head_dim, page_size=page)
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("table", [False, True])
+def test_rows_are_at_the_plans_positions(head_dim, table):
+    cfg = _config(head_dim)
+    attn = Attention(cfg, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    pool, lists, held, raw = _cache(cfg, 3), [[] for _ in range(3)], [0] * 3, [[] for _ in range(3)]
+    rope = RopeTable(*rope_cos_sin(torch.arange(200, device="cuda"), head_dim, cfg.rope_theta), None) if table else None
+    g = torch.Generator().manual_seed(5)
+    for counts, each in [([20, 7, 0], 20), ([1, 1, 1], 1), ([1, 0, 1], 1), ([3, 3, 3], 3), ([5, 2, 0], 5), ([1, 1, 1], 1)]:
+        x = torch.randn(3, each, cfg.hidden_size, generator=g).bfloat16().cuda()
+        pool.begin(_i32(counts), each)
+        with torch.no_grad():
+            y = attn(x, cache=pool.layers[0], position_embeddings=rope)
+            rows = attn.qkv(x)
+        for r, c in enumerate(counts):
+            if c > 0:
+                want = attn(x[r:r + 1, :c], cache=lists[r])[0].float()
+                assert (y[r, :c].float() - want).abs().max() <= 2.0 ** -5 * want.abs().max(), (counts, r)
+                held[r] += c
+                raw[r].append(rows[r, :c])
+        assert pool.lengths.tolist() == held and pool.sync() >= 0
+    for r in range(3):
+        hk, hv = pool.layers[0].history(held[r], r)
+        heads = torch.cat(raw[r]).view(held[r], -1, head_dim).transpose(0, 1)[None]
+        assert torch.equal(hv, heads[:, -cfg.num_kv_heads:])
+        k = heads[:, cfg.num_heads:cfg.num_heads + cfg.num_kv_heads].double()
+        k = k / (k.square().mean(-1, keepdim=True) + attn.k_norm.eps).sqrt()
+        cos, sin = (t.double() for t in rope_cos_sin(torch.arange(held[r], device="cuda"), head_dim, cfg.rope_theta))
+        turned = torch.cat([-k[..., head_dim // 2:], k[..., :head_dim // 2]], -1) * sin
+        # fp32 arithmetic (some d 2^-24) and one or two roundings to bf16, the first before the turn
+        bound = 2.0 ** -8 * 1.02 * ((k * cos).abs() + turned.abs()) + 2.0 ** -8 * (k * cos + turned).abs()
+        assert bool(((hk.double() - (k * cos + turned)).abs() <= bound).all())
+
+
+def test_several_tokens_are_not_captured():
+    cfg = _config(64)
+    attn = Attention(cfg, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    pool = _cache(cfg, 2)
+    x = torch.randn(2, 4, cfg.hidden_size, device="cuda").bfloat16()
+    counts = _i32([4, 4])
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.no_grad(), torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        pool.begin(counts, 4)
+        with pytest.raises(RuntimeError, match="captured"):
+            attn(x, cache=pool.layers[0])
+    torch.cuda.synchronize()
+    assert pool.lengths.tolist() == [0, 0]

@@ -1,0 +1,124 @@
+"""A ``PagedLayer`` given to the decoder's attention: every row at the position that the plan has for it, and every part
+of a prompt behind what its own request holds.  On the CPU, the operators in plain torch operations.
+
+Against the same attention over a list cache for each request alone, in fp32: the two do the same arithmetic in
+other orders over at most 128 terms a sum (128 * 2^-24 of the terms' sizes) through four stages, well inside
+2^-12 of the largest output; a row at another position differs by the output's own size."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import butterfly_amd as bf
+from butterfly_amd.decoder import Attention, Decoder, DecoderConfig, RopeTable, rope_cos_sin
+
+from . import paged_plain
+
+CFG = DecoderConfig(vocab_size=64, hidden_size=128, num_layers=2, num_heads=2, num_kv_heads=1, head_dim=64, intermediate_size=128)
+
+
+@pytest.fixture(autouse=True)
+def _plain(monkeypatch):
+    paged_plain.install(monkeypatch)
+
+
+def _attention():
+    return Attention(CFG, generator=torch.Generator().manual_seed(3), device="cpu").float()
+
+
+def _cache(requests, dtype=torch.float32, pages=40, page=16, layers=1):
+    return bf.PagedKVCache(num_layers=layers, num_pages=pages, max_requests=requests, num_kv_heads=CFG.num_kv_heads,
+                           head_dim=CFG.head_dim, page_size=page, dtype=dtype, device="cpu")
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _close(got, want):
+    assert got.shape == want.shape
+    assert (got - want).abs().max() <= 2.0 ** -12 * want.abs().max()
+
+
+class _Requests:
+    """Requests over pages, and each of them over a list cache of its own."""
+
+    def __init__(self, n):
+        self.attn, self.pool, self.lists = _attention(), _cache(n), [[] for _ in range(n)]
+        self.held, self.g = [0] * n, torch.Generator().manual_seed(n)
+
+    def step(self, counts, each, rope=None):
+        x = torch.randn(len(counts), each, CFG.hidden_size, generator=self.g)
+        self.pool.begin(_i32(counts), each)
+        y = self.attn(x, cache=self.pool.layers[0], position_embeddings=rope(self) if rope else None)
+        for r, c in enumerate(counts):
+            if c > 0:
+                _close(y[r, :c], self.attn(x[r:r + 1, :c], cache=self.lists[r])[0])
+                self.held[r] += c
+        assert self.pool.lengths.tolist() == self.held and self.pool.sync() >= 0
+
+
+def _table(_):
+    return RopeTable(*rope_cos_sin(torch.arange(200), CFG.head_dim, CFG.rope_theta), None)
+
+
+@pytest.mark.parametrize("rope", [None, _table])
+def test_one_token_of_requests_of_different_lengths(rope):
+    s = _Requests(4)
+    s.step([7, 20, 0, 1], 20, rope)
+    for counts in ([1, 1, 1, 1], [1, 0, 1, 1], [1, 1, 0, 0]):
+        s.step(counts, 1, rope)
+
+
+@pytest.mark.parametrize("rope", [None, _table])
+def test_parts_behind_what_each_request_holds(rope):
+    s = _Requests(3)
+    s.step([20, 20, 20], 20, rope)        # prompts of one length
+    s.step([3, 3, 3], 3, rope)            # drafts behind them
+    s.step([5, 2, 0], 5, rope)            # counts below the step's rows, an idle request
+    s.step([4, 4, 4], 4, rope)            # requests of different lengths
+    s.step([0, 0, 0], 2, rope)
+    s.step([1, 1, 1], 1, rope)
+
+
+def test_rows_of_position_embeddings_of_each_requests_own():
+    s = _Requests(2)
+    s.step([9, 4], 9)
+    own = lambda s: rope_cos_sin(torch.cat([torch.arange(n, n + 3) for n in s.held]), CFG.head_dim, CFG.rope_theta)
+    s.step([3, 3], 3, own)
+    one = lambda s: rope_cos_sin(torch.tensor(s.held), CFG.head_dim, CFG.rope_theta)
+    s.step([1, 1], 1, one)
+    shared = lambda s: rope_cos_sin(torch.arange(12, 15), CFG.head_dim, CFG.rope_theta)
+    with pytest.raises(ValueError, match="own"):
+        s.step([3, 3], 3, shared)
+    with pytest.raises(ValueError, match="rows of position_embeddings"):
+        s.step([3, 3], 3, lambda s: rope_cos_sin(torch.arange(4), CFG.head_dim, CFG.rope_theta))
+
+
+def test_a_step_that_starts_elsewhere_is_refused():
+    pool = _cache(2)
+    pool.begin(_i32([7, 7]), 7, start=0)
+    before = [x.clone() for x in (pool.lengths, pool.state, pool.block_table)]
+    for start in (0, 6, 8):
+        with pytest.raises(ValueError, match="hold"):
+            pool.begin(_i32([2, 2]), 2, start=start)
+    assert all(torch.equal(a, b) for a, b in zip(before, (pool.lengths, pool.state, pool.block_table)))
+    pool.begin(_i32([2, 1]), 2, start=7)
+    with pytest.raises(ValueError, match="hold"):
+        pool.begin(_i32([2, 2]), 2, start=9)
+    pool.begin(_i32([2, 2]), 2)
+
+
+def test_a_part_of_a_prompt_goes_behind_the_tokens_that_are_there():
+    model = Decoder(CFG, seed=1, device="cpu")
+    tokens = torch.randint(0, CFG.vocab_size, (2, 30), generator=torch.Generator().manual_seed(1))
+    pool = _cache(2, torch.bfloat16, layers=2)
+    model.forward(tokens[:, :20], pool.layers, 0)
+    for start in (0, 19, 30):
+        with pytest.raises(ValueError, match="hold"):
+            model.forward(tokens[:, 20:], pool.layers, start)
+    got = model.forward(tokens[:, 20:], pool.layers, 20)
+    lists = [[] for _ in range(2)]
+    model.forward(tokens[:, :20], lists, 0)
+    assert torch.equal(got, model.forward(tokens[:, 20:], lists, 20))
+    assert pool.lengths.tolist() == [30, 30]
