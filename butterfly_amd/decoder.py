@@ -973,15 +973,18 @@ class Decoder(nn.Module):
         eagerly, then the compressed caches switch to device counters; the first decode step
         runs eagerly and the next one (every layer, argmax, position advance) is
         captured and replayed ``new_tokens - 2`` times with no host
-        synchronisation in between.
+        synchronisation in between.  A paged cache is empty before.
         """
+        for pool in self._paged_pools(caches, prompt.shape[0]):
+            pool.require(0)
         logits = self.forward(prompt, caches, 0)
         return self.greedy_graph_from_logits(logits, prompt.shape[1], new_tokens, caches)
 
     @torch.no_grad()
     def greedy_graph_from_logits(self, logits: torch.Tensor, t: int, new_tokens: int, caches: List,
                                  timed: bool = False, on_step: Optional[Callable[[int], None]] = None) -> torch.Tensor:
-        """The decode part of ``greedy_graph`` after a prefill of ``t`` tokens that produced ``logits``.
+        """The decode part of ``greedy_graph`` after a prefill of ``t`` tokens that produced ``logits`` (over pages alone, of
+        at most ``t`` tokens a request).
 
         With ``timed`` the replays are bracketed by device synchronisations and
         their wall time is kept in ``self.last_graph_decode_s``.  ``on_step(i)`` is called after
@@ -1002,6 +1005,8 @@ class Decoder(nn.Module):
                     f"of at most 16 blocks, or a dense layer over a PagedLayer); use greedy() for this configuration")
         compressed = [c for c in caches if isinstance(c, CompressedKVCache)]
         pools = self._paged_pools(caches, b)
+        for pool in pools:
+            pool.require(t, at_most=not compressed)
         for c in compressed:
             c.use_device_counters()
         one_each = torch.ones(b, dtype=torch.int32, device=dev)
@@ -1138,7 +1143,10 @@ class Decoder(nn.Module):
     @torch.no_grad()
     def greedy(self, prompt: torch.Tensor, new_tokens: int, caches: List,
                on_token: Optional[Callable[[int], None]] = None) -> torch.Tensor:
-        """Prefill ``prompt`` [B, T] in one call, then ``new_tokens`` greedy steps; returns [B, new_tokens]."""
+        """Prefill ``prompt`` [B, T] in one call, then ``new_tokens`` greedy steps; returns [B, new_tokens].  A paged cache
+        is empty before."""
+        for pool in self._paged_pools(caches, prompt.shape[0]):
+            pool.require(0)
         logits = self.forward(prompt, caches, 0)
         out = []
         pos = prompt.shape[1]

@@ -479,14 +479,15 @@ class PagedKVCache:
         """A step whose rows follow each other, request by request: ragged prompts."""
         return self._begin(counts, num_rows, 0)
 
-    def require(self, tokens: int) -> bool:
-        """``ValueError`` unless every request holds ``tokens`` tokens (waits for the current stream).  ``False`` where an
-        earlier step did not fit: lengths stand still then, until :meth:`sync` reports it."""
+    def require(self, tokens: int, *, at_most: bool = False) -> bool:
+        """``ValueError`` unless every request holds ``tokens`` tokens, or ``at_most`` as many (waits for the current
+        stream).  ``False`` where an earlier step did not fit: lengths stand still then, until :meth:`sync` reports it."""
         *lengths, _, error = self._read(torch.cat([self.lengths, self.state]))
         if error:
             return False
-        if any(n != tokens for n in lengths):
-            raise ValueError(f"the paged cache's requests hold {lengths} tokens, not {tokens} each (release() empties them)")
+        if any(n > tokens or n < tokens and not at_most for n in lengths):
+            raise ValueError(f"the paged cache's requests hold {lengths} tokens, not {'at most ' * at_most}{tokens} each "
+                             "(release() empties them)")
         return True
 
     def held(self) -> List[Optional[int]]:

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import butterfly_amd as bf
-from butterfly_amd.decoder import Attention, DecoderConfig, RopeTable, rope_cos_sin
+from butterfly_amd.decoder import Attention, Decoder, DecoderConfig, RopeTable, rope_cos_sin
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,19 @@ def test_several_tokens_are_not_captured():
             attn(x, cache=pool.layers[0])
     torch.cuda.synchronize()
     assert pool.lengths.tolist() == [0, 0]
+
+
+def test_greedy_graph_goes_on_from_the_prefill_it_is_told():
+    cfg = _config(64)
+    model = Decoder(cfg, seed=1)
+    prompt = torch.randint(0, cfg.vocab_size, (2, 9), generator=torch.Generator().manual_seed(1)).cuda()
+    pool, other = _cache(cfg, 2), _cache(cfg, 2)
+    out = model.greedy_graph(prompt, 6, pool.layers)
+    with pytest.raises(ValueError, match="hold"):
+        model.greedy_graph(prompt, 6, pool.layers)
+    with pytest.raises(ValueError, match="hold"):
+        model.greedy_graph(prompt[:, :1], 6, pool.layers)
+    logits = model.forward(prompt, other.layers, 0)
+    with pytest.raises(ValueError, match="at most 8"):       # the tables of its steps would be too short
+        model.greedy_graph_from_logits(logits, 8, 6, other.layers)
+    assert torch.equal(model.greedy_graph_from_logits(logits, 9, 6, other.layers), out)

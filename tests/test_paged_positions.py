@@ -122,3 +122,18 @@ def test_a_part_of_a_prompt_goes_behind_the_tokens_that_are_there():
     model.forward(tokens[:, :20], lists, 0)
     assert torch.equal(got, model.forward(tokens[:, 20:], lists, 20))
     assert pool.lengths.tolist() == [30, 30]
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_greedy_starts_from_an_empty_cache(tokens):
+    model = Decoder(CFG, seed=1, device="cpu")
+    prompt = torch.randint(0, CFG.vocab_size, (2, tokens), generator=torch.Generator().manual_seed(1))
+    pool = _cache(2, torch.bfloat16, layers=2)
+    out = model.greedy(prompt, 4, pool.layers)
+    held = pool.lengths.clone()
+    for run in (model.greedy, model.greedy_graph):
+        with pytest.raises(ValueError, match="hold"):
+            run(prompt, 4, pool.layers)
+    assert torch.equal(pool.lengths, held)
+    pool.release(range(2))
+    assert torch.equal(model.greedy(prompt, 4, pool.layers), out)
