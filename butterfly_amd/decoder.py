@@ -675,6 +675,7 @@ class Attention(nn.Module):
         hold and the part itself, for which the lengths are read back once a step; requests of different lengths
         one by one.  Rows without a token (idle requests, counts below the step's rows) are undefined."""
         b, t, _ = x.shape
+        cache.check_step(b, t)
         if self.takes_paged_rows(x, cache, rope):
             return self.forward_paged_rows(self.qkv(x), cache, rope)
         held = cache.cache.held() if t > 1 else []

@@ -398,6 +398,14 @@ class PagedLayer:
             raise RuntimeError("begin() a step of the paged cache before its layers")
         return self.cache.plan
 
+    def check_step(self, requests: int, rows_each: int) -> None:
+        """``ValueError`` unless the step has ``rows_each`` rows of each of ``requests`` requests."""
+        c = self.cache
+        if c.plan is not None and (c.max_requests != requests or c.rows_each != rows_each):
+            has = f"{c.rows_each} rows of each" if c.rows_each else "packed rows"
+            raise ValueError(f"the paged cache's step has {has} of its {c.max_requests} requests, not {rows_each} of each of "
+                             f"{requests}")
+
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """The step's rows of keys and values [N, Hkv, d] into their slots."""
         paged_append(k, v, self.k_pages, self.v_pages, self.plan.slots)
@@ -476,7 +484,8 @@ class PagedKVCache:
         return plan
 
     def begin_packed(self, counts: torch.Tensor, num_rows: int) -> PagedPlan:
-        """A step whose rows follow each other, request by request: ragged prompts."""
+        """A step whose rows follow each other, request by request: ragged prompts (for the layers' operators; an
+        attention module has rows of every request, :meth:`begin`)."""
         return self._begin(counts, num_rows, 0)
 
     def require(self, tokens: int, *, at_most: bool = False) -> bool:

@@ -137,3 +137,19 @@ def test_greedy_starts_from_an_empty_cache(tokens):
     assert torch.equal(pool.lengths, held)
     pool.release(range(2))
     assert torch.equal(model.greedy(prompt, 4, pool.layers), out)
+
+
+def test_steps_of_other_rows_are_refused():
+    attn, pool = _attention(), _cache(3)
+    x = torch.randn(3, 4, CFG.hidden_size)
+    pool.begin_packed(_i32([6, 2, 4]), 12)
+    for y in (x, x.view(1, 12, -1), x.view(12, 1, -1)):
+        with pytest.raises(ValueError, match="packed rows"):
+            attn(y, cache=pool.layers[0])
+    pool.begin_packed(_i32([2, 0, 1]), 3)                     # three rows of two requests
+    with pytest.raises(ValueError, match="packed rows"):
+        attn(x[:, :1], cache=pool.layers[0])
+    pool.begin(_i32([4, 4, 4]), 4)
+    for y in (x.view(4, 3, -1), x.view(1, 12, -1), x[:, :1]):
+        with pytest.raises(ValueError, match="4 rows of each"):
+            attn(y, cache=pool.layers[0])
