@@ -542,6 +542,10 @@ class RopeTable:
     def rows(self):
         return self.cos_tab.index_select(0, self.pos), self.sin_tab.index_select(0, self.pos)
 
+    def plain(self) -> bool:
+        """Whether the rows are the tables' (``rows`` as it stands above)."""
+        return type(self).rows is RopeTable.rows and "rows" not in self.__dict__
+
     def at(self, positions: torch.Tensor):
         """The tables' rows of ``positions`` [N]; NaN for a position outside them."""
         n = self.cos_tab.shape[0]
@@ -555,7 +559,7 @@ class RopeTable:
         ``d`` columns on ``x``'s device, ``rows`` as it stands above.  Two row selections and their launches less for each layer: a step of
         eight sequences through four layers is 214 us so, 231 with the selections."""
         tabs, pos = (self.cos_tab, self.sin_tab), self.pos
-        return (type(self).rows is RopeTable.rows and "rows" not in self.__dict__ and pos.dtype == torch.int64 and pos.numel() == 1 and pos.device == x.device
+        return (self.plain() and pos.dtype == torch.int64 and pos.numel() == 1 and pos.device == x.device
                 and tabs[0].shape == tabs[1].shape
                 and all(t.dtype == torch.float32 and t.ndim == 2 and t.shape[1] == d and t.shape[0] > 0
                         and t.is_contiguous() and t.device == x.device for t in tabs))
@@ -643,7 +647,7 @@ class Attention(nn.Module):
         """``cache``: a list ``[k, v]`` of the full history (empty before the first call), or a ``PagedLayer``
         whose cache has begun the step; ``position_embeddings``: ``(cos, sin)`` rows of the call's positions
         (or a ``RopeTable``), else computed from the cache length.  Over pages the plan has the positions: a ``RopeTable``
-        is read at those."""
+        is read at those (one with ``rows`` of its own gives the call's)."""
         if isinstance(cache, PagedLayer):
             return self._forward_paged(x, cache, position_embeddings)
         positions = None
@@ -705,7 +709,7 @@ class Attention(nn.Module):
         b, t, _ = x.shape
         positions = cache.plan.positions
         if isinstance(rope, RopeTable):
-            rope = rope.at(positions)
+            rope = rope.at(positions) if rope.plain() else rope.rows()
         if rope is not None:
             rope = tuple(r.reshape(-1, r.shape[-1]) for r in rope)
             rows = rope[0].shape[0]
@@ -723,7 +727,8 @@ class Attention(nn.Module):
     @staticmethod
     def takes_paged_rows(x: torch.Tensor, cache, rope) -> bool:
         """Whether this call is one token of every request over pages, fed with the raw q|k|v rows."""
-        return isinstance(cache, PagedLayer) and isinstance(rope, RopeTable) and x.shape[1] == 1 and _hip(x)
+        return (isinstance(cache, PagedLayer) and isinstance(rope, RopeTable) and rope.plain() and x.shape[1] == 1
+                and _hip(x))
 
     def forward_paged_rows(self, qkv: torch.Tensor, cache: PagedLayer, rope: "RopeTable") -> torch.Tensor:
         """The paged step from the fused projection's raw output rows (``takes_paged_rows`` held), through the

@@ -92,3 +92,33 @@ def test_greedy_graph_goes_on_from_the_prefill_it_is_told():
     with pytest.raises(ValueError, match="at most 8"):       # the tables of its steps would be too short
         model.greedy_graph_from_logits(logits, 8, 6, other.layers)
     assert torch.equal(model.greedy_graph_from_logits(logits, 9, 6, other.layers), out)
+
+
+class _Scaled(RopeTable):
+    """Positions at half their distance."""
+
+    def rows(self):
+        return rope_cos_sin(self.pos.double() / 2, self.cos_tab.shape[1], 1e4)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+def test_a_table_with_rows_of_its_own_is_asked_for_them(head_dim, own):
+    """A list cache asks it (``RopeTable.fits``): one token over pages turns as over a list."""
+    cfg = _config(head_dim)
+    attn = Attention(cfg, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    tabs = rope_cos_sin(torch.arange(64, device="cuda"), head_dim, cfg.rope_theta)
+    pool, lists = _cache(cfg, 2), []
+    g = torch.Generator().manual_seed(5)
+    for i in range(8):
+        x = torch.randn(2, 1, cfg.hidden_size, generator=g).bfloat16().cuda()
+        pos = torch.tensor([i], device="cuda")
+        table = _Scaled(*tabs, pos) if own else RopeTable(*tabs, pos)
+        if not own:
+            table.rows = lambda: rope_cos_sin(pos.double() / 2, head_dim, 1e4)
+        pool.begin(_i32([1, 1]))
+        with torch.no_grad():
+            y = attn(x, cache=pool.layers[0], position_embeddings=table)
+        want = attn(x, cache=lists, position_embeddings=table).float()
+        assert (y.float() - want).abs().max() <= 2.0 ** -5 * want.abs().max()
+    assert torch.equal(pool.layers[0].history(8)[0], lists[0]) and torch.equal(pool.layers[0].history(8)[1], lists[1])
