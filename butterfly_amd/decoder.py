@@ -680,6 +680,7 @@ class Attention(nn.Module):
         one by one.  Rows without a token (idle requests, counts below the step's rows) are undefined."""
         b, t, _ = x.shape
         cache.check_step(b, t)
+        cache.cache.check_heads(self.n_kv_heads, self.head_dim, x.dtype)
         if self.takes_paged_rows(x, cache, rope):
             return self.forward_paged_rows(self.qkv(x), cache, rope)
         held = cache.cache.held() if t > 1 else []
@@ -962,10 +963,11 @@ class Decoder(nn.Module):
             rope = RopeTable(*self._rope_tab, positions)
         return self._last_logits(x, positions, caches, rope).float()
 
-    @staticmethod
-    def _paged_pools(caches: List, batch: int) -> List[PagedKVCache]:
-        """The paged caches behind ``caches``, each once."""
+    def _paged_pools(self, caches: List, batch: int) -> List[PagedKVCache]:
+        """The paged caches behind ``caches``, each once, after what can be refused before a step of theirs."""
         pools = list({id(c.cache): c.cache for c in caches if isinstance(c, PagedLayer)}.values())
+        for pool in pools:
+            pool.check_heads(self.cfg.num_kv_heads, self.cfg.head_dim, self.embed_tokens.dtype)
         if any(pool.max_requests != batch for pool in pools):
             raise ValueError(f"a paged cache of {[p.max_requests for p in pools]} requests cannot take a batch of {batch}")
         return pools
@@ -1095,6 +1097,7 @@ class Decoder(nn.Module):
                              "each layer of the model")
         if not _hip(self.embed_tokens) or not all(isinstance(layer.self_attn, Attention) for layer in self.layers):
             raise ValueError("greedy_requests needs a bf16 model on the GPU whose layers all have stock attention")
+        self._paged_pools(cache.layers, b)
         if bool(cache.lengths.any()):
             raise ValueError("greedy_requests starts from an empty cache (release the requests it holds)")
         if new_tokens <= 0:

@@ -34,6 +34,7 @@ _PLAN, _APPEND, _ROPE, _ATTN = (_native.PAGED_STRUCTS["bfly_paged_" + x].pack
                                 for x in ("plan", "append", "rope_append", "attention"))
 _EMPTY = torch.empty_strided     # (0.95 us a call; torch.empty, which also sorts out layouts, 1.8)
 PAGE_SIZES = frozenset(1 << i for i in range(4, 11))
+HEAD_DIMS = (64, 128, 256)       # of paged_rope_append and paged_attention
 
 # state[1] after a plan that did not fit (include/butterfly_amd_paged.h)
 PLAN_ERRORS = {
@@ -487,6 +488,16 @@ class PagedKVCache:
         """A step whose rows follow each other, request by request: ragged prompts (for the layers' operators; an
         attention module has rows of every request, :meth:`begin`)."""
         return self._begin(counts, num_rows, 0)
+
+    def check_heads(self, num_kv_heads: int, head_dim: int, dtype: torch.dtype) -> None:
+        """``NotImplementedError`` or ``ValueError`` unless attention of such heads runs over these pages: before a
+        step begins, not in the middle of a generation."""
+        if head_dim not in HEAD_DIMS:
+            raise NotImplementedError(f"attention over pages: head_dim={head_dim} unsupported {HEAD_DIMS}")
+        _, _, heads, _, d = self.k_pages.shape
+        if (heads, d, self.k_pages.dtype) != (num_kv_heads, head_dim, dtype):
+            raise ValueError(f"a paged cache of {heads} kv heads of {d} in {self.k_pages.dtype} cannot take {num_kv_heads} of "
+                             f"{head_dim} in {dtype}")
 
     def require(self, tokens: int, *, at_most: bool = False) -> bool:
         """``ValueError`` unless every request holds ``tokens`` tokens, or ``at_most`` as many (waits for the current

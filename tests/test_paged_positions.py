@@ -6,6 +6,8 @@ other orders over at most 128 terms a sum (128 * 2^-24 of the terms' sizes) thro
 2^-12 of the largest output; a row at another position differs by the output's own size."""
 from __future__ import annotations
 
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -153,3 +155,27 @@ def test_steps_of_other_rows_are_refused():
     for y in (x.view(4, 3, -1), x.view(1, 12, -1), x[:, :1]):
         with pytest.raises(ValueError, match="4 rows of each"):
             attn(y, cache=pool.layers[0])
+
+
+@pytest.mark.parametrize("head_dim,dtype,kv,error", [(32, torch.bfloat16, 1, NotImplementedError),
+                                                     (96, torch.bfloat16, 1, NotImplementedError),
+                                                     (64, torch.float32, 1, ValueError), (64, torch.bfloat16, 2, ValueError),
+                                                     (128, torch.bfloat16, 1, ValueError)])
+def test_a_cache_the_model_cannot_decode_over_is_refused_before_the_prompt(head_dim, dtype, kv, error):
+    """head_dim is the cache's; the model has it too where no decode step would take it, else 64."""
+    cfg = replace(CFG, head_dim=head_dim if head_dim in (32, 96) else 64)
+    model = Decoder(cfg, seed=1, device="cpu")
+    pool = bf.PagedKVCache(num_layers=2, num_pages=8, max_requests=2, num_kv_heads=kv, head_dim=head_dim, page_size=16,
+                           dtype=dtype, device="cpu")
+    prompt = torch.zeros(2, 5, dtype=torch.long)
+    for run in (lambda: model.forward(prompt, pool.layers, 0), lambda: model.greedy(prompt, 3, pool.layers),
+                lambda: model.greedy_graph(prompt, 3, pool.layers)):
+        with pytest.raises(error):
+            run()
+    assert pool.lengths.tolist() == [0, 0] and pool.plan is None
+    pool.begin(_i32([5, 5]), 5)
+    x = torch.zeros(2, 5, CFG.hidden_size, dtype=torch.bfloat16)
+    pages = pool.k_pages.zero_().clone()
+    with pytest.raises(error):
+        model.layers[0].self_attn(x, cache=pool.layers[0])
+    assert torch.equal(pages, pool.k_pages)
