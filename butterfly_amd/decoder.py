@@ -965,7 +965,10 @@ class Decoder(nn.Module):
 
     def _paged_pools(self, caches: List, batch: int) -> List[PagedKVCache]:
         """The paged caches behind ``caches``, each once, after what can be refused before a step of theirs."""
-        pools = list({id(c.cache): c.cache for c in caches if isinstance(c, PagedLayer)}.values())
+        layers = [c for c in caches if isinstance(c, PagedLayer)]
+        if len({id(c) for c in layers}) != len(layers):
+            raise ValueError("every layer takes a PagedLayer of its own")
+        pools = list({id(c.cache): c.cache for c in layers}.values())
         for pool in pools:
             pool.check_heads(self.cfg.num_kv_heads, self.cfg.head_dim, self.embed_tokens.dtype)
         if any(pool.max_requests != batch for pool in pools):

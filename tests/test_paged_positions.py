@@ -179,3 +179,12 @@ def test_a_cache_the_model_cannot_decode_over_is_refused_before_the_prompt(head_
     with pytest.raises(error):
         model.layers[0].self_attn(x, cache=pool.layers[0])
     assert torch.equal(pages, pool.k_pages)
+
+
+def test_two_layers_do_not_share_their_pages():
+    model, pool = Decoder(CFG, seed=1, device="cpu"), _cache(2, torch.bfloat16, layers=2)
+    prompt = torch.zeros(2, 5, dtype=torch.long)
+    for run in (lambda c: model.forward(prompt, c, 0), lambda c: model.greedy(prompt, 3, c)):
+        with pytest.raises(ValueError, match="its own"):
+            run([pool.layers[0]] * 2)
+    assert pool.lengths.tolist() == [0, 0]
