@@ -15,8 +15,8 @@ Requests have lengths of their own, and nothing on the way of a decode step need
 
 :class:`PagedKVCache` holds the tensors of all layers and the bookkeeping they share.  Every call runs on
 the current stream of its tensors' device, allocates only its outputs (and a workspace of its own, so
-captured graphs share none), and can be captured in a HIP graph.  The operators are for inference: with
-gradients enabled they refuse tensors that require them.
+captured graphs share none), and can be captured in a HIP graph.  The operators are for inference: they refuse
+tensors that require gradients (with gradients enabled) or carry tangents, and traces.
 """
 from __future__ import annotations
 
@@ -26,6 +26,8 @@ from operator import index
 from typing import Iterable, List, NamedTuple, Optional
 
 import torch
+from torch import _C
+from torch.autograd import forward_ad
 
 from . import _native
 from ._device import _GET_DEVICE, stream_of
@@ -60,6 +62,14 @@ class PagedPlan(NamedTuple):
 # The checks below cost a decode step's host time (these calls take 4 to 8 us on the GPU): each tests what a
 # well-formed call has in as few attribute reads as it takes, and only then, case by case, what is wrong.
 _GRAD = "the paged operators are for inference: call them under torch.no_grad()"
+
+
+def _check_followed(*tensors: Optional[torch.Tensor]) -> None:
+    """Refuses what a native call would hide itself from: a trace, or a tangent of one of ``tensors``."""
+    if _C._get_tracing_state() is not None:
+        raise ValueError("the paged operators cannot be traced: a trace would hold this call's result as a constant")
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(_GRAD + " and without tangents")
 
 
 def _device_of(t: torch.Tensor) -> int:
@@ -175,6 +185,8 @@ def paged_plan(block_table: torch.Tensor, lengths: torch.Tensor, counts: torch.T
         with torch.cuda.device(dev):
             return paged_plan(block_table, lengths, counts, free_pages, state, page_size=page_size, num_rows=num_rows,
                               rows_each=rows_each, in_place=in_place)
+    if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
+        _check_followed()
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
     if lengths.dim() != 1:
@@ -235,6 +247,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
             return paged_append(k, v, k_pages, v_pages, slots)
     if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise ValueError(_GRAD)
+    if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
+        _check_followed(k, v, k_pages, v_pages)
     shape, strides = _pages(k_pages, v_pages, dev, True)
     n, hkv, d = _check_rows(k, v, shape, k_pages.dtype, slots, dev)
     code = _dtype_code(k_pages.dtype)
@@ -276,6 +290,8 @@ def paged_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
                                     or q_weight is not None and q_weight.requires_grad
                                     or k_weight is not None and k_weight.requires_grad):
         raise ValueError(_GRAD)
+    if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
+        _check_followed(q, k, v, k_pages, v_pages, cos, sin, q_weight, k_weight)
     shape, strides = _pages(k_pages, v_pages, dev, True)
     dtype = k_pages.dtype
     n, hkv, d = _check_rows(k, v, shape, dtype, slots, dev)
@@ -345,6 +361,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
                                    return_stats=return_stats)
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise ValueError(_GRAD)
+    if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
+        _check_followed(q, k_pages, v_pages)
     shape, strides = _pages(k_pages, v_pages, dev, False)
     pages, hkv, page_size, d = shape
     sq, dtype = q.shape, q.dtype
