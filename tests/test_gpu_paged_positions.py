@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import butterfly_amd as bf
-from butterfly_amd.decoder import Attention, Decoder, DecoderConfig, RopeTable, rope_cos_sin
+from butterfly_amd.decoder import Attention, Decoder, DecoderConfig, RopeTable, add_rms_norm, rope_cos_sin
 
 pytestmark = pytest.mark.gpu
 
@@ -27,6 +27,21 @@ def _cache(cfg, requests, pages=40, page=16):
 
 def _i32(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _check_history(attn, cfg, layer, request, rows, start):
+    """The request's keys and values from ``start`` on are those of the projection ``rows`` at their positions."""
+    n, d = rows.shape[0], cfg.head_dim
+    hk, hv = (x[:, :, start:] for x in layer.history(start + n, request))
+    heads = rows.view(n, -1, d).transpose(0, 1)[None]
+    assert torch.equal(hv, heads[:, -cfg.num_kv_heads:])
+    k = heads[:, cfg.num_heads:cfg.num_heads + cfg.num_kv_heads].double()
+    k = k / (k.square().mean(-1, keepdim=True) + attn.k_norm.eps).sqrt() * attn.k_norm.weight.double()
+    cos, sin = (t.double() for t in rope_cos_sin(torch.arange(start, start + n, device="cuda"), d, cfg.rope_theta))
+    turned = torch.cat([-k[..., d // 2:], k[..., :d // 2]], -1) * sin
+    # fp32 arithmetic (some d 2^-24) and one or two roundings to bf16, the first before the turn
+    bound = 2.0 ** -8 * 1.02 * ((k * cos).abs() + turned.abs()) + 2.0 ** -8 * (k * cos + turned).abs()
+    assert bool(((hk.double() - (k * cos + turned)).abs() <= bound).all())
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
@@ -51,16 +66,7 @@ def test_rows_are_at_the_plans_positions(head_dim, table):
                 raw[r].append(rows[r, :c])
         assert pool.lengths.tolist() == held and pool.sync() >= 0
     for r in range(3):
-        hk, hv = pool.layers[0].history(held[r], r)
-        heads = torch.cat(raw[r]).view(held[r], -1, head_dim).transpose(0, 1)[None]
-        assert torch.equal(hv, heads[:, -cfg.num_kv_heads:])
-        k = heads[:, cfg.num_heads:cfg.num_heads + cfg.num_kv_heads].double()
-        k = k / (k.square().mean(-1, keepdim=True) + attn.k_norm.eps).sqrt()
-        cos, sin = (t.double() for t in rope_cos_sin(torch.arange(held[r], device="cuda"), head_dim, cfg.rope_theta))
-        turned = torch.cat([-k[..., head_dim // 2:], k[..., :head_dim // 2]], -1) * sin
-        # fp32 arithmetic (some d 2^-24) and one or two roundings to bf16, the first before the turn
-        bound = 2.0 ** -8 * 1.02 * ((k * cos).abs() + turned.abs()) + 2.0 ** -8 * (k * cos + turned).abs()
-        assert bool(((hk.double() - (k * cos + turned)).abs() <= bound).all())
+        _check_history(attn, cfg, pool.layers[0], r, torch.cat(raw[r]), 0)
 
 
 def test_several_tokens_are_not_captured():
@@ -122,3 +128,28 @@ def test_a_table_with_rows_of_its_own_is_asked_for_them(head_dim, own):
         want = attn(x, cache=lists, position_embeddings=table).float()
         assert (y.float() - want).abs().max() <= 2.0 ** -5 * want.abs().max()
     assert torch.equal(pool.layers[0].history(8)[0], lists[0]) and torch.equal(pool.layers[0].history(8)[1], lists[1])
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_captured_ragged_steps_leave_each_requests_own_rows(head_dim):
+    """First layer: the prompts' keys and values are the list cache's, bit for bit, and each later row is its token's
+    projection at its own position."""
+    cfg = _config(head_dim)
+    model = Decoder(cfg, seed=7)
+    attn, norm = model.layers[0].self_attn, model.layers[0].input_layernorm
+    g = torch.Generator(device="cuda").manual_seed(head_dim)
+    for w in (attn.q_norm.weight, attn.k_norm.weight, norm.weight):
+        w.data = (1 + 0.3 * torch.randn(w.shape, generator=g, device="cuda")).bfloat16()
+    prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=torch.Generator().manual_seed(n)).cuda() for n in (1, 33, 120, 64)]
+    pool = _cache(cfg, 4)
+    out = model.greedy_requests(prompts, 30, pool)
+    steps = []
+    with torch.no_grad():
+        for i in range(29):
+            x = torch.nn.functional.embedding(out[:, i:i + 1], model.embed_tokens)
+            steps.append(attn.qkv(add_rms_norm(x, None, norm.weight, norm.eps)[1]))
+    for r, p in enumerate(prompts):
+        lists = [[]]
+        model.forward(p[None], lists, 0)
+        assert all(torch.equal(a, b) for a, b in zip(pool.layers[0].history(p.numel(), r), lists[0]))
+        _check_history(attn, cfg, pool.layers[0], r, torch.cat([s[r] for s in steps]), p.numel())
