@@ -253,8 +253,14 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a) {
 // kHeads = 1: a decode step's few rows, spread as wide as they go; what they write stays in the caches for the
 // attention that follows.  kHeads = 4, from kManyHeads heads' rows on: a group takes four heads of a token, so
 // four loads are under way over one position's cos and sin, and moves them past the caches.
-// Both sides, us (16/4 heads of d 128, bf16, whole rotation; one head / four): 32 rows 3.1 / 6.0, 1024 6.2 / 7.8, 2048
-// 9.3 / 9.4, 4096 15.1 / 14.5, 16384 52 / 47; d 256 in bf16, 16384 rows: 103 / 83.
+// Both sides, us (16/4 heads, whole rotation; one head / four; the rule changes at 2731 rows):
+//            32 rows     1024         2048         2731         4096         16384
+//   bf16  64  2.8 / 5.5   4.4 / 6.5    6.0 / 7.2    6.8 / 7.7    8.9 / 9.0   29.2 / 25.8
+//   bf16 128  2.9 / 5.9   6.0 / 7.4    9.0 / 9.5   10.5 / 11.1  16.0 / 15.3  51.6 / 45.3
+//   bf16 256  2.9 / 6.3   9.1 / 9.7   16.1 / 14.9  20.7 / 18.9  29.5 / 26.8   102 / 84.6
+//   fp32  64  2.5 / 4.6   5.0 / 6.0    7.4 / 7.6    8.7 / 8.8   13.0 / 11.9  41.9 / 39.8
+//   fp32 128  2.6 / 4.8   7.7 / 7.7   13.5 / 11.8  16.8 / 15.5  23.7 / 23.3  85.1 / 73.9
+//   fp32 256  2.7 / 4.9  13.8 / 12.4  24.5 / 23.7  30.1 / 28.7  44.9 / 40.1   176 / 142
 constexpr int64_t kManyHeads = 1 << 16;
 
 struct RopeAppendArgs {

@@ -22,30 +22,44 @@
 // Rows that hold no token the request sees (behind the last one, before the window) are read with their tile; their
 // scores become -inf and their V zero, whatever they hold.
 //
-// Bound by HBM: keys and values are read once (4 hq / (2 hkv size) flops a byte, 4 to 32 here, against some 250 that
-// the card's product and copy rates take).  Kernel times: 1.36 GB of 32 requests of up to 131072 tokens 209 us
-// (6.5 TB/s; a large copy on this card moves 4.96), 262144 tokens of d 256 161 us (6.7); 32768 tokens of one
-// request 15.5 us, of which some 3 us are four dependent reads (arguments, lengths, page, K) and the sums' way
+// Bound by HBM: keys and values are read once (2 group / size flops a byte for groups of `group` query heads over a kv
+// head: 4 for groups of 4 in bf16, 2 in fp32, 1 without groups in bf16, 16 for groups of 16, against some 250 that the
+// card's product and copy rates take).  Kernel times: 1.36 GB of 32 requests of up to 131072 tokens 207 us
+// (6.6 TB/s; reading alone reaches 7.0 on this card), 262144 tokens of d 256 160 us (6.7); 32768 tokens of one
+// request 16.0 us, of which some 3 us are four dependent reads (arguments, lengths, page, K) and the sums' way
 // through LDS, and 3.9 us for the join.
+//
+// The schedule is every workgroup's own work over all lengths: hidden up to some hundreds of requests, and beyond as
+// many passes as there are workgroups.  One request of 40000 tokens among requests of 100 (8/2 heads of 128), us: alone
+// 17, 64 requests 20, 512 44, 4096 769, 16384 10248; 4096 and 16384 of 100 tokens over tables that hold no more
+// (no schedule): 122, 479.  Batches beyond a thousand requests pass short contexts with the first columns of
+// their table.
 #include "paged.h"
 
 namespace bfly {
 
 constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
-// Whole calls, us, with 256 / 512 / 1024 runs: one request of 32768 tokens 21.6 / 22.0 / 22.1, 131072 tokens x 32 247 /
-// 248 / 247, 262144 tokens of d 256 193 / 196 / 199, 64 of up to 2000 tokens with 32/8 heads 39.8 / 43.6 / 40.6.
-// c at least 1 / 2: one request of 1024 tokens 9.9 / 11.4.  Two tiles of a wave under way instead of one: 131072 tokens x 32
-// 227 -> 237 (334 registers), 64 of up to 2000 38.5 -> 41.2.
-// Workgroups of 4 / 8 waves: 64 of up to 2000 tokens 39.8 / 46.9, one of 32768 21.6 / 21.6.
+// Calls replayed from a graph, us, with 256 / 512 / 1024 runs (d 128 where nothing else stands): one request of 32768 tokens
+// 19.1 / 19.7 / 23.6, 131072 tokens x 32 223 / 223 / 222, 262144 tokens of d 256 174 / 177 / 182, 64 of 4096 tokens with 32/8
+// heads 174 / 173 / 180; fp32: 32768 tokens 30.9 / 31.8 / 35.9, 8 of 30000 160 / 164 / 165, 4 of 30000 of d 256 163 / 168 / 176.
+// c at least 1 / 2: one request of 1024 tokens 9.6 / 11.3, four of up to 4096 in fp32 11.4 / 13.0.
+// Two tiles of a wave under way instead of one: 131072 tokens x 32 223 -> 231, 64 of up to 2000 with 32/8 heads 37.9 -> 40.8,
+// 262144 tokens of d 256 174 -> 367 (226 registers spill).
+// Workgroups of 4 / 8 waves: 131072 tokens x 32 223 / 227, 64 of up to 2000 37.9 / 36.7, one of 1024 9.6 / 15.2, fp32 of d 256
+// 164 / 207.
 // Tiles of d 64 have half the bytes and half the registers: two runs a CU (512 / 256 runs: 8 requests of 60000 tokens
-// 86.0 / 88.0, fp32 8 of 30000 86.7 / 92.5; d 128 in fp32 166 / 161).
+// 83.7 / 86.6, fp32 8 of 30000 85.4 / 90.4).
 constexpr int runs_for(int head_dim) { return head_dim <= 64 ? 512 : 256; }   // in all, where requests and heads leave them
 constexpr int kMaxRuns = 512;
 constexpr int kMinRun = 1;            // c at least
 // Rounds that stay one run, and without a second launch where the tables hold no more: 512 keys (bf16) are done before a
 // join of two runs, and the more pairs of request and head (x16 query heads) there are, the longer runs hide behind each
-// other.  Measured, this many / the next fewer, us: 128 pairs of 1000 tokens 18.3 / 20.9, 512 of up to 2000 87.6 / 90.7
-// (all 2000), 2048 and more of up to 3000 287 / 380; 512 of up to 4000 with 32 instead of 16: 69.6 / 63.4.
+// other.  Measured, half as many / this many / twice as many for all pairs, us: 128 pairs of 1000 tokens 19.8 / 18.0 /
+// 18.1; 512 pairs of 2000 tokens 90.7 / 86.5 / 86.8, of up to 2000 (a mixed load) 37.8 / 45.1 / 45.1, of up to 4000
+// 58.8 / 58.9 / 84.4, fp32 of up to 2000 62.7 / 62.7 / 98.1; 2048 pairs of up to 3000 164 / 146 (32 rounds either way
+// for twice); one request of 1024 tokens 9.6 / 9.6 / 15.3.
+// The pairs are the call's, idle requests among them: one request of 4000 tokens among 127 idle ones of 4 kv heads 13.7
+// us, alone 10.7.
 constexpr int whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 // A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
 // c >= total / runs_for, fewer than twice runs_for: the partials there can be.  (kSlack: the total is a sum of floats.)
@@ -242,8 +256,8 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 // V rows are read once, whole lines an instruction, past the caches' replacement: the K half-lines of two
 // neighbouring instructions then stay until both have been taken.  Measured, V past the caches / nothing / K and V,
-// us: 131072 tokens x 32 227 / 247 / 246, 262144 tokens of d 256 175 / 193 / 172, 64 requests of 4096 tokens 175 / 194 /
-// 177, one of 1024 (in the caches) 10.3 / 9.9 / 10.6.
+// us: 131072 tokens x 32 223 / 246 / 241, 262144 tokens of d 256 174 / 191 / 172, 64 requests of 4096 tokens 174 / 192 /
+// 175, one of 1024 (in the caches) 9.6 / 9.3 / 10.2.
 template <typename V>
 __device__ __forceinline__ V stream_load(const char* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
@@ -326,8 +340,8 @@ struct Sweep<__bf16, D> {
       for (int w = 0; w < W; ++w) v[j][h][w] = 0;
   }
   // The weights enter as two bf16 parts, 16 bits of them: with one part (8 bits) a weight would be off by
-  // as much as the output's own rounding, and the second part hides behind the loads (131072 tokens x 32: 249 us
-  // with it, 246 without).  kSafe: the second part skips V's infinities and NaN, which the
+  // as much as the output's own rounding, and the second part hides behind the loads (131072 tokens x 32: 223 us
+  // with it, 222 without).  kSafe: the second part skips V's infinities and NaN, which the
   // first one has carried into the sums already (p * inf is inf, but the rest of p may be 0).
   template <bool kSafe>
   __device__ __forceinline__ void add(const float (&p)[8]) {
