@@ -153,3 +153,23 @@ def test_captured_ragged_steps_leave_each_requests_own_rows(head_dim):
         model.forward(p[None], lists, 0)
         assert all(torch.equal(a, b) for a, b in zip(pool.layers[0].history(p.numel(), r), lists[0]))
         _check_history(attn, cfg, pool.layers[0], r, torch.cat([s[r] for s in steps]), p.numel())
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_rows_of_position_embeddings_that_are_not_the_calls_are_refused(paged):
+    """Their numbers of rows and columns are the kernel's bounds."""
+    cfg = _config(128)
+    attn = Attention(cfg, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    x = torch.randn(2, 6, cfg.hidden_size, device="cuda").bfloat16()
+    cos, sin = rope_cos_sin(torch.arange(6, device="cuda"), 128, cfg.rope_theta)
+    cache = []
+    if paged:
+        pool = _cache(cfg, 2)
+        pool.begin(_i32([6, 6]), 6)
+        cache = pool.layers[0]
+    with torch.no_grad():
+        for rope in [(cos[:, :64], sin[:, :64]), (cos[:5], sin[:5]), (cos, sin[:5]), (cos, sin[:, :64]), (cos.cpu(), sin.cpu()),
+                     (cos, sin.cpu())]:
+            with pytest.raises(ValueError):
+                attn(x, cache=cache, position_embeddings=rope)
+        attn(x, cache=cache, position_embeddings=(cos[None], sin[None]))
