@@ -682,12 +682,12 @@ class Attention(nn.Module):
         one by one.  Rows without a token (idle requests, counts below the step's rows) are undefined."""
         b, t, _ = x.shape
         cache.check_step(b, t)
-        cache.cache.check_heads(self.n_kv_heads, self.head_dim, x.dtype)
         if self.takes_paged_rows(x, cache, rope):
             return self.forward_paged_rows(self.qkv(x), cache, rope)
         held = cache.cache.held() if t > 1 else []
         starts = sorted({n for n in held if n is not None})
         q, k, v = self._project_paged(x, cache, rope, shared=len(starts) <= 1)
+        cache.cache.check_heads(self.n_kv_heads, self.head_dim, k.dtype)
         cache.append(k.transpose(1, 2).reshape(b * t, *k.shape[1::2]), v.transpose(1, 2).reshape(b * t, *v.shape[1::2]))
         if t == 1:
             return self.output(cache.attend(q, scale=self.scale))
@@ -972,7 +972,9 @@ class Decoder(nn.Module):
             raise ValueError("every layer takes a PagedLayer of its own")
         pools = list({id(c.cache): c.cache for c in layers}.values())
         for pool in pools:
-            pool.check_heads(self.cfg.num_kv_heads, self.cfg.head_dim, self.embed_tokens.dtype)
+            # (under autocast the products' type is not the weights': the operators see it)
+            pool.check_heads(self.cfg.num_kv_heads, self.cfg.head_dim,
+                             pool.k_pages.dtype if torch.is_autocast_enabled() else self.embed_tokens.dtype)
         if any(pool.max_requests != batch for pool in pools):
             raise ValueError(f"a paged cache of {[p.max_requests for p in pools]} requests cannot take a batch of {batch}")
         return pools

@@ -188,3 +188,17 @@ def test_two_layers_do_not_share_their_pages():
         with pytest.raises(ValueError, match="its own"):
             run([pool.layers[0]] * 2)
     assert pool.lengths.tolist() == [0, 0]
+
+
+def test_an_fp32_attention_under_autocast_takes_bf16_pages():
+    """The products' type counts.  (q, k and v are the same bf16 rows for both caches; the softmax's weights and its output
+    are rounded at other places, half steps of 2^-8: 2^-5 of the largest covers them.)"""
+    attn, pool, lists = _attention(), _cache(2, torch.bfloat16), []
+    with torch.no_grad(), torch.autocast("cpu", torch.bfloat16):
+        for t in (5, 1):
+            x = torch.randn(2, t, CFG.hidden_size)
+            pool.begin(_i32([t, t]), t)
+            rope = rope_cos_sin(torch.arange(6)[-t:] if t == 1 else torch.arange(t), CFG.head_dim, CFG.rope_theta)
+            y = attn(x, cache=pool.layers[0], position_embeddings=rope)
+            want = attn(x, cache=lists, position_embeddings=rope)
+            assert (y.float() - want.float()).abs().max() <= 2.0 ** -5 * want.float().abs().max()
