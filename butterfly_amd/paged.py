@@ -418,9 +418,10 @@ class PagedLayer:
         return self.cache.plan
 
     def check_step(self, requests: int, rows_each: int) -> None:
-        """``ValueError`` unless the step has ``rows_each`` rows of each of ``requests`` requests."""
-        c = self.cache
-        if c.plan is not None and (c.max_requests != requests or c.rows_each != rows_each):
+        """``ValueError`` unless the step has ``rows_each`` rows of each of ``requests`` requests, ``RuntimeError`` where none
+        has begun."""
+        c, _ = self.cache, self.plan
+        if c.max_requests != requests or c.rows_each != rows_each:
             has = f"{c.rows_each} rows of each" if c.rows_each else "packed rows"
             raise ValueError(f"the paged cache's step has {has} of its {c.max_requests} requests, not {rows_each} of each of "
                              f"{requests}")

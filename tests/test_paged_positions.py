@@ -202,3 +202,9 @@ def test_an_fp32_attention_under_autocast_takes_bf16_pages():
             y = attn(x, cache=pool.layers[0], position_embeddings=rope)
             want = attn(x, cache=lists, position_embeddings=rope)
             assert (y.float() - want.float()).abs().max() <= 2.0 ** -5 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("tokens", [1, 4])
+def test_a_step_that_has_not_begun_is_refused(tokens):
+    with pytest.raises(RuntimeError, match="begin"):
+        _attention()(torch.zeros(2, tokens, CFG.hidden_size), cache=_cache(2).layers[0])
