@@ -623,7 +623,8 @@ class Attention(nn.Module):
         base, ld, es = qkv.data_ptr(), qkv.shape[-1], qkv.element_size()
         if table is None:
             cos, sin = rope if rope is not None else rope_cos_sin(positions, c.head_dim, c.rope_theta)
-            if cos.numel() != t * c.head_dim or sin.numel() != t * c.head_dim or not cos.device == sin.device == qkv.device:
+            if (not cos.shape[-1] == sin.shape[-1] == c.head_dim or min(cos.numel(), sin.numel()) < t * c.head_dim
+                    or not cos.device == sin.device == qkv.device):
                 raise ValueError(f"position_embeddings must be [{t}, {c.head_dim}] cos and sin rows on {qkv.device}")
             cos, sin = cos.float().contiguous(), sin.float().contiguous()
         qo = torch.empty(b, c.num_heads, t, c.head_dim, dtype=qkv.dtype, device=qkv.device)

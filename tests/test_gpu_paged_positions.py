@@ -173,3 +173,7 @@ def test_rows_of_position_embeddings_that_are_not_the_calls_are_refused(paged):
             with pytest.raises(ValueError):
                 attn(x, cache=cache, position_embeddings=rope)
         attn(x, cache=cache, position_embeddings=(cos[None], sin[None]))
+        if not paged:                  # rows behind the call's are not read
+            want = attn(x, cache=[], position_embeddings=(cos, sin))
+            longer = rope_cos_sin(torch.arange(9, device="cuda"), 128, cfg.rope_theta)
+            assert torch.equal(attn(x, cache=[], position_embeddings=longer), want)
