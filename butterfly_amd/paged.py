@@ -404,6 +404,10 @@ def _workspace_bytes(*sizes: int) -> int:
     return _native.lib().bfly_paged_attention_workspace_bytes(*sizes)
 
 
+def _capturing(x: torch.Tensor) -> bool:
+    return x.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class PagedLayer:
     """One layer's pages of a :class:`PagedKVCache`: what an attention module takes as its ``cache``.  Between the
     cache's :meth:`PagedKVCache.begin` and the next one, its rows are the step's."""
@@ -481,6 +485,7 @@ class PagedKVCache:
         self.plan: Optional[PagedPlan] = None
         self.rows_each = 0             # the step's rows of every request; 0: packed
         self._held: Optional[List[Optional[int]]] = None
+        self._replayed = False         # the step was captured: replays make others of it
 
     @property
     def nbytes(self) -> int:
@@ -489,7 +494,7 @@ class PagedKVCache:
     def _begin(self, counts: torch.Tensor, num_rows: int, rows_each: int) -> PagedPlan:
         self.plan = paged_plan(self.block_table, self.lengths, counts, self.free_pages, self.state,
                                page_size=self.page_size, num_rows=num_rows, rows_each=rows_each, in_place=True)
-        self.rows_each, self._held = rows_each, None
+        self.rows_each, self._held, self._replayed = rows_each, None, _capturing(self.lengths)
         return self.plan
 
     def begin(self, counts: torch.Tensor, rows_each: int = 1, *, start: Optional[int] = None) -> PagedPlan:
@@ -531,8 +536,9 @@ class PagedKVCache:
 
     def held(self) -> List[Optional[int]]:
         """How many tokens each request held before the step (``None``: one that adds none in it), for a step of
-        ``rows_each`` rows.  Read back once a step, which waits for the current stream."""
-        if self._held is None:
+        ``rows_each`` rows.  Read back once a step (a captured one: every time, for its latest replay), which waits for
+        the current stream."""
+        if self._held is None or self._replayed:
             p = self.plan
             first = torch.where(p.slots >= 0, p.positions, -1).view(-1, self.rows_each)[:, 0]
             self._held = [None if n < 0 else n for n in self._read(first)]
@@ -540,7 +546,7 @@ class PagedKVCache:
 
     @staticmethod
     def _read(x: torch.Tensor) -> List[int]:
-        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        if _capturing(x):
             raise RuntimeError("a paged step that needs its lengths on the host cannot be captured (steps of one token can)")
         return x.tolist()
 

@@ -177,3 +177,23 @@ def test_rows_of_position_embeddings_that_are_not_the_calls_are_refused(paged):
             want = attn(x, cache=[], position_embeddings=(cos, sin))
             longer = rope_cos_sin(torch.arange(9, device="cuda"), 128, cfg.rope_theta)
             assert torch.equal(attn(x, cache=[], position_embeddings=longer), want)
+
+
+def test_a_captured_begin_and_its_replays():
+    """The bookkeeping of several tokens captured, the attention outside: every replay is a step of its own."""
+    cfg = _config(64)
+    attn = Attention(cfg, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    pool, lists = _cache(cfg, 2), [[], []]
+    counts, g = _i32([3, 2]), torch.Generator().manual_seed(1)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        pool.begin(counts, 3)
+    for _ in range(4):
+        graph.replay()
+        x = torch.randn(2, 3, cfg.hidden_size, generator=g).bfloat16().cuda()
+        with torch.no_grad():
+            y = attn(x, cache=pool.layers[0])
+        for r, c in enumerate((3, 2)):
+            want = attn(x[r:r + 1, :c], cache=lists[r])[0].float()
+            assert (y[r, :c].float() - want).abs().max() <= 2.0 ** -5 * want.abs().max()
+    assert pool.lengths.tolist() == [12, 8]
