@@ -351,7 +351,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     ``swa_stream_attention``, which ``online_softmax_merge`` takes.  A request without tokens gives zeros and
     the empty stream ``(0, 0, -1e30)``; a length beyond its table row, or a page id outside the pages among
     those that are read, gives NaN for that request.  Rows of a page behind the request's last token are never
-    part of the result, whatever they hold.  float32 or bfloat16, head_dim 64, 128 or 256."""
+    part of the result, whatever they hold.  Sums are divided by ``l`` at the end: values whose weighted sum passes the
+    largest fp32 number give infinities.  float32 or bfloat16, head_dim 64, 128 or 256."""
     dev = _device_of(q)
     if not block_table.get_device() == lengths.get_device() == dev:
         _other_device()
