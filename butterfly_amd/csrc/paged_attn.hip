@@ -34,11 +34,10 @@
 // 17, 64 requests 20, 512 44, 4096 769, 16384 10248; 4096 and 16384 of 100 tokens over tables that hold no more
 // (no schedule): 122, 479.  Batches beyond a thousand requests pass short contexts with the first columns of
 // their table.
-#include "paged.h"
+#include "paged_runs.h"
 
 namespace bfly {
 
-constexpr float kPagedNeg = -1e30f;   // the largest score of a request without tokens
 // Calls replayed from a graph, us, with 256 / 512 / 1024 runs (d 128 where nothing else stands): one request of 32768 tokens
 // 19.1 / 19.7 / 23.6, 131072 tokens x 32 223 / 223 / 222, 262144 tokens of d 256 174 / 177 / 182, 64 of 4096 tokens with 32/8
 // heads 174 / 173 / 180; fp32: 32768 tokens 30.9 / 31.8 / 35.9, 8 of 30000 160 / 164 / 165, 4 of 30000 of d 256 163 / 168 / 176.
@@ -50,8 +49,7 @@ constexpr float kPagedNeg = -1e30f;   // the largest score of a request without 
 // Tiles of d 64 have half the bytes and half the registers: two runs a CU (512 / 256 runs: 8 requests of 60000 tokens
 // 83.7 / 86.6, fp32 8 of 30000 85.4 / 90.4).
 constexpr int runs_for(int head_dim) { return head_dim <= 64 ? 512 : 256; }   // in all, where requests and heads leave them
-constexpr int kMaxRuns = 512;
-constexpr int kMinRun = 1;            // c at least
+static_assert(runs_for(64) <= kMaxRuns && runs_for(256) <= kMaxRuns, "");
 // Rounds that stay one run, and without a second launch where the tables hold no more: 512 keys (bf16) are done before a
 // join of two runs, and the more pairs of request and head (x16 query heads) there are, the longer runs hide behind each
 // other.  Measured, half as many / this many / twice as many for all pairs, us: 128 pairs of 1000 tokens 19.8 / 18.0 /
@@ -61,198 +59,22 @@ constexpr int kMinRun = 1;            // c at least
 // The pairs are the call's, idle requests among them: one request of 4000 tokens among 127 idle ones of 4 kv heads 13.7
 // us, alone 10.7.
 constexpr int whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
-// A request of several runs has more than c rounds, so fewer than 2 rounds_b / c runs; all of them together, with
-// c >= total / runs_for, fewer than twice runs_for: the partials there can be.  (kSlack: the total is a sum of floats.)
-constexpr int kSlack = 64;
-constexpr int kMaxSlots = 2 * kMaxRuns + kSlack;
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
 constexpr int kTile = sizeof(T) == 2 ? 32 : 16;
-constexpr int kWaves = 4;             // waves of a workgroup, tiles of a round
 
-typedef __attribute__((ext_vector_type(2))) float f32x2;
-
-struct PagedAttnArgs {
+struct PagedAttnArgs : RunArgs {
   const char* q;
   PagePtr kp, vp;
-  const int32_t* table;
-  const int32_t* lengths;
-  void* out;
-  float* l;
-  float* m;
-  float* part;                           // partials: [slot][rows][D], then [slot][rows] m and l
-  float* part_ml;
-  int4* join;                            // what to join: request, unit, runs, first slot
-  int* joins;                            // how many of them
-  int64_t q_req, q_head, table_stride;   // bytes, bytes, elements
-  int64_t capacity;                      // tokens a table row holds
-  int requests, num_pages, hq, hkv, shift, window;
-  int group, row_tiles, rows;            // query heads a kv head; 16-row parts of them; rows of a part at most
-  int units;                             // hkv * row_tiles
-  int runs;                              // runs_for(D)
-  int whole;                             // rounds that stay one run
-  int direct;                            // every request is one run (its table row is that short)
-  float scale;
+  int64_t q_req, q_head;                 // bytes
 };
 
-// What a request's workgroups do, from its length.
-struct Span {
-  int lo, n;      // positions seen: [lo, n)
-  int t0, tiles;  // tiles that hold them
-  int rounds;     // four tiles each
-  bool off;       // the length is beyond the table
-};
-template <int KT>
-__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int len) {
-  Span s;
-  s.off = (int64_t)len > a.capacity;
-  s.n = len <= 0 || s.off ? 0 : len;
-  s.lo = a.window > 0 && s.n > a.window ? s.n - a.window : 0;
-  s.t0 = s.lo / KT;
-  s.tiles = s.n > 0 ? (s.n - 1) / KT + 1 - s.t0 : 0;
-  s.rounds = (s.tiles + kWaves - 1) / kWaves;
-  return s;
-}
-
-struct Run {
-  int b, len;     // request (-1: none) and its length
-  int sub;        // index inside the request
-  int splits;     // runs of the request (per unit)
-  int slot;       // partials before the request's
-  int join;       // (request, unit) pairs of several runs before the request's
-  int joins;      // and in all
-};
-
-// Sums over the wave's lanes on DPP (row shifts inside 16 lanes, then the rows' last lanes broadcast): lane 63
-// of the inclusive scan holds the total.
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int dpp_shift(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, kRows, 0xf, false); }
-__device__ __forceinline__ int wave_scan(int x) {
-  x += dpp_shift<0x111, 0xf>(x);     // row_shr:1, 2, 4, 8
-  x += dpp_shift<0x112, 0xf>(x);
-  x += dpp_shift<0x114, 0xf>(x);
-  x += dpp_shift<0x118, 0xf>(x);
-  x += dpp_shift<0x142, 0xa>(x);     // row_bcast:15 into rows 1 and 3
-  x += dpp_shift<0x143, 0xc>(x);     // row_bcast:31 into rows 2 and 3
-  return x;
-}
-__device__ __forceinline__ float wave_total(float x) {
-  const auto step = [](float v, int w) { return v + __int_as_float(w); };
-  x = step(x, dpp_shift<0x111, 0xf>(__float_as_int(x)));
-  x = step(x, dpp_shift<0x112, 0xf>(__float_as_int(x)));
-  x = step(x, dpp_shift<0x114, 0xf>(__float_as_int(x)));
-  x = step(x, dpp_shift<0x118, 0xf>(__float_as_int(x)));
-  x = step(x, dpp_shift<0x142, 0xa>(__float_as_int(x)));
-  x = step(x, dpp_shift<0x143, 0xc>(__float_as_int(x)));
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
-}
-
-// The largest over the wave's lanes, in every lane (col_max4 over the lanes of a row of 16, which hold the
-// same then).
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return col_max4(x);
-}
-
-// The request that item `idx` falls into, where request b has units * splits_b items.  Every wave does it by
-// itself: a lane sums a stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
-template <int KT>
-__device__ __forceinline__ Run plan_run(const PagedAttnArgs& a, int64_t idx) {
-  if (a.direct) {                                   // no request can have several runs: item = (request, unit)
-    const int b = (int)idx / a.units;
-    return Run{b, a.lengths[b], (int)idx - b * a.units, 1, 0, 0, 0};
-  }
-  const int lane = threadIdx.x & 63;
-  const int per = (a.requests + 63) >> 6;
-  const int b0 = lane * per < a.requests ? lane * per : a.requests;
-  const int b1 = b0 + per < a.requests ? b0 + per : a.requests;
-  // (up to 64 requests a lane has one, in registers)
-  const int len0 = b0 < b1 ? a.lengths[b0] : 0;
-  const int first = span_of<KT>(a, len0).rounds;
-  const auto each = [&](auto&& f) {
-    if (per == 1) {
-      if (b0 < b1) f(first);
-    } else {
-#pragma unroll 4
-      for (int b = b0; b < b1; ++b) f(span_of<KT>(a, a.lengths[b]).rounds);
-    }
-  };
-  float total = 0.f;
-  each([&](int n) { total += (float)n; });
-  total = wave_total(total) * (float)a.units;
-  // c fills the runs exactly if the requests' last, shorter runs fit among them; else room is left for one each
-  const auto over = [&](float to) { return fminf(fmaxf(ceilf(total / to), (float)kMinRun), 1e9f); };
-  int c = __builtin_amdgcn_readfirstlane((int)over((float)a.runs));
-  const auto runs = [&](int n) { return n > c && n > a.whole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
-  int items = 0;
-  each([&](int n) { items += runs(n); });
-  const int64_t pairs = (int64_t)a.requests * a.units;
-  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs)
-    c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
-  int slots = 0;                                    // low half: partials; high half: requests that have them (both
-  items = 0;                                        // below kMaxSlots in all)
-  const auto parts = [](int s) { return s > 1 ? s | 0x10000 : 0; };
-  each([&](int n) {
-    const int s = runs(n);
-    items += s;
-    slots += parts(s);
-  });
-  const int i_up = wave_scan(items), s_up = wave_scan(slots);
-  const uint64_t mine = __ballot((int64_t)i_up * a.units > idx);
-  Run r{-1, 0, 0, 0, 0, 0, (__builtin_amdgcn_readlane(s_up, 63) >> 16) * a.units};
-  if (mine == 0) return r;
-  const int owner = __builtin_ctzll(mine);
-  int at = __builtin_amdgcn_readlane(i_up - items, owner), slot = __builtin_amdgcn_readlane(s_up - slots, owner);
-  for (int b = owner * per;; ++b) {               // (a request of the owner's stretch holds idx)
-    const int len = per == 1 ? __builtin_amdgcn_readlane(len0, owner) : a.lengths[b];
-    const int s = runs(span_of<KT>(a, len).rounds);
-    const int next = at + s;
-    if ((int64_t)next * a.units > idx) {
-      r.b = b;
-      r.len = len;
-      r.sub = (int)(idx - (int64_t)at * a.units);
-      r.splits = s;
-      r.slot = (slot & 0xffff) * a.units;
-      r.join = (slot >> 16) * a.units;
-      return r;
-    }
-    at = next;
-    slot += parts(s);
-  }
-}
-
-__device__ __forceinline__ void store4(float* o, f32x4 y, float f) { *reinterpret_cast<f32x4*>(o) = y * f; }
-__device__ __forceinline__ void store4(__bf16* o, f32x4 y, float f) {
-  y *= f;
-  *reinterpret_cast<bf16x4*>(o) = __builtin_convertvector(y, bf16x4);
-}
-
-// The statistics of a row from its joined sums.  A row that sees nothing but scores of -inf has no softmax: its sum is
-// NaN, as exp(-inf - -inf) gives (its output is 0 / 0).  NaN scores make the sum NaN, and then the maximum, which
-// has passed over them (a maximum of +inf makes a NaN sum by itself).
-template <typename T>
-__device__ __forceinline__ void finish_stats(const PagedAttnArgs& a, int64_t row, float m, float l) {
-  if (a.l == nullptr) return;
-  const bool nan = l != l;
-  a.l[row] = m == -INFINITY ? __builtin_nanf("") : l;
-  a.m[row] = nan && m != INFINITY ? l : m;
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
-}
 // The word without its bf16 infinities and NaN.
 __device__ __forceinline__ uint32_t finite_bf16(uint32_t w) {
   if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
   if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
   return w;
 }
-
-typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
 
 // V rows are read once, whole lines an instruction, past the caches' replacement: the K half-lines of two
 // neighbouring instructions then stay until both have been taken.  Measured, V past the caches / nothing / K and V,
@@ -430,30 +252,6 @@ struct Sweep<float, D> {
   }
 };
 
-// The pages of tile t: one base per 16 keys, with the page's and the rows' offsets.  Keys outside [lo, n)
-// share the page of the nearest key inside, so no entry behind the last page (or before the window) is read.
-template <int U>
-__device__ __forceinline__ bool tile_pages(const PagedAttnArgs& a, const int32_t* row, int first, const Span& s, int (&id)[U]) {
-  bool bad = false;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    unsigned t = (unsigned)first + 16 * u;
-    t = t < (unsigned)s.lo ? s.lo : t > (unsigned)s.n - 1 ? s.n - 1 : t;
-    id[u] = row[t >> a.shift];
-    if ((unsigned)id[u] >= (unsigned)a.num_pages) {
-      bad = true;
-      id[u] = 0;
-    }
-  }
-  return bad;
-}
-template <int U>
-__device__ __forceinline__ void tile_base(const PagedAttnArgs& a, const PagePtr& p, int h, int first, const int (&id)[U],
-                                          const char* (&base)[U]) {
-#pragma unroll
-  for (int u = 0; u < U; ++u) base[u] = p.row(id[u], h, (first + 16 * u) & ((1 << a.shift) - 1));
-}
-
 // Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.
 template <typename T, int D, bool kSafe>
 __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, const int32_t* row, const Span& s, int kvh,
@@ -622,7 +420,7 @@ __global__ void __launch_bounds__(64 * kWaves) paged_attn_kernel(PagedAttnArgs a
 // weights exp(m_i - m) are made once, in LDS; then 16 lanes across the elements, the runs dealt to 16 groups
 // of lanes, four loads under way in each.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
+__global__ void __launch_bounds__(256) paged_merge_kernel(RunArgs a) {
   constexpr int G = 16;
   __shared__ f32x4 sy[G][16];
   __shared__ float weight[kMaxSlots], sl[4], smx[4];
@@ -681,21 +479,22 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(PagedAttnArgs a) {
   if (c == 0) finish_stats<T>(a, row, mm, l);
 }
 
-// The rounds of a request at most; only one of more than whole_rounds can have several runs.
-static int64_t most_rounds(int64_t capacity, int window, int esize) {
-  const int kt = esize == 2 ? kTile<__bf16> : kTile<float>;
-  const int64_t keys = window > 0 && window < capacity ? (int64_t)window + kt - 1 : capacity;
-  return (keys + kWaves * kt - 1) / (kWaves * kt);
+template <typename T>
+static void launch_merge(const RunArgs& a, int head_dim, hipStream_t stream) {
+  const int64_t pairs = (int64_t)a.requests * a.units;
+  const dim3 grid((unsigned)(pairs < a.runs ? pairs : a.runs), (unsigned)a.rows, (unsigned)head_dim / 64), block(256);
+  if (head_dim == 64) hipLaunchKernelGGL((paged_merge_kernel<T, 64>), grid, block, 0, stream, a);
+  else if (head_dim == 128) hipLaunchKernelGGL((paged_merge_kernel<T, 128>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((paged_merge_kernel<T, 256>), grid, block, 0, stream, a);
 }
-template <typename T, int D>
-static void launch_paged(const PagedAttnArgs& a, int64_t items, bool splits, hipStream_t stream) {
-  hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(64 * kWaves), 0, stream, a);
-  if (splits) {
-    const int64_t pairs = (int64_t)a.requests * a.units;
-    const unsigned x = (unsigned)(pairs < a.runs ? pairs : a.runs);
-    hipLaunchKernelGGL((paged_merge_kernel<T, D>), dim3(x, (unsigned)a.rows, D / 64), dim3(256), 0, stream, a);
-  }
+void paged_merge(const RunArgs& a, int dtype, int head_dim, hipStream_t stream) {
+  if (a.direct) return;
+  if (dtype == BFLY_DTYPE_BF16) launch_merge<__bf16>(a, head_dim, stream);
+  else launch_merge<float>(a, head_dim, stream);
 }
+
+template <typename T>
+static int64_t rounds_at_most(int64_t capacity, int window) { return most_rounds(capacity, window, kTile<T>); }
 
 }  // namespace bfly
 
@@ -706,8 +505,9 @@ extern "C" int64_t bfly_paged_attention_workspace_bytes(int dtype, int64_t reque
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   const int64_t pairs = requests * hkv * ((group + 15) / 16);
-  if (most_rounds(table_width * page_size, window, dtype == BFLY_DTYPE_F32 ? 4 : 2) <= whole_rounds(pairs)) return 0;
-  return (int64_t)kMaxSlots * (rows * (head_dim + 2) * 4 + 16) + 16;
+  const int64_t capacity = table_width * page_size;
+  const int64_t rounds = dtype == BFLY_DTYPE_F32 ? rounds_at_most<float>(capacity, window) : rounds_at_most<__bf16>(capacity, window);
+  return rounds <= whole_rounds(pairs) ? 0 : run_workspace_bytes(rows, head_dim);
 }
 
 extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hipStream_t stream) {
@@ -744,27 +544,17 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
   a.q = static_cast<const char*>(x.q);
   a.kp = k_page_ptr(x.pages, es); a.vp = v_page_ptr(x.pages, es);
   a.table = x.block_table; a.lengths = x.lengths; a.out = x.out; a.l = x.l; a.m = x.m;
-  a.q_req = x.q_request_stride * es; a.q_head = x.q_head_stride * es; a.table_stride = x.table_stride;
-  a.shift = __builtin_ctzll(x.pages.page_size); a.capacity = x.table_width << a.shift;
-  a.requests = (int)x.requests; a.num_pages = (int)x.pages.num_pages; a.hq = (int)x.hq; a.hkv = (int)x.hkv;
-  a.window = (int)x.window; a.scale = (float)x.scale;
-  a.group = a.hq / a.hkv; a.row_tiles = (a.group + 15) / 16; a.rows = a.group < 16 ? a.group : 16;
-  BFLY_CHECK_ARG((int64_t)a.hkv * a.row_tiles <= 65535, "too many heads");
-  a.units = a.hkv * a.row_tiles;
-  a.join = static_cast<int4*>(x.workspace);
-  a.joins = reinterpret_cast<int*>(a.join + kMaxSlots);
-  a.part = reinterpret_cast<float*>(a.join + kMaxSlots + 1);
-  a.part_ml = a.part + (int64_t)kMaxSlots * a.rows * x.head_dim;
-  // runs: one for each (request, unit), and as many more as the splits make (plan_run)
-  const int64_t rounds = most_rounds(a.capacity, a.window, (int)es), pairs = x.requests * a.units;
+  a.q_req = x.q_request_stride * es; a.q_head = x.q_head_stride * es; a.scale = (float)x.scale;
+  BFLY_CHECK_ARG(run_shape(a, x.requests, x.hq, x.hkv, x.pages.page_size, x.pages.num_pages, x.table_width, x.table_stride,
+                           x.window),
+                 "too many heads");
+  run_workspace(a, x.workspace, x.head_dim);
   a.runs = runs_for((int)x.head_dim);
-  a.whole = whole_rounds(pairs);
-  const bool splits = rounds > a.whole;
-  a.direct = !splits;
-  const int64_t most = pairs * ((rounds + kMinRun - 1) / kMinRun), some = pairs + a.runs + kSlack;
-  const int64_t items = !splits ? pairs : most < some ? most : some;
+  a.whole = whole_rounds((int64_t)a.requests * a.units);
+  const int64_t items = run_items(a, es == 4 ? rounds_at_most<float>(a.capacity, a.window)
+                                             : rounds_at_most<__bf16>(a.capacity, a.window));
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads
-#define BFLY_PAGED(T, D) launch_paged<T, D>(a, items, splits, stream)
+#define BFLY_PAGED(T, D) hipLaunchKernelGGL((paged_attn_kernel<T, D>), dim3((unsigned)items), dim3(64 * kWaves), 0, stream, a)
   if (x.dtype == BFLY_DTYPE_BF16) {
     if (x.head_dim == 64) BFLY_PAGED(__bf16, 64);
     else if (x.head_dim == 128) BFLY_PAGED(__bf16, 128);
@@ -775,6 +565,7 @@ extern "C" int bfly_paged_attention(const bfly_paged_attention_args_t* args, hip
     else BFLY_PAGED(float, 256);
   }
 #undef BFLY_PAGED
+  paged_merge(a, (int)x.dtype, (int)x.head_dim, stream);
   BFLY_CHECK_LAUNCH("bfly_paged_attention");
   return BFLY_OK;
 }
