@@ -115,6 +115,12 @@ SIGNATURES = {
     "bfly_paged_rope_append": (_int, [C.c_char_p, _vp]),
     "bfly_paged_attention_workspace_bytes": (_i64, [_int, _i64, _int, _int, _int, _i64, _int, _int]),
     "bfly_paged_attention": (_int, [C.c_char_p, _vp]),
+    # include/butterfly_amd_paged_q4.h (packed too, PAGED_Q4_STRUCTS)
+    "bfly_paged_q4_append": (_int, [C.c_char_p, _vp]),
+    "bfly_paged_q4_rope_append": (_int, [C.c_char_p, _vp]),
+    "bfly_paged_q4_read": (_int, [C.c_char_p, _vp]),
+    "bfly_paged_q4_attention_workspace_bytes": (_i64, [_i64, _int, _int, _int, _i64, _int, _int]),
+    "bfly_paged_q4_attention": (_int, [C.c_char_p, _vp]),
 }
 
 # The argument structs of include/butterfly_amd_paged.h, as struct formats: eight bytes a member, pointers
@@ -125,6 +131,13 @@ PAGED_STRUCTS = {
     "bfly_paged_append": struct.Struct("21q"),
     "bfly_paged_rope_append": struct.Struct("16qd17q"),
     "bfly_paged_attention": struct.Struct("23qd5q"),
+}
+# Those of include/butterfly_amd_paged_q4.h, the same way (19 members of each are the pages).
+PAGED_Q4_STRUCTS = {
+    "bfly_paged_q4_append": struct.Struct("30q"),
+    "bfly_paged_q4_rope_append": struct.Struct("16qd26q"),
+    "bfly_paged_q4_read": struct.Struct("29q"),
+    "bfly_paged_q4_attention": struct.Struct("32qd5q"),
 }
 
 _lib = None
