@@ -109,6 +109,8 @@ SIGNATURES = {
     "bfly_add_rms_norm_q4_gemv_argmax": (_int, [_vp, _vp, _vp, _f32, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp,
                                                 _i64, _vp]),
     "bfly_greedy_advance": (_int, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "bfly_token_logprobs_workspace_bytes": (_i64, [_i64, _i64, _int]),
+    "bfly_token_logprobs": (_int, [_vp, _int, _i64, _i64, _i64, _vp, _int, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     # include/butterfly_amd_paged.h (the structs of arguments are packed bytes, PAGED_STRUCTS below)
     "bfly_paged_plan": (_int, [C.c_char_p, _vp]),
     "bfly_paged_append": (_int, [C.c_char_p, _vp]),

@@ -203,6 +203,22 @@ int bfly_add_rms_norm_q4_gemv_silu_parts(const float* x_parts, int n_parts, cons
                                          const void* scale_bias, int64_t out_features, int64_t in_features,
                                          int group, int64_t up_row_offset, void* out, hipStream_t stream);
 
+/*
+ * Device: for each of `rows` rows of `vocab` logits (dtype fp32 or bf16; rows row_stride elements apart, any
+ * alignment): the log probability of tokens[row] under the row's softmax (NaN for a token outside it), the
+ * softmax's entropy in nats, and its `top` largest entries in order (log probability and index; equal logits by the
+ * lower index, NaN above every number).  One pass over the logits, sums in fp32.  logprobs, entropy [rows],
+ * top_logprobs, top_tokens [rows][top] (NULL for top 0).  A logit of -inf has probability 0; a row that holds a NaN or
+ * +inf, or nothing but -inf, gives NaN (its top_tokens stay defined).  top at most 64 and at most vocab; vocab below 2^30.
+ * workspace: bfly_token_logprobs_workspace_bytes bytes, 16-byte aligned (it need not be cleared; calls that
+ * overlap need one each).  No counterpart in the reference's own code (its quality smoke compares the top
+ * entries and the divergence of host arrays, scripts/quality_smoke.py).
+ */
+int64_t bfly_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top);
+int bfly_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                        const int64_t* tokens, int top, float* logprobs, float* entropy, float* top_logprobs,
+                        int64_t* top_tokens, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,7 +68,7 @@ def test_c_abi_refuses_pages(name, kw, rc, msg):
     (_append, dict(k=I + 8), INVALID, b"aligned"),
     (_append, dict(slots=None), INVALID, b"null"),
     (_append, dict(rows=1 << 29), INVALID, b"too many"),
-    (_append, dict(rows=1 << 28, d=256), INVALID, b"too many"),
+    (_append, dict(rows=1 << 27, d=256, ksr=16, vsr=16), INVALID, b"too many"),
     (_rope, dict(rot=24), INVALID, b"rotary_dim"),
     (_rope, dict(rot=144), INVALID, b"rotary_dim"),
     (_rope, dict(table=0), INVALID, b"rows"),
