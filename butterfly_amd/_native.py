@@ -121,7 +121,7 @@ SIGNATURES = {
     "bfly_paged_q4_append": (_int, [C.c_char_p, _vp]),
     "bfly_paged_q4_rope_append": (_int, [C.c_char_p, _vp]),
     "bfly_paged_q4_read": (_int, [C.c_char_p, _vp]),
-    "bfly_paged_q4_attention_workspace_bytes": (_i64, [_i64, _int, _int, _int, _i64, _int, _int]),
+    "bfly_paged_q4_attention_workspace_bytes": (_i64, [_int, _i64, _int, _int, _int, _i64, _int, _int]),
     "bfly_paged_q4_attention": (_int, [C.c_char_p, _vp]),
 }
 

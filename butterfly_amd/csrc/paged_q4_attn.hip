@@ -17,7 +17,6 @@
 
 namespace bfly {
 
-constexpr int kQ4Tile = 32;
 constexpr int q4_runs_for(int) { return 512; }   // in all, where requests and heads leave them
 static_assert(q4_runs_for(64) <= kMaxRuns, "");
 constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
@@ -32,13 +31,19 @@ struct Q4AttnArgs : RunArgs {
 template <int R>
 __device__ __forceinline__ float of_four(float x) {
   constexpr int ctrl = R | R << 2 | R << 4 | R << 6;
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xf, 0xf, false));
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
 }
-// codes number j of both half-words of r as 16 + c in bf16
+// codes number j of both half-words of r as 16 + c in bf16; `ones` is 16 in both halves of a VGPR (with both constants as
+// scalars or literals the two operations below cannot be one)
 template <int J>
-__device__ __forceinline__ uint32_t codes_of(uint32_t r) {
+__device__ __forceinline__ uint32_t codes_of(uint32_t r, uint32_t ones) {
   const uint32_t x = J == 0 ? r << 3 : r >> (4 * J - 3);
-  return (x & 0x00780078u) | 0x41804180u;
+  return (x & 0x00780078u) | ones;
+}
+__device__ __forceinline__ uint32_t sixteens() {
+  uint32_t x = 0x41804180u;
+  asm("" : "+v"(x));
+  return x;
 }
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -67,49 +72,63 @@ struct Words {                                      // N dwords (or a half-word:
   }
 };
 
-// One wave's sums over its tiles.  acc[4 h + j][r] of lane (n = lane & 15, g = lane >> 4): query row n, element
-// d_of(4 h + j, 4 g + r).
-template <typename T, int D, int G>
+// Columns of a product in J blocks of C = 16 / J: a block's columns are the rows of q for one subtile (16 keys) of J, so a
+// lane's four results are of its own block's subtile and every lane of a unit with few query heads has
+// weights to work on.  Rows of q are kept J times, each zero outside its block: the chain over J subtiles then ends in
+// one accumulator.  Every column keeps a maximum and sums of its own until the end.
+template <typename T, int D, int G, int J>
 struct Q4Sweep {
-  static constexpr int KT = kQ4Tile;
+  static constexpr int C = 16 / J;                  // rows of q
+  static constexpr int U = J > 2 ? J : 2;           // subtiles of a tile
+  static constexpr int A = U / J;                   // of them in a block: results 4 a + r of a lane
+  static constexpr int KT = 16 * U;
   static constexpr int H = D / 64;                  // half-words of a piece
   static constexpr int NG = D / G;                  // groups of a row
-  static constexpr int N = D / 16;                  // second products a tile
+  static constexpr int N = D / 16;                  // second products for 32 keys
   static constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;   // bf16 parts of q, of the weights
   static constexpr int VW = D == 256 ? 2 : 1;       // dwords of a piece (d 64: half of one)
-  f32x4 acc[N];
+  f32x4 acc[N];                                     // acc[4 h + j][r]: row n of q's columns, element d_of(4 h + j, 4 g + r)
   float accb[NG];                                   // this lane's keys only, as l
   float m, l;                                       // m: the largest q . k, unscaled
-  u32x4 q[QP][D / 32];
+  u32x4 q[J][QP][D / 32];
   float qs[NG];                                     // sums of q over a group
-  Words<2 * H> k[2];
-  Words<NG> ks[2], vs[2];
-  Words<VW> v[8];
+  Words<2 * H> k[U];
+  Words<NG> ks[A], vs[A];
+  Words<VW> v[4 * U];
+  uint32_t ones, mine[J];                           // mine[j]: all bits in the lanes of block j
 
   static __device__ __forceinline__ int group_of(int i) { return G == 64 ? i / 4 : 2 * (i / 4) + (i % 4) / 2; }
   // element of acc[i] at row m of the product
   static __device__ __forceinline__ int d_of(int i, int m) {
     return G == 64 ? 64 * (i / 4) + 4 * m + i % 4 : 32 * group_of(i) + 2 * m + i % 2;
   }
-  __device__ __forceinline__ void clear() {
+  __device__ __forceinline__ void clear(int n) {
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NG; ++i) accb[i] = 0.f;
     m = -INFINITY;
     l = 0.f;
+    ones = sixteens();
+#pragma unroll
+    for (int j = 0; j < J; ++j) mine[j] = n / C == j ? ~0u : 0u;
   }
   // q times `sign`: a quarter of each group, in the codes' order
-  __device__ __forceinline__ void load_q(const T* row, int g, float sign) {
-    constexpr int E = G / 4;
+  __device__ __forceinline__ void load_q(const T* row, int n, int g, float sign) {
+    constexpr int E = G / 4, VE = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(VE)));
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
       float x[E], sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        x[e] = row != nullptr ? to_f32(row[G * b + E * g + e]) * sign : 0.f;
-        sum += x[e];
+      for (int i = 0; i < E; i += VE) {
+        vec y;
+        if (row != nullptr) y = *reinterpret_cast<const vec*>(row + G * b + E * g + i);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[i + e] = row != nullptr ? to_f32(y[e]) * sign : 0.f;
       }
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += x[e];
       qs[b] = col_sum4(sum);
 #pragma unroll
       for (int part = 0; part < QP; ++part) {
@@ -124,205 +143,253 @@ struct Q4Sweep {
           x[f] -= hi_f(w[i]);
         }
 #pragma unroll
-        for (int i = 0; i < E / 8; ++i) q[part][b * (E / 8) + i] = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int i = 0; i < E / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[j][part][b * (E / 8) + i][e] = n / C == j ? w[4 * i + e] : 0;
       }
     }
   }
-  __device__ __forceinline__ void load_k(const char* const (&base)[2], const char* const (&sbase)[2], const Q4Ptr& p, int n, int g) {
+  // subtile of this lane's results a
+  static __device__ __forceinline__ int subtile(int a, int n) { return a * J + n / C; }
+  __device__ __forceinline__ void load_k(const char* const (&base)[U], const Q4Ptr& p, int n, int g) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      k[u].load(base[u] + (uint32_t)(n * p.kc.row_bytes + (D / 8) * g));
-      ks[u].load(sbase[u] + (uint32_t)((4 * g + (n & 3)) * p.ks.row_bytes));
+    for (int u = 0; u < U; ++u) k[u].load(base[u] + (uint32_t)(n * p.kc.row_bytes + (D / 8) * g));
+  }
+  __device__ __forceinline__ void load_v(const char* const (&base)[U], const Q4Ptr& p, int n, int g) {
+#pragma unroll
+    for (int i = 0; i < 4 * U; ++i) {
+      const char* at = base[i >> 2] + (uint32_t)((4 * g + (i & 3)) * p.vc.row_bytes + (D / 32) * n);
+      if constexpr (D == 64) v[i].w[0] = *reinterpret_cast<const uint16_t*>(at);
+      else v[i].load(at);
     }
   }
-  __device__ __forceinline__ void load_v(const char* const (&base)[2], const char* const (&sbase)[2], const Q4Ptr& p, int n, int g) {
+  // scales of the keys 4 g + (n & 3) of this lane's subtiles (the address of its block's by masks: a choice among
+  // elements of `base` would take the array to memory)
+  __device__ __forceinline__ void load_scales(Words<NG> (&s)[A], const char* const (&base)[U], int row_bytes, int n, int g) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const char* at = base[j >> 2] + (uint32_t)((4 * g + (j & 3)) * p.vc.row_bytes + (D / 32) * n);
-      if constexpr (D == 64) v[j].w[0] = *reinterpret_cast<const uint16_t*>(at);
-      else v[j].load(at);
+    for (int a = 0; a < A; ++a) {
+      uint64_t at = reinterpret_cast<uint64_t>(base[a * J]);
+      if constexpr (J > 1) {
+        uint32_t lo = 0, hi = 0;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const uint64_t x = reinterpret_cast<uint64_t>(base[a * J + j]);
+          lo |= (uint32_t)x & mine[j];
+          hi |= (uint32_t)(x >> 32) & mine[j];
+        }
+        at = (uint64_t)hi << 32 | lo;
+      }
+      s[a].load(reinterpret_cast<const char*>(at) + (uint32_t)((4 * g + (n & 3)) * row_bytes));
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) vs[u].load(sbase[u] + (uint32_t)((4 * g + (n & 3)) * p.vs.row_bytes));
   }
   static __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int h) {   // half-word h of a and of b
     return __builtin_amdgcn_perm(b, a, h & 1 ? 0x07060302u : 0x05040100u);
   }
-  // this lane's keys 16 u + 4 g + r: s[4 u + r] = q . k
-  __device__ __forceinline__ void scores(float (&s)[8]) const {
+  // s[4 a + r] = q . k of key 16 subtile(a) + 4 g + r
+  __device__ __forceinline__ void scores(float (&s)[4 * A]) const {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      uint32_t r[2][H];                             // r[p][h]: half-words h of pieces 4 g + 2 p and the next
+    for (int a = 0; a < A; ++a) {
+      f32x4 c[NG];
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
+      for (int b = 0; b < NG; ++b) c[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const Words<2 * H>& x = k[a * J + j];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          if constexpr (H == 1) r[p][h] = k[u].w[p];
-          else if constexpr (H == 2) r[p][h] = halves(k[u].w[2 * p], k[u].w[2 * p + 1], h);
-          else r[p][h] = halves(k[u].w[4 * p + (h >> 1)], k[u].w[4 * p + 2 + (h >> 1)], h);
+          uint32_t r[2];                            // half-words h of pieces 4 g + 2 p and the next
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            if constexpr (H == 1) r[p] = x.w[p];
+            else if constexpr (H == 2) r[p] = halves(x.w[2 * p], x.w[2 * p + 1], h);
+            else r[p] = halves(x.w[4 * p + (h >> 1)], x.w[4 * p + 2 + (h >> 1)], h);
+          }
+          if constexpr (G == 64) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              const u32x4 y = {codes_of<0>(r[p], ones), codes_of<1>(r[p], ones), codes_of<2>(r[p], ones), codes_of<3>(r[p], ones)};
+#pragma unroll
+              for (int i = QP - 1; i >= 0; --i) c[h] = mfma(y, q[j][i][2 * h + p], c[h]);
+            }
+          } else {
+            const u32x4 y = {codes_of<0>(r[0], ones), codes_of<1>(r[0], ones), codes_of<0>(r[1], ones), codes_of<1>(r[1], ones)};
+            const u32x4 z = {codes_of<2>(r[0], ones), codes_of<3>(r[0], ones), codes_of<2>(r[1], ones), codes_of<3>(r[1], ones)};
+#pragma unroll
+            for (int i = QP - 1; i >= 0; --i) {
+              c[2 * h] = mfma(y, q[j][i][2 * h], c[2 * h]);
+              c[2 * h + 1] = mfma(z, q[j][i][2 * h + 1], c[2 * h + 1]);
+            }
+          }
         }
+      }
       float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int b = 0; b < NG; ++b) {
-        f32x4 c = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (G == 64) {
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const u32x4 x = {codes_of<0>(r[p][b]), codes_of<1>(r[p][b]), codes_of<2>(r[p][b]), codes_of<3>(r[p][b])};
-#pragma unroll
-            for (int i = QP - 1; i >= 0; --i) c = mfma(x, q[i][2 * b + p], c);
-          }
-        } else {
-          const int h = b >> 1;
-          const u32x4 x = b & 1 ? u32x4{codes_of<2>(r[0][h]), codes_of<3>(r[0][h]), codes_of<2>(r[1][h]), codes_of<3>(r[1][h])}
-                                : u32x4{codes_of<0>(r[0][h]), codes_of<1>(r[0][h]), codes_of<0>(r[1][h]), codes_of<1>(r[1][h])};
-#pragma unroll
-          for (int i = QP - 1; i >= 0; --i) c = mfma(x, q[i][b], c);
-        }
-        const float sc = lo_f(ks[u].w[b]), bias = fmaf(-16.f, sc, hi_f(ks[u].w[b]));
-        t[0] = fmaf(of_four<0>(sc), c[0], fmaf(of_four<0>(bias), qs[b], t[0]));
-        t[1] = fmaf(of_four<1>(sc), c[1], fmaf(of_four<1>(bias), qs[b], t[1]));
-        t[2] = fmaf(of_four<2>(sc), c[2], fmaf(of_four<2>(bias), qs[b], t[2]));
-        t[3] = fmaf(of_four<3>(sc), c[3], fmaf(of_four<3>(bias), qs[b], t[3]));
+        const float sc = lo_f(ks[a].w[b]), bias = fmaf(-16.f, sc, hi_f(ks[a].w[b]));
+        t[0] = fmaf(of_four<0>(sc), c[b][0], fmaf(of_four<0>(bias), qs[b], t[0]));
+        t[1] = fmaf(of_four<1>(sc), c[b][1], fmaf(of_four<1>(bias), qs[b], t[1]));
+        t[2] = fmaf(of_four<2>(sc), c[b][2], fmaf(of_four<2>(bias), qs[b], t[2]));
+        t[3] = fmaf(of_four<3>(sc), c[b][3], fmaf(of_four<3>(bias), qs[b], t[3]));
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * u + i] = t[i];
+      for (int i = 0; i < 4; ++i) s[4 * a + i] = t[i];
     }
   }
-  static __device__ __forceinline__ int key(int i, int g) { return 16 * (i >> 2) + 4 * g + (i & 3); }
-  __device__ __forceinline__ void drop_v(int u) {   // the scales that this lane holds for subtile u
+  // Leaves out the keys outside [lo, n) of the tile that begins at `first`: scores of -inf, scales of zero.
+  __device__ __forceinline__ void cut(float (&s)[4 * A], unsigned first, unsigned lo, unsigned end, int n, int g) {
 #pragma unroll
-    for (int b = 0; b < NG; ++b) vs[u].w[b] = 0;
+    for (int a = 0; a < A; ++a) {
+      const unsigned at = first + 16 * subtile(a, n) + 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (at + r < lo || at + r >= end) s[4 * a + r] = -INFINITY;
+      if (at + (n & 3) < lo || at + (n & 3) >= end) {
+#pragma unroll
+        for (int b = 0; b < NG; ++b) vs[a].w[b] = 0;
+      }
+    }
   }
-  __device__ __forceinline__ void add(const float (&p)[8]) {
+  __device__ __forceinline__ void add(const float (&p)[4 * A]) {
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
-      float w[8];
+      uint32_t part[PP][2 * A];                     // the weights of this lane's keys for the group
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const float sc = lo_f(vs[u].w[b]), bias = fmaf(-16.f, sc, hi_f(vs[u].w[b]));
-        w[4 * u + 0] = p[4 * u + 0] * of_four<0>(sc);
-        w[4 * u + 1] = p[4 * u + 1] * of_four<1>(sc);
-        w[4 * u + 2] = p[4 * u + 2] * of_four<2>(sc);
-        w[4 * u + 3] = p[4 * u + 3] * of_four<3>(sc);
-        accb[b] = fmaf(p[4 * u + 0], of_four<0>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * u + 1], of_four<1>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * u + 2], of_four<2>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * u + 3], of_four<3>(bias), accb[b]);
-      }
-      u32x4 part[PP];
+      for (int a = 0; a < A; ++a) {
+        const float sc = lo_f(vs[a].w[b]), bias = fmaf(-16.f, sc, hi_f(vs[a].w[b]));
+        float w[4];
+        w[0] = p[4 * a + 0] * of_four<0>(sc);
+        w[1] = p[4 * a + 1] * of_four<1>(sc);
+        w[2] = p[4 * a + 2] * of_four<2>(sc);
+        w[3] = p[4 * a + 3] * of_four<3>(sc);
+        accb[b] = fmaf(p[4 * a + 0], of_four<0>(bias), accb[b]);
+        accb[b] = fmaf(p[4 * a + 1], of_four<1>(bias), accb[b]);
+        accb[b] = fmaf(p[4 * a + 2], of_four<2>(bias), accb[b]);
+        accb[b] = fmaf(p[4 * a + 3], of_four<3>(bias), accb[b]);
 #pragma unroll
-      for (int i = 0; i < PP; ++i)
+        for (int i = 0; i < PP; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          part[i][j] = pack_bf16(w[2 * j], w[2 * j + 1]);
-          if (i + 1 < PP) {
-            w[2 * j] -= lo_f(part[i][j]);
-            w[2 * j + 1] -= hi_f(part[i][j]);
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x = pack_bf16(w[2 * j], w[2 * j + 1]);
+            part[i][2 * a + j] = x;
+            if (i + 1 < PP) {
+              w[2 * j] -= lo_f(x);
+              w[2 * j + 1] -= hi_f(x);
+            }
           }
-        }
+      }
       // G 64: half-word b, its four codes; G 32: two of half-word b / 2
       const int h = G == 64 ? b : b >> 1;
-      uint32_t r[4];                                // half-words h of the keys 2 j and 2 j + 1
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (D == 64) r[j] = v[2 * j].w[0] | v[2 * j + 1].w[0] << 16;
-        else r[j] = halves(v[2 * j].w[h >> 1], v[2 * j + 1].w[h >> 1], h);
-      }
-      const auto product = [&](auto jc) {
-        constexpr int J = decltype(jc)::value;
-        const u32x4 x = {codes_of<J>(r[0]), codes_of<J>(r[1]), codes_of<J>(r[2]), codes_of<J>(r[3])};
+      for (int e = 0; e < U / 2; ++e) {             // 32 keys: subtiles 2 e and 2 e + 1
+        u32x4 w[PP];
 #pragma unroll
-        for (int i = PP - 1; i >= 0; --i) acc[4 * h + J] = mfma(x, part[i], acc[4 * h + J]);
-      };
-      using std::integral_constant;
-      if (G == 64 || !(b & 1)) {
-        product(integral_constant<int, 0>{});
-        product(integral_constant<int, 1>{});
-      }
-      if (G == 64 || (b & 1)) {
-        product(integral_constant<int, 2>{});
-        product(integral_constant<int, 3>{});
+        for (int i = 0; i < PP; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int u = 2 * e + (j >> 1);
+            w[i][j] = part[i][2 * (u / J) + (j & 1)];
+            if constexpr (J > 1) w[i][j] &= mine[u % J];
+          }
+        uint32_t r[4];                              // half-words h of the keys 2 j and 2 j + 1
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const Words<VW>&x = v[8 * e + 2 * j], &y = v[8 * e + 2 * j + 1];
+          if constexpr (D == 64) r[j] = x.w[0] | y.w[0] << 16;
+          else r[j] = halves(x.w[h >> 1], y.w[h >> 1], h);
+        }
+        const auto product = [&](auto jc) __attribute__((always_inline)) {
+          constexpr int K = decltype(jc)::value;
+          const u32x4 x = {codes_of<K>(r[0], ones), codes_of<K>(r[1], ones), codes_of<K>(r[2], ones), codes_of<K>(r[3], ones)};
+#pragma unroll
+          for (int i = PP - 1; i >= 0; --i) acc[4 * h + K] = mfma(x, w[i], acc[4 * h + K]);
+        };
+        using std::integral_constant;
+        if (G == 64 || !(b & 1)) {
+          product(integral_constant<int, 0>{});
+          product(integral_constant<int, 1>{});
+        }
+        if (G == 64 || (b & 1)) {
+          product(integral_constant<int, 2>{});
+          product(integral_constant<int, 3>{});
+        }
       }
     }
   }
 };
 
 // Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.
-template <typename T, int D, int G>
-__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, Q4Sweep<T, D, G>& w, const int32_t* row, const Span& s, int kvh,
-                                         int t, int t_end, float unit) {
-  constexpr int KT = kQ4Tile;
+template <typename S>
+__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end,
+                                         float unit) {
+  constexpr int KT = S::KT, U = S::U;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  w.clear();
+  w.clear(n);
   if (t >= t_end) return false;
-  int id[2];
-  const char *base[2], *sbase[2];
-  const auto bases = [&](const PagePtr& codes, const PagePtr& scales, int first) {
-    tile_base<2>(a, codes, kvh, first, id, base);
-    tile_base<2>(a, scales, kvh, first, id, sbase);
+  int id[U];
+  const char* base[U];
+  bool bad = tile_pages<U>(a, row, t * KT, s, id);
+  const auto load_k = [&](int first) __attribute__((always_inline)) {
+    tile_base<U>(a, a.p.kc, kvh, first, id, base);
+    w.load_k(base, a.p, n, g);
+    tile_base<U>(a, a.p.ks, kvh, first, id, base);
+    w.load_scales(w.ks, base, a.p.ks.row_bytes, n, g);
   };
-  bool bad = tile_pages<2>(a, row, t * KT, s, id);
-  bases(a.p.kc, a.p.ks, t * KT);
-  w.load_k(base, sbase, a.p, n, g);
-  bases(a.p.vc, a.p.vs, t * KT);
-  w.load_v(base, sbase, a.p, n, g);
+  const auto load_v = [&](int first) __attribute__((always_inline)) {
+    tile_base<U>(a, a.p.vc, kvh, first, id, base);
+    w.load_v(base, a.p, n, g);
+    tile_base<U>(a, a.p.vs, kvh, first, id, base);
+    w.load_scales(w.vs, base, a.p.vs.row_bytes, n, g);
+  };
+  load_k(t * KT);
+  load_v(t * KT);
   while (true) {
     const int next = t + kWaves;
     const bool more = next < t_end;
-    if (more) bad |= tile_pages<2>(a, row, next * KT, s, id);
-    float p[8];
+    if (more) bad |= tile_pages<U>(a, row, next * KT, s, id);
+    float p[4 * S::A];
     w.scores(p);
-    if (more) {
-      bases(a.p.kc, a.p.ks, next * KT);
-      w.load_k(base, sbase, a.p, n, g);
-    }
+    if (more) load_k(next * KT);
     const unsigned first = (unsigned)t * KT, lo = s.lo, end = s.n;
-    if (first < lo || first + KT > end) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const unsigned at = first + w.key(i, g);
-        if (at < lo || at >= end) p[i] = -INFINITY;
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const unsigned at = first + 16 * u + 4 * g + (n & 3);
-        if (at < lo || at >= end) w.drop_v(u);
-      }
-    }
+    if (first < lo || first + KT > end) w.cut(p, first, lo, end, n, g);
     float mx = p[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, p[i]);
+    for (int i = 1; i < 4 * S::A; ++i) mx = fmaxf(mx, p[i]);
     mx = col_max4(mx);
     if (__any(mx > w.m)) {
       const float nm = fmaxf(w.m, mx);
       const float f = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m - nm) * unit);
       w.l *= f;
 #pragma unroll
-      for (int i = 0; i < w.N; ++i) w.acc[i] *= f;
+      for (int i = 0; i < S::N; ++i) w.acc[i] *= f;
 #pragma unroll
-      for (int i = 0; i < w.NG; ++i) w.accb[i] *= f;
+      for (int i = 0; i < S::NG; ++i) w.accb[i] *= f;
       w.m = nm;
     }
     const float ref = w.m == -INFINITY ? 0.f : w.m;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4 * S::A; ++i) {
       p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * unit);
       sum += p[i];
     }
     w.l += sum;
     w.add(p);
     if (!more) return bad;
-    bases(a.p.vc, a.p.vs, next * KT);
-    w.load_v(base, sbase, a.p, n, g);
+    load_v(next * KT);
     t = next;
   }
 }
 
-template <typename T, int D, int G>
-__global__ void __launch_bounds__(64 * kWaves) q4_attn_kernel(Q4AttnArgs a) {
-  constexpr int KT = kQ4Tile, LD = D + 4;
+// Waves of a SIMD that the registers are cut for: two need no more than 256 (and no moves to accumulation registers
+// and back), but for the widest rows.
+constexpr int q4_waves(int esize, int d, int g, int j) { return d < 256 || (esize == 2 && g == 64 && j == 2) ? 2 : 1; }
+
+template <typename T, int D, int G, int J>
+__global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_attn_kernel(Q4AttnArgs a) {
+  typedef Q4Sweep<T, D, G, J> S;
+  constexpr int KT = S::KT, C = S::C, LD = D + 4;
   __shared__ float so[kWaves][16 * LD];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int sbad;
@@ -336,7 +403,7 @@ __global__ void __launch_bounds__(64 * kWaves) q4_attn_kernel(Q4AttnArgs a) {
   const int sub = __builtin_amdgcn_readfirstlane(run.sub), slot = __builtin_amdgcn_readfirstlane(run.slot) + sub;
   const int unit = sub / splits, split = sub - unit * splits;
   const int kvh = unit / a.row_tiles, part = unit - kvh * a.row_tiles;
-  const int rows = a.group - 16 * part < 16 ? a.group - 16 * part : 16;
+  const int rows = a.group - 16 * part < 16 ? a.group - 16 * part : 16;   // (at most C: there are more than C with J = 1 only)
   const int head0 = kvh * a.group + 16 * part;
   const Span s = span_of<KT>(a, __builtin_amdgcn_readfirstlane(run.len));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -359,17 +426,17 @@ __global__ void __launch_bounds__(64 * kWaves) q4_attn_kernel(Q4AttnArgs a) {
   if (threadIdx.x == 0) sbad = 0;
   // scores stay q . k up to the exponential; a scale below zero turns q over, one of zero clears it
   const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : a.scale, size = a.scale == 0.f ? 1.f : fabsf(a.scale);
-  Q4Sweep<T, D, G> w;
-  w.load_q(n < rows ? reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + n) * a.q_head) : nullptr, g, sign);
-  const bool bad = q4_sweep<T, D, G>(a, w, table, s, kvh, t0 + wave, t1, size * kLog2e);
+  S w;
+  w.load_q(n % C < rows ? reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + n % C) * a.q_head) : nullptr, n, g, sign);
+  const bool bad = q4_sweep(a, w, table, s, kvh, t0 + wave, t1, size * kLog2e);
   const float l = col_sum4(w.l);
-  float accb[w.NG];
+  float accb[S::NG];
 #pragma unroll
-  for (int i = 0; i < w.NG; ++i) accb[i] = col_sum4(w.accb[i]);
+  for (int i = 0; i < S::NG; ++i) accb[i] = col_sum4(w.accb[i]);
   __syncthreads();
-  if (n < rows) {
+  if (n % C < rows) {
 #pragma unroll
-    for (int i = 0; i < w.N; i += G / 16)
+    for (int i = 0; i < S::N; i += G / 16)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float bias = accb[w.group_of(i)];
@@ -394,17 +461,18 @@ __global__ void __launch_bounds__(64 * kWaves) q4_attn_kernel(Q4AttnArgs a) {
     const int r = i / (D / 4), c = 4 * (i % (D / 4));
     float mm = sm[0][r];
 #pragma unroll
-    for (int k = 1; k < kWaves; ++k) mm = fmaxf(mm, sm[k][r]);
+    for (int k = 1; k < kWaves * J; ++k) mm = fmaxf(mm, sm[k / J][k % J * C + r]);
     const float ref = mm == -INFINITY ? 0.f : mm;
     f32x4 y = {0.f, 0.f, 0.f, 0.f};
     float ll = poison;
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float f = __builtin_amdgcn_exp2f((sm[k][r] - ref) * kLog2e);
+    for (int k = 0; k < kWaves * J; ++k) {
+      const int col = k % J * C + r;
+      const float f = __builtin_amdgcn_exp2f((sm[k / J][col] - ref) * kLog2e);
       // a wave without tiles has no part in it (0 * its sums would do, but for a reference of +inf)
-      if (t0 + k < t1) {
-        ll += f * sl[k][r];
-        y += f * *reinterpret_cast<const f32x4*>(&so[k][r * LD + c]);
+      if (t0 + k / J < t1) {
+        ll += f * sl[k / J][col];
+        y += f * *reinterpret_cast<const f32x4*>(&so[k / J][col * LD + c]);
       }
     }
     if (splits == 1) {
@@ -418,16 +486,45 @@ __global__ void __launch_bounds__(64 * kWaves) q4_attn_kernel(Q4AttnArgs a) {
   }
 }
 
+// Blocks of columns: as many as leave room for a unit's rows of q, and as the copies of q leave registers for.
+constexpr int q4_most_blocks(int esize, int head_dim) {
+  return esize == 2 ? (head_dim <= 128 ? 4 : 2) : head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;
+}
+static int q4_blocks(int esize, int64_t head_dim, int64_t group) {
+  const int most = q4_most_blocks(esize, (int)head_dim), fit = group <= 4 ? 4 : group <= 8 ? 2 : 1;
+  return most < fit ? most : fit;
+}
+static int q4_tile(int blocks) { return blocks > 2 ? 64 : 32; }
+
+template <typename T, int D, int G>
+static void launch_q4(const Q4AttnArgs& a, int blocks, int64_t items, hipStream_t stream) {
+  const dim3 grid((unsigned)items), block(64 * kWaves);
+  if constexpr (q4_most_blocks(sizeof(T), D) >= 4) {
+    if (blocks == 4) {
+      hipLaunchKernelGGL((q4_attn_kernel<T, D, G, 4>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  if constexpr (q4_most_blocks(sizeof(T), D) >= 2) {
+    if (blocks == 2) {
+      hipLaunchKernelGGL((q4_attn_kernel<T, D, G, 2>), grid, block, 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((q4_attn_kernel<T, D, G, 1>), grid, block, 0, stream, a);
+}
+
 }  // namespace bfly
 
 using namespace bfly;
 
-extern "C" int64_t bfly_paged_q4_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim, int64_t table_width,
-                                                           int page_size, int window) {
+extern "C" int64_t bfly_paged_q4_attention_workspace_bytes(int dtype, int64_t requests, int hq, int hkv, int head_dim,
+                                                           int64_t table_width, int page_size, int window) {
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   const int64_t pairs = requests * hkv * ((group + 15) / 16);
-  return most_rounds(table_width * page_size, window, kQ4Tile) <= q4_whole_rounds(pairs) ? 0 : run_workspace_bytes(rows, head_dim);
+  const int tile = q4_tile(q4_blocks(dtype == BFLY_DTYPE_F32 ? 4 : 2, head_dim, group));
+  return most_rounds(table_width * page_size, window, tile) <= q4_whole_rounds(pairs) ? 0 : run_workspace_bytes(rows, head_dim);
 }
 
 extern "C" int bfly_paged_q4_attention(const bfly_paged_q4_attention_args_t* args, hipStream_t stream) {
@@ -452,8 +549,8 @@ extern "C" int bfly_paged_q4_attention(const bfly_paged_q4_attention_args_t* arg
   BFLY_CHECK_ARG(x.table_width == 0 || x.block_table, "null pointer");
   BFLY_CHECK_ARG((x.l == nullptr) == (x.m == nullptr), "both l and m or neither");
   BFLY_CHECK_ARG(aligned16(x.q) && aligned16(x.out) && q4_aligned(x.pages), "pointers must be 16-byte aligned");
-  const int64_t need = bfly_paged_q4_attention_workspace_bytes(x.requests, (int)x.hq, (int)x.hkv, (int)x.head_dim, x.table_width,
-                                                               (int)x.pages.page_size, (int)x.window);
+  const int64_t need = bfly_paged_q4_attention_workspace_bytes((int)x.dtype, x.requests, (int)x.hq, (int)x.hkv, (int)x.head_dim,
+                                                               x.table_width, (int)x.pages.page_size, (int)x.window);
   BFLY_CHECK_ARG(need == 0 || (x.workspace && x.workspace_bytes >= need && aligned16(x.workspace)), "workspace too small");
   Q4AttnArgs a{};
   a.q = static_cast<const char*>(x.q);
@@ -466,9 +563,10 @@ extern "C" int bfly_paged_q4_attention(const bfly_paged_q4_attention_args_t* arg
   run_workspace(a, x.workspace, x.head_dim);
   a.runs = q4_runs_for((int)x.head_dim);
   a.whole = q4_whole_rounds((int64_t)a.requests * a.units);
-  const int64_t items = run_items(a, most_rounds(a.capacity, a.window, kQ4Tile));
+  const int blocks = q4_blocks((int)es, x.head_dim, a.group);
+  const int64_t items = run_items(a, most_rounds(a.capacity, a.window, q4_tile(blocks)));
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads
-#define BFLY_Q4(T, D, G) hipLaunchKernelGGL((q4_attn_kernel<T, D, G>), dim3((unsigned)items), dim3(64 * kWaves), 0, stream, a)
+#define BFLY_Q4(T, D, G) launch_q4<T, D, G>(a, blocks, items, stream)
 #define BFLY_Q4_G(T, D)                       \
   do {                                        \
     if (x.pages.group == 32) BFLY_Q4(T, D, 32); \

@@ -286,7 +286,7 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
             q = q.clone(memory_format=torch.contiguous_format)
             q0, q1, _, _ = q.stride()
         lengths = lengths.contiguous()
-        need = _workspace_bytes(b, hq, hkv, d, width, size, window)
+        need = _workspace_bytes(code, b, hq, hkv, d, width, size, window)
         if need:
             ws = _EMPTY((need,), (1,), dtype=torch.uint8, device=cuda)
         _native.call("bfly_paged_q4_attention", _ATTN(

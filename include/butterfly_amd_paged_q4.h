@@ -103,8 +103,8 @@ int bfly_paged_q4_read(const bfly_paged_q4_read_args_t* args, hipStream_t stream
  * workspace: bfly_paged_q4_attention_workspace_bytes bytes, 16-byte aligned (it need not be cleared; calls
  * that overlap need one each).
  */
-int64_t bfly_paged_q4_attention_workspace_bytes(int64_t requests, int hq, int hkv, int head_dim, int64_t table_width,
-                                                int page_size, int window);
+int64_t bfly_paged_q4_attention_workspace_bytes(int dtype, int64_t requests, int hq, int hkv, int head_dim,
+                                                int64_t table_width, int page_size, int window);
 typedef struct bfly_paged_q4_attention_args {
   const void* q;
   int64_t dtype, requests, hq, hkv, head_dim;

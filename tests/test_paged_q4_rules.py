@@ -137,10 +137,10 @@ def test_the_packed_formats_are_the_headers_structs():
 
 def test_workspace_only_where_requests_can_be_split():
     need = _native.lib().bfly_paged_q4_attention_workspace_bytes
-    assert need(1, 8, 2, 128, 1, 128, 0) == 0 and need(0, 8, 2, 128, 1000, 128, 0) == 0 and need(1, 8, 3, 128, 1000, 128, 0) == 0
-    big = need(1, 8, 2, 128, 1000, 128, 0)
-    assert big > 0 and need(1, 8, 2, 128, 1000, 128, 100) == 0
-    assert need(1, 64, 2, 256, 1000, 128, 0) > big
+    assert need(1, 1, 8, 2, 128, 1, 128, 0) == 0 and need(1, 0, 8, 2, 128, 1000, 128, 0) == 0 and need(0, 1, 8, 3, 128, 1000, 128, 0) == 0
+    big = need(1, 1, 8, 2, 128, 1000, 128, 0)
+    assert big > 0 and need(1, 1, 8, 2, 128, 1000, 128, 100) == 0
+    assert need(0, 1, 64, 2, 256, 1000, 128, 0) > big
 
 
 def test_operators_refuse_cpu_tensors():
