@@ -262,7 +262,8 @@ __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, co
   if (t >= t_end) return false;
   int id[U];
   const char* base[U];
-  bool bad = tile_pages<U>(a, row, t * KT, s, id);
+  tile_ids<U>(a, row, t * KT, s, id);
+  bool bad = tile_bad<U>(a, id);
   tile_base<U>(a, a.kp, kvh, t * KT, id, base);
   w.load_k(base, a.kp.row_bytes, n, g);
   tile_base<U>(a, a.vp, kvh, t * KT, id, base);
@@ -270,7 +271,10 @@ __device__ __forceinline__ bool sweep(const PagedAttnArgs& a, Sweep<T, D>& w, co
   while (true) {
     const int next = t + kWaves;
     const bool more = next < t_end;
-    if (more) bad |= tile_pages<U>(a, row, next * KT, s, id);
+    if (more) {
+      tile_ids<U>(a, row, next * KT, s, id);
+      bad |= tile_bad<U>(a, id);
+    }
     float p[P];
     w.scores(p, a.scale);
     if (more) {

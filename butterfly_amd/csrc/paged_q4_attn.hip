@@ -11,7 +11,7 @@
 //   * A row's 16 pieces hold a sixteenth of every group each.  S^T = K Q^T: lane (n, g) takes four pieces of key n
 //     (a quarter of every group), so each product is over one group.  O^T += V^T P^T: lane n takes piece n of a lane's 8
 //     keys, so the 16 rows of each product are of one group, and P carries that group's scale.
-//   * Scales are read as lane (n, g) needs them, for keys 4g + (n & 3), and reach the other lanes of a four by DPP.
+//   * Scales are read as lane (n, g) needs them, for keys 4 (n & 3) + g, and reach the other lanes of a four by DPP.
 #include "paged_runs.h"
 #include "paged_q4.h"
 
@@ -51,23 +51,54 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 __device__ __forceinline__ float lo_f(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// Rows of one page and head, through a buffer descriptor: the row of a tile is a scalar offset, so a lane's offset is
+// the same for every tile.
+struct Rows {
+  __amdgpu_buffer_rsrc_t page;
+  int at;                                           // the tile's first row, in bytes
+};
+__device__ __forceinline__ Rows page_rows(const PagePtr& p, int64_t id, int h, int row, int page_size, int row_length) {
+  return Rows{__builtin_amdgcn_make_buffer_rsrc(p.row(id, h, 0), (short)0, (page_size - 1) * p.row_bytes + row_length, 0x00020000),
+              row * p.row_bytes};
+}
+
 template <int N>
-struct Words {                                      // N dwords (or a half-word: N = 0) as they lie
+struct Words {                                      // N dwords as they lie
   uint32_t w[N];
-  __device__ __forceinline__ void load(const char* p) {
+  template <int kPolicy>
+  __device__ __forceinline__ void load(const Rows& r, int lane_at, int at) {
     if constexpr (N >= 4) {
 #pragma unroll
       for (int i = 0; i < N; i += 4) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 4 * i);
+        const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r.page, lane_at + 4 * i, r.at + at, kPolicy));
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[i + j] = x[j];
       }
     } else if constexpr (N == 2) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r.page, lane_at, r.at + at, kPolicy));
       w[0] = x[0];
       w[1] = x[1];
     } else {
-      w[0] = *reinterpret_cast<const uint32_t*>(p);
+      w[0] = __builtin_amdgcn_raw_buffer_load_b32(r.page, lane_at, r.at + at, kPolicy);
+    }
+  }
+  __device__ __forceinline__ void load(uint64_t address) {   // (somewhere else for every lane)
+    typedef __attribute__((address_space(1))) const uint32_t* ptr;
+    typedef __attribute__((address_space(1))) const u32x2* ptr2;
+    typedef __attribute__((address_space(1))) const u32x4* ptr4;
+    if constexpr (N >= 4) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const u32x4 x = *(ptr4)(address + 4 * i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[i + j] = x[j];
+      }
+    } else if constexpr (N == 2) {
+      const u32x2 x = *(ptr2)address;
+      w[0] = x[0];
+      w[1] = x[1];
+    } else {
+      w[0] = *(ptr)address;
     }
   }
 };
@@ -82,19 +113,26 @@ struct Q4Sweep {
   static constexpr int U = J > 2 ? J : 2;           // subtiles of a tile
   static constexpr int A = U / J;                   // of them in a block: results 4 a + r of a lane
   static constexpr int KT = 16 * U;
+  static constexpr int kPolicyK = 2, kPolicyV = 0, kPolicyS = 0;
+  static constexpr int kCodes = D / 2, kScales = 4 * (D / G);   // bytes of a row
   static constexpr int H = D / 64;                  // half-words of a piece
   static constexpr int NG = D / G;                  // groups of a row
   static constexpr int N = D / 16;                  // second products for 32 keys
-  static constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;   // bf16 parts of q, of the weights
+  static constexpr bool kBytes = sizeof(T) == 2;    // scores from codes as bytes (else as bf16)
+  static constexpr int QP = kBytes ? 2 : 3, PP = kBytes ? 2 : 3;   // parts of q, of the weights
+  static constexpr int QW = kBytes ? 2 : 4;         // words of an operand
   static constexpr int VW = D == 256 ? 2 : 1;       // dwords of a piece (d 64: half of one)
   f32x4 acc[N];                                     // acc[4 h + j][r]: row n of q's columns, element d_of(4 h + j, 4 g + r)
   float accb[NG];                                   // this lane's keys only, as l
   float m, l;                                       // m: the largest q . k, unscaled
-  u32x4 q[J][QP][D / 32];
-  float qs[NG];                                     // sums of q over a group
-  Words<2 * H> k[U];
-  Words<NG> ks[A], vs[A];
-  Words<VW> v[4 * U];
+  uint32_t q[J][QP][D / 32][QW];
+  float qs[NG];                                     // sums of q over a group, in the scores' unit
+  float unit;                                       // what a score counts
+  struct Tile {                                     // a tile as it lies
+    Words<2 * H> k[U];
+    Words<NG> ks[A], vs[A];
+    Words<VW> v[4 * U];
+  };
   uint32_t ones, mine[J];                           // mine[j]: all bits in the lanes of block j
 
   static __device__ __forceinline__ int group_of(int i) { return G == 64 ? i / 4 : 2 * (i / 4) + (i % 4) / 2; }
@@ -113,82 +151,171 @@ struct Q4Sweep {
 #pragma unroll
     for (int j = 0; j < J; ++j) mine[j] = n / C == j ? ~0u : 0u;
   }
-  // q times `sign`: a quarter of each group, in the codes' order
-  __device__ __forceinline__ void load_q(const T* row, int n, int g, float sign) {
+  // q times `sign`: a quarter of each group, in the codes' order.  `size`: the scale's size, times log2 e.
+  __device__ __forceinline__ void load_q(const T* row, int n, int g, float sign, float size) {
     constexpr int E = G / 4, VE = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(VE)));
+    float x[NG][E], most = 0.f;
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
-      float x[E], sum = 0.f;
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < E; i += VE) {
         vec y;
         if (row != nullptr) y = *reinterpret_cast<const vec*>(row + G * b + E * g + i);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[i + e] = row != nullptr ? to_f32(y[e]) * sign : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += x[e];
-      qs[b] = col_sum4(sum);
-#pragma unroll
-      for (int part = 0; part < QP; ++part) {
-        uint32_t w[E / 2];
-#pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-          // G 64: product i / 4, word j = i % 4: elements 8 (i / 4) + j and 4 further;
-          // G 32: word i = 2 p + j: elements 4 p + j and 2 further
-          const int e = G == 64 ? 8 * (i / 4) + i % 4 : 4 * (i / 2) + i % 2, f = e + (G == 64 ? 4 : 2);
-          w[i] = pack_bf16(x[e], x[f]);
-          x[e] -= lo_f(w[i]);
-          x[f] -= hi_f(w[i]);
+        for (int e = 0; e < VE; ++e) {
+          x[b][i + e] = row != nullptr ? to_f32(y[e]) * sign : 0.f;
+          most = fmaxf(most, fabsf(x[b][i + e]));
+          sum += x[b][i + e];
         }
-#pragma unroll
-        for (int j = 0; j < J; ++j)
-#pragma unroll
-          for (int i = 0; i < E / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[j][part][b * (E / 8) + i][e] = n / C == j ? w[4 * i + e] : 0;
       }
+      qs[b] = col_sum4(sum);
+    }
+    unit = size;
+    if constexpr (kBytes) {
+      // q as two bytes (4 bits each, E4M3) of q f, f the power of two that takes the row's largest to [2^7, 2^8): eight bits
+      // for elements of 2^-10 of it and more, 2^-18 of it for what is below.  A byte of 0..15 is 2^-9 of its number in that
+      // format, so scores count f 2^-9.  (An infinity or NaN in q makes the unit, and with it every weight, NaN.)
+      most = col_max4(most);
+      const int e = most > 0.f ? (int)(__float_as_uint(most) >> 23) : 127;
+      const float f = __uint_as_float((uint32_t)(e < 8 ? 253 : 261 - e) << 23);   // 2^(134 - e), at most 2^126
+      float any = 0.f;
+#pragma unroll
+      for (int b = 0; b < NG; ++b) {
+        any += qs[b] - qs[b];
+        qs[b] = qs[b] * f * 0.001953125f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[b][i] *= f;
+      }
+      unit = size / f * 512.f + any;
+#pragma unroll
+      for (int b = 0; b < NG; ++b)
+#pragma unroll
+        for (int part = 0; part < QP; ++part)
+#pragma unroll
+          for (int i = 0; i < E / 8; ++i) {         // a product: 8 elements, even ones of four codes (two of G 32) first
+            uint32_t w[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float y[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int at = G == 64 ? 8 * i + 4 * (k >> 1) + 2 * (k & 1) + j : 2 * k + j;
+                y[k] = x[b][at];
+              }
+              int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+              word = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], word, true);
+              w[j] = (uint32_t)word;
+              const float z[4] = {__builtin_amdgcn_cvt_f32_fp8(word, 0), __builtin_amdgcn_cvt_f32_fp8(word, 1),
+                                  __builtin_amdgcn_cvt_f32_fp8(word, 2), __builtin_amdgcn_cvt_f32_fp8(word, 3)};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int at = G == 64 ? 8 * i + 4 * (k >> 1) + 2 * (k & 1) + j : 2 * k + j;
+                x[b][at] -= z[k];
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) q[j][part][b * (E / 8) + i][k] = n / C == j ? w[k] : 0;
+          }
+    } else {
+#pragma unroll
+      for (int b = 0; b < NG; ++b)
+#pragma unroll
+        for (int part = 0; part < QP; ++part) {
+          uint32_t w[E / 2];
+#pragma unroll
+          for (int i = 0; i < E / 2; ++i) {
+            // G 64: product i / 4, word j = i % 4: elements 8 (i / 4) + j and 4 further;
+            // G 32: word i = 2 p + j: elements 4 p + j and 2 further
+            const int e = G == 64 ? 8 * (i / 4) + i % 4 : 4 * (i / 2) + i % 2, f = e + (G == 64 ? 4 : 2);
+            w[i] = pack_bf16(x[b][e], x[b][f]);
+            x[b][e] -= lo_f(w[i]);
+            x[b][f] -= hi_f(w[i]);
+          }
+#pragma unroll
+          for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < E / 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) q[j][part][b * (E / 8) + i][e] = n / C == j ? w[4 * i + e] : 0;
+        }
     }
   }
   // subtile of this lane's results a
   static __device__ __forceinline__ int subtile(int a, int n) { return a * J + n / C; }
-  __device__ __forceinline__ void load_k(const char* const (&base)[U], const Q4Ptr& p, int n, int g) {
+  // The key of a subtile in row n of the first product: results r of lane g are of keys 4 r + g then, and an instruction
+  // takes four rows of v that follow each other.
+  static __device__ __forceinline__ int key_of(int n) { return 4 * (n & 3) + (n >> 2); }
+  // A tile inside one page.  Codes of k: key_of(n), its pieces 4 g and on; of v: keys 4 r + g, piece n; scales: of the
+  // keys 4 (n & 3) + g of this lane's subtiles.
+  static __device__ __forceinline__ void load_k(Tile& x, const Q4Ptr& p, const Rows& codes, const Rows& scales, int n, int g) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) k[u].load(base[u] + (uint32_t)(n * p.kc.row_bytes + (D / 8) * g));
+    for (int u = 0; u < U; ++u) x.k[u].template load<kPolicyK>(codes, key_of(n) * p.kc.row_bytes + (D / 8) * g, 16 * u * p.kc.row_bytes);
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+      x.ks[a].template load<kPolicyS>(scales, (16 * (n / C) + 4 * (n & 3) + g) * p.ks.row_bytes, 16 * a * J * p.ks.row_bytes);
   }
-  __device__ __forceinline__ void load_v(const char* const (&base)[U], const Q4Ptr& p, int n, int g) {
+  static __device__ __forceinline__ void load_v(Tile& x, const Q4Ptr& p, const Rows& codes, const Rows& scales, int n, int g) {
 #pragma unroll
-    for (int i = 0; i < 4 * U; ++i) {
-      const char* at = base[i >> 2] + (uint32_t)((4 * g + (i & 3)) * p.vc.row_bytes + (D / 32) * n);
-      if constexpr (D == 64) v[i].w[0] = *reinterpret_cast<const uint16_t*>(at);
-      else v[i].load(at);
+    for (int i = 0; i < 4 * U; ++i) load_v_row(x.v[i], p, codes, (16 * (i >> 2) + 4 * (i & 3)) * p.vc.row_bytes, n, g);
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+      x.vs[a].template load<kPolicyS>(scales, (16 * (n / C) + 4 * (n & 3) + g) * p.vs.row_bytes, 16 * a * J * p.vs.row_bytes);
+  }
+  static __device__ __forceinline__ void load_v_row(Words<VW>& v, const Q4Ptr& p, const Rows& codes, int at, int n, int g) {
+    const int lane_at = g * p.vc.row_bytes + (D / 32) * n;
+    if constexpr (D == 64) v.w[0] = __builtin_amdgcn_raw_buffer_load_b16(codes.page, lane_at, codes.at + at, kPolicyV);
+    else v.template load<kPolicyV>(codes, lane_at, at);
+  }
+  // A tile over several pages: subtile by subtile, and for the scales the address of a lane's block by masks.
+  __device__ __forceinline__ void load_k(Tile& x, const RunArgs& a, const Q4Ptr& p, const int (&id)[U], int kvh, int first, int n,
+                                         int g) const {
+    const int size = 1 << a.shift;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      x.k[u].template load<kPolicyK>(page_rows(p.kc, id[u], kvh, (first + 16 * u) & (size - 1), size, D / 2), key_of(n) * p.kc.row_bytes + (D / 8) * g, 0);
+    load_scales(x.ks, p.ks, id, kvh, first, size, n, g);
+  }
+  __device__ __forceinline__ void load_v(Tile& x, const RunArgs& a, const Q4Ptr& p, const int (&id)[U], int kvh, int first, int n,
+                                         int g) const {
+    const int size = 1 << a.shift;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Rows codes = page_rows(p.vc, id[u], kvh, (first + 16 * u) & (size - 1), size, D / 2);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) load_v_row(x.v[4 * u + r], p, codes, 4 * r * p.vc.row_bytes, n, g);
     }
+    load_scales(x.vs, p.vs, id, kvh, first, size, n, g);
   }
-  // scales of the keys 4 g + (n & 3) of this lane's subtiles (the address of its block's by masks: a choice among
-  // elements of `base` would take the array to memory)
-  __device__ __forceinline__ void load_scales(Words<NG> (&s)[A], const char* const (&base)[U], int row_bytes, int n, int g) const {
+  __device__ __forceinline__ void load_scales(Words<NG> (&s)[A], const PagePtr& p, const int (&id)[U], int kvh, int first, int size,
+                                              int n, int g) const {
 #pragma unroll
     for (int a = 0; a < A; ++a) {
-      uint64_t at = reinterpret_cast<uint64_t>(base[a * J]);
-      if constexpr (J > 1) {
-        uint32_t lo = 0, hi = 0;
+      uint32_t lo = 0, hi = 0;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const uint64_t x = reinterpret_cast<uint64_t>(base[a * J + j]);
-          lo |= (uint32_t)x & mine[j];
-          hi |= (uint32_t)(x >> 32) & mine[j];
-        }
-        at = (uint64_t)hi << 32 | lo;
+      for (int j = 0; j < J; ++j) {
+        const uint64_t x = reinterpret_cast<uint64_t>(p.row(id[a * J + j], kvh, (first + 16 * (a * J + j)) & (size - 1)));
+        lo |= (uint32_t)x & mine[j];
+        hi |= (uint32_t)(x >> 32) & mine[j];
       }
-      s[a].load(reinterpret_cast<const char*>(at) + (uint32_t)((4 * g + (n & 3)) * row_bytes));
+      s[a].load(((uint64_t)hi << 32 | lo) + (uint32_t)((4 * (n & 3) + g) * p.row_bytes));
     }
   }
   static __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int h) {   // half-word h of a and of b
     return __builtin_amdgcn_perm(b, a, h & 1 ? 0x07060302u : 0x05040100u);
   }
-  // s[4 a + r] = q . k of key 16 subtile(a) + 4 g + r
-  __device__ __forceinline__ void scores(float (&s)[4 * A]) const {
+  __device__ __forceinline__ f32x4 score(const uint32_t (&codes)[QW], int j, int part, int i, f32x4 c) const {
+    const uint32_t(&y)[QW] = q[j][part][i];
+    if constexpr (kBytes)
+      return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8((uint64_t)codes[1] << 32 | codes[0], (uint64_t)y[1] << 32 | y[0], c, 0, 0, 0);
+    else
+      return mfma(u32x4{codes[0], codes[1], codes[2], codes[3]}, u32x4{y[0], y[1], y[2], y[3]}, c);
+  }
+  // s[4 a + r] = q . k of key 16 subtile(a) + 4 r + g, in the row's unit
+  __device__ __forceinline__ void scores(const Tile& in, float (&s)[4 * A]) const {
 #pragma unroll
     for (int a = 0; a < A; ++a) {
       f32x4 c[NG];
@@ -196,7 +323,7 @@ struct Q4Sweep {
       for (int b = 0; b < NG; ++b) c[b] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const Words<2 * H>& x = k[a * J + j];
+        const Words<2 * H>& x = in.k[a * J + j];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t r[2];                            // half-words h of pieces 4 g + 2 p and the next
@@ -206,28 +333,49 @@ struct Q4Sweep {
             else if constexpr (H == 2) r[p] = halves(x.w[2 * p], x.w[2 * p + 1], h);
             else r[p] = halves(x.w[4 * p + (h >> 1)], x.w[4 * p + 2 + (h >> 1)], h);
           }
-          if constexpr (G == 64) {
+          uint32_t y[2][QW];                        // G 64: products of group h; G 32: of groups 2 h and 2 h + 1
+          if constexpr (kBytes) {
+            uint32_t w[2][2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-              const u32x4 y = {codes_of<0>(r[p], ones), codes_of<1>(r[p], ones), codes_of<2>(r[p], ones), codes_of<3>(r[p], ones)};
+              w[p][0] = r[p] & 0x0f0f0f0fu;
+              w[p][1] = r[p] >> 4 & 0x0f0f0f0fu;
+            }
 #pragma unroll
-              for (int i = QP - 1; i >= 0; --i) c[h] = mfma(y, q[j][i][2 * h + p], c[h]);
+            for (int p = 0; p < 2; ++p)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)           // (a G 32 group: every other byte of both words)
+                y[p][e] = G == 64 ? w[p][e] : __builtin_amdgcn_perm(w[1][e], w[0][e], p ? 0x07050301u : 0x06040200u);
+          } else if constexpr (G == 64) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              y[p][0] = codes_of<0>(r[p], ones);
+              y[p][1] = codes_of<1>(r[p], ones);
+              y[p][2] = codes_of<2>(r[p], ones);
+              y[p][3] = codes_of<3>(r[p], ones);
             }
           } else {
-            const u32x4 y = {codes_of<0>(r[0], ones), codes_of<1>(r[0], ones), codes_of<0>(r[1], ones), codes_of<1>(r[1], ones)};
-            const u32x4 z = {codes_of<2>(r[0], ones), codes_of<3>(r[0], ones), codes_of<2>(r[1], ones), codes_of<3>(r[1], ones)};
 #pragma unroll
-            for (int i = QP - 1; i >= 0; --i) {
-              c[2 * h] = mfma(y, q[j][i][2 * h], c[2 * h]);
-              c[2 * h + 1] = mfma(z, q[j][i][2 * h + 1], c[2 * h + 1]);
+            for (int p = 0; p < 2; ++p) {
+              y[0][2 * p] = codes_of<0>(r[p], ones);
+              y[0][2 * p + 1] = codes_of<1>(r[p], ones);
+              y[1][2 * p] = codes_of<2>(r[p], ones);
+              y[1][2 * p + 1] = codes_of<3>(r[p], ones);
             }
           }
+#pragma unroll
+          for (int i = QP - 1; i >= 0; --i)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              f32x4& to = c[G == 64 ? h : 2 * h + p];
+              to = score(y[p], j, i, 2 * h + p, to);
+            }
         }
       }
       float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int b = 0; b < NG; ++b) {
-        const float sc = lo_f(ks[a].w[b]), bias = fmaf(-16.f, sc, hi_f(ks[a].w[b]));
+        const float sc = lo_f(in.ks[a].w[b]), bias = kBytes ? hi_f(in.ks[a].w[b]) : fmaf(-16.f, sc, hi_f(in.ks[a].w[b]));
         t[0] = fmaf(of_four<0>(sc), c[b][0], fmaf(of_four<0>(bias), qs[b], t[0]));
         t[1] = fmaf(of_four<1>(sc), c[b][1], fmaf(of_four<1>(bias), qs[b], t[1]));
         t[2] = fmaf(of_four<2>(sc), c[b][2], fmaf(of_four<2>(bias), qs[b], t[2]));
@@ -238,26 +386,26 @@ struct Q4Sweep {
     }
   }
   // Leaves out the keys outside [lo, n) of the tile that begins at `first`: scores of -inf, scales of zero.
-  __device__ __forceinline__ void cut(float (&s)[4 * A], unsigned first, unsigned lo, unsigned end, int n, int g) {
+  static __device__ __forceinline__ void cut(Tile& in, float (&s)[4 * A], unsigned first, unsigned lo, unsigned end, int n, int g) {
 #pragma unroll
     for (int a = 0; a < A; ++a) {
-      const unsigned at = first + 16 * subtile(a, n) + 4 * g;
+      const unsigned at = first + 16 * subtile(a, n) + g;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        if (at + r < lo || at + r >= end) s[4 * a + r] = -INFINITY;
-      if (at + (n & 3) < lo || at + (n & 3) >= end) {
+        if (at + 4 * r < lo || at + 4 * r >= end) s[4 * a + r] = -INFINITY;
+      if (at + 4 * (n & 3) < lo || at + 4 * (n & 3) >= end) {
 #pragma unroll
-        for (int b = 0; b < NG; ++b) vs[a].w[b] = 0;
+        for (int b = 0; b < NG; ++b) in.vs[a].w[b] = 0;
       }
     }
   }
-  __device__ __forceinline__ void add(const float (&p)[4 * A]) {
+  __device__ __forceinline__ void add(const Tile& in, const float (&p)[4 * A]) {
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
       uint32_t part[PP][2 * A];                     // the weights of this lane's keys for the group
 #pragma unroll
       for (int a = 0; a < A; ++a) {
-        const float sc = lo_f(vs[a].w[b]), bias = fmaf(-16.f, sc, hi_f(vs[a].w[b]));
+        const float sc = lo_f(in.vs[a].w[b]), bias = fmaf(-16.f, sc, hi_f(in.vs[a].w[b]));
         float w[4];
         w[0] = p[4 * a + 0] * of_four<0>(sc);
         w[1] = p[4 * a + 1] * of_four<1>(sc);
@@ -295,7 +443,7 @@ struct Q4Sweep {
         uint32_t r[4];                              // half-words h of the keys 2 j and 2 j + 1
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const Words<VW>&x = v[8 * e + 2 * j], &y = v[8 * e + 2 * j + 1];
+          const Words<VW>&x = in.v[8 * e + 2 * j], &y = in.v[8 * e + 2 * j + 1];
           if constexpr (D == 64) r[j] = x.w[0] | y.w[0] << 16;
           else r[j] = halves(x.w[h >> 1], y.w[h >> 1], h);
         }
@@ -319,47 +467,67 @@ struct Q4Sweep {
   }
 };
 
-// Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.
-template <typename S>
-__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end,
-                                         float unit) {
+// Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.  The next tile is requested
+// whole before this one is worked on (kAhead), or its keys once this one's scores are done and its values at the end; the page
+// ids of the one behind it before that.
+template <typename S, bool kAhead>
+__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end) {
   constexpr int KT = S::KT, U = S::U;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   w.clear(n);
   if (t >= t_end) return false;
+  const int size = 1 << a.shift;
+  const bool whole = size >= KT;                    // a tile lies inside one page
   int id[U];
-  const char* base[U];
-  bool bad = tile_pages<U>(a, row, t * KT, s, id);
-  const auto load_k = [&](int first) __attribute__((always_inline)) {
-    tile_base<U>(a, a.p.kc, kvh, first, id, base);
-    w.load_k(base, a.p, n, g);
-    tile_base<U>(a, a.p.ks, kvh, first, id, base);
-    w.load_scales(w.ks, base, a.p.ks.row_bytes, n, g);
+  bool bad = false;
+  const auto ids = [&](int first) __attribute__((always_inline)) {
+    if (whole) id[0] = row[(unsigned)first >> a.shift];
+    else tile_ids<U>(a, row, first, s, id);
   };
-  const auto load_v = [&](int first) __attribute__((always_inline)) {
-    tile_base<U>(a, a.p.vc, kvh, first, id, base);
-    w.load_v(base, a.p, n, g);
-    tile_base<U>(a, a.p.vs, kvh, first, id, base);
-    w.load_scales(w.vs, base, a.p.vs.row_bytes, n, g);
+  const auto check = [&]() __attribute__((always_inline)) {
+    if (whole) {
+      if ((unsigned)id[0] >= (unsigned)a.num_pages) {
+        bad = true;
+        id[0] = 0;
+      }
+    } else {
+      bad |= tile_bad<U>(a, id);
+    }
   };
-  load_k(t * KT);
-  load_v(t * KT);
-  while (true) {
+  const auto load_k = [&](typename S::Tile& x, int first) __attribute__((always_inline)) {
+    const int at = first & (size - 1);
+    if (whole) w.load_k(x, a.p, page_rows(a.p.kc, id[0], kvh, at, size, S::kCodes), page_rows(a.p.ks, id[0], kvh, at, size, S::kScales), n, g);
+    else w.load_k(x, a, a.p, id, kvh, first, n, g);
+  };
+  const auto load_v = [&](typename S::Tile& x, int first) __attribute__((always_inline)) {
+    const int at = first & (size - 1);
+    if (whole) w.load_v(x, a.p, page_rows(a.p.vc, id[0], kvh, at, size, S::kCodes), page_rows(a.p.vs, id[0], kvh, at, size, S::kScales), n, g);
+    else w.load_v(x, a, a.p, id, kvh, first, n, g);
+  };
+  // one tile (in x), the next one's requests (to y); whether there is another
+  const auto step = [&](typename S::Tile& x, typename S::Tile& y) __attribute__((always_inline)) {
     const int next = t + kWaves;
     const bool more = next < t_end;
-    if (more) bad |= tile_pages<U>(a, row, next * KT, s, id);
+    if (more) {
+      check();
+      if (kAhead) {
+        load_k(y, next * KT);
+        load_v(y, next * KT);
+        if (next + kWaves < t_end) ids((next + kWaves) * KT);
+      }
+    }
     float p[4 * S::A];
-    w.scores(p);
-    if (more) load_k(next * KT);
+    w.scores(x, p);
+    if (!kAhead && more) load_k(x, next * KT);
     const unsigned first = (unsigned)t * KT, lo = s.lo, end = s.n;
-    if (first < lo || first + KT > end) w.cut(p, first, lo, end, n, g);
+    if (first < lo || first + KT > end) w.cut(x, p, first, lo, end, n, g);
     float mx = p[0];
 #pragma unroll
     for (int i = 1; i < 4 * S::A; ++i) mx = fmaxf(mx, p[i]);
     mx = col_max4(mx);
     if (__any(mx > w.m)) {
       const float nm = fmaxf(w.m, mx);
-      const float f = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m - nm) * unit);
+      const float f = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m - nm) * w.unit);
       w.l *= f;
 #pragma unroll
       for (int i = 0; i < S::N; ++i) w.acc[i] *= f;
@@ -371,20 +539,40 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4 * S::A; ++i) {
-      p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * unit);
+      p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * w.unit);
       sum += p[i];
     }
     w.l += sum;
-    w.add(p);
-    if (!more) return bad;
-    load_v(next * KT);
+    w.add(x, p);
+    if (!kAhead && more) {
+      load_v(x, next * KT);
+      if (next + kWaves < t_end) ids((next + kWaves) * KT);
+    }
     t = next;
+    return more;
+  };
+  typename S::Tile tiles[kAhead ? 2 : 1];
+  ids(t * KT);
+  check();
+  load_k(tiles[0], t * KT);
+  load_v(tiles[0], t * KT);
+  if (t + kWaves < t_end) ids((t + kWaves) * KT);
+  if constexpr (kAhead) {
+    while (step(tiles[0], tiles[1]) && step(tiles[1], tiles[0])) {
+    }
+  } else {
+    while (step(tiles[0], tiles[0])) {
+    }
   }
+  return bad;
 }
 
 // Waves of a SIMD that the registers are cut for: two need no more than 256 (and no moves to accumulation registers
 // and back), but for the widest rows.
 constexpr int q4_waves(int esize, int d, int g, int j) { return d < 256 || (esize == 2 && g == 64 && j == 2) ? 2 : 1; }
+
+// Whether the registers hold two tiles.
+constexpr bool q4_ahead(int d) { return d < 0; }
 
 template <typename T, int D, int G, int J>
 __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_attn_kernel(Q4AttnArgs a) {
@@ -427,8 +615,8 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
   // scores stay q . k up to the exponential; a scale below zero turns q over, one of zero clears it
   const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : a.scale, size = a.scale == 0.f ? 1.f : fabsf(a.scale);
   S w;
-  w.load_q(n % C < rows ? reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + n % C) * a.q_head) : nullptr, n, g, sign);
-  const bool bad = q4_sweep(a, w, table, s, kvh, t0 + wave, t1, size * kLog2e);
+  w.load_q(n % C < rows ? reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + n % C) * a.q_head) : nullptr, n, g, sign, size * kLog2e);
+  const bool bad = q4_sweep<S, q4_ahead(D)>(a, w, table, s, kvh, t0 + wave, t1);
   const float l = col_sum4(w.l);
   float accb[S::NG];
 #pragma unroll
@@ -448,7 +636,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
           *reinterpret_cast<f32x2*>(to) = f32x2{w.acc[i][r] + bias, w.acc[i + 1][r] + bias};
       }
     if (g == 0) {
-      sm[wave][n] = w.m * size;
+      sm[wave][n] = w.m * (w.unit * 0.6931471805599453f);
       sl[wave][n] = l;
     }
   }

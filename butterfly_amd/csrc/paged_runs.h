@@ -190,16 +190,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 
-// The pages of tile t: one base per 16 keys, with the page's and the rows' offsets.  Keys outside [lo, n)
-// share the page of the nearest key inside, so no entry behind the last page (or before the window) is read.
+// The pages of the tile at key `first`: one for each 16 keys.  Keys outside [lo, n) share the page of the nearest key
+// inside, so no entry behind the last page (or before the window) is read.
 template <int U>
-__device__ __forceinline__ bool tile_pages(const RunArgs& a, const int32_t* row, int first, const Span& s, int (&id)[U]) {
-  bool bad = false;
+__device__ __forceinline__ void tile_ids(const RunArgs& a, const int32_t* row, int first, const Span& s, int (&id)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     unsigned t = (unsigned)first + 16 * u;
     t = t < (unsigned)s.lo ? s.lo : t > (unsigned)s.n - 1 ? s.n - 1 : t;
     id[u] = row[t >> a.shift];
+  }
+}
+// Whether one of them is outside the pages: it is page 0 then.
+template <int U>
+__device__ __forceinline__ bool tile_bad(const RunArgs& a, int (&id)[U]) {
+  bool bad = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
     if ((unsigned)id[u] >= (unsigned)a.num_pages) {
       bad = true;
       id[u] = 0;
@@ -207,6 +214,7 @@ __device__ __forceinline__ bool tile_pages(const RunArgs& a, const int32_t* row,
   }
   return bad;
 }
+// Where their rows lie.
 template <int U>
 __device__ __forceinline__ void tile_base(const RunArgs& a, const PagePtr& p, int h, int first, const int (&id)[U],
                                           const char* (&base)[U]) {
