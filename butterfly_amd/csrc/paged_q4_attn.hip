@@ -21,6 +21,10 @@ constexpr int q4_runs_for(int) { return 512; }   // in all, where requests and h
 static_assert(q4_runs_for(64) <= kMaxRuns, "");
 constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 
+// A column's sums keep their reference until its maximum is more than this many powers of two above it: 16 columns of a
+// tile hardly ever rise together, and one that rises would turn all sums over.  (Weights are at most 2^4 then.)
+constexpr float kQ4Lag = 4.f;
+
 struct Q4AttnArgs : RunArgs {
   const char* q;
   Q4Ptr p;
@@ -124,7 +128,7 @@ struct Q4Sweep {
   static constexpr int VW = D == 256 ? 2 : 1;       // dwords of a piece (d 64: half of one)
   f32x4 acc[N];                                     // acc[4 h + j][r]: row n of q's columns, element d_of(4 h + j, 4 g + r)
   float accb[NG];                                   // this lane's keys only, as l
-  float m, l;                                       // m: the largest q . k, unscaled
+  float m, l, most;                                 // most: the largest q . k, unscaled; m: what the sums refer to
   uint32_t q[J][QP][D / 32][QW];
   float qs[NG];                                     // sums of q over a group, in the scores' unit
   float unit;                                       // what a score counts
@@ -145,7 +149,7 @@ struct Q4Sweep {
     for (int i = 0; i < N; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NG; ++i) accb[i] = 0.f;
-    m = -INFINITY;
+    m = most = -INFINITY;
     l = 0.f;
     ones = sixteens();
 #pragma unroll
@@ -385,6 +389,16 @@ struct Q4Sweep {
       for (int i = 0; i < 4; ++i) s[4 * a + i] = t[i];
     }
   }
+  // The sums with the largest score as their reference.
+  __device__ __forceinline__ void settle() {
+    const float f = most == m ? 1.f : __builtin_amdgcn_exp2f((m - most) * unit);
+    l *= f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) accb[i] *= f;
+    m = most;
+  }
   // Leaves out the keys outside [lo, n) of the tile that begins at `first`: scores of -inf, scales of zero.
   static __device__ __forceinline__ void cut(Tile& in, float (&s)[4 * A], unsigned first, unsigned lo, unsigned end, int n, int g) {
 #pragma unroll
@@ -525,7 +539,9 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
 #pragma unroll
     for (int i = 1; i < 4 * S::A; ++i) mx = fmaxf(mx, p[i]);
     mx = col_max4(mx);
-    if (__any(mx > w.m)) {
+    w.most = fmaxf(w.most, mx);
+    // (not `> kQ4Lag`: a unit of NaN, or one of 0 on the first maximum, goes the careful way)
+    if (__any(mx > w.m && !((mx - w.m) * w.unit <= kQ4Lag))) {
       const float nm = fmaxf(w.m, mx);
       const float f = nm == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m - nm) * w.unit);
       w.l *= f;
@@ -564,6 +580,7 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     while (step(tiles[0], tiles[0])) {
     }
   }
+  w.settle();
   return bad;
 }
 
@@ -581,7 +598,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
   __shared__ float so[kWaves][16 * LD];
   __shared__ float sm[kWaves][16], sl[kWaves][16];
   __shared__ int sbad;
-  const Run run = plan_run<KT>(a, blockIdx.x);
+  const Run run = plan_run<KT, true>(a, blockIdx.x);
   if (run.b < 0) return;
   // (every store comes after the last page id is read, as in paged_attn_kernel)
   const auto leave = [&]() {

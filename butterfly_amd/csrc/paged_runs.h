@@ -103,7 +103,7 @@ __device__ __forceinline__ float wave_max(float x) {
 
 // The request that item `idx` falls into, where request b has units * splits_b items.  Every wave does it by
 // itself: a lane sums a stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
-template <int KT>
+template <int KT, bool kEven = false>
 __device__ __forceinline__ Run plan_run(const RunArgs& a, int64_t idx) {
   if (a.direct) {                                   // no request can have several runs: item = (request, unit)
     const int b = (int)idx / a.units;
@@ -134,8 +134,23 @@ __device__ __forceinline__ Run plan_run(const RunArgs& a, int64_t idx) {
   int items = 0;
   each([&](int n) { items += runs(n); });
   const int64_t pairs = (int64_t)a.requests * a.units;
-  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs)
-    c = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
+  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs) {
+    int fits = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
+    if (kEven && per == 1) {
+      // the least c between the two whose runs fit, or near it: the longest run is the call's time
+#pragma unroll 1
+      for (int i = 0; i < 5 && fits - c > 1; ++i) {
+        const int low = c, mid = c + (fits - c) / 2;
+        c = mid;                                    // (what `runs` counts with)
+        const int n = b0 < b1 ? runs(first) : 0;
+        if ((int64_t)__builtin_amdgcn_readlane(wave_scan(n), 63) * a.units <= a.runs) {
+          fits = mid;
+          c = low;
+        }
+      }
+    }
+    c = fits;
+  }
   int slots = 0;                                    // low half: partials; high half: requests that have them (both
   items = 0;                                        // below kMaxSlots in all)
   const auto parts = [](int s) { return s > 1 ? s | 0x10000 : 0; };
