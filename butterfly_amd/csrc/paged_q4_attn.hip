@@ -151,28 +151,35 @@ struct Q4Sweep {
     for (int i = 0; i < NG; ++i) accb[i] = 0.f;
     m = most = -INFINITY;
     l = 0.f;
+    unit = 0.f;
     ones = sixteens();
 #pragma unroll
     for (int j = 0; j < J; ++j) mine[j] = n / C == j ? ~0u : 0u;
   }
-  // q times `sign`: a quarter of each group, in the codes' order.  `size`: the scale's size, times log2 e.
-  __device__ __forceinline__ void load_q(const T* row, int n, int g, float sign, float size) {
-    constexpr int E = G / 4, VE = 16 / sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(VE)));
+  // A row of q as it lies: a quarter of each group.
+  static constexpr int kVec = 16 / sizeof(T);
+  typedef T QVec __attribute__((ext_vector_type(kVec)));
+  struct QRow {
+    QVec x[NG][G / 4 / kVec];
+  };
+  static __device__ __forceinline__ void fetch_q(QRow& q, const T* row, int g) {
+#pragma unroll
+    for (int b = 0; b < NG; ++b)
+#pragma unroll
+      for (int i = 0; i < G / 4 / kVec; ++i) q.x[b][i] = *reinterpret_cast<const QVec*>(row + G * b + G / 4 * g + kVec * i);
+  }
+  // q times `sign` (nothing where it is not `there`), in the codes' order.  `size`: the scale's size, times log2 e.
+  __device__ __forceinline__ void take_q(const QRow& raw, bool there, int n, float sign, float size) {
+    constexpr int E = G / 4;
     float x[NG][E], most = 0.f;
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
       float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < E; i += VE) {
-        vec y;
-        if (row != nullptr) y = *reinterpret_cast<const vec*>(row + G * b + E * g + i);
-#pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          x[b][i + e] = row != nullptr ? to_f32(y[e]) * sign : 0.f;
-          most = fmaxf(most, fabsf(x[b][i + e]));
-          sum += x[b][i + e];
-        }
+      for (int i = 0; i < E; ++i) {
+        x[b][i] = there ? to_f32(raw.x[b][i / kVec][i % kVec]) * sign : 0.f;
+        most = fmaxf(most, fabsf(x[b][i]));
+        sum += x[b][i];
       }
       qs[b] = col_sum4(sum);
     }
@@ -484,8 +491,9 @@ struct Q4Sweep {
 // Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.  The next tile is requested
 // whole before this one is worked on (kAhead), or its keys once this one's scores are done and its values at the end; the page
 // ids of the one behind it before that.
-template <typename S, bool kAhead>
-__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end) {
+template <typename S, bool kAhead, typename T>
+__device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end,
+                                         const T* q, bool there, float sign, float unit) {
   constexpr int KT = S::KT, U = S::U;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   w.clear(n);
@@ -568,11 +576,14 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     return more;
   };
   typename S::Tile tiles[kAhead ? 2 : 1];
+  typename S::QRow raw;                             // (before the tile: loads return in order)
+  S::fetch_q(raw, q, g);
   ids(t * KT);
   check();
   load_k(tiles[0], t * KT);
   load_v(tiles[0], t * KT);
   if (t + kWaves < t_end) ids((t + kWaves) * KT);
+  w.take_q(raw, there, n, sign, unit);
   if constexpr (kAhead) {
     while (step(tiles[0], tiles[1]) && step(tiles[1], tiles[0])) {
     }
@@ -632,8 +643,9 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
   // scores stay q . k up to the exponential; a scale below zero turns q over, one of zero clears it
   const float sign = a.scale > 0.f ? 1.f : a.scale < 0.f ? -1.f : a.scale, size = a.scale == 0.f ? 1.f : fabsf(a.scale);
   S w;
-  w.load_q(n % C < rows ? reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + n % C) * a.q_head) : nullptr, n, g, sign, size * kLog2e);
-  const bool bad = q4_sweep<S, q4_ahead(D)>(a, w, table, s, kvh, t0 + wave, t1);
+  const bool there = n % C < rows;                  // (a column without a row of q reads the first one's)
+  const T* q = reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + (there ? n % C : 0)) * a.q_head);
+  const bool bad = q4_sweep<S, q4_ahead(D)>(a, w, table, s, kvh, t0 + wave, t1, q, there, sign, size * kLog2e);
   const float l = col_sum4(w.l);
   float accb[S::NG];
 #pragma unroll
@@ -653,7 +665,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
           *reinterpret_cast<f32x2*>(to) = f32x2{w.acc[i][r] + bias, w.acc[i + 1][r] + bias};
       }
     if (g == 0) {
-      sm[wave][n] = w.m * (w.unit * 0.6931471805599453f);
+      sm[wave][n] = w.m == -INFINITY ? w.m : w.m * (w.unit * 0.6931471805599453f);   // (a wave without tiles has no unit)
       sl[wave][n] = l;
     }
   }
