@@ -17,8 +17,6 @@
 
 namespace bfly {
 
-constexpr int q4_runs_for(int) { return 512; }   // in all, where requests and heads leave them
-static_assert(q4_runs_for(64) <= kMaxRuns, "");
 constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 
 // A column's sums keep their reference until its maximum is more than this many powers of two above it: 16 columns of a
@@ -712,6 +710,13 @@ static int q4_blocks(int esize, int64_t head_dim, int64_t group) {
   return most < fit ? most : fit;
 }
 static int q4_tile(int blocks) { return blocks > 2 ? 64 : 32; }
+// Runs in all, where requests and heads leave them: as many workgroups as a CU holds by its registers.  Measured, us, half as
+// many / these: 32 requests of up to 131072 tokens 90 / 73, one of 262144 of d 256 66 / 62, 8 of 60000 of d 64 29 / 26; twice as
+// many: 90, 80, 24.  Fewer runs of two rounds before as many of one: one request of 32768 tokens 15.8 -> 14.0.
+static int q4_runs(int esize, int64_t head_dim, int64_t group, int blocks) {
+  return 256 * q4_waves(esize, (int)head_dim, (int)group, blocks);
+}
+static_assert(256 * 2 <= kMaxRuns, "");
 
 template <typename T, int D, int G>
 static void launch_q4(const Q4AttnArgs& a, int blocks, int64_t items, hipStream_t stream) {
@@ -778,9 +783,9 @@ extern "C" int bfly_paged_q4_attention(const bfly_paged_q4_attention_args_t* arg
                            x.window),
                  "too many heads");
   run_workspace(a, x.workspace, x.head_dim);
-  a.runs = q4_runs_for((int)x.head_dim);
   a.whole = q4_whole_rounds((int64_t)a.requests * a.units);
   const int blocks = q4_blocks((int)es, x.head_dim, a.group);
+  a.runs = q4_runs((int)es, x.head_dim, x.pages.group, blocks);
   const int64_t items = run_items(a, most_rounds(a.capacity, a.window, q4_tile(blocks)));
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads
 #define BFLY_Q4(T, D, G) launch_q4<T, D, G>(a, blocks, items, stream)

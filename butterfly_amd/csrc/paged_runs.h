@@ -101,6 +101,7 @@ __device__ __forceinline__ float wave_max(float x) {
   return col_max4(x);
 }
 
+// kEven: the runs as even as they can be (and fewer of them before they are short).
 // The request that item `idx` falls into, where request b has units * splits_b items.  Every wave does it by
 // itself: a lane sums a stretch of requests, one scan over the lanes, then the lane of the item walks its stretch.
 template <int KT, bool kEven = false>
@@ -127,15 +128,17 @@ __device__ __forceinline__ Run plan_run(const RunArgs& a, int64_t idx) {
   float total = 0.f;
   each([&](int n) { total += (float)n; });
   total = wave_total(total) * (float)a.units;
+  // fewer runs, of two rounds, before as many of one (kEven)
+  const int most = __builtin_amdgcn_readfirstlane(kEven && total < 2.f * (float)a.runs ? a.runs / 2 : a.runs);
   // c fills the runs exactly if the requests' last, shorter runs fit among them; else room is left for one each
   const auto over = [&](float to) { return fminf(fmaxf(ceilf(total / to), (float)kMinRun), 1e9f); };
-  int c = __builtin_amdgcn_readfirstlane((int)over((float)a.runs));
+  int c = __builtin_amdgcn_readfirstlane((int)over((float)most));
   const auto runs = [&](int n) { return n > c && n > a.whole ? (int)(((unsigned)n + c - 1) / (unsigned)c) : 1; };
   int items = 0;
   each([&](int n) { items += runs(n); });
   const int64_t pairs = (int64_t)a.requests * a.units;
-  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > a.runs && pairs < a.runs) {
-    int fits = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < a.runs / 2 ? a.runs - (int)pairs : a.runs / 2)));
+  if ((int64_t)__builtin_amdgcn_readlane(wave_scan(items), 63) * a.units > most && pairs < most) {
+    int fits = __builtin_amdgcn_readfirstlane((int)over((float)(pairs < most / 2 ? most - (int)pairs : most / 2)));
     if (kEven && per == 1) {
       // the least c between the two whose runs fit, or near it: the longest run is the call's time
 #pragma unroll 1
@@ -143,7 +146,7 @@ __device__ __forceinline__ Run plan_run(const RunArgs& a, int64_t idx) {
         const int low = c, mid = c + (fits - c) / 2;
         c = mid;                                    // (what `runs` counts with)
         const int n = b0 < b1 ? runs(first) : 0;
-        if ((int64_t)__builtin_amdgcn_readlane(wave_scan(n), 63) * a.units <= a.runs) {
+        if ((int64_t)__builtin_amdgcn_readlane(wave_scan(n), 63) * a.units <= most) {
           fits = mid;
           c = low;
         }
