@@ -67,17 +67,17 @@ def test_rows_of_all_sizes(rows, vocab, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_orders_that_fill_the_list(dtype):
+@pytest.mark.parametrize("v", [70001, 700001])
+def test_orders_that_fill_the_list(dtype, v):
     """Rows that rise, fall, are all equal, hold few values, or rise in jumps: every round has more than its part of
-    the top, and ties everywhere."""
-    v = 70001
+    the top, and ties everywhere; 700001: two rounds of a workgroup to a kept maximum where it has the whole row."""
     i = torch.arange(v, device="cuda")
     rows = [i / v * 8, -i / v * 8, torch.zeros(v, device="cuda"), (i % 3).float(), (i * 7919 % v) / v * 8,
             (i // 8192).float(), -(i // 8192).float(), torch.where(i >= v - 64, 5.0, 0.0), torch.where(i % 257 == 0, 5.0, -1.0)]
     for parts in (1, len(rows)):                     # few rows: parts of a row; many: a workgroup a row
         x = torch.stack(rows).to(dtype)
         if parts == 1:
-            x = x.repeat(150, 1)
+            x = x.repeat(150 if v < 100000 else 120, 1)
         tokens = torch.arange(x.shape[0], device="cuda") * 31 % v
         for top in (1, 20, 64):
             _check(x, tokens, top)
