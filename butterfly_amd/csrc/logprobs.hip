@@ -273,6 +273,7 @@ struct RowOf {
   typedef T Vec __attribute__((ext_vector_type(VE)));
   const T* x;
   int skew, vocab, v0, v1;
+  bool stream;                                      // long: past the caches' replacement (short ones are read again there)
   __device__ __forceinline__ RowOf(const LogprobArgs& a, int64_t row, int part) {
     x = reinterpret_cast<const T*>(a.logits + row * a.stride);
     skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
@@ -280,6 +281,7 @@ struct RowOf {
     const int vectors = (int)(((int64_t)a.vocab + skew + VE - 1) / VE);
     v0 = part * a.per < vectors ? part * a.per : vectors;
     v1 = v0 + a.per < vectors ? v0 + a.per : vectors;
+    stream = a.per > 4 * kRound;
   }
   // Element i of thread t's in the round at vector `base`; whether it is one.
   __device__ __forceinline__ int at(int base, int t, int i) const { return (base + t + kThreads * (i / VE)) * VE - skew + i % VE; }
@@ -293,7 +295,13 @@ struct RowOf {
     for (int i = 0; i < NV; ++i) {
       const int v = base + t + kThreads * i, p = v * VE - skew;
       if (v < v1 && p >= 0 && p + VE <= vocab) {
-        y[i] = __builtin_nontemporal_load(reinterpret_cast<const Vec*>(x + p));
+        const Vec* q = reinterpret_cast<const Vec*>(x + p);
+        if (stream) {
+          y[i] = __builtin_nontemporal_load(q);
+        } else {
+          asm("" : "+v"(q));                        // (else both loads become one, of the second kind)
+          y[i] = *q;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) y[i][e] = v < v1 && p + e >= 0 && p + e < vocab ? x[p + e] : (T)-INFINITY;
@@ -429,25 +437,37 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_kernel(LogprobArgs a) {
   }
   if constexpr (kTop) {
     __syncthreads();
+    constexpr uint32_t kNone = 0x007FFFFFu;         // the rank of -inf
     uint32_t from = in.v0 < in.v1 ? rank_bound<kThreads>(sh, all, a.top) : 0xFFFFFFFFu;
-    if (from <= rank_of(-INFINITY))                 // (mostly -inf: the exact k-th of all threads may be above)
+    if (from <= kNone)                              // (mostly -inf: the exact k-th of all threads may be above)
       from = (uint32_t)(kth_of_threads<kThreads>(sh, in.v0 < in.v1 ? (uint64_t)all << 32 | (uint32_t)(kThreads - t) : 0, a.top) >> 32);
+    const bool sparse = from <= kNone;              // fewer than k threads have any other: all of those, and the first -inf
+    const uint32_t reach = sparse ? kNone + 1 : from;
     for (int i = 0; i < slot; ++i)
-      if (ranks[i * kThreads + t] >= RankOf<T>::pack(from)) {
+      if (ranks[i * kThreads + t] >= RankOf<T>::pack(reach)) {
         const int at = atomicAdd(sh.segments, 1);
         if (at < kLpSegments) sh.segment[at] = (uint16_t)(i * kThreads + t);
       }
     __syncthreads();
     const int segments = *sh.segments;
     const bool fits = segments <= kLpSegments;
-    const float least = key_value((uint64_t)from << 32);
+    const float least = key_value((uint64_t)reach << 32);
+    const auto push = [&](float v, int at) {
+      const int to = atomicAdd(sh.count, 1);
+      if (to < sh.room) sh.list[to] = argmax_key(v, (uint32_t)at);
+    };
     for (int f = 0; fits && f < a.fold; ++f)
       each_element<T, kThreads>(sh, in, segments, a.fold, f, [&](float v, int at) {
-        if (!(v < least)) {
-          const int to = atomicAdd(sh.count, 1);
-          if (to < sh.room) sh.list[to] = argmax_key(v, (uint32_t)at);
-        }
+        if (!(v < least)) push(v, at);
       });
+    if (sparse) {                                   // (where they do not make up k, k -inf are among the first 2 k)
+      const int first = in.v0 * Row::VE - in.skew > 0 ? in.v0 * Row::VE - in.skew : 0;
+      const int64_t end = (int64_t)in.v1 * Row::VE - in.skew < in.vocab ? (int64_t)in.v1 * Row::VE - in.skew : in.vocab;
+      for (int i = t; i < 2 * a.top && first + i < end; i += kThreads) {
+        const float v = to_f32(in.x[first + i]);
+        if (v == -INFINITY) push(v, first + i);
+      }
+    }
     __syncthreads();
     if (fits && *sh.count <= sh.room) cut_list<kThreads>(sh, *sh.count, a.top);
     else top_by_keys<T, kThreads>(a, sh, in, from, slot);

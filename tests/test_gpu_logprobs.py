@@ -117,6 +117,23 @@ def test_masks_infinities_and_nan(dtype, vocab):
         _check(x[r:r + 1], tokens[r:r + 1], 5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [3, 1100])
+def test_few_tokens_left(dtype, rows):
+    """Constrained rows: from none to some hundred logits are not -inf, in one place or all over; the rest of the top is
+    the first -inf ones."""
+    v = 20001
+    x = torch.full((rows, v), -math.inf, device="cuda")
+    g = _gen(rows)
+    for r in range(rows):
+        n = (0, 1, 3, 49, 50, 51, 64, 65, 200, 2000)[r % 10] if rows > 3 else (3, 63, 700)[r]
+        at = torch.randperm(v, generator=g, device="cuda")[:n] if r % 3 else torch.arange(v - n, v, device="cuda") if r % 2 else \
+            torch.arange(n, device="cuda")
+        x[r, at] = torch.randn(n, generator=g, device="cuda") * 2
+    for top in (5, 50, 64):
+        _check(x.to(dtype), torch.arange(rows, device="cuda") % v, top)
+
+
 def test_sure_rows():
     """One logit far above the rest: entropies near zero."""
     x = torch.randn(6, 4000, generator=_gen(5), device="cuda")
