@@ -78,17 +78,26 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
         logits = logits.clone(memory_format=torch.contiguous_format)
     tokens = tokens.contiguous()
     rows, cuda = logits.shape[0], logits.device
-    # one allocation for the fp32 results
-    out = _EMPTY((rows * (2 + top),), (1,), dtype=torch.float32, device=cuda)
-    logprobs, entropy, tops = out.split_with_sizes((rows, rows, rows * top))
-    ids = _EMPTY((rows, top), (top, 1), dtype=torch.int64, device=cuda)
+    f32, many = torch.float32, (*shape, top)
+    strides, by = (1,) if len(shape) == 1 else _strides(shape), _strides(many)
+    logprobs, entropy = _EMPTY(shape, strides, dtype=f32, device=cuda), _EMPTY(shape, strides, dtype=f32, device=cuda)
+    tops, ids = _EMPTY(many, by, dtype=f32, device=cuda), _EMPTY(many, by, dtype=torch.int64, device=cuda)
     if rows:
         need = _workspace_bytes(rows, vocab, top)
         ws = _EMPTY((need,), (1,), dtype=torch.uint8, device=cuda) if need else None
         _native.call("bfly_token_logprobs", logits.data_ptr(), code, rows, vocab, logits.stride(0) if rows > 1 else vocab,
                      tokens.data_ptr(), top, logprobs.data_ptr(), entropy.data_ptr(), tops.data_ptr(), ids.data_ptr(),
                      0 if ws is None else ws.data_ptr(), need, stream_of(dev))
-    return TokenLogprobs(logprobs.view(shape), entropy.view(shape), tops.view(*shape, top), ids.view(*shape, top))
+    return TokenLogprobs(logprobs, entropy, tops, ids)
+
+
+def _strides(shape):
+    """Strides of a contiguous tensor."""
+    out, n = [], 1
+    for s in reversed(shape):
+        out.append(n)
+        n *= max(1, s)
+    return tuple(reversed(out))
 
 
 @lru_cache(maxsize=1024)

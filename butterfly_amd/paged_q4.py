@@ -70,45 +70,56 @@ def empty_q4_pages(num_pages: int, num_kv_heads: int, page_size: int, head_dim: 
 
 
 def _pages(pages: Q4Pages, dev: int, written: bool):
-    """(num_pages, Hkv, page_size, d), group, and what the packed structs hold of the pages."""
+    """(num_pages, Hkv, page_size, d), and what the packed structs hold of the pages."""
     kc, ks, vc, vs = pages
-    shape, sshape = kc.shape, ks.shape
-    if len(shape) != 4 or len(sshape) != 5 or vc.shape != shape or vs.shape != sshape or sshape[:3] != shape[:3] \
-            or sshape[4] != 2 or sshape[3] == 0 or not kc.dtype is vc.dtype is torch.uint8 \
-            or not ks.dtype is vs.dtype is torch.bfloat16:
-        raise ValueError("pages must be uint8 codes [num_pages, Hkv, page_size, d / 2] and bfloat16 scales "
-                         "[num_pages, Hkv, page_size, d / group, 2], k's and v's alike")
+    if not kc.dtype is vc.dtype is torch.uint8 or not ks.dtype is vs.dtype is torch.bfloat16:
+        raise ValueError("pages must be uint8 codes and bfloat16 scales")
     if not kc.get_device() == ks.get_device() == vc.get_device() == vs.get_device() == dev:
         _other_device()
-    num, hkv, size, half = shape
-    d, groups = 2 * half, sshape[3]
+    shape, sizes = _layout(kc.shape, kc.stride(), ks.shape, ks.stride(), vc.shape, vc.stride(), vs.shape, vs.stride(), written)
+    a, b, c, d = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    if (a | b | c | d) & 15:
+        raise ValueError("pages must be 16-byte aligned")
+    if written and len({a, b, c, d}) < 4:
+        raise ValueError("pages that are written must not overlap themselves or each other")
+    return shape, (a, b, c, d, *sizes)
+
+
+@lru_cache(maxsize=1024)
+def _layout(kc, kc_strides, ks, ks_strides, vc, vc_strides, vs, vs_strides, written):
+    """The checks of the pages' shapes and strides, which a decode step would repeat for every layer: (num_pages, Hkv,
+    page_size, d) and (num_pages, page_size, group, strides in bytes)."""
+    if len(kc) != 4 or len(ks) != 5 or vc != kc or vs != ks or ks[:3] != kc[:3] or ks[4] != 2 or ks[3] == 0:
+        raise ValueError("pages must be codes [num_pages, Hkv, page_size, d / 2] and scales [num_pages, Hkv, page_size, "
+                         "d / group, 2], k's and v's alike")
+    num, hkv, size, half = kc
+    d, groups = 2 * half, ks[3]
     group = d // groups
     if size not in PAGE_SIZES:
         raise ValueError(f"page_size {size} must be a power of two from 16 to 1024")
+    if 0 in kc:
+        raise ValueError("the pages hold nothing")
     if d not in HEAD_DIMS:
         raise NotImplementedError(f"pages in 4 bits: head_dim={d} unsupported {HEAD_DIMS}")
     if group not in GROUPS or group * groups != d:
         raise ValueError(f"groups of {d} / {groups} elements: must be of 32 or 64")
-    if 0 in shape:
-        raise ValueError("the pages hold nothing")
-    unit = min(16, 4 * groups)
-    strides, ptrs = [], []
-    for t, last, by in ((kc, (1,), 16), (ks, (2, 1), unit), (vc, (1,), 16), (vs, (2, 1), unit)):
-        st, es = t.stride(), t.element_size()
+    out = []
+    for shape, strides, last, es, unit in ((kc, kc_strides, (1,), 1, 16), (ks, ks_strides, (2, 1), 2, min(16, 4 * groups)),
+                                           (vc, vc_strides, (1,), 1, 16), (vs, vs_strides, (2, 1), 2, min(16, 4 * groups))):
         # (a dimension of one element has no stride to speak of)
-        own = [s * es if n > 1 else 0 for s, n in zip(st[:3], shape)]
-        inner = [s for s, n in zip(st[3:], t.shape[3:]) if n > 1]
-        ptr = t.data_ptr()
-        if inner != [s for s, n in zip(last, t.shape[3:]) if n > 1] or ptr & 15 or any(s % by for s in own):
+        own = [s * es if n > 1 else 0 for s, n in zip(strides[:3], shape)]
+        if any(s != x for s, n, x in zip(strides[3:], shape[3:], last) if n > 1) or any(s % unit for s in own):
             raise ValueError("a row's codes and its scales must be contiguous, 16-byte aligned in every other dimension "
                              "(scales of less than 16 bytes a row: as long as that)")
         if written and any(s == 0 and n > 1 for s, n in zip(own, shape)):
             raise ValueError("pages that are written must not overlap themselves or each other")
-        strides += own
-        ptrs.append(ptr)
-    if written and len(set(ptrs)) < 4:
-        raise ValueError("pages that are written must not overlap themselves or each other")
-    return (num, hkv, size, d), (*ptrs, num, size, group, *strides)
+        out += own
+    return (num, hkv, size, d), (num, size, group, *out)
+
+
+def _grad(pages: Q4Pages) -> bool:
+    a, b, c, d = pages
+    return a.requires_grad or b.requires_grad or c.requires_grad or d.requires_grad
 
 
 def _check_rows(k, v, shape, slots, dev):
@@ -135,7 +146,7 @@ def paged_q4_append(k: torch.Tensor, v: torch.Tensor, pages: Q4Pages, slots: tor
     if dev != _GET_DEVICE():
         with torch.cuda.device(dev):
             return paged_q4_append(k, v, pages, slots)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or any(t.requires_grad for t in pages)):
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or _grad(pages)):
         raise ValueError(_GRAD)
     if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
         _check_followed(k, v, *pages)
@@ -170,7 +181,7 @@ def paged_q4_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page
             return paged_q4_rope_append(q, k, v, pages, slots, positions, cos, sin, q_weight=q_weight, k_weight=k_weight,
                                         eps=eps)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or cos.requires_grad
-                                    or sin.requires_grad or any(t.requires_grad for t in pages)
+                                    or sin.requires_grad or _grad(pages)
                                     or q_weight is not None and q_weight.requires_grad
                                     or k_weight is not None and k_weight.requires_grad):
         raise ValueError(_GRAD)
@@ -220,7 +231,7 @@ def paged_q4_read(pages: Q4Pages, block_table: torch.Tensor, tokens: int, *,
     if dev != _GET_DEVICE():
         with torch.cuda.device(dev):
             return paged_q4_read(pages, block_table, tokens, dtype=dtype)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in pages):
+    if torch.is_grad_enabled() and _grad(pages):
         raise ValueError(_GRAD)
     if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
         _check_followed(*pages)
@@ -257,7 +268,7 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
     if dev != _GET_DEVICE():
         with torch.cuda.device(dev):
             return paged_q4_attention(q, pages, block_table, lengths, scale=scale, window=window, return_stats=return_stats)
-    if torch.is_grad_enabled() and (q.requires_grad or any(t.requires_grad for t in pages)):
+    if torch.is_grad_enabled() and (q.requires_grad or _grad(pages)):
         raise ValueError(_GRAD)
     if forward_ad._current_level >= 0 or _C._get_tracing_state() is not None:
         _check_followed(q, *pages)
