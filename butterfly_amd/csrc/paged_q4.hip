@@ -12,59 +12,64 @@
 namespace bfly {
 
 // --------------------------------------------------------------------------- one row's codes
-// DPP within 8 lanes: the neighbour in a pair, the other pair of four, the other four of eight (mirrored: every
-// lane of a four holds the same by then).
-constexpr int kPair = 0xB1, kQuad = 0x4E, kEight = 0x141;
+// DPP within 16 lanes: the neighbour in a pair, the other pair of four, the other four of eight and the other eight
+// (mirrored: every lane of a four or eight holds the same by then).
+constexpr int kPair = 0xB1, kQuad = 0x4E, kEight = 0x141, kRow = 0x140;
 template <int kCtrl>
-__device__ __forceinline__ double dpp_double(double x) {
+__device__ __forceinline__ int dpp(int x) { return __builtin_amdgcn_update_dpp(0, x, kCtrl, 0xf, 0xf, false); }
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float x) { return __int_as_float(dpp<kCtrl>(__float_as_int(x))); }
+template <int kCtrl>
+__device__ __forceinline__ double dpp(double x) {
   const uint64_t u = __double_as_longlong(x);
-  const int lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, kCtrl, 0xf, 0xf, false);
-  const int hi = __builtin_amdgcn_update_dpp(0, (int)(u >> 32), kCtrl, 0xf, 0xf, false);
-  return __longlong_as_double((int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo));
+  return __longlong_as_double((int64_t)(((uint64_t)(uint32_t)dpp<kCtrl>((int)(u >> 32)) << 32) | (uint32_t)dpp<kCtrl>((int)(uint32_t)u)));
 }
-template <int kCtrl>
-__device__ __forceinline__ void extremes(double& lo, double& hi, int& bad) {
-  lo = fmin(lo, dpp_double<kCtrl>(lo));
-  hi = fmax(hi, dpp_double<kCtrl>(hi));
-  bad |= __builtin_amdgcn_update_dpp(0, bad, kCtrl, 0xf, 0xf, false);
+// over the 8 to 32 lanes of a row, in each of them
+template <int kLanes, typename F>
+__device__ __forceinline__ F row_sum(F x) {
+  x += dpp<kPair>(x);
+  x += dpp<kQuad>(x);
+  x += dpp<kEight>(x);
+  if constexpr (kLanes > 8) x += dpp<kRow>(x);
+  if constexpr (kLanes > 16) x += __shfl_xor(x, 16);
+  return x;
 }
+__device__ __forceinline__ float least(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double least(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
 
 __device__ __forceinline__ uint32_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
 
 // 8 elements y of a row in each of D / 8 lanes (gl: which): the row's codes, a dword a lane, and the scale and bias
-// of a group in its first lane.
-template <int D, int G>
-__device__ __forceinline__ void q4_store(const double (&y)[8], int gl, char* codes, char* scales) {
+// of a group in its first lane.  F: what the elements are exact in (a row as it lies: fp32).
+template <int D, int G, typename F>
+__device__ __forceinline__ void q4_store(const F (&y)[8], int gl, char* codes, char* scales) {
   constexpr int LG = G / 8;                         // lanes of a group
-  double lo = y[0], hi = y[0];
-  int bad = 0;
+  F lo = y[0], hi = y[0], nan = y[0] - y[0];        // (0, or NaN where there is an infinity or NaN)
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo = fmin(lo, y[e]);
-    hi = fmax(hi, y[e]);
-    bad |= y[e] - y[e] == 0.0 ? 0 : 1;              // an infinity or NaN
+  for (int e = 1; e < 8; ++e) {
+    lo = least(lo, y[e]);
+    hi = most(hi, y[e]);
+    nan += y[e] - y[e];
   }
-  extremes<kPair>(lo, hi, bad);
-  extremes<kQuad>(lo, hi, bad);
-  if constexpr (LG == 8) extremes<kEight>(lo, hi, bad);
-  uint32_t sb = bf16_bits((float)fmax((hi - lo) / 15.0, 1e-8)), bb = bf16_bits((float)lo);
+  int bad = nan == 0 ? 0 : 1;
+  lo = least(lo, dpp<kPair>(lo)), hi = most(hi, dpp<kPair>(hi)), bad |= dpp<kPair>(bad);
+  lo = least(lo, dpp<kQuad>(lo)), hi = most(hi, dpp<kQuad>(hi)), bad |= dpp<kQuad>(bad);
+  if constexpr (LG == 8) lo = least(lo, dpp<kEight>(lo)), hi = most(hi, dpp<kEight>(hi)), bad |= dpp<kEight>(bad);
+  // (a 15th as a product: the same but for values within 2^-52 of themselves of a border between two fp32 numbers)
+  uint32_t sb = bf16_bits((float)fmax(((double)hi - (double)lo) * (1.0 / 15.0), 1e-8)), bb = bf16_bits((float)lo);
   bad |= (sb & 0x7f80u) == 0x7f80u || (bb & 0x7f80u) == 0x7f80u;
   if (bad) sb = bb = 0x7fc0u;
-  const double s = __uint_as_float(sb << 16), b = __uint_as_float(bb << 16), inv = 1.0 / s, half = 0.5 * s;
+  const double s = __uint_as_float(sb << 16), b = __uint_as_float(bb << 16), inv = 1.0 / s;
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    // the nearest whole number to d / s: the product with 1 / s may be off by a rounding, the rest of the
-    // division tells (and where two are as near)
-    const double d = y[e] - b;
-    double q = fmin(fmax(rint(d * inv), -1.0), 16.0);
-    const double r = fma(-q, s, d);
-    const bool odd = ((int)q & 1) != 0;
-    if (r > half || (r == half && odd)) q += 1.0;
-    else if (r < -half || (r == -half && odd)) q -= 1.0;
-    const int c = bad ? 0 : (int)fmin(fmax(q, 0.0), 15.0);
-    w |= (uint32_t)c << (4 * e);
+    // d / s rounded as a division is: a first quotient, the rest of it, and the rest's part (1 / s is rounded so)
+    const double d = (double)y[e] - b, t = d * inv, q = fma(fma(-t, s, d), inv, t);
+    w |= (uint32_t)(int)fmin(fmax(rint(q), 0.0), 15.0) << (4 * e);   // (NaN: 0)
   }
+  if (bad) w = 0;
   // dword gl of the row: half-words hw = c * H + h, c the piece (of 16) and h the pair of groups (G = 32) or the group
   constexpr int H = D / 64;
   const int lane = threadIdx.x & 63, base = lane - gl;
@@ -90,7 +95,11 @@ struct Row8;                                        // 8 elements as they lie
 template <>
 struct Row8<__bf16> {
   bf16x8 x;
-  __device__ __forceinline__ void load(const char* p) { x = *reinterpret_cast<const bf16x8*>(p); }
+  template <bool kStream = false>
+  __device__ __forceinline__ void load(const char* p) {
+    const bf16x8* q = reinterpret_cast<const bf16x8*>(p);
+    x = kStream ? __builtin_nontemporal_load(q) : *q;
+  }
   __device__ __forceinline__ float get(int e) const { return (float)x[e]; }
   __device__ __forceinline__ Row8 from(int lane) const {
     typedef __attribute__((ext_vector_type(4))) int i32x4;
@@ -100,19 +109,23 @@ struct Row8<__bf16> {
     for (int i = 0; i < 4; ++i) y[i] = __shfl(v[i], lane);
     return Row8{__builtin_bit_cast(bf16x8, y)};
   }
+  template <bool kStream = false>
   static __device__ __forceinline__ void store(char* p, const float (&y)[8]) {
     bf16x8 o;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = (__bf16)y[e];
-    *reinterpret_cast<bf16x8*>(p) = o;
+    if (kStream) __builtin_nontemporal_store(o, reinterpret_cast<bf16x8*>(p));
+    else *reinterpret_cast<bf16x8*>(p) = o;
   }
 };
 template <>
 struct Row8<float> {
   f32x4 x[2];
+  template <bool kStream = false>
   __device__ __forceinline__ void load(const char* p) {
-    x[0] = *reinterpret_cast<const f32x4*>(p);
-    x[1] = *reinterpret_cast<const f32x4*>(p + 16);
+    const f32x4* q = reinterpret_cast<const f32x4*>(p);
+    x[0] = kStream ? __builtin_nontemporal_load(q) : q[0];
+    x[1] = kStream ? __builtin_nontemporal_load(q + 1) : q[1];
   }
   __device__ __forceinline__ float get(int e) const { return x[e >> 2][e & 3]; }
   __device__ __forceinline__ Row8 from(int lane) const {
@@ -121,9 +134,17 @@ struct Row8<float> {
     for (int i = 0; i < 8; ++i) y.x[i >> 2][i & 3] = __shfl(x[i >> 2][i & 3], lane);
     return y;
   }
+  template <bool kStream = false>
   static __device__ __forceinline__ void store(char* p, const float (&y)[8]) {
-    *reinterpret_cast<f32x4*>(p) = f32x4{y[0], y[1], y[2], y[3]};
-    *reinterpret_cast<f32x4*>(p + 16) = f32x4{y[4], y[5], y[6], y[7]};
+    f32x4* q = reinterpret_cast<f32x4*>(p);
+    const f32x4 a = {y[0], y[1], y[2], y[3]}, b = {y[4], y[5], y[6], y[7]};
+    if (kStream) {
+      __builtin_nontemporal_store(a, q);
+      __builtin_nontemporal_store(b, q + 1);
+    } else {
+      q[0] = a;
+      q[1] = b;
+    }
   }
 };
 
@@ -135,7 +156,7 @@ struct Q4AppendArgs {
   Q4Ptr pages;
   int64_t k_row, k_head, v_row, v_head;   // bytes
   int64_t limit;                          // num_pages * page_size
-  unsigned items;                         // rows x (k and v heads), below 2^31
+  unsigned items;                         // rows x heads, below 2^31
   unsigned hkv;
   int shift;
 };
@@ -146,19 +167,21 @@ __global__ void __launch_bounds__(256) q4_append_kernel(Q4AppendArgs a) {
   const int gl = threadIdx.x % LPR;
   const unsigned item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
   if (item >= a.items) return;                      // whole groups of lanes, here and below
-  const unsigned r = item / (2 * a.hkv), i = item - r * (2 * a.hkv);
-  const bool is_v = i >= a.hkv;
-  const unsigned h = is_v ? i - a.hkv : i;
+  const unsigned r = item / a.hkv, h = item - r * a.hkv;
   const int64_t slot = a.slots[r];
   if (slot < 0 || slot >= a.limit) return;
+  const bool is_v = blockIdx.y != 0;
+  const char* from = is_v ? a.v : a.k;
+  const int64_t row = is_v ? a.v_row : a.k_row, head = is_v ? a.v_head : a.k_head;
   Row8<T> x;
-  x.load((is_v ? a.v + r * a.v_row + h * a.v_head : a.k + r * a.k_row + h * a.k_head) + 8 * sizeof(T) * gl);
-  double y[8];
+  x.load(from + r * row + h * head + 8 * sizeof(T) * gl);
+  float y[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) y[e] = x.get(e);
   const int64_t id = slot >> a.shift;
   const int at = (int)(slot & ((1 << a.shift) - 1));
-  q4_store<D, G>(y, gl, (is_v ? a.pages.vc : a.pages.kc).row(id, h, at), (is_v ? a.pages.vs : a.pages.ks).row(id, h, at));
+  const PagePtr codes = is_v ? a.pages.vc : a.pages.kc, scales = is_v ? a.pages.vs : a.pages.ks;
+  q4_store<D, G>(y, gl, codes.row(id, h, at), scales.row(id, h, at));
 }
 
 // --------------------------------------------------------------------------- norm, RoPE, rows into pages
@@ -178,20 +201,38 @@ struct Q4RopeArgs {
   Q4Ptr pages;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;   // bytes
   int64_t limit, table_rows;
-  unsigned items;                         // rows x heads, below 2^31
+  unsigned rows, q_blocks, k_blocks;      // workgroups of q heads, of k heads; the others are v's
   int hq, hkv, shift, rot;
   double eps;
 };
 
-template <typename T, int D, typename F>
-__device__ __forceinline__ void rope_row(const Q4RopeArgs& a, const Row8<T>& x, const T* w, int gl, int64_t pos, F (&z)[8]) {
+// cos and sin of a lane's 8 elements (1 and 0 beyond the rotation; si: with the sign of the other half's part).
+struct Turn {
+  float c[8], si[8];
+  int step;                                         // lanes to the other half
+  bool inside;
+  __device__ __forceinline__ void load(const Q4RopeArgs& a, int gl, int64_t pos) {
+    const int half = a.rot / 2 / 8;
+    step = gl < half ? half : gl < 2 * half ? -half : 0;
+    inside = pos >= 0 && pos < a.table_rows;
+    const int64_t at = step != 0 ? (inside ? pos : 0) * a.rot + 8 * gl : 0;
+#pragma unroll
+    for (int e4 = 0; e4 < 8; e4 += 4) {
+      const f32x4 cv = *reinterpret_cast<const f32x4*>(a.cos + at + e4), sv = *reinterpret_cast<const f32x4*>(a.sin + at + e4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        c[e4 + e] = step != 0 ? cv[e] : 1.f;
+        si[e4 + e] = step > 0 ? -sv[e] : sv[e];
+      }
+    }
+  }
+};
+
+// A head's row after norm and rotation, in F.
+template <int D, typename T, typename F>
+__device__ __forceinline__ void rope_row(const Q4RopeArgs& a, const Row8<T>& x, const T* w, int gl, const Turn& turn, F (&z)[8]) {
   constexpr int LPR = D / 8;
-  const int half = a.rot / 2 / 8;                   // lanes to the other half
-  const int lane = threadIdx.x & 63;
-  const int step = gl < half ? half : gl < 2 * half ? -half : 0;
-  const bool inside = pos >= 0 && pos < a.table_rows;
-  const Row8<T> o = x.from(lane + step);            // (every lane of the row takes part)
-  F r = 1;
+  const Row8<T> o = x.from((threadIdx.x & 63) + turn.step);   // (every lane of the row takes part)
   F y[8], t[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
@@ -202,72 +243,72 @@ __device__ __forceinline__ void rope_row(const Q4RopeArgs& a, const Row8<T>& x, 
     F ss = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = y[e] * y[e] + ss;
-#pragma unroll
-    for (int i = 1; i < LPR; i <<= 1) ss += __shfl_xor(ss, i);
-    if constexpr (sizeof(F) == 8) r = 1.0 / sqrt(ss / (double)D + a.eps);
-    else r = rsqrtf(ss / (float)D + (float)a.eps);
+    ss = row_sum<LPR>(ss);
+    F r;
+    if constexpr (sizeof(F) == 8) r = 1.0 / sqrt(ss * (1.0 / D) + a.eps);
+    else r = rsqrtf(ss * (1.f / D) + (float)a.eps);
     Row8<T> wv, wo;
     wv.load(reinterpret_cast<const char*>(w + 8 * gl));
-    wo.load(reinterpret_cast<const char*>(w + 8 * (gl + step)));
+    wo.load(reinterpret_cast<const char*>(w + 8 * (gl + turn.step)));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       y[e] = y[e] * r * (F)wv.get(e);
       t[e] = t[e] * r * (F)wo.get(e);
     }
   }
-  if (step != 0) {
-    const int64_t at = (inside ? pos : 0) * a.rot + 8 * gl;
 #pragma unroll
-    for (int e4 = 0; e4 < 8; e4 += 4) {
-      const f32x4 c = *reinterpret_cast<const f32x4*>(a.cos + at + e4), s = *reinterpret_cast<const f32x4*>(a.sin + at + e4);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const F si = step > 0 ? -(F)s[e] : (F)s[e];
-        z[e4 + e] = y[e4 + e] * (F)c[e] + t[e4 + e] * si;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = y[e];
-  }
-  if (!inside) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) z[e] = __builtin_nanf("");
+  for (int e = 0; e < 8; ++e) {
+    const F v = y[e] * (F)turn.c[e] + t[e] * (F)turn.si[e];
+    z[e] = !turn.inside ? (F)__builtin_nanf("") : turn.step != 0 ? v : y[e];
   }
 }
 
-template <typename T, int D, int G>
+// A group of D / 8 lanes takes kHeads heads of a token, all of q, of k or of v.  kHeads = 1: a decode step's few rows, spread as
+// wide as they go; what they write stays in the caches for the attention that follows.  kHeads = 4, from kManyHeads heads'
+// rows on: four loads are under way over one position's cos and sin, and q moves past the caches.
+constexpr int64_t kManyHeads = 1 << 16;
+
+template <typename T, int D, int G, int kHeads>
 __global__ void __launch_bounds__(256) q4_rope_append_kernel(Q4RopeArgs a) {
-  constexpr int LPR = D / 8;
+  constexpr int LPR = D / 8, kGroups = 256 / LPR;
   const int gl = threadIdx.x % LPR;
-  const unsigned item = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
-  if (item >= a.items) return;                      // whole groups of lanes, here and below
-  const unsigned nh = a.hq + 2 * a.hkv, r = item / nh;
-  const int head = (int)(item - r * nh);
-  const int64_t row = r;
-  const bool is_q = head < a.hq, is_v = head >= a.hq + a.hkv;
-  const int h = is_q ? head : is_v ? head - a.hq - a.hkv : head - a.hq;
-  const int64_t slot = a.slots[row], pos = a.positions[row];
+  const bool is_q = blockIdx.x < a.q_blocks, is_k = !is_q && blockIdx.x < a.q_blocks + a.k_blocks;
+  const unsigned block = blockIdx.x - (is_q ? 0 : is_k ? a.q_blocks : a.q_blocks + a.k_blocks);
+  const unsigned heads = is_q ? a.hq : a.hkv, chunks = (heads + kHeads - 1) / kHeads;
+  const unsigned item = block * kGroups + threadIdx.x / LPR, r = item / chunks;
+  if (r >= a.rows) return;                          // whole groups of lanes, here and below
+  const unsigned head0 = (item - r * chunks) * kHeads;
+  const char* from = is_q ? a.q : is_k ? a.k : a.v;
+  const int64_t row = is_q ? a.q_row : is_k ? a.k_row : a.v_row, head = is_q ? a.q_head : is_k ? a.k_head : a.v_head;
+  const int64_t slot = a.slots[r];
   if (!is_q && (slot < 0 || slot >= a.limit)) return;
-  Row8<T> x;
-  x.load((is_q ? a.q + row * a.q_row + h * a.q_head : is_v ? a.v + row * a.v_row + h * a.v_head
-                                                           : a.k + row * a.k_row + h * a.k_head) + 8 * sizeof(T) * gl);
-  if (is_q) {
-    float z[8];
-    rope_row<T, D, float>(a, x, static_cast<const T*>(a.qw), gl, pos, z);
-    Row8<T>::store(a.q_out + ((row * a.hq + h) * D + 8 * gl) * (int64_t)sizeof(T), z);
-    return;
-  }
-  double y[8];
-  if (is_v) {
+  Row8<T> x[kHeads];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = x.get(e);
-  } else {
-    rope_row<T, D, double>(a, x, static_cast<const T*>(a.kw), gl, pos, y);
-  }
+  for (int i = 0; i < kHeads; ++i)
+    if (kHeads == 1 || head0 + i < heads) x[i].template load<(kHeads > 1)>(from + r * row + (head0 + i) * head + 8 * sizeof(T) * gl);
+  Turn turn;
+  if (is_q || is_k) turn.load(a, gl, a.positions[r]);
   const int64_t id = slot >> a.shift;
   const int at = (int)(slot & ((1 << a.shift) - 1));
-  q4_store<D, G>(y, gl, (is_v ? a.pages.vc : a.pages.kc).row(id, h, at), (is_v ? a.pages.vs : a.pages.ks).row(id, h, at));
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = (int)head0 + i;
+    if (kHeads > 1 && h >= (int)heads) break;
+    if (is_q) {
+      float z[8];
+      rope_row<D>(a, x[i], static_cast<const T*>(a.qw), gl, turn, z);
+      Row8<T>::template store<(kHeads > 1)>(a.q_out + (((int64_t)r * a.hq + h) * D + 8 * gl) * (int64_t)sizeof(T), z);
+    } else if (is_k) {
+      double z[8];
+      rope_row<D>(a, x[i], static_cast<const T*>(a.kw), gl, turn, z);
+      q4_store<D, G>(z, gl, a.pages.kc.row(id, h, at), a.pages.ks.row(id, h, at));
+    } else {
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = x[i].get(e);
+      q4_store<D, G>(z, gl, a.pages.vc.row(id, h, at), a.pages.vs.row(id, h, at));
+    }
+  }
 }
 
 // --------------------------------------------------------------------------- rows out of pages
@@ -389,11 +430,11 @@ extern "C" int bfly_paged_q4_append(const bfly_paged_q4_append_args_t* args, hip
   a.k_row = x.k_row_stride * es; a.k_head = x.k_head_stride * es; a.v_row = x.v_row_stride * es; a.v_head = x.v_head_stride * es;
   a.limit = x.pages.num_pages * x.pages.page_size; a.hkv = (unsigned)x.hkv;
   a.shift = __builtin_ctzll(x.pages.page_size);
-  BFLY_CHECK_ARG(x.rows * 2 * x.hkv < ((int64_t)1 << 31) - 256, "too many rows");
-  a.items = (unsigned)(x.rows * 2 * x.hkv);
+  BFLY_CHECK_ARG(x.rows * x.hkv < ((int64_t)1 << 30), "too many rows");
+  a.items = (unsigned)(x.rows * x.hkv);
   const int64_t blocks = (a.items * (x.head_dim / 8) + 255) / 256;
-  BFLY_CHECK_ARG(blocks < (1 << 24), "too many rows");        // a grid holds fewer than 2^32 threads
-  BFLY_Q4_LAUNCH(q4_append_kernel, dim3((unsigned)blocks), a);
+  BFLY_CHECK_ARG(blocks < (1 << 23), "too many rows");        // a grid (of k and v) holds fewer than 2^32 threads
+  BFLY_Q4_LAUNCH(q4_append_kernel, dim3((unsigned)blocks, 2), a);
   BFLY_CHECK_LAUNCH("bfly_paged_q4_append");
   return BFLY_OK;
 }
@@ -430,10 +471,32 @@ extern "C" int bfly_paged_q4_rope_append(const bfly_paged_q4_rope_append_args_t*
   a.shift = __builtin_ctzll(x.pages.page_size); a.rot = (int)x.rotary_dim; a.eps = x.eps;
   const int64_t heads = x.hq + 2 * x.hkv;
   BFLY_CHECK_ARG(x.rows * heads < ((int64_t)1 << 31) - 256, "too many rows");
-  a.items = (unsigned)(x.rows * heads);
-  const int64_t blocks = (a.items * (x.head_dim / 8) + 255) / 256;
-  BFLY_CHECK_ARG(blocks < (1 << 24), "too many rows");
-  BFLY_Q4_LAUNCH(q4_rope_append_kernel, dim3((unsigned)blocks), a);
+  const int64_t each = x.rows * heads >= kManyHeads ? 4 : 1, groups = 256 / (x.head_dim / 8);
+  const auto blocks = [&](int64_t h) { return (x.rows * ((h + each - 1) / each) + groups - 1) / groups; };
+  BFLY_CHECK_ARG(blocks(x.hq) + 2 * blocks(x.hkv) < (1 << 24), "too many rows");   // a grid holds fewer than 2^32 threads
+  a.rows = (unsigned)x.rows; a.q_blocks = (unsigned)blocks(x.hq); a.k_blocks = (unsigned)blocks(x.hkv);
+  const dim3 grid(a.q_blocks + 2 * a.k_blocks);
+#define BFLY_Q4_ROPE(T, D, G)                                                                                    \
+  do {                                                                                                           \
+    if (each == 4) hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 4>), grid, dim3(256), 0, stream, a);       \
+    else hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 1>), grid, dim3(256), 0, stream, a);                 \
+  } while (0)
+#define BFLY_Q4_ROPE_G(T, D)                        \
+  do {                                              \
+    if (x.pages.group == 32) BFLY_Q4_ROPE(T, D, 32); \
+    else BFLY_Q4_ROPE(T, D, 64);                    \
+  } while (0)
+#define BFLY_Q4_ROPE_D(T)                            \
+  do {                                               \
+    if (x.head_dim == 64) BFLY_Q4_ROPE_G(T, 64);     \
+    else if (x.head_dim == 128) BFLY_Q4_ROPE_G(T, 128); \
+    else BFLY_Q4_ROPE_G(T, 256);                     \
+  } while (0)
+  if (x.dtype == BFLY_DTYPE_BF16) BFLY_Q4_ROPE_D(__bf16);
+  else BFLY_Q4_ROPE_D(float);
+#undef BFLY_Q4_ROPE_D
+#undef BFLY_Q4_ROPE_G
+#undef BFLY_Q4_ROPE
   BFLY_CHECK_LAUNCH("bfly_paged_q4_rope_append");
   return BFLY_OK;
 }
