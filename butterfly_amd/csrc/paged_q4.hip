@@ -268,12 +268,14 @@ __device__ __forceinline__ void rope_row(const Q4RopeArgs& a, const Row8<T>& x, 
 // rows on: four loads are under way over one position's cos and sin, and q moves past the caches.
 constexpr int64_t kManyHeads = 1 << 16;
 
-template <typename T, int D, int G, int kHeads>
+// Then q has a launch of its own as well (kPart 1, k and v: 2, all: 0): without k's fp64 its lanes need half the registers.
+template <typename T, int D, int G, int kHeads, int kPart>
 __global__ void __launch_bounds__(256) q4_rope_append_kernel(Q4RopeArgs a) {
   constexpr int LPR = D / 8, kGroups = 256 / LPR;
   const int gl = threadIdx.x % LPR;
-  const bool is_q = blockIdx.x < a.q_blocks, is_k = !is_q && blockIdx.x < a.q_blocks + a.k_blocks;
-  const unsigned block = blockIdx.x - (is_q ? 0 : is_k ? a.q_blocks : a.q_blocks + a.k_blocks);
+  const unsigned q_blocks = kPart == 0 ? a.q_blocks : 0;
+  const bool is_q = kPart == 0 ? blockIdx.x < q_blocks : kPart == 1, is_k = !is_q && blockIdx.x < q_blocks + a.k_blocks;
+  const unsigned block = blockIdx.x - (is_q ? 0 : is_k ? q_blocks : q_blocks + a.k_blocks);
   const unsigned heads = is_q ? a.hq : a.hkv, chunks = (heads + kHeads - 1) / kHeads;
   const unsigned item = block * kGroups + threadIdx.x / LPR, r = item / chunks;
   if (r >= a.rows) return;                          // whole groups of lanes, here and below
@@ -475,11 +477,14 @@ extern "C" int bfly_paged_q4_rope_append(const bfly_paged_q4_rope_append_args_t*
   const auto blocks = [&](int64_t h) { return (x.rows * ((h + each - 1) / each) + groups - 1) / groups; };
   BFLY_CHECK_ARG(blocks(x.hq) + 2 * blocks(x.hkv) < (1 << 24), "too many rows");   // a grid holds fewer than 2^32 threads
   a.rows = (unsigned)x.rows; a.q_blocks = (unsigned)blocks(x.hq); a.k_blocks = (unsigned)blocks(x.hkv);
-  const dim3 grid(a.q_blocks + 2 * a.k_blocks);
 #define BFLY_Q4_ROPE(T, D, G)                                                                                    \
   do {                                                                                                           \
-    if (each == 4) hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 4>), grid, dim3(256), 0, stream, a);       \
-    else hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 1>), grid, dim3(256), 0, stream, a);                 \
+    if (each == 1) {                                                                                             \
+      hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 1, 0>), dim3(a.q_blocks + 2 * a.k_blocks), dim3(256), 0, stream, a); \
+    } else {                                                                                                     \
+      hipLaunchKernelGGL((q4_rope_append_kernel<T, D, 64, 4, 1>), dim3(a.q_blocks), dim3(256), 0, stream, a);     \
+      hipLaunchKernelGGL((q4_rope_append_kernel<T, D, G, 4, 2>), dim3(2 * a.k_blocks), dim3(256), 0, stream, a); \
+    }                                                                                                            \
   } while (0)
 #define BFLY_Q4_ROPE_G(T, D)                        \
   do {                                              \
