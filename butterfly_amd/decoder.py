@@ -38,7 +38,7 @@ from __future__ import annotations
 import math
 import time
 from dataclasses import dataclass
-from typing import Callable, List, Optional
+from typing import Callable, List, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -53,6 +53,7 @@ from . import _native
 from ._device import on, stream_of
 from .compressed_cache import CompressedKVCache
 from .integrations import QwenButterflyAttention, QwenButterflyConfig, register_butterfly_attention
+from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .paged import PagedKVCache, PagedLayer
 
 
@@ -236,6 +237,9 @@ FUSE_O_PROJ = True
 # per-workgroup candidates and advance token, output, counters and the next input in one more
 # launch (GreedyState); False keeps torch's embedding, index_copy and add and the argmax passes
 FUSE_GREEDY = True
+
+# logits that Decoder.score makes at a time (a gigabyte of float32)
+SCORE_LOGITS = 1 << 28
 
 
 def _one_row(x: torch.Tensor) -> bool:
@@ -491,6 +495,21 @@ def argmax_rows(x: torch.Tensor, parallel: bool = True) -> torch.Tensor:
         _native.call("bfly_argmax_rows", x.data_ptr(), rows, n, x.stride(0), x.stride(1),
                      ws.data_ptr() if parallel else None, ws.numel(), out.data_ptr(), stream_of(x))
     return out
+
+
+def _token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> TokenLogprobs:
+    """``token_logprobs``; on the CPU its PyTorch form."""
+    if logits.is_cuda:
+        return token_logprobs(logits, tokens, top=top)
+    lp = torch.log_softmax(logits.float(), -1)
+    entropy = -torch.where(lp > -math.inf, lp.exp() * lp, lp.exp()).sum(-1)
+    return TokenLogprobs(lp.gather(-1, tokens[:, None])[:, 0], entropy, *lp.topk(top))
+
+
+def _no_logprobs(b: int, n: int, top: int, device) -> TokenLogprobs:
+    """Rows [b, n(, top)] that hold NaN and -1."""
+    one, many = (torch.full(x, math.nan, device=device) for x in ((2, b, n), (b, n, top)))
+    return TokenLogprobs(one[0], one[1], many, torch.full((b, n, top), -1, dtype=torch.long, device=device))
 
 
 def argmax_rows_noalloc(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -956,6 +975,10 @@ class Decoder(nn.Module):
         """tokens [B, T] at positions [start, start+T); returns logits [B, vocab] of the last position.
         A paged cache's requests hold ``start`` tokens each (several tokens: else ``ValueError``; one token: each
         request goes on at its own length, at most ``start``)."""
+        return self._last_logits(*self._begin(tokens, caches, start)).float()
+
+    def _begin(self, tokens: torch.Tensor, caches: List, start: int):
+        """A call's embedded rows, positions, caches and RoPE rows, with the paged caches' step begun."""
         x = F.embedding(tokens, self.embed_tokens)
         positions = torch.arange(start, start + tokens.shape[1], device=tokens.device)
         rope = self._rope(start, tokens.shape[1], tokens.device)
@@ -964,7 +987,40 @@ class Decoder(nn.Module):
             pool.begin(torch.full_like(pool.lengths, t), t, start=start if t > 1 else None)
         if pools and t == 1:
             rope = RopeTable(*self._rope_tab, positions)
-        return self._last_logits(x, positions, caches, rope).float()
+        return x, positions, caches, rope
+
+    @torch.no_grad()
+    def score(self, tokens: torch.Tensor, caches: List, *, top: int = 0) -> TokenLogprobs:
+        """The log probability of each token of ``tokens`` [B, T] behind the first, given those before it, with the
+        distributions' entropies and ``top`` most probable tokens (``token_logprobs``): tensors [B, T - 1(, top)].
+
+        ``caches`` as ``forward``'s, empty before; they hold the first T - 1 tokens afterwards.  The logits are the rows of
+        one product over the table, made and read some ``SCORE_LOGITS`` at a time and never all held."""
+        if tokens.dim() != 2 or tokens.shape[1] == 0:
+            raise ValueError("score takes tokens [B, T] of at least one token")
+        b, t = tokens.shape[0], tokens.shape[1] - 1
+        for pool in self._paged_pools(caches, b):
+            pool.require(0)
+        if t == 0 or b == 0:
+            h = self.embed_tokens.new_zeros(0, self.cfg.hidden_size)
+        else:
+            h = self._normed(*self._begin(tokens[:, :-1], caches, 0)).reshape(b * t, -1)
+        given = tokens[:, 1:].reshape(-1).long()
+        step = max(1, SCORE_LOGITS // self.cfg.vocab_size)
+        parts = [_token_logprobs(F.linear(x, self.embed_tokens), n, top)
+                 for x, n in zip(h.split(step), given.split(step))]
+        return TokenLogprobs(*(torch.cat(x).view(b, t, *x[0].shape[1:]) for x in zip(*parts)))
+
+    def _normed(self, x: torch.Tensor, positions: torch.Tensor, caches: List, rope) -> torch.Tensor:
+        """Every layer over the embedded ``x``, then the final norm of every row."""
+        if _hip(x) and x.shape[-1] % 256 == 0:
+            m = None
+            for layer, cache in zip(self.layers, caches):
+                x, m = layer.forward_split(x, m, positions, cache, rope)
+            return add_rms_norm(x, m, self.norm.weight, self.norm.eps)[1]
+        for layer, cache in zip(self.layers, caches):
+            x = layer(x, positions, cache, rope)
+        return self.norm(x)
 
     def _paged_pools(self, caches: List, batch: int) -> List[PagedKVCache]:
         """The paged caches behind ``caches``, each once, after what can be refused before a step of theirs."""
@@ -975,7 +1031,7 @@ class Decoder(nn.Module):
         for pool in pools:
             # (under autocast the products' type is not the weights': the operators see it)
             pool.check_heads(self.cfg.num_kv_heads, self.cfg.head_dim,
-                             pool.k_pages.dtype if torch.is_autocast_enabled() else self.embed_tokens.dtype)
+                             pool.dtype if torch.is_autocast_enabled() else self.embed_tokens.dtype)
         if any(pool.max_requests != batch for pool in pools):
             raise ValueError(f"a paged cache of {[p.max_requests for p in pools]} requests cannot take a batch of {batch}")
         return pools
@@ -1089,13 +1145,16 @@ class Decoder(nn.Module):
 
     @torch.no_grad()
     def greedy_requests(self, prompts: List[torch.Tensor], new_tokens: int, cache: PagedKVCache, *,
-                        eos_token: Optional[int] = None) -> torch.Tensor:
+                        eos_token: Optional[int] = None, top_logprobs: Optional[int] = None
+                        ) -> Union[torch.Tensor, Tuple[torch.Tensor, TokenLogprobs]]:
         """Greedy decoding of requests of different lengths together, over the dense layers' paged cache.
 
         ``prompts``: one 1-D tensor of tokens per request (``cache.max_requests`` of them, the cache empty).
         Each is prefilled by itself and its keys and values go into pages; then all requests decode together,
         a step captured once in a HIP graph and replayed, each request at its own position.  Returns
         [B, new_tokens]; after ``eos_token`` a request idles (its row repeats the token, its pages stay).
+        ``top_logprobs``: also the tokens' log probabilities, entropies and that many alternatives (``token_logprobs``,
+        in the captured step), [B, new_tokens(, top_logprobs)]; where a request idles NaN, and -1 for a token.
         Every layer has stock attention (a compressed cache holds one length for its batch)."""
         b = len(prompts)
         dev = self.embed_tokens.device
@@ -1108,13 +1167,18 @@ class Decoder(nn.Module):
         self._paged_pools(cache.layers, b)
         if bool(cache.lengths.any()):
             raise ValueError("greedy_requests starts from an empty cache (release the requests it holds)")
+        said = top_logprobs is not None
+        if said and not 0 <= top_logprobs <= min(MAX_TOP, self.cfg.vocab_size):
+            raise ValueError(f"top_logprobs {top_logprobs} must be 0 to {min(MAX_TOP, self.cfg.vocab_size)}")
         if new_tokens <= 0:
-            return torch.empty(b, 0, dtype=torch.long, device=dev)
-        first = []
+            out = torch.empty(b, 0, dtype=torch.long, device=dev)
+            return (out, _no_logprobs(b, 0, top_logprobs, dev)) if said else out
+        first, logits = [], []
         for r, prompt in enumerate(prompts):
             n = prompt.numel()
             held = [[] for _ in self.layers]
-            first.append(self.forward(prompt[None].to(dev), held, 0).argmax(-1))
+            logits.append(self.forward(prompt[None].to(dev), held, 0))
+            first.append(logits[-1].argmax(-1))
             counts = torch.zeros_like(cache.lengths)
             counts[r] = n
             cache.begin_packed(counts, n)
@@ -1128,6 +1192,11 @@ class Decoder(nn.Module):
         alive = torch.ones(b, dtype=torch.int32, device=dev)
         if eos_token is not None:
             alive.copy_((tok[:, 0] != eos_token).int())
+        if said:
+            lps = _no_logprobs(b, new_tokens, top_logprobs, dev)
+            for x, y in zip(lps, token_logprobs(torch.cat(logits), tok[:, 0], top=top_logprobs)):
+                x[:, 0] = y
+        del logits
         self._rope(0, max(p.numel() for p in prompts) + new_tokens + 1, dev)
         rope = RopeTable(*self._rope_tab, None)
 
@@ -1135,6 +1204,11 @@ class Decoder(nn.Module):
             cache.begin(alive)
             lg = self._last_logits(F.embedding(tok, self.embed_tokens), None, cache.layers, rope)
             nxt = argmax_rows(lg)
+            if said:
+                # (an idle request's column keeps its NaN and -1)
+                for x, y in zip(lps, token_logprobs(lg, nxt[:, 0], top=top_logprobs)):
+                    live = (alive != 0).view(-1, *[1] * (y.dim() - 1))
+                    x.index_copy_(1, column, torch.where(live, y, -1 if y.dtype is torch.long else math.nan)[:, None])
             if eos_token is not None:
                 nxt = torch.where(alive[:, None] != 0, nxt, tok)
                 alive.copy_((nxt[:, 0] != eos_token).int())
@@ -1155,7 +1229,7 @@ class Decoder(nn.Module):
             for _ in range(new_tokens - 2):
                 graph.replay()
         cache.sync()
-        return out
+        return (out, lps) if said else out
 
     @torch.no_grad()
     def greedy(self, prompt: torch.Tensor, new_tokens: int, caches: List,

@@ -461,23 +461,37 @@ class PagedKVCache:
     ``[num_layers, num_pages, Hkv, page_size, d]`` and one block table, lengths and free list on the device,
     which all layers share (page ``p`` of a request is page ``p`` in every layer).
 
-    ``max_tokens`` bounds a request (default: all pages).  A step is :meth:`begin` (or :meth:`begin_packed`), then
+    ``max_tokens`` bounds a request (default: all pages).  ``quant_bits=4`` holds keys and values as 4-bit codes in groups of
+    ``quant_group`` (32 or 64) elements (:mod:`butterfly_amd.paged_q4`; ``pages`` instead of ``k_pages`` and ``v_pages``):
+    ``dtype`` is the rows' then.  A step is :meth:`begin` (or :meth:`begin_packed`), then
     every layer's rows and attention through ``layers[i]``; :meth:`sync` reads the state back."""
 
     def __init__(self, *, num_layers: int, num_pages: int, max_requests: int, num_kv_heads: int, head_dim: int,
-                 page_size: int = 128, max_tokens: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None):
+                 page_size: int = 128, max_tokens: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None,
+                 quant_bits: Optional[int] = None, quant_group: int = 64):
         if page_size not in PAGE_SIZES:
             raise ValueError(f"page_size {page_size} must be a power of two from 16 to 1024")
         if min(num_layers, num_pages, max_requests, num_kv_heads, head_dim) <= 0 or max_tokens is not None and max_tokens <= 0:
             raise ValueError("the cache's sizes must be positive")
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"unsupported dtype {dtype}; expected float32 or bfloat16")
+        if quant_bits not in (None, 4):
+            raise ValueError(f"unsupported quant_bits {quant_bits}; expected 4 or None")
         device = torch.device("cuda" if device is None else device)
         width = num_pages if max_tokens is None else min(num_pages, -(-max_tokens // page_size))
         self.page_size, self.max_requests, self.max_tokens = page_size, max_requests, width * page_size
-        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
-        self.k_pages, self.v_pages = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
-        self.layers = [PagedLayer(self, k, v) for k, v in zip(self.k_pages, self.v_pages)]
+        self.num_kv_heads, self.head_dim, self.dtype = num_kv_heads, head_dim, dtype
+        self.k_pages = self.v_pages = self.pages = None
+        if quant_bits is None:
+            shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+            self.k_pages, self.v_pages = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+            self.layers = [PagedLayer(self, k, v) for k, v in zip(self.k_pages, self.v_pages)]
+        else:
+            from .paged_q4 import PagedQ4Layer, Q4Pages, empty_q4_pages
+
+            self.pages = empty_q4_pages(num_pages, num_kv_heads, page_size, head_dim, group=quant_group,
+                                        layers=(num_layers,), device=device)
+            self.layers = [PagedQ4Layer(self, Q4Pages(*layer)) for layer in zip(*self.pages)]
         i32 = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((max_requests, width), -1, **i32)
         self.lengths = torch.zeros(max_requests, **i32)
@@ -490,7 +504,7 @@ class PagedKVCache:
 
     @property
     def nbytes(self) -> int:
-        return self.k_pages.nbytes + self.v_pages.nbytes
+        return self.pages.nbytes if self.pages is not None else self.k_pages.nbytes + self.v_pages.nbytes
 
     def _begin(self, counts: torch.Tensor, num_rows: int, rows_each: int) -> PagedPlan:
         self.plan = paged_plan(self.block_table, self.lengths, counts, self.free_pages, self.state,
@@ -519,9 +533,9 @@ class PagedKVCache:
         step begins, not in the middle of a generation."""
         if head_dim not in HEAD_DIMS:
             raise NotImplementedError(f"attention over pages: head_dim={head_dim} unsupported {HEAD_DIMS}")
-        _, _, heads, _, d = self.k_pages.shape
-        if (heads, d, self.k_pages.dtype) != (num_kv_heads, head_dim, dtype):
-            raise ValueError(f"a paged cache of {heads} kv heads of {d} in {self.k_pages.dtype} cannot take {num_kv_heads} of "
+        heads, d = self.num_kv_heads, self.head_dim
+        if (heads, d, self.dtype) != (num_kv_heads, head_dim, dtype):
+            raise ValueError(f"a paged cache of {heads} kv heads of {d} in {self.dtype} cannot take {num_kv_heads} of "
                              f"{head_dim} in {dtype}")
 
     def require(self, tokens: int, *, at_most: bool = False) -> bool:

@@ -28,7 +28,7 @@ from torch.autograd import forward_ad
 
 from . import _native
 from ._device import _GET_DEVICE, stream_of
-from .paged import (_EMPTY, _GRAD, HEAD_DIMS, PAGE_SIZES, _check_followed, _check_ints, _device_of, _dtype_code, _flat,
+from .paged import (_EMPTY, _GRAD, HEAD_DIMS, PAGE_SIZES, PagedLayer, _check_followed, _check_ints, _device_of, _dtype_code, _flat,
                     _other_device, _rows, _table_stride)
 
 _APPEND, _ROPE, _READ, _ATTN = (_native.PAGED_Q4_STRUCTS["bfly_paged_q4_" + x].pack
@@ -310,3 +310,34 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
 @lru_cache(maxsize=1024)
 def _workspace_bytes(*sizes: int) -> int:
     return _native.lib().bfly_paged_q4_attention_workspace_bytes(*sizes)
+
+
+class PagedQ4Layer(PagedLayer):
+    """One layer's pages of a :class:`butterfly_amd.PagedKVCache` in 4 bits, as :class:`butterfly_amd.PagedLayer`."""
+
+    def __init__(self, cache, pages: Q4Pages):
+        super().__init__(cache, None, None)
+        self.pages = pages
+
+    def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
+        """The step's rows of keys and values [N, Hkv, d] into their slots."""
+        paged_q4_append(k, v, self.pages, self.plan.slots)
+
+    def rope_append(self, q, k, v, cos, sin, *, q_weight=None, k_weight=None, eps: float = 1e-6) -> torch.Tensor:
+        """The step's projection rows: :func:`paged_q4_rope_append` at the plan's positions and slots."""
+        p = self.plan
+        return paged_q4_rope_append(q, k, v, self.pages, p.slots, p.positions, cos, sin, q_weight=q_weight,
+                                    k_weight=k_weight, eps=eps)
+
+    def attend(self, q: torch.Tensor, *, scale: Optional[float] = None, window: int = 0, return_stats: bool = False):
+        """:func:`paged_q4_attention` of one new token ``q`` [B, Hq, 1, d] of every request over its pages."""
+        return paged_q4_attention(q, self.pages, self.cache.block_table, self.plan.lengths, scale=scale, window=window,
+                                  return_stats=return_stats)
+
+    def history(self, tokens: int, request: Optional[int] = None):
+        """The first ``tokens`` keys and values of every request, or of one, as dense [B, Hkv, tokens, d] tensors of
+        the rows' type; the requests hold that many."""
+        table = self.cache.block_table
+        if request is not None:
+            table = table[request:request + 1]
+        return paged_q4_read(self.pages, table, tokens, dtype=self.cache.dtype)
