@@ -266,7 +266,7 @@ __device__ __forceinline__ void rope_row(const Q4RopeArgs& a, const Row8<T>& x, 
 // A group of D / 8 lanes takes kHeads heads of a token, all of q, of k or of v.  kHeads = 1: a decode step's few rows, spread as
 // wide as they go; what they write stays in the caches for the attention that follows.  kHeads = 4, from kManyHeads heads'
 // rows on: four loads are under way over one position's cos and sin, and q moves past the caches.
-constexpr int64_t kManyHeads = 1 << 16;
+constexpr int64_t kManyHeads = 1 << 17;
 
 // Then q has a launch of its own as well (kPart 1, k and v: 2, all: 0): without k's fp64 its lanes need half the registers.
 template <typename T, int D, int G, int kHeads, int kPart>

@@ -4,23 +4,37 @@
 //   s_t = scale q . k_t = scale sum_groups (s_t (q . c_t) + b_t sum q),   m = max s_t, l = sum exp(s_t - m),
 //   o = (sum exp(s_t - m) v_t) / l,  v's scales and biases on the weights: sum (p_t s_t) c_t + sum p_t b_t.
 //
-// The schedule, runs and joins are those of paged_attn.hip (paged_runs.h).  Inside a tile of 32 keys the two products
-// run over the codes themselves: a code is exact in bf16 (as 16 + c: two operations for two codes, an operand word
-// is ((w >> n) & 0x00780078) | 0x41804180), so nothing is rounded on the way from the cache to the sums but the weights, which
-// enter as two bf16 parts (three, and q as three, for fp32).
-//   * A row's 16 pieces hold a sixteenth of every group each.  S^T = K Q^T: lane (n, g) takes four pieces of key n
-//     (a quarter of every group), so each product is over one group.  O^T += V^T P^T: lane n takes piece n of a lane's 8
-//     keys, so the 16 rows of each product are of one group, and P carries that group's scale.
-//   * Scales are read as lane (n, g) needs them, for keys 4 (n & 3) + g, and reach the other lanes of a four by DPP.
+// The schedule, runs and joins are those of paged_attn.hip (paged_runs.h); a workgroup's four waves take every fourth tile of
+// 32 or 64 keys.  Both products run over the codes themselves, so nothing is rounded on the way from the cache to the sums but
+// what stands against the codes:
+//   * scores, bf16: a code is a byte, two operations make four, and a byte of 0..15 is 2^-9 of its number as E4M3: the
+//     8-bit matrix instruction takes eight codes in two registers.  q enters as two E4M3 parts (take_q says how exactly).
+//     fp32: a code as 16 + c in bf16, an operand word of two codes is ((w >> n) & 0x00780078) | 0x41804180, and q as three
+//     bf16 parts;
+//   * values: codes as 16 + c in bf16, weights as two bf16 parts (2^-17 of the weight is left; fp32: three).
+// Layout: a row's 16 pieces hold a sixteenth of every group each.  S^T = K Q^T: lane (n, g) takes four pieces of key n (a
+// quarter of every group), so each product is over one group.  O^T += V^T P^T: lane n takes piece n of a lane's keys, so the 16
+// rows of each product are of one group, and P carries that group's scale.  Scales are read as lane (n, g) needs them, for keys
+// 4 (n & 3) + g, and reach the other lanes of a four by DPP.
+//
+// Bound: the cache is read once, 72 + 72 bytes a key and head of 128 in groups of 64 against 512 in bf16.  Four query heads a kv
+// head, bf16, d 128, 32 requests of 131072 tokens and less (385 MB): 72 us, 5.4 TB/s with the join (a copy reaches 6.6);
+// there the vector instructions between the loads and the products (codes, scales, weights) take two thirds of the time, which
+// is why they are counted: scores through bytes instead of 16 + c 90 -> 82 us, columns in blocks (below) 101 -> 73.  One
+// request of 32768 tokens (19 MB): 14 us, mostly the two launches and two rounds of latency.
 #include "paged_runs.h"
 #include "paged_q4.h"
 
 namespace bfly {
 
+// Rounds (four tiles) of a request that one workgroup takes alone: the more pairs of a request and a kv head the
+// more.  Measured, us, 4 for all / this rule / 32 for all: 64 requests of 2048 tokens and 4 kv heads 24.6 / 20.4 / 20.4, 256 of
+// 1 to 4096 and 8 heads 99.5 / 83.4 / 83.2; 8 of 8192 and 4 heads 18.0 / 18.0 / 54.1.
 constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs >= 512 ? 16 : pairs >= 128 ? 8 : 4; }
 
 // A column's sums keep their reference until its maximum is more than this many powers of two above it: 16 columns of a
-// tile hardly ever rise together, and one that rises would turn all sums over.  (Weights are at most 2^4 then.)
+// tile hardly ever rise together, and one that rises would turn all sums over (32 requests of 131072: 77.4 -> 75.9 us, of 2000
+// tokens 25.9 -> 25.5).  Weights are at most 2^4 then.
 constexpr float kQ4Lag = 4.f;
 
 struct Q4AttnArgs : RunArgs {
@@ -115,6 +129,9 @@ struct Q4Sweep {
   static constexpr int U = J > 2 ? J : 2;           // subtiles of a tile
   static constexpr int A = U / J;                   // of them in a block: results 4 a + r of a lane
   static constexpr int KT = 16 * U;
+  // Keys pass the caches (2: non-temporal), values and scales do not: a row of values is read by four instructions, rows of
+  // scales lie in a line with their neighbours'.  32 requests of 131072 tokens: keys through the caches 85.6 us, values past them
+  // too 81.4, so 75.9 (one request of 60000 of d 64: 24.4, 25.9, 25.7).
   static constexpr int kPolicyK = 2, kPolicyV = 0, kPolicyS = 0;
   static constexpr int kCodes = D / 2, kScales = 4 * (D / G);   // bytes of a row
   static constexpr int H = D / 64;                  // half-words of a piece
@@ -486,10 +503,10 @@ struct Q4Sweep {
   }
 };
 
-// Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.  The next tile is requested
-// whole before this one is worked on (kAhead), or its keys once this one's scores are done and its values at the end; the page
-// ids of the one behind it before that.
-template <typename S, bool kAhead, typename T>
+// Tiles t, t + kWaves, ... below t_end.  Returns whether a page id was outside the pages.  The next tile's keys are requested
+// once this one's scores are done and its values at the end, the page ids of the one behind it after them.  (Two tiles in
+// registers, the next one requested whole before: level, 73 us for 32 requests of up to 131072 tokens either way.)
+template <typename S, typename T>
 __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_t* row, const Span& s, int kvh, int t, int t_end,
                                          const T* q, bool there, float sign, float unit) {
   constexpr int KT = S::KT, U = S::U;
@@ -524,21 +541,15 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     if (whole) w.load_v(x, a.p, page_rows(a.p.vc, id[0], kvh, at, size, S::kCodes), page_rows(a.p.vs, id[0], kvh, at, size, S::kScales), n, g);
     else w.load_v(x, a, a.p, id, kvh, first, n, g);
   };
-  // one tile (in x), the next one's requests (to y); whether there is another
-  const auto step = [&](typename S::Tile& x, typename S::Tile& y) __attribute__((always_inline)) {
+  typename S::Tile x;
+  // one tile, the next one's requests; whether there is another
+  const auto step = [&]() __attribute__((always_inline)) {
     const int next = t + kWaves;
     const bool more = next < t_end;
-    if (more) {
-      check();
-      if (kAhead) {
-        load_k(y, next * KT);
-        load_v(y, next * KT);
-        if (next + kWaves < t_end) ids((next + kWaves) * KT);
-      }
-    }
+    if (more) check();
     float p[4 * S::A];
     w.scores(x, p);
-    if (!kAhead && more) load_k(x, next * KT);
+    if (more) load_k(x, next * KT);
     const unsigned first = (unsigned)t * KT, lo = s.lo, end = s.n;
     if (first < lo || first + KT > end) w.cut(x, p, first, lo, end, n, g);
     float mx = p[0];
@@ -566,28 +577,22 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     }
     w.l += sum;
     w.add(x, p);
-    if (!kAhead && more) {
+    if (more) {
       load_v(x, next * KT);
       if (next + kWaves < t_end) ids((next + kWaves) * KT);
     }
     t = next;
     return more;
   };
-  typename S::Tile tiles[kAhead ? 2 : 1];
   typename S::QRow raw;                             // (before the tile: loads return in order)
   S::fetch_q(raw, q, g);
   ids(t * KT);
   check();
-  load_k(tiles[0], t * KT);
-  load_v(tiles[0], t * KT);
+  load_k(x, t * KT);
+  load_v(x, t * KT);
   if (t + kWaves < t_end) ids((t + kWaves) * KT);
   w.take_q(raw, there, n, sign, unit);
-  if constexpr (kAhead) {
-    while (step(tiles[0], tiles[1]) && step(tiles[1], tiles[0])) {
-    }
-  } else {
-    while (step(tiles[0], tiles[0])) {
-    }
+  while (step()) {
   }
   w.settle();
   return bad;
@@ -596,9 +601,6 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
 // Waves of a SIMD that the registers are cut for: two need no more than 256 (and no moves to accumulation registers
 // and back), but for the widest rows.
 constexpr int q4_waves(int esize, int d, int g, int j) { return d < 256 || (esize == 2 && g == 64 && j == 2) ? 2 : 1; }
-
-// Whether the registers hold two tiles.
-constexpr bool q4_ahead(int d) { return d < 0; }
 
 template <typename T, int D, int G, int J>
 __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_attn_kernel(Q4AttnArgs a) {
@@ -643,7 +645,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
   S w;
   const bool there = n % C < rows;                  // (a column without a row of q reads the first one's)
   const T* q = reinterpret_cast<const T*>(a.q + b * a.q_req + (int64_t)(head0 + (there ? n % C : 0)) * a.q_head);
-  const bool bad = q4_sweep<S, q4_ahead(D)>(a, w, table, s, kvh, t0 + wave, t1, q, there, sign, size * kLog2e);
+  const bool bad = q4_sweep<S>(a, w, table, s, kvh, t0 + wave, t1, q, there, sign, size * kLog2e);
   const float l = col_sum4(w.l);
   float accb[S::NG];
 #pragma unroll
@@ -701,13 +703,17 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
   }
 }
 
-// Blocks of columns: as many as leave room for a unit's rows of q, and as the copies of q leave registers for.
+// Blocks of columns: as many as leave room for a unit's rows of q, and as the copies of q leave registers for; one where
+// all requests together have few keys (their tables' widths; a window) and what counts is how soon the first results are there.
+// Measured, us, one / two / these: 32 requests of 131072 tokens 101 / 88 / 76, one of 32768 15.8 / 15.3 / 13.9, 16 of 1024 and 4 kv
+// heads (2^16 keys) 11.9 / 11.7 / 11.9; one of 8192 (2^15) 10.6 / 10.7 / 11.6, of 1024 10.2 / 10.3 / 11.6.
 constexpr int q4_most_blocks(int esize, int head_dim) {
   return esize == 2 ? (head_dim <= 128 ? 4 : 2) : head_dim == 64 ? 4 : head_dim == 128 ? 2 : 1;
 }
-static int q4_blocks(int esize, int64_t head_dim, int64_t group) {
+static int q4_blocks(int esize, int64_t head_dim, int64_t group, int64_t pairs, int64_t tokens, int64_t window) {
   const int most = q4_most_blocks(esize, (int)head_dim), fit = group <= 4 ? 4 : group <= 8 ? 2 : 1;
-  return most < fit ? most : fit;
+  if (window > 0 && window < tokens) tokens = window;
+  return tokens < (1 << 16) && pairs * tokens < (1 << 16) ? 1 : most < fit ? most : fit;
 }
 static int q4_tile(int blocks) { return blocks > 2 ? 64 : 32; }
 // Runs in all, where requests and heads leave them: as many workgroups as a CU holds by its registers.  Measured, us, half as
@@ -745,7 +751,7 @@ extern "C" int64_t bfly_paged_q4_attention_workspace_bytes(int dtype, int64_t re
   if (requests <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || head_dim <= 0 || table_width <= 0 || page_size <= 0) return 0;
   const int64_t group = hq / hkv, rows = group < 16 ? group : 16;
   const int64_t pairs = requests * hkv * ((group + 15) / 16);
-  const int tile = q4_tile(q4_blocks(dtype == BFLY_DTYPE_F32 ? 4 : 2, head_dim, group));
+  const int tile = q4_tile(q4_blocks(dtype == BFLY_DTYPE_F32 ? 4 : 2, head_dim, group, pairs, table_width * page_size, window));
   return most_rounds(table_width * page_size, window, tile) <= q4_whole_rounds(pairs) ? 0 : run_workspace_bytes(rows, head_dim);
 }
 
@@ -784,7 +790,7 @@ extern "C" int bfly_paged_q4_attention(const bfly_paged_q4_attention_args_t* arg
                  "too many heads");
   run_workspace(a, x.workspace, x.head_dim);
   a.whole = q4_whole_rounds((int64_t)a.requests * a.units);
-  const int blocks = q4_blocks((int)es, x.head_dim, a.group);
+  const int blocks = q4_blocks((int)es, x.head_dim, a.group, (int64_t)a.requests * a.units, x.table_width * x.pages.page_size, x.window);
   a.runs = q4_runs((int)es, x.head_dim, x.pages.group, blocks);
   const int64_t items = run_items(a, most_rounds(a.capacity, a.window, q4_tile(blocks)));
   BFLY_CHECK_ARG(items < (1 << 24), "too many requests and heads");   // a grid holds fewer than 2^32 threads

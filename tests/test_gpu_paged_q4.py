@@ -161,6 +161,27 @@ def test_rope_append(dtype, d, rot, group):
             assert _same(a, b), (rows, name)
 
 
+@pytest.mark.parametrize("dtype,d,group,hq,hkv", [(torch.bfloat16, 64, 64, 14, 1), (torch.bfloat16, 128, 32, 6, 6),
+                                                  (torch.float32, 256, 64, 5, 5), (torch.bfloat16, 256, 32, 8, 4)])
+def test_rope_append_of_many_rows_is_that_of_its_parts(dtype, d, group, hq, hkv):
+    """Rows enough that heads are taken four at a time, against calls of a few hundred: the same bits."""
+    rows, page = (1 << 17) // (hq + 2 * hkv) + 37, 128
+    q, k, v = torch.randn(rows, hq + 2 * hkv, d, generator=_gen(1), device="cuda").to(dtype).split((hq, hkv, hkv), 1)
+    ang = torch.rand(500, d // 2, generator=_gen(2), device="cuda") * 9
+    positions = torch.randint(-1, 501, (rows,), generator=_gen(3), device="cuda")
+    slots = torch.randperm(-(-rows // page) * page, generator=torch.Generator().manual_seed(1))[:rows].cuda()
+    slots[5::11] = -1
+    qw, kw = (torch.rand(d, generator=_gen(4 + i), device="cuda").to(dtype) for i in range(2))
+    outs, pools = [], []
+    for part in (rows, 700):
+        pages = _pages(-(-rows // page), hkv, page, d, group)
+        outs.append(torch.cat([bf.paged_q4_rope_append(a, b, c, pages, s, p, ang.cos(), ang.sin(), q_weight=qw, k_weight=kw, eps=1e-6)
+                               for a, b, c, s, p in zip(*(x.split(part) for x in (q, k, v, slots, positions)))]))
+        pools.append(pages)
+    assert torch.equal(outs[0].nan_to_num(9.0), outs[1].nan_to_num(9.0))
+    assert all(_same(a, b) for a, b in zip(*pools))
+
+
 # --------------------------------------------------------------------------- rows out of pages
 @pytest.mark.parametrize("group", [32, 64])
 @pytest.mark.parametrize("d", [64, 128, 256])
@@ -235,6 +256,38 @@ def test_attention_of_split_requests(dtype, d, group, hq, hkv, lens, page, windo
     q = torch.randn(len(lens), hq, 1, d, generator=_gen(3), device="cuda").to(dtype)
     out, l, m = bf.paged_q4_attention(q, pages, table, _i32(lens), window=window, return_stats=True)
     _check(out, q, pages, table, _i32(lens), (l, m), window=window)
+
+
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("hq,hkv", [(8, 2), (6, 2), (14, 2), (17, 1)])
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (256, 32), (256, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attention_of_narrow_and_wide_tables(dtype, d, group, hq, hkv, page):
+    """Tables of the same requests on both sides of 2^16 keys in all, where the kernel's form changes: entries behind
+    a request's pages say nothing, keys that it does not see are never part of the result."""
+    lens, window = [300, 0, 47, 129, 1], 90 if page == 32 else 0
+    pages = _pages(sum(-(-n // page) for n in lens) + 1, hkv, page, d, group, seed=hq)
+    units = len(lens) * hkv * -(-hq // hkv // 16)
+    q = torch.randn(len(lens), hq, 1, d, generator=_gen(hq), device="cuda").to(dtype)
+    q[3, 1] *= 8.0                                    # a row whose maximum moves a lot
+    seen = torch.zeros(pages.k_codes.shape[0], page, dtype=torch.bool, device="cuda")
+    narrow = _table(lens, page, pages.k_codes.shape[0])
+    for b, n in enumerate(lens):
+        for t in range(max(0, n - window) if window else 0, n):
+            seen[int(narrow[b, t // page]), t % page] = True
+    for codes, scales in ((pages.k_codes, pages.k_scales), (pages.v_codes, pages.v_scales)):
+        codes.masked_fill_(~seen[:, None, :, None], 0xff)
+        scales.masked_fill_(~seen[:, None, :, None, None], math.nan)
+    clean = bf.Q4Pages(pages.k_codes, pages.k_scales.nan_to_num(0.0), pages.v_codes, pages.v_scales.nan_to_num(0.0))
+    for width in (narrow.shape[1], -(-(1 << 16) // (units * page))):
+        table = _table(lens, page, pages.k_codes.shape[0], width=width)
+        out, l, m = bf.paged_q4_attention(q, pages, table, _i32(lens), window=window, return_stats=True)
+        _check(out, q, clean, table, _i32(lens), (l, m), window=window)
+        bad = table.clone()
+        bad[3, (lens[3] - 1) // page] = pages.k_codes.shape[0]
+        bad[4, 0] = -1
+        nan = bf.paged_q4_attention(q, pages, bad, _i32(lens), window=window)
+        assert bool(nan[3:].isnan().all()) and torch.equal(nan[:3], out[:3])
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.25, 3.0, 1e-4])
