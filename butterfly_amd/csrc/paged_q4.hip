@@ -39,7 +39,11 @@ __device__ __forceinline__ double least(double a, double b) { return fmin(a, b);
 __device__ __forceinline__ float most(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double most(double a, double b) { return fmax(a, b); }
 
-__device__ __forceinline__ uint32_t bf16_bits(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+// (opaque: from fp64 through fp32 to bf16 are two roundings by definition, which the compiler would contract into one)
+__device__ __forceinline__ uint32_t bf16_bits(float x) {
+  asm("" : "+v"(x));
+  return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
 
 // 8 elements y of a row in each of D / 8 lanes (gl: which): the row's codes, a dword a lane, and the scale and bias
 // of a group in its first lane.  F: what the elements are exact in (a row as it lies: fp32).

@@ -5,22 +5,21 @@
 //   o = (sum exp(s_t - m) v_t) / l,  v's scales and biases on the weights: sum (p_t s_t) c_t + sum p_t b_t.
 //
 // The schedule, runs and joins are those of paged_attn.hip (paged_runs.h); a workgroup's four waves take every fourth tile of
-// 32 or 64 keys.  Both products run over the codes themselves, so nothing is rounded on the way from the cache to the sums but
-// what stands against the codes:
-//   * scores, bf16: a code is a byte, two operations make four, and a byte of 0..15 is 2^-9 of its number as E4M3: the
-//     8-bit matrix instruction takes eight codes in two registers.  q enters as two E4M3 parts (take_q says how exactly).
-//     fp32: a code as 16 + c in bf16, an operand word of two codes is ((w >> n) & 0x00780078) | 0x41804180, and q as three
-//     bf16 parts;
-//   * values: codes as 16 + c in bf16, weights as two bf16 parts (2^-17 of the weight is left; fp32: three).
+// 32 or 64 keys.  Both products run over the codes themselves: a code is exact in bf16 as c 2^-130, a number below the smallest
+// exponent (a shift and an and for two codes), so nothing is rounded on the way from the cache to the sums but the weights, which
+// enter as two bf16 parts (2^-17 of them is left; fp32: three, and q as three).  Codes as 16 + c would do too, and need no care
+// for the exponents, but the 16 q has to go again: scores were off by three times as much and fp32 outputs by 2^-20, and the
+// step of 32 requests below took 1 to 2 us more.  (Codes and q as 8-bit floats: as fast, but that instruction sums 8
+// products short of fp32, which puts scores 2^-16 of their size off.)
 // Layout: a row's 16 pieces hold a sixteenth of every group each.  S^T = K Q^T: lane (n, g) takes four pieces of key n (a
 // quarter of every group), so each product is over one group.  O^T += V^T P^T: lane n takes piece n of a lane's keys, so the 16
 // rows of each product are of one group, and P carries that group's scale.  Scales are read as lane (n, g) needs them, for keys
 // 4 (n & 3) + g, and reach the other lanes of a four by DPP.
 //
 // Bound: the cache is read once, 72 + 72 bytes a key and head of 128 in groups of 64 against 512 in bf16.  Four query heads a kv
-// head, bf16, d 128, 32 requests of 131072 tokens and less (385 MB): 72 us, 5.4 TB/s with the join (a copy reaches 6.6);
+// head, bf16, d 128, 32 requests of 131072 tokens and less (385 MB): 73 us, 5.3 TB/s with the join (a copy reaches 6.6);
 // there the vector instructions between the loads and the products (codes, scales, weights) take two thirds of the time, which
-// is why they are counted: scores through bytes instead of 16 + c 90 -> 82 us, columns in blocks (below) 101 -> 73.  One
+// is why they are counted: columns in blocks (below) took 101 us to 76.  One
 // request of 32768 tokens (19 MB): 14 us, mostly the two launches and two rounds of latency.
 #include "paged_runs.h"
 #include "paged_q4.h"
@@ -36,6 +35,8 @@ constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs
 // tile hardly ever rise together, and one that rises would turn all sums over (32 requests of 131072: 77.4 -> 75.9 us, of 2000
 // tokens 25.9 -> 25.5).  Weights are at most 2^4 then.
 constexpr float kQ4Lag = 4.f;
+// Weights, and l with them, count 2^-40, which keeps their products with codes far from fp32's smallest numbers.
+constexpr float kQ4Up = 40.f;
 
 struct Q4AttnArgs : RunArgs {
   const char* q;
@@ -49,17 +50,11 @@ __device__ __forceinline__ float of_four(float x) {
   constexpr int ctrl = R | R << 2 | R << 4 | R << 6;
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), ctrl, 0xf, 0xf, true));
 }
-// codes number j of both half-words of r as 16 + c in bf16; `ones` is 16 in both halves of a VGPR (with both constants as
-// scalars or literals the two operations below cannot be one)
+// codes number j of both half-words of r as c 2^-130 in bf16, number 0 as c 2^-133: below the smallest exponent a word's bits are
+// its number, and nothing is added to a code.  (The matrix instructions take such operands as they are.)
 template <int J>
-__device__ __forceinline__ uint32_t codes_of(uint32_t r, uint32_t ones) {
-  const uint32_t x = J == 0 ? r << 3 : r >> (4 * J - 3);
-  return (x & 0x00780078u) | ones;
-}
-__device__ __forceinline__ uint32_t sixteens() {
-  uint32_t x = 0x41804180u;
-  asm("" : "+v"(x));
-  return x;
+__device__ __forceinline__ uint32_t codes_of(uint32_t r) {
+  return J == 0 ? r & 0x000f000fu : r >> (4 * J - 3) & 0x00780078u;
 }
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -137,14 +132,12 @@ struct Q4Sweep {
   static constexpr int H = D / 64;                  // half-words of a piece
   static constexpr int NG = D / G;                  // groups of a row
   static constexpr int N = D / 16;                  // second products for 32 keys
-  static constexpr bool kBytes = sizeof(T) == 2;    // scores from codes as bytes (else as bf16)
-  static constexpr int QP = kBytes ? 2 : 3, PP = kBytes ? 2 : 3;   // parts of q, of the weights
-  static constexpr int QW = kBytes ? 2 : 4;         // words of an operand
+  static constexpr int QP = sizeof(T) == 2 ? 1 : 3, PP = sizeof(T) == 2 ? 2 : 3;   // bf16 parts of q, of the weights
   static constexpr int VW = D == 256 ? 2 : 1;       // dwords of a piece (d 64: half of one)
   f32x4 acc[N];                                     // acc[4 h + j][r]: row n of q's columns, element d_of(4 h + j, 4 g + r)
   float accb[NG];                                   // this lane's keys only, as l
   float m, l, most;                                 // most: the largest q . k, unscaled; m: what the sums refer to
-  uint32_t q[J][QP][D / 32][QW];
+  u32x4 q[J][QP][D / 32];
   float qs[NG];                                     // sums of q over a group, in the scores' unit
   float unit;                                       // what a score counts
   struct Tile {                                     // a tile as it lies
@@ -152,7 +145,7 @@ struct Q4Sweep {
     Words<NG> ks[A], vs[A];
     Words<VW> v[4 * U];
   };
-  uint32_t ones, mine[J];                           // mine[j]: all bits in the lanes of block j
+  uint32_t mine[J];                           // mine[j]: all bits in the lanes of block j
 
   static __device__ __forceinline__ int group_of(int i) { return G == 64 ? i / 4 : 2 * (i / 4) + (i % 4) / 2; }
   // element of acc[i] at row m of the product
@@ -167,7 +160,6 @@ struct Q4Sweep {
     m = most = -INFINITY;
     l = 0.f;
     unit = 0.f;
-    ones = sixteens();
 #pragma unroll
     for (int j = 0; j < J; ++j) mine[j] = n / C == j ? ~0u : 0u;
   }
@@ -198,77 +190,43 @@ struct Q4Sweep {
       }
       qs[b] = col_sum4(sum);
     }
-    unit = size;
-    if constexpr (kBytes) {
-      // q as two bytes (4 bits each, E4M3) of q f, f the power of two that takes the row's largest to [2^7, 2^8): eight bits
-      // for elements of 2^-10 of it and more, 2^-18 of it for what is below.  A byte of 0..15 is 2^-9 of its number in that
-      // format, so scores count f 2^-9.  (An infinity or NaN in q makes the unit, and with it every weight, NaN.)
-      most = col_max4(most);
-      const int e = most > 0.f ? (int)(__float_as_uint(most) >> 23) : 127;
-      const float f = __uint_as_float((uint32_t)(e < 8 ? 253 : 261 - e) << 23);   // 2^(134 - e), at most 2^126
-      float any = 0.f;
+    // q f against codes c 2^-130, f the power of two that takes the row's largest to [2^110, 2^111) (at most 2^124): sums are of
+    // ordinary size.  (An infinity or NaN in q makes the unit, and with it every weight, NaN.)
+    most = col_max4(most);
+    const int e = (int)(__float_as_uint(most) >> 23);
+    const float f = __uint_as_float((uint32_t)(e < 113 ? 251 : 364 - e) << 23);
+    unit = size * 0x1p65f / f * 0x1p65f;
 #pragma unroll
-      for (int b = 0; b < NG; ++b) {
-        any += qs[b] - qs[b];
-        qs[b] = qs[b] * f * 0.001953125f;
+    for (int b = 0; b < NG; ++b) {
+      unit += qs[b] - qs[b];
+      qs[b] = qs[b] * f * 0x1p-65f * 0x1p-65f;
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[b][i] *= f;
-      }
-      unit = size / f * 512.f + any;
+      for (int i = 0; i < E; ++i)                   // (codes number 0 are an eighth)
+        x[b][i] *= (G == 64 ? i % 4 == 0 : (b | i) % 2 == 0) ? 8.f * f : f;
+    }
 #pragma unroll
-      for (int b = 0; b < NG; ++b)
+    for (int b = 0; b < NG; ++b)
 #pragma unroll
-        for (int part = 0; part < QP; ++part)
+      for (int part = 0; part < QP; ++part) {
+        uint32_t w[E / 2];
 #pragma unroll
-          for (int i = 0; i < E / 8; ++i) {         // a product: 8 elements, even ones of four codes (two of G 32) first
-            uint32_t w[2] = {0, 0};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float y[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int at = G == 64 ? 8 * i + 4 * (k >> 1) + 2 * (k & 1) + j : 2 * k + j;
-                y[k] = x[b][at];
-              }
-              int word = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-              word = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], word, true);
-              w[j] = (uint32_t)word;
-              const float z[4] = {__builtin_amdgcn_cvt_f32_fp8(word, 0), __builtin_amdgcn_cvt_f32_fp8(word, 1),
-                                  __builtin_amdgcn_cvt_f32_fp8(word, 2), __builtin_amdgcn_cvt_f32_fp8(word, 3)};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int at = G == 64 ? 8 * i + 4 * (k >> 1) + 2 * (k & 1) + j : 2 * k + j;
-                x[b][at] -= z[k];
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) q[j][part][b * (E / 8) + i][k] = n / C == j ? w[k] : 0;
-          }
-    } else {
-#pragma unroll
-      for (int b = 0; b < NG; ++b)
-#pragma unroll
-        for (int part = 0; part < QP; ++part) {
-          uint32_t w[E / 2];
-#pragma unroll
-          for (int i = 0; i < E / 2; ++i) {
-            // G 64: product i / 4, word j = i % 4: elements 8 (i / 4) + j and 4 further;
-            // G 32: word i = 2 p + j: elements 4 p + j and 2 further
-            const int e = G == 64 ? 8 * (i / 4) + i % 4 : 4 * (i / 2) + i % 2, f = e + (G == 64 ? 4 : 2);
-            w[i] = pack_bf16(x[b][e], x[b][f]);
+        for (int i = 0; i < E / 2; ++i) {
+          // G 64: product i / 4, word j = i % 4: elements 8 (i / 4) + j and 4 further;
+          // G 32: word i = 2 p + j: elements 4 p + j and 2 further
+          const int e = G == 64 ? 8 * (i / 4) + i % 4 : 4 * (i / 2) + i % 2, f = e + (G == 64 ? 4 : 2);
+          w[i] = pack_bf16(x[b][e], x[b][f]);
+          if (part + 1 < QP) {
             x[b][e] -= lo_f(w[i]);
             x[b][f] -= hi_f(w[i]);
           }
-#pragma unroll
-          for (int j = 0; j < J; ++j)
-#pragma unroll
-            for (int i = 0; i < E / 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) q[j][part][b * (E / 8) + i][e] = n / C == j ? w[4 * i + e] : 0;
         }
-    }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int i = 0; i < E / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[j][part][b * (E / 8) + i][e] = w[4 * i + e] & mine[j];
+      }
   }
   // subtile of this lane's results a
   static __device__ __forceinline__ int subtile(int a, int n) { return a * J + n / C; }
@@ -333,13 +291,6 @@ struct Q4Sweep {
   static __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, int h) {   // half-word h of a and of b
     return __builtin_amdgcn_perm(b, a, h & 1 ? 0x07060302u : 0x05040100u);
   }
-  __device__ __forceinline__ f32x4 score(const uint32_t (&codes)[QW], int j, int part, int i, f32x4 c) const {
-    const uint32_t(&y)[QW] = q[j][part][i];
-    if constexpr (kBytes)
-      return __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8((uint64_t)codes[1] << 32 | codes[0], (uint64_t)y[1] << 32 | y[0], c, 0, 0, 0);
-    else
-      return mfma(u32x4{codes[0], codes[1], codes[2], codes[3]}, u32x4{y[0], y[1], y[2], y[3]}, c);
-  }
   // s[4 a + r] = q . k of key 16 subtile(a) + 4 r + g, in the row's unit
   __device__ __forceinline__ void scores(const Tile& in, float (&s)[4 * A]) const {
 #pragma unroll
@@ -352,41 +303,20 @@ struct Q4Sweep {
         const Words<2 * H>& x = in.k[a * J + j];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          uint32_t r[2];                            // half-words h of pieces 4 g + 2 p and the next
+          u32x4 y[2];                               // G 64: products of group h; G 32: of groups 2 h and 2 h + 1
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            if constexpr (H == 1) r[p] = x.w[p];
-            else if constexpr (H == 2) r[p] = halves(x.w[2 * p], x.w[2 * p + 1], h);
-            else r[p] = halves(x.w[4 * p + (h >> 1)], x.w[4 * p + 2 + (h >> 1)], h);
-          }
-          uint32_t y[2][QW];                        // G 64: products of group h; G 32: of groups 2 h and 2 h + 1
-          if constexpr (kBytes) {
-            uint32_t w[2][2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              w[p][0] = r[p] & 0x0f0f0f0fu;
-              w[p][1] = r[p] >> 4 & 0x0f0f0f0fu;
-            }
-#pragma unroll
-            for (int p = 0; p < 2; ++p)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)           // (a G 32 group: every other byte of both words)
-                y[p][e] = G == 64 ? w[p][e] : __builtin_amdgcn_perm(w[1][e], w[0][e], p ? 0x07050301u : 0x06040200u);
-          } else if constexpr (G == 64) {
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              y[p][0] = codes_of<0>(r[p], ones);
-              y[p][1] = codes_of<1>(r[p], ones);
-              y[p][2] = codes_of<2>(r[p], ones);
-              y[p][3] = codes_of<3>(r[p], ones);
-            }
-          } else {
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              y[0][2 * p] = codes_of<0>(r[p], ones);
-              y[0][2 * p + 1] = codes_of<1>(r[p], ones);
-              y[1][2 * p] = codes_of<2>(r[p], ones);
-              y[1][2 * p + 1] = codes_of<3>(r[p], ones);
+            uint32_t r;                             // half-words h of pieces 4 g + 2 p and the next
+            if constexpr (H == 1) r = x.w[p];
+            else if constexpr (H == 2) r = halves(x.w[2 * p], x.w[2 * p + 1], h);
+            else r = halves(x.w[4 * p + (h >> 1)], x.w[4 * p + 2 + (h >> 1)], h);
+            if constexpr (G == 64) {
+              y[p] = u32x4{codes_of<0>(r), codes_of<1>(r), codes_of<2>(r), codes_of<3>(r)};
+            } else {
+              y[0][2 * p] = codes_of<0>(r);
+              y[0][2 * p + 1] = codes_of<1>(r);
+              y[1][2 * p] = codes_of<2>(r);
+              y[1][2 * p + 1] = codes_of<3>(r);
             }
           }
 #pragma unroll
@@ -394,14 +324,14 @@ struct Q4Sweep {
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
               f32x4& to = c[G == 64 ? h : 2 * h + p];
-              to = score(y[p], j, i, 2 * h + p, to);
+              to = mfma(y[p], q[j][i][2 * h + p], to);
             }
         }
       }
       float t[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int b = 0; b < NG; ++b) {
-        const float sc = lo_f(in.ks[a].w[b]), bias = kBytes ? hi_f(in.ks[a].w[b]) : fmaf(-16.f, sc, hi_f(in.ks[a].w[b]));
+        const float sc = lo_f(in.ks[a].w[b]), bias = hi_f(in.ks[a].w[b]);
         t[0] = fmaf(of_four<0>(sc), c[b][0], fmaf(of_four<0>(bias), qs[b], t[0]));
         t[1] = fmaf(of_four<1>(sc), c[b][1], fmaf(of_four<1>(bias), qs[b], t[1]));
         t[2] = fmaf(of_four<2>(sc), c[b][2], fmaf(of_four<2>(bias), qs[b], t[2]));
@@ -441,7 +371,7 @@ struct Q4Sweep {
       uint32_t part[PP][2 * A];                     // the weights of this lane's keys for the group
 #pragma unroll
       for (int a = 0; a < A; ++a) {
-        const float sc = lo_f(in.vs[a].w[b]), bias = fmaf(-16.f, sc, hi_f(in.vs[a].w[b]));
+        const float sc = lo_f(in.vs[a].w[b]), bias = hi_f(in.vs[a].w[b]);
         float w[4];
         w[0] = p[4 * a + 0] * of_four<0>(sc);
         w[1] = p[4 * a + 1] * of_four<1>(sc);
@@ -485,7 +415,7 @@ struct Q4Sweep {
         }
         const auto product = [&](auto jc) __attribute__((always_inline)) {
           constexpr int K = decltype(jc)::value;
-          const u32x4 x = {codes_of<K>(r[0], ones), codes_of<K>(r[1], ones), codes_of<K>(r[2], ones), codes_of<K>(r[3], ones)};
+          const u32x4 x = {codes_of<K>(r[0]), codes_of<K>(r[1]), codes_of<K>(r[2]), codes_of<K>(r[3])};
 #pragma unroll
           for (int i = PP - 1; i >= 0; --i) acc[4 * h + K] = mfma(x, w[i], acc[4 * h + K]);
         };
@@ -572,7 +502,7 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4 * S::A; ++i) {
-      p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * w.unit);
+      p[i] = __builtin_amdgcn_exp2f(fmaf(p[i] - ref, w.unit, kQ4Up));
       sum += p[i];
     }
     w.l += sum;
@@ -656,17 +586,17 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
     for (int i = 0; i < S::N; i += G / 16)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float bias = accb[w.group_of(i)];
+        const float bias = accb[w.group_of(i)] * 0x1p-40f, c0 = 0x1p93f, c = 0x1p90f;   // (c 2^-133, c 2^-130)
         float* to = &so[wave][n * LD + w.d_of(i, 4 * g + r)];
         if constexpr (G == 64)
-          *reinterpret_cast<f32x4*>(to) =
-              f32x4{w.acc[i][r] + bias, w.acc[i + 1][r] + bias, w.acc[i + 2][r] + bias, w.acc[i + 3][r] + bias};
+          *reinterpret_cast<f32x4*>(to) = f32x4{fmaf(w.acc[i][r], c0, bias), fmaf(w.acc[i + 1][r], c, bias),
+                                                fmaf(w.acc[i + 2][r], c, bias), fmaf(w.acc[i + 3][r], c, bias)};
         else
-          *reinterpret_cast<f32x2*>(to) = f32x2{w.acc[i][r] + bias, w.acc[i + 1][r] + bias};
+          *reinterpret_cast<f32x2*>(to) = f32x2{fmaf(w.acc[i][r], i % 4 == 0 ? c0 : c, bias), fmaf(w.acc[i + 1][r], c, bias)};
       }
     if (g == 0) {
       sm[wave][n] = w.m == -INFINITY ? w.m : w.m * (w.unit * 0.6931471805599453f);   // (a wave without tiles has no unit)
-      sl[wave][n] = l;
+      sl[wave][n] = l * 0x1p-40f;
     }
   }
   if (bad && lane == 0) sbad = 1;

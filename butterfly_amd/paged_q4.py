@@ -261,9 +261,8 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
     without tokens gives zeros and the empty stream ``(0, 0, -1e30)``; a length beyond its table row, or a page id outside
     the pages among those that are read, gives NaN for that request, and so do infinities and NaN in its queries or
     scales (in v's scales: in that group).  Rows of a page that the request does not see are never part of the result, whatever
-    they hold.  Sums are taken over 16 + code and of weights up to 2^4: where 2^11 times a query's element times a scale
-    of k, or 2^9 times the number of keys times a scale of v, passes 2^127 the result may be infinite or NaN.  A bfloat16
-    query enters with eight bits down to 2^-10 of its row's largest element, and to 2^-18 of that element below."""
+    they hold.  Queries of
+    2^110 and more, and scales of v whose product with the number of keys passes 2^75, may give infinities or NaN."""
     dev = _device_of(q)
     if not block_table.get_device() == lengths.get_device() == dev:
         _other_device()

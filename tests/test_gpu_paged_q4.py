@@ -2,14 +2,14 @@
 
 Codes, scales and biases are defined by 64-bit arithmetic and have to be equal, bit for bit.  Tolerances of the
 attention, with u = 2^-24 and a row's terms at most t = 31 scale + |bias| of v:
-  * scores: sums of d products q (16 + c) and their scales in fp32, errors of u each that add up like a random
+  * scores: sums of d products q c and their scales in fp32, errors of u each that add up like a random
     walk: below 2^-18 of the weights for the sizes here, twice (in the sum and in l);
   * weights: two bf16 parts are off by 2^-17 (half a step of the second one), three by 2^-25;
   * so |error| <= t (2^-17 + 2^-16) = 0.75 * 2^-15 t, rounded up to 2^-15 t, and half a step of the output's type.
 A relative 2-norm of 2^-16 holds fp32 outputs to more: their errors are independent, 2^-18 at the most each.
 The statistics are held to the worst case.  A score's terms, scale |q_e| (31 scale + |bias|) summed over its elements, are A
 at the most (of all rows and keys), and each of its fp32 roundings is of a partial sum of them, so at most u A: some 6
-for the products of a group (up to three, of 32 products each, and the term of 16), two for each of up to 8 groups, two
+for the products of a group (up to three, of 32 products each, and the bias's term), two for each of up to 8 groups, two
 for the scale.  So m is off by at most delta = 24 u A, however small it is itself, and l, a sum of exp(s - m), by a
 part of 2 delta and the 2^-18 of its own sum."""
 from __future__ import annotations
@@ -123,6 +123,23 @@ def test_append_of_groups_at_the_edges(dtype):
         assert torch.equal(nan, want[..., None].expand_as(nan))
 
 
+def test_scales_are_rounded_to_fp32_and_then_to_bf16():
+    """Ranges whose 15th is within 2^-30 of a middle between two bf16 numbers: its fp32 number is that middle, and
+    goes to the even one of the two."""
+    rows = []
+    for t in (1 + 2.0 ** -8, 1 + 3 * 2.0 ** -8):
+        for lo in (-2.0 ** -30, 0.0, 2.0 ** -30):
+            r = torch.linspace(1, 14, 64)
+            r[3], r[40] = lo, 15 * t
+            rows.append(r)
+    x = torch.stack(rows).cuda()[:, None]
+    pages = _pages(1, 1, 16, 64, 64)
+    bf.paged_q4_append(x, x, pages, torch.arange(len(rows), device="cuda"))
+    assert pages.k_scales[0, 0, :6, 0, 0].tolist() == [1.0] * 3 + [1 + 2.0 ** -6] * 3
+    c, s = q4_plain.packed(x, 64)
+    assert torch.equal(pages.k_codes[0, 0, :6], c[:, 0]) and _same(pages.v_scales[0, 0, :6], s[:, 0])
+
+
 # --------------------------------------------------------------------------- norm and RoPE on the way
 @pytest.mark.parametrize("group", [32, 64])
 @pytest.mark.parametrize("d,rot", [(64, 64), (64, 16), (128, 128), (128, 64), (256, 256), (256, 64), (256, 48)])
@@ -159,6 +176,24 @@ def test_rope_append(dtype, d, rot, group):
             scales[slots[live] // page, :, slots[live] % page] = s[live]
         for name, a, b in zip(pages._fields, pages, before):
             assert _same(a, b), (rows, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rope_append_of_many_groups_equals_the_definition(dtype):
+    """Half a million groups: each rounding of a scale and a bias meets its ties."""
+    rows, hq, hkv, d, group = 8000, 8, 8, 256, 32
+    q, k, v = torch.randn(rows, hq + 2 * hkv, d, generator=_gen(5), device="cuda").to(dtype).split((hq, hkv, hkv), 1)
+    ang = torch.rand(500, d // 4, generator=_gen(2), device="cuda") * 9
+    positions = torch.randint(500, (rows,), generator=_gen(3), device="cuda")
+    pages = _pages(63, hkv, 128, d, group)
+    kw = torch.rand(d, generator=_gen(4), device="cuda").to(dtype)
+    bf.paged_q4_rope_append(q, k, v, pages, torch.arange(rows, device="cuda"), positions, ang.cos(), ang.sin(),
+                            q_weight=kw, k_weight=kw, eps=1e-6)
+    for x, codes, scales in ((q4_plain.rope(k, kw, ang.cos(), ang.sin(), positions, 1e-6), pages.k_codes, pages.k_scales),
+                             (v, pages.v_codes, pages.v_scales)):
+        c, s = q4_plain.packed(x, group)
+        for got, want in ((codes, c), (scales, s)):
+            assert _same(got.transpose(1, 2).flatten(0, 1)[:rows], want)
 
 
 @pytest.mark.parametrize("dtype,d,group,hq,hkv", [(torch.bfloat16, 64, 64, 14, 1), (torch.bfloat16, 128, 32, 6, 6),
