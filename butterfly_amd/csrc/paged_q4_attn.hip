@@ -35,8 +35,8 @@ constexpr int q4_whole_rounds(int64_t pairs) { return pairs >= 2048 ? 32 : pairs
 // tile hardly ever rise together, and one that rises would turn all sums over (32 requests of 131072: 77.4 -> 75.9 us, of 2000
 // tokens 25.9 -> 25.5).  Weights are at most 2^4 then.
 constexpr float kQ4Lag = 4.f;
-// Weights, and l with them, count 2^-40, which keeps their products with codes far from fp32's smallest numbers.
-constexpr float kQ4Up = 40.f;
+// v's scales are taken times this, which keeps the weights' products with codes far from fp32's smallest numbers.
+constexpr float kQ4Up = 0x1p40f;
 
 struct Q4AttnArgs : RunArgs {
   const char* q;
@@ -371,16 +371,16 @@ struct Q4Sweep {
       uint32_t part[PP][2 * A];                     // the weights of this lane's keys for the group
 #pragma unroll
       for (int a = 0; a < A; ++a) {
-        const float sc = lo_f(in.vs[a].w[b]), bias = hi_f(in.vs[a].w[b]);
+        const float sc = lo_f(in.vs[a].w[b]) * kQ4Up, bias = hi_f(in.vs[a].w[b]);
         float w[4];
         w[0] = p[4 * a + 0] * of_four<0>(sc);
         w[1] = p[4 * a + 1] * of_four<1>(sc);
         w[2] = p[4 * a + 2] * of_four<2>(sc);
         w[3] = p[4 * a + 3] * of_four<3>(sc);
-        accb[b] = fmaf(p[4 * a + 0], of_four<0>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * a + 1], of_four<1>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * a + 2], of_four<2>(bias), accb[b]);
-        accb[b] = fmaf(p[4 * a + 3], of_four<3>(bias), accb[b]);
+        // (four keys' sum first: the long one is rounded once for them)
+        const float some = fmaf(p[4 * a + 3], of_four<3>(bias), fmaf(p[4 * a + 2], of_four<2>(bias),
+                                                                     fmaf(p[4 * a + 1], of_four<1>(bias), p[4 * a] * of_four<0>(bias))));
+        accb[b] += some;
 #pragma unroll
         for (int i = 0; i < PP; ++i)
 #pragma unroll
@@ -415,9 +415,13 @@ struct Q4Sweep {
         }
         const auto product = [&](auto jc) __attribute__((always_inline)) {
           constexpr int K = decltype(jc)::value;
+          // (fp32: the long sum is rounded once for 32 keys, not at each part)
+          f32x4 sum = PP == 3 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[4 * h + K];
           const u32x4 x = {codes_of<K>(r[0]), codes_of<K>(r[1]), codes_of<K>(r[2]), codes_of<K>(r[3])};
 #pragma unroll
-          for (int i = PP - 1; i >= 0; --i) acc[4 * h + K] = mfma(x, w[i], acc[4 * h + K]);
+          for (int i = PP - 1; i >= 0; --i) sum = mfma(x, w[i], sum);
+          if constexpr (PP == 3) acc[4 * h + K] += sum;
+          else acc[4 * h + K] = sum;
         };
         using std::integral_constant;
         if (G == 64 || !(b & 1)) {
@@ -502,7 +506,7 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4 * S::A; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(fmaf(p[i] - ref, w.unit, kQ4Up));
+      p[i] = __builtin_amdgcn_exp2f((p[i] - ref) * w.unit);
       sum += p[i];
     }
     w.l += sum;
@@ -586,7 +590,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
     for (int i = 0; i < S::N; i += G / 16)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float bias = accb[w.group_of(i)] * 0x1p-40f, c0 = 0x1p93f, c = 0x1p90f;   // (c 2^-133, c 2^-130)
+        const float bias = accb[w.group_of(i)], c0 = 0x1p93f, c = 0x1p90f;   // (2^133 and 2^130 / kQ4Up)
         float* to = &so[wave][n * LD + w.d_of(i, 4 * g + r)];
         if constexpr (G == 64)
           *reinterpret_cast<f32x4*>(to) = f32x4{fmaf(w.acc[i][r], c0, bias), fmaf(w.acc[i + 1][r], c, bias),
@@ -596,7 +600,7 @@ __global__ void __launch_bounds__(64 * kWaves, q4_waves(sizeof(T), D, G, J)) q4_
       }
     if (g == 0) {
       sm[wave][n] = w.m == -INFINITY ? w.m : w.m * (w.unit * 0.6931471805599453f);   // (a wave without tiles has no unit)
-      sl[wave][n] = l * 0x1p-40f;
+      sl[wave][n] = l;
     }
   }
   if (bad && lane == 0) sbad = 1;
