@@ -195,7 +195,7 @@ struct Q4Sweep {
     most = col_max4(most);
     const int e = (int)(__float_as_uint(most) >> 23);
     const float f = __uint_as_float((uint32_t)(e < 113 ? 251 : 364 - e) << 23);
-    unit = size * 0x1p65f / f * 0x1p65f;
+    unit = size * (0x1p65f / f) * 0x1p65f;
 #pragma unroll
     for (int b = 0; b < NG; ++b) {
       unit += qs[b] - qs[b];

@@ -336,6 +336,18 @@ def test_attention_scales(dtype, scale):
     _check(out, q, pages, table, _i32(lens), (l, m), scale=scale)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [-80, -20, 50, 100])
+def test_attention_of_small_and_large_queries(dtype, power):
+    """Powers of two between queries and scale move every number on the way alike: the same bits."""
+    pages, lens = _pages(20, 2, 32, 128, 64), [500, 33]
+    table = _table(lens, 32, 20)
+    q = (torch.randn(2, 8, 1, 128, generator=_gen(1), device="cuda")).to(dtype)
+    want = bf.paged_q4_attention(q, pages, table, _i32(lens), scale=0.125, return_stats=True)
+    got = bf.paged_q4_attention(q * 2.0 ** power, pages, table, _i32(lens), scale=0.125 * 2.0 ** -power, return_stats=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("group", [32, 64])
 @pytest.mark.parametrize("d", [64, 128, 256])
 def test_attention_reads_nothing_that_a_request_does_not_see(d, group):
