@@ -52,7 +52,7 @@ from torch.utils._device import DeviceContext
 from . import _native
 from ._device import on, stream_of
 from .compressed_cache import CompressedKVCache
-from .integrations import QwenButterflyAttention, QwenButterflyConfig, register_butterfly_attention
+from .integrations import QwenButterflyAttention, QwenButterflyConfig, _cache_offset, register_butterfly_attention
 from .logprobs import MAX_TOP, TokenLogprobs, token_logprobs
 from .paged import PagedKVCache, PagedLayer
 
@@ -504,6 +504,13 @@ def _token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> Tok
     lp = torch.log_softmax(logits.float(), -1)
     entropy = -torch.where(lp > -math.inf, lp.exp() * lp, lp.exp()).sum(-1)
     return TokenLogprobs(lp.gather(-1, tokens[:, None])[:, 0], entropy, *lp.topk(top))
+
+
+def _tokens_held(cache) -> int:
+    """Tokens that one layer's cache holds (0 for pages: their pool says)."""
+    if isinstance(cache, list):
+        return int(cache[0].shape[2]) if cache else 0
+    return _cache_offset(cache)
 
 
 def _no_logprobs(b: int, n: int, top: int, device) -> TokenLogprobs:
@@ -999,6 +1006,9 @@ class Decoder(nn.Module):
         if tokens.dim() != 2 or tokens.shape[1] == 0:
             raise ValueError("score takes tokens [B, T] of at least one token")
         b, t = tokens.shape[0], tokens.shape[1] - 1
+        for i, cache in enumerate(caches):
+            if _tokens_held(cache):
+                raise ValueError(f"score starts from empty caches: layer {i}'s holds {_tokens_held(cache)} tokens")
         for pool in self._paged_pools(caches, b):
             pool.require(0)
         if t == 0 or b == 0:

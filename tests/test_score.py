@@ -1,0 +1,50 @@
+"""``Decoder.score``: what it refuses, and before what.  On the CPU, the paged operators in plain torch operations."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import butterfly_amd as bf
+from butterfly_amd.decoder import Decoder, DecoderConfig
+
+from . import paged_plain, q4_plain
+
+CFG = DecoderConfig(vocab_size=64, hidden_size=128, num_layers=2, num_heads=2, num_kv_heads=1, head_dim=64, intermediate_size=128)
+
+
+@pytest.fixture(autouse=True)
+def _plain(monkeypatch):
+    paged_plain.install(monkeypatch)
+    q4_plain.install(monkeypatch)
+
+
+def _model():
+    return Decoder(CFG, seed=1, device="cpu").float()
+
+
+def _cache(requests, pages=40, quant_bits=4, **kw):
+    return bf.PagedKVCache(num_layers=CFG.num_layers, num_pages=pages, max_requests=requests, num_kv_heads=CFG.num_kv_heads,
+                           head_dim=CFG.head_dim, page_size=16, dtype=torch.float32, device="cpu", quant_bits=quant_bits, **kw)
+
+
+def _text(b, t, seed=4):
+    return torch.randint(0, CFG.vocab_size, (b, t), generator=torch.Generator().manual_seed(seed))
+
+
+# --------------------------------------------------------------------------- caches that hold something
+def test_list_caches_that_hold_a_text_are_refused():
+    model, text, lists = _model(), _text(2, 9), [[] for _ in range(2)]
+    first = model.score(text, lists)
+    with pytest.raises(ValueError, match="empty caches: layer 0's holds 8"):
+        model.score(text, lists)
+    assert lists[0][0].shape[2] == 8
+    with pytest.raises(ValueError, match="layer 1's holds 8"):
+        model.score(text, [[], lists[1]])
+    assert torch.equal(model.score(text, [None, None]).logprobs, first.logprobs)     # no cache at all
+
+
+def test_a_compressed_cache_that_holds_a_text_is_refused():
+    cache = bf.CompressedKVCache(block_size=16, local_window_tokens=32)
+    cache.offset = 5
+    with pytest.raises(ValueError, match="layer 1's holds 5"):
+        _model().score(_text(2, 9), [[], cache])
