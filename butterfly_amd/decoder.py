@@ -38,6 +38,7 @@ from __future__ import annotations
 import math
 import time
 from dataclasses import dataclass
+from operator import index
 from typing import Callable, List, Optional, Tuple, Union
 
 import torch
@@ -1005,6 +1006,7 @@ class Decoder(nn.Module):
         one product over the table, made and read some ``SCORE_LOGITS`` at a time and never all held."""
         if tokens.dim() != 2 or tokens.shape[1] == 0:
             raise ValueError("score takes tokens [B, T] of at least one token")
+        top = self._top("top", top)
         b, t = tokens.shape[0], tokens.shape[1] - 1
         for i, cache in enumerate(caches):
             if _tokens_held(cache):
@@ -1020,6 +1022,13 @@ class Decoder(nn.Module):
         parts = [_token_logprobs(F.linear(x, self.embed_tokens), n, top)
                  for x, n in zip(h.split(step), given.split(step))]
         return TokenLogprobs(*(torch.cat(x).view(b, t, *x[0].shape[1:]) for x in zip(*parts)))
+
+    def _top(self, name: str, top: int) -> int:
+        """A number of alternatives, before anything is done for them."""
+        top, most = index(top), min(MAX_TOP, self.cfg.vocab_size)
+        if not 0 <= top <= most:
+            raise ValueError(f"{name} {top} must be 0 to {most}")
+        return top
 
     def _normed(self, x: torch.Tensor, positions: torch.Tensor, caches: List, rope) -> torch.Tensor:
         """Every layer over the embedded ``x``, then the final norm of every row."""
@@ -1178,8 +1187,8 @@ class Decoder(nn.Module):
         if bool(cache.lengths.any()):
             raise ValueError("greedy_requests starts from an empty cache (release the requests it holds)")
         said = top_logprobs is not None
-        if said and not 0 <= top_logprobs <= min(MAX_TOP, self.cfg.vocab_size):
-            raise ValueError(f"top_logprobs {top_logprobs} must be 0 to {min(MAX_TOP, self.cfg.vocab_size)}")
+        if said:
+            top_logprobs = self._top("top_logprobs", top_logprobs)
         if new_tokens <= 0:
             out = torch.empty(b, 0, dtype=torch.long, device=dev)
             return (out, _no_logprobs(b, 0, top_logprobs, dev)) if said else out

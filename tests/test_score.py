@@ -48,3 +48,20 @@ def test_a_compressed_cache_that_holds_a_text_is_refused():
     cache.offset = 5
     with pytest.raises(ValueError, match="layer 1's holds 5"):
         _model().score(_text(2, 9), [[], cache])
+
+
+# --------------------------------------------------------------------------- tops
+@pytest.mark.parametrize("top,error", [(-1, ValueError), (65, ValueError), (2.5, TypeError)])
+def test_a_top_out_of_range_is_refused_before_the_caches_change(top, error):
+    model, text, pool, lists = _model(), _text(2, 9), _cache(2), [[], []]
+    for caches in (pool.layers, lists):
+        with pytest.raises(error, match="top 65|top -1|float"):
+            model.score(text, caches, top=top)
+    assert pool.lengths.tolist() == [0, 0] and pool.plan is None and lists == [[], []]
+
+
+def test_a_top_beyond_a_small_vocabulary_is_refused():
+    model = Decoder(DecoderConfig(**{**vars(CFG), "vocab_size": 40}), seed=1, device="cpu").float()
+    with pytest.raises(ValueError, match="top 41 must be 0 to 40"):
+        model.score(_text(1, 5) % 40, [[], []], top=41)
+    assert model.score(_text(1, 5) % 40, [[], []], top=40).top_tokens.shape == (1, 4, 40)
