@@ -1002,7 +1002,8 @@ class Decoder(nn.Module):
         """The log probability of each token of ``tokens`` [B, T] behind the first, given those before it, with the
         distributions' entropies and ``top`` most probable tokens (``token_logprobs``): tensors [B, T - 1(, top)].
 
-        ``caches`` as ``forward``'s, empty before; they hold the first T - 1 tokens afterwards.  The logits are the rows of
+        ``caches`` as ``forward``'s, empty before; they hold the first T - 1 tokens afterwards (pages that cannot:
+        ``RuntimeError``).  The logits are the rows of
         one product over the table, made and read some ``SCORE_LOGITS`` at a time and never all held."""
         if tokens.dim() != 2 or tokens.shape[1] == 0:
             raise ValueError("score takes tokens [B, T] of at least one token")
@@ -1011,8 +1012,10 @@ class Decoder(nn.Module):
         for i, cache in enumerate(caches):
             if _tokens_held(cache):
                 raise ValueError(f"score starts from empty caches: layer {i}'s holds {_tokens_held(cache)} tokens")
-        for pool in self._paged_pools(caches, b):
-            pool.require(0)
+        pools = self._paged_pools(caches, b)
+        for pool in pools:
+            if not pool.require(0):
+                pool.sync()
         if t == 0 or b == 0:
             h = self.embed_tokens.new_zeros(0, self.cfg.hidden_size)
         else:
@@ -1021,6 +1024,8 @@ class Decoder(nn.Module):
         step = max(1, SCORE_LOGITS // self.cfg.vocab_size)
         parts = [_token_logprobs(F.linear(x, self.embed_tokens), n, top)
                  for x, n in zip(h.split(step), given.split(step))]
+        for pool in pools:
+            pool.sync()
         return TokenLogprobs(*(torch.cat(x).view(b, t, *x[0].shape[1:]) for x in zip(*parts)))
 
     def _top(self, name: str, top: int) -> int:

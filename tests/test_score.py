@@ -65,3 +65,23 @@ def test_a_top_beyond_a_small_vocabulary_is_refused():
     with pytest.raises(ValueError, match="top 41 must be 0 to 40"):
         model.score(_text(1, 5) % 40, [[], []], top=41)
     assert model.score(_text(1, 5) % 40, [[], []], top=40).top_tokens.shape == (1, 4, 40)
+
+
+# --------------------------------------------------------------------------- pages that cannot hold the text
+@pytest.mark.parametrize("quant_bits", [4, None])
+@pytest.mark.parametrize("kw,msg", [(dict(pages=3), "too few pages"), (dict(max_tokens=32), "outgrow")])
+def test_a_text_that_does_not_fit_is_an_error(quant_bits, kw, msg):
+    model, pool = _model(), _cache(2, quant_bits=quant_bits, **kw)
+    with pytest.raises(RuntimeError, match=msg):
+        model.score(_text(2, 40), pool.layers)
+    assert pool.lengths.tolist() == [0, 0] and pool.state[1] == 0
+    assert model.score(_text(2, 16), pool.layers).logprobs.shape == (2, 15)
+
+
+def test_an_earlier_steps_error_is_reported_before_the_prefill():
+    model, pool = _model(), _cache(1, pages=1)
+    pool.begin(torch.tensor([20], dtype=torch.int32), 20)        # does not fit
+    with pytest.raises(RuntimeError, match="outgrow"):
+        model.score(_text(1, 9), pool.layers)
+    assert pool.lengths.tolist() == [0]
+    model.score(_text(1, 9), pool.layers)
