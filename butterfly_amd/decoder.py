@@ -502,9 +502,13 @@ def _token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int) -> Tok
     """``token_logprobs``; on the CPU its PyTorch form."""
     if logits.is_cuda:
         return token_logprobs(logits, tokens, top=top)
-    lp = torch.log_softmax(logits.float(), -1)
+    x = logits.float()
+    lp, vocab = torch.log_softmax(x, -1), x.shape[-1]
     entropy = -torch.where(lp > -math.inf, lp.exp() * lp, lp.exp()).sum(-1)
-    return TokenLogprobs(lp.gather(-1, tokens[:, None])[:, 0], entropy, *lp.topk(top))
+    own = lp.gather(-1, tokens.clamp(0, vocab - 1)[:, None])[:, 0].masked_fill((tokens < 0) | (tokens >= vocab), math.nan)
+    # (a stable order: NaN first, equal logits by the lower token)
+    ids = x.sort(stable=True, dim=-1, descending=True).indices[:, :top] if top else tokens.new_empty(len(x), 0)
+    return TokenLogprobs(own, entropy, lp.gather(-1, ids), ids)
 
 
 def _tokens_held(cache) -> int:

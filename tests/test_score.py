@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import butterfly_amd as bf
-from butterfly_amd.decoder import Decoder, DecoderConfig
+from butterfly_amd.decoder import Decoder, DecoderConfig, _token_logprobs
 
 from . import paged_plain, q4_plain
 
@@ -85,3 +85,26 @@ def test_an_earlier_steps_error_is_reported_before_the_prefill():
         model.score(_text(1, 9), pool.layers)
     assert pool.lengths.tolist() == [0]
     model.score(_text(1, 9), pool.layers)
+
+
+# --------------------------------------------------------------------------- the CPU form
+def test_the_cpu_form_ranks_and_marks_as_the_operator_does():
+    """Ties go to the lower token, NaN above every number, a token outside the vocabulary is NaN."""
+    nan, inf = float("nan"), float("inf")
+    logits = torch.tensor([[1.0, 3.0, -0.0, 3.0, 0.0, -inf], [0.0, nan, 2.0, nan, inf, 1.0], [-inf] * 6, [5.0] * 6])
+    own, entropy, tops, ids = _token_logprobs(logits, torch.tensor([5, 0, 1, -1]), 5)
+    assert ids.tolist() == [[1, 3, 0, 2, 4], [1, 3, 4, 2, 5], [0, 1, 2, 3, 4], [0, 1, 2, 3, 4]]
+    assert own[0] == -inf and bool(own[1:].isnan().all()) and bool(entropy[1:3].isnan().all())
+    assert bool(tops[1:3].isnan().all()) and bool((tops[3] == tops[3, 0]).all()) and bool((tops[0].diff() <= 0).all())
+    # one unit in the last place of log 6 and of the sum of six terms
+    assert abs(entropy[3].item() - 1.791759469228055) <= 8 * 2.0 ** -24 * 1.8
+    many = torch.zeros(3, 5000)
+    assert _token_logprobs(many, torch.tensor([0, 5000, 4999]), 64).top_tokens.tolist() == [list(range(64))] * 3
+    assert _token_logprobs(many, torch.tensor([0, 5000, 4999]), 0).logprobs.isnan().tolist() == [False, True, False]
+
+
+def test_a_last_token_outside_the_vocabulary_scores_nan():
+    text = _text(1, 6)
+    text[0, -1] = CFG.vocab_size
+    got = _model().score(text, [[], []]).logprobs[0]
+    assert got.isnan().tolist() == [False] * 4 + [True]
