@@ -1002,18 +1002,28 @@ class Decoder(nn.Module):
         return x, positions, caches, rope
 
     @torch.no_grad()
-    def score(self, tokens: torch.Tensor, caches: List, *, top: int = 0) -> TokenLogprobs:
+    def score(self, tokens: torch.Tensor, caches: List, *, top: int = 0, part: Optional[int] = None) -> TokenLogprobs:
         """The log probability of each token of ``tokens`` [B, T] behind the first, given those before it, with the
         distributions' entropies and ``top`` most probable tokens (``token_logprobs``): tensors [B, T - 1(, top)].
 
+        ``part``: tokens that go through the layers at a time (None: all in one call).  In dense layers the tokens of a call
+        attend to each other exactly, and to those of earlier calls as ``caches`` hold them (one token alone also to itself).
+        So over pages in 4 bits one call reads no code and scores what exact pages score; ``part=1`` scores what decode steps
+        over those pages see, larger parts what a prompt's further parts see.
+
         ``caches`` as ``forward``'s, empty before; they hold the first T - 1 tokens afterwards (pages that cannot:
-        ``RuntimeError``).  The logits are the rows of
-        one product over the table, made and read some ``SCORE_LOGITS`` at a time and never all held."""
+        ``RuntimeError``).  The logits are the rows of one product over the table, made and read some ``SCORE_LOGITS`` at a
+        time and never all held."""
         if tokens.dim() != 2 or tokens.shape[1] == 0:
             raise ValueError("score takes tokens [B, T] of at least one token")
         top = self._top("top", top)
         b, t = tokens.shape[0], tokens.shape[1] - 1
+        part = max(t, 1) if part is None else index(part)
+        if part < 1:
+            raise ValueError(f"part {part} must be a number of tokens, at least 1")
         for i, cache in enumerate(caches):
+            if cache is None and part < t:
+                raise ValueError(f"score in parts reads earlier tokens from caches: layer {i} has none")
             if _tokens_held(cache):
                 raise ValueError(f"score starts from empty caches: layer {i}'s holds {_tokens_held(cache)} tokens")
         pools = self._paged_pools(caches, b)
@@ -1023,7 +1033,8 @@ class Decoder(nn.Module):
         if t == 0 or b == 0:
             h = self.embed_tokens.new_zeros(0, self.cfg.hidden_size)
         else:
-            h = self._normed(*self._begin(tokens[:, :-1], caches, 0)).reshape(b * t, -1)
+            h = [self._normed(*self._begin(tokens[:, i:min(i + part, t)], caches, i)) for i in range(0, t, part)]
+            h = (torch.cat(h, 1) if len(h) > 1 else h[0]).reshape(b * t, -1)
         given = tokens[:, 1:].reshape(-1).long()
         step = max(1, SCORE_LOGITS // self.cfg.vocab_size)
         parts = [_token_logprobs(F.linear(x, self.embed_tokens), n, top)

@@ -108,3 +108,61 @@ def test_a_last_token_outside_the_vocabulary_scores_nan():
     text[0, -1] = CFG.vocab_size
     got = _model().score(text, [[], []]).logprobs[0]
     assert got.isnan().tolist() == [False] * 4 + [True]
+
+
+# --------------------------------------------------------------------------- in parts
+# Logits of some unit's size, fp32 sums of at most 128 terms through the layers in other orders: 2^-14 is 2^10 steps.
+NEAR = dict(rtol=0, atol=2.0 ** -14)
+
+
+@pytest.mark.parametrize("part", [1, 2, 7, 39, 100])
+def test_parts_over_exact_caches_score_as_one_call(part):
+    model, text = _model(), _text(2, 40)
+    want = model.score(text, [[], []], top=3)
+    for caches in ([[], []], _cache(2, quant_bits=None).layers):
+        got = model.score(text, caches, top=3, part=part)
+        for x, y in zip(got[:3], want[:3]):
+            torch.testing.assert_close(x, y, **NEAR)
+        held = caches[0][0].shape[2] if isinstance(caches[0], list) else caches[0].cache.lengths.tolist()[0]
+        assert held == 39
+
+
+@pytest.mark.parametrize("group", [32, 64])
+@pytest.mark.parametrize("part", [2, 7, 20])
+def test_parts_over_pages_in_4_bits_read_their_codes(part, group):
+    """Each token's score from a list cache of what the pages hold of earlier parts, and of its own part exactly."""
+    model, text, pool = _model(), _text(2, 41), _cache(2, quant_group=group)
+    got, exact = model.score(text, pool.layers, part=part), model.score(text, [[], []])
+    for i in range(40):
+        s = i // part * part
+        lists = [[x.clone() for x in layer.history(s)] if s else [] for layer in pool.layers]
+        lp = torch.log_softmax(model.forward(text[:, s:i + 1], lists, s).double(), -1)
+        torch.testing.assert_close(got.logprobs[:, i].double(), lp.gather(1, text[:, i + 1:i + 2])[:, 0], **NEAR)
+        torch.testing.assert_close(got.entropy[:, i].double(), -(lp.exp() * lp).sum(-1), **NEAR)
+    # the first part reads no code; what 4 bits leave of the others is far from rounding
+    torch.testing.assert_close(got.logprobs[:, :part], exact.logprobs[:, :part], **NEAR)
+    assert (got.logprobs - exact.logprobs)[:, part:].abs().max() > 16 * NEAR["atol"]
+
+
+def test_one_token_at_a_time_scores_what_decode_steps_see():
+    model, text, pool, steps = _model(), _text(2, 30), _cache(2), _cache(2)
+    got, exact = model.score(text, pool.layers, part=1), model.score(text, [[], []])
+    for i in range(29):
+        lp = torch.log_softmax(model.forward(text[:, i:i + 1], steps.layers, i).double(), -1)
+        torch.testing.assert_close(got.logprobs[:, i].double(), lp.gather(1, text[:, i + 1:i + 2])[:, 0], **NEAR)
+    assert (got.logprobs - exact.logprobs).abs().max() > 16 * NEAR["atol"]
+
+
+def test_parts_that_are_refused():
+    model, text, pool = _model(), _text(2, 9), _cache(2)
+    for part, error in ((0, ValueError), (-3, ValueError), (2.5, TypeError)):
+        with pytest.raises(error, match="at least 1|float"):
+            model.score(text, pool.layers, part=part)
+        with pytest.raises(error, match="at least 1|float"):
+            model.score(text[:, :1], pool.layers, part=part)
+    with pytest.raises(ValueError, match="layer 1 has none"):
+        model.score(text, [[], None], part=4)
+    with pytest.raises(RuntimeError, match="too few pages"):
+        model.score(_text(2, 40), _cache(2, pages=3).layers, part=8)
+    assert pool.lengths.tolist() == [0, 0] and pool.plan is None
+    assert model.score(text, [None, None], part=8).logprobs.shape == (2, 8)
