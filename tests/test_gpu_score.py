@@ -1,13 +1,15 @@
-"""GPU: ``Decoder.score`` in parts over each kind of cache.
+"""GPU: ``Decoder.score`` in parts over each kind of cache, and ``greedy_requests``' log probabilities by value.
 
 Log probabilities of logits that went other ways (products of one row and of many round at other places) agree as far as bf16
-noise lets them: half the logits' standard deviation, as for scores in one call."""
+noise lets them: half the logits' standard deviation, as for scores in one call.  Those of the same logits agree to fp32
+rounding."""
 from __future__ import annotations
 
 import pytest
 import torch
 
 import butterfly_amd as bf
+from butterfly_amd.decoder import RopeTable
 
 from .test_gpu_paged_q4_decoder import _cache, _model, _tokens
 
@@ -55,3 +57,40 @@ def test_codes_count_in_parts_and_not_in_one_call():
     assert torch.equal(one, one4)
     first = parts[:, :16] - parts4[:, :16]
     assert not bool(first.any()) and float((parts - parts4)[:, 16:].abs().mean()) > 0
+
+
+@pytest.mark.parametrize("quant_bits", [4, None])
+@pytest.mark.parametrize("head_dim,requests,top", [(64, 3, 5), (128, 35, 1), (128, 1, 0)])
+def test_requests_log_probabilities_are_those_of_their_steps(head_dim, requests, top, quant_bits):
+    """``greedy_requests``' steps once more, eagerly: the same logits, whose log-softmax in 64 bits is what it said."""
+    model, cfg = _model(head_dim)
+    prompts = [_tokens(cfg, (40, 1, 77)[r % 3], seed=r) for r in range(requests)]
+    make = lambda: _cache(cfg, requests, pages=5 * requests, quant_bits=quant_bits)
+    out, said = model.greedy_requests(prompts, 12, make(), top_logprobs=top)
+    assert said.top_tokens.shape == said.top_logprobs.shape == (requests, 12, top)
+    cache = make()
+    steps = [torch.cat([model.forward(p[None], [[] for _ in range(cfg.num_layers)], 0) for p in prompts])]
+    for r, p in enumerate(prompts):
+        held = [[] for _ in range(cfg.num_layers)]
+        model.forward(p[None], held, 0)
+        counts = torch.zeros_like(cache.lengths)
+        counts[r] = len(p)
+        cache.begin_packed(counts, len(p))
+        for layer, (k, v) in zip(cache.layers, held):
+            layer.append(k[0].transpose(0, 1), v[0].transpose(0, 1))
+    model._rope(0, 200, out.device)
+    for i in range(11):
+        cache.begin(torch.ones_like(cache.lengths))
+        x = torch.nn.functional.embedding(out[:, i:i + 1], model.embed_tokens)
+        steps.append(model._last_logits(x, None, cache.layers, RopeTable(*model._rope_tab, None)))
+    for i, lg in enumerate(steps):
+        assert torch.equal(lg.argmax(-1), out[:, i])
+        lp = lg.double().log_softmax(-1)
+        # sums of 2048 positive fp32 terms, 32 of them one after another and the rest pairwise: fewer than 64 steps of
+        # 2^-24 of l, whose logarithm moves by as much; the entropy's second sum counts terms up to |x - m| <= 64
+        near = dict(rtol=2.0 ** -20, atol=2.0 ** -17)
+        torch.testing.assert_close(said.logprobs[:, i].double(), lp.gather(1, out[:, i:i + 1])[:, 0], **near)
+        torch.testing.assert_close(said.entropy[:, i].double(), -(lp.exp() * lp).sum(-1), rtol=2.0 ** -14, atol=2.0 ** -14)
+        torch.testing.assert_close(said.top_logprobs[:, i].double(), lp.sort(-1, descending=True).values[:, :top], **near)
+        order = lg.float().sort(stable=True, dim=-1, descending=True).indices[:, :top]
+        assert torch.equal(said.top_tokens[:, i], order)
