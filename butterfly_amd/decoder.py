@@ -1212,12 +1212,17 @@ class Decoder(nn.Module):
         if new_tokens <= 0:
             out = torch.empty(b, 0, dtype=torch.long, device=dev)
             return (out, _no_logprobs(b, 0, top_logprobs, dev)) if said else out
-        first, logits = [], []
+        lps = _no_logprobs(b, new_tokens, top_logprobs, dev) if said else None
+        first = []
         for r, prompt in enumerate(prompts):
             n = prompt.numel()
             held = [[] for _ in self.layers]
-            logits.append(self.forward(prompt[None].to(dev), held, 0))
-            first.append(logits[-1].argmax(-1))
+            lg = self.forward(prompt[None].to(dev), held, 0)
+            first.append(lg.argmax(-1))
+            if said:
+                for x, y in zip(lps, token_logprobs(lg, first[-1], top=top_logprobs)):
+                    x[r, 0] = y[0]
+            del lg                                           # (a vocabulary's row a request adds up)
             counts = torch.zeros_like(cache.lengths)
             counts[r] = n
             cache.begin_packed(counts, n)
@@ -1231,11 +1236,6 @@ class Decoder(nn.Module):
         alive = torch.ones(b, dtype=torch.int32, device=dev)
         if eos_token is not None:
             alive.copy_((tok[:, 0] != eos_token).int())
-        if said:
-            lps = _no_logprobs(b, new_tokens, top_logprobs, dev)
-            for x, y in zip(lps, token_logprobs(torch.cat(logits), tok[:, 0], top=top_logprobs)):
-                x[:, 0] = y
-        del logits
         self._rope(0, max(p.numel() for p in prompts) + new_tokens + 1, dev)
         rope = RopeTable(*self._rope_tab, None)
 

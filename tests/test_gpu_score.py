@@ -5,6 +5,8 @@ noise lets them: half the logits' standard deviation, as for scores in one call.
 rounding."""
 from __future__ import annotations
 
+import weakref
+
 import pytest
 import torch
 
@@ -94,3 +96,19 @@ def test_requests_log_probabilities_are_those_of_their_steps(head_dim, requests,
         torch.testing.assert_close(said.top_logprobs[:, i].double(), lp.sort(-1, descending=True).values[:, :top], **near)
         order = lg.float().sort(stable=True, dim=-1, descending=True).indices[:, :top]
         assert torch.equal(said.top_tokens[:, i], order)
+
+
+@pytest.mark.parametrize("top", [None, 2])
+def test_no_prompts_logits_wait_for_the_next(monkeypatch, top):
+    model, cfg = _model(64)
+    seen, alive, forward = [], [], model.forward
+
+    def one(*args):
+        alive.append(sum(x() is not None for x in seen))
+        lg = forward(*args)
+        seen.append(weakref.ref(lg))
+        return lg
+
+    monkeypatch.setattr(model, "forward", one)
+    model.greedy_requests([_tokens(cfg, n, seed=n) for n in (20, 7, 50, 3)], 3, _cache(cfg, 4), top_logprobs=top)
+    assert alive == [0] * 4 and not any(x() is not None for x in seen)
