@@ -47,6 +47,14 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
   return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
 
+// a / b rounded as a division is, inv = 1 / b rounded so too: a first quotient, the rest of it, and the rest's part.
+// (A 15th as the product alone is a step off where the quotient lies next to a border between two fp32 numbers that is also
+// one between two bf16 numbers.)
+__device__ __forceinline__ double quotient(double a, double b, double inv) {
+  const double t = a * inv;
+  return fma(fma(-t, b, a), inv, t);
+}
+
 // 8 elements y of a row in each of D / 8 lanes (gl: which): the row's codes, a dword a lane, and the scale and bias
 // of a group in its first lane.  F: what the elements are exact in (a row as it lies: fp32).
 template <int D, int G, typename F>
@@ -63,17 +71,14 @@ __device__ __forceinline__ void q4_store(const F (&y)[8], int gl, char* codes, c
   lo = least(lo, dpp<kPair>(lo)), hi = most(hi, dpp<kPair>(hi)), bad |= dpp<kPair>(bad);
   lo = least(lo, dpp<kQuad>(lo)), hi = most(hi, dpp<kQuad>(hi)), bad |= dpp<kQuad>(bad);
   if constexpr (LG == 8) lo = least(lo, dpp<kEight>(lo)), hi = most(hi, dpp<kEight>(hi)), bad |= dpp<kEight>(bad);
-  // (a 15th as a product: the same but for values within 2^-52 of themselves of a border between two fp32 numbers)
-  uint32_t sb = bf16_bits((float)fmax(((double)hi - (double)lo) * (1.0 / 15.0), 1e-8)), bb = bf16_bits((float)lo);
+  uint32_t sb = bf16_bits((float)fmax(quotient((double)hi - (double)lo, 15.0, 1.0 / 15.0), 1e-8)), bb = bf16_bits((float)lo);
   bad |= (sb & 0x7f80u) == 0x7f80u || (bb & 0x7f80u) == 0x7f80u;
   if (bad) sb = bb = 0x7fc0u;
   const double s = __uint_as_float(sb << 16), b = __uint_as_float(bb << 16), inv = 1.0 / s;
   uint32_t w = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    // d / s rounded as a division is: a first quotient, the rest of it, and the rest's part (1 / s is rounded so)
-    const double d = (double)y[e] - b, t = d * inv, q = fma(fma(-t, s, d), inv, t);
-    w |= (uint32_t)(int)fmin(fmax(rint(q), 0.0), 15.0) << (4 * e);   // (NaN: 0)
+    w |= (uint32_t)(int)fmin(fmax(rint(quotient((double)y[e] - b, s, inv)), 0.0), 15.0) << (4 * e);   // (NaN: 0)
   }
   if (bad) w = 0;
   // dword gl of the row: half-words hw = c * H + h, c the piece (of 16) and h the pair of groups (G = 32) or the group
