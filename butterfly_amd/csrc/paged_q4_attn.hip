@@ -191,7 +191,8 @@ struct Q4Sweep {
       qs[b] = col_sum4(sum);
     }
     // q f against codes c 2^-130, f the power of two that takes the row's largest to [2^110, 2^111) (at most 2^124): sums are of
-    // ordinary size.  (An infinity or NaN in q makes the unit, and with it every weight, NaN.)
+    // ordinary size.  (An infinity or NaN in q makes the unit, and with it every weight, NaN.  The unit is finite while the
+    // largest of |q| times the scale is below 2^107.)
     most = col_max4(most);
     const int e = (int)(__float_as_uint(most) >> 23);
     const float f = __uint_as_float((uint32_t)(e < 113 ? 251 : 364 - e) << 23);

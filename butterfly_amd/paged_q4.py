@@ -262,7 +262,8 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
     the pages among those that are read, gives NaN for that request, and so do infinities and NaN in its queries or
     scales (in v's scales: in that group).  Rows of a page that the request does not see are never part of the result, whatever
     they hold.  Queries of
-    2^110 and more, and scales of v of 2^80 and more, may give infinities or NaN."""
+    2^110 and more, or of 2^107 and more times the size of ``scale``, and scales of v of 2^80 and more, may give infinities
+    or NaN."""
     dev = _device_of(q)
     if not block_table.get_device() == lengths.get_device() == dev:
         _other_device()
