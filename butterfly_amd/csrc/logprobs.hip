@@ -510,7 +510,7 @@ static_assert(kLpParts <= 32 && kLpSlots * kLpWhole <= 1 << 16 && kLpSegments >=
 
 // Parts of a row: enough workgroups for the card, of at most 8192 elements each where the rows leave so many (kLpParts at most).
 // Measured, us, at most 4096 / 8192: one row of 151936 bf16, top 5, 13.2 / 12.4, 32 of them 16.2 / 14.1, 32 of 32003 fp32, top 50,
-// 20.1 / 19.3 (at most 2048: 23.3); at least 8192 (one part fewer), top 20: one row of 151936 14.8 / 12.6, of 32003 13.6 / 13.7.
+// 20.1 / 19.3 (at most 2048: 23.3); at least 8192 (one part fewer) / at most, top 20: one row of 151936 14.8 / 12.6, of 32003 13.6 / 13.7.
 // Two parts of a row below 16384 are not worth their join, two / one: one row of 8193, top 20, 12.2 / 9.3, of 12000 11.3 / 8.7 (16384,
 // in two parts, 11.6), 32 of 12000 13.2 / 10.1, 200 fp32 ones 14.2 / 10.4.  2048 workgroups instead of 1024: 512 rows of 151936
 // fp32 58 -> 65, 1024 mostly masked ones of bf16 70 -> 95.

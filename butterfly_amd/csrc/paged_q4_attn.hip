@@ -7,20 +7,21 @@
 // The schedule, runs and joins are those of paged_attn.hip (paged_runs.h); a workgroup's four waves take every fourth tile of
 // 32 or 64 keys.  Both products run over the codes themselves: a code is exact in bf16 as c 2^-130, a number below the smallest
 // exponent (a shift and an and for two codes), so nothing is rounded on the way from the cache to the sums but the weights, which
-// enter as two bf16 parts (2^-17 of them is left; fp32: three, and q as three).  Codes as 16 + c would do too, and need no care
-// for the exponents, but the 16 q has to go again: scores were off by three times as much and fp32 outputs by 2^-20, and the
-// step of 32 requests below took 1 to 2 us more.  (Codes and q as 8-bit floats: as fast, but that instruction sums 8
-// products short of fp32, which puts scores 2^-16 of their size off.)
+// enter as two bf16 parts (2^-17 of them is left; fp32: three, and q as three).  Three for bf16 brought its outputs no nearer to
+// 64 bits and made the step of 32 requests below 82 us for 74.  Codes as 16 + c would do too, and need no care for the
+// exponents, but the 16 q has to go again: scores were off by three times as much and fp32 outputs by 2^-20, and that step took 1 to
+// 2 us more.  (Codes and q as 8-bit floats: as fast, but that instruction sums 8 products short of fp32, which puts scores 2^-16
+// of their size off.)
 // Layout: a row's 16 pieces hold a sixteenth of every group each.  S^T = K Q^T: lane (n, g) takes four pieces of key n (a
 // quarter of every group), so each product is over one group.  O^T += V^T P^T: lane n takes piece n of a lane's keys, so the 16
 // rows of each product are of one group, and P carries that group's scale.  Scales are read as lane (n, g) needs them, for keys
 // 4 (n & 3) + g, and reach the other lanes of a four by DPP.
 //
 // Bound: the cache is read once, 72 + 72 bytes a key and head of 128 in groups of 64 against 512 in bf16.  Four query heads a kv
-// head, bf16, d 128, 32 requests of 131072 tokens and less (385 MB): 73 us, 5.3 TB/s with the join (a copy reaches 6.6);
-// there the vector instructions between the loads and the products (codes, scales, weights) take two thirds of the time, which
-// is why they are counted: columns in blocks (below) took 101 us to 76.  One
-// request of 32768 tokens (19 MB): 14 us, mostly the two launches and two rounds of latency.
+// head, bf16, d 128, 32 requests of 131072 tokens and less (385 MB): 73 us, 5.3 TB/s with the join (that of bf16 pages reads
+// at 6.6, a copy runs at 5.8); there the vector instructions between the loads and the products (codes, scales, weights) take
+// two thirds of the time, which is why they are counted: columns in blocks (below) took 101 us to 76.  One request of 32768
+// tokens (19 MB): 14 us, mostly the two launches and two rounds of latency.
 #include "paged_runs.h"
 #include "paged_q4.h"
 
@@ -534,7 +535,8 @@ __device__ __forceinline__ bool q4_sweep(const Q4AttnArgs& a, S& w, const int32_
 }
 
 // Waves of a SIMD that the registers are cut for: two need no more than 256 (and no moves to accumulation registers
-// and back), but for the widest rows.
+// and back), but for the widest rows.  (Those in groups of 32 with one block of columns spill all the same: 5 registers in bf16, 3
+// in fp32.)
 constexpr int q4_waves(int esize, int d, int g, int j) { return d < 256 || (esize == 2 && g == 64 && j == 2) ? 2 : 1; }
 
 template <typename T, int D, int G, int J>
@@ -651,9 +653,10 @@ static int q4_blocks(int esize, int64_t head_dim, int64_t group, int64_t pairs, 
   return tokens < (1 << 16) && pairs * tokens < (1 << 16) ? 1 : most < fit ? most : fit;
 }
 static int q4_tile(int blocks) { return blocks > 2 ? 64 : 32; }
-// Runs in all, where requests and heads leave them: as many workgroups as a CU holds by its registers.  Measured, us, half as
-// many / these: 32 requests of up to 131072 tokens 90 / 73, one of 262144 of d 256 66 / 62, 8 of 60000 of d 64 29 / 26; twice as
-// many: 90, 80, 24.  Fewer runs of two rounds before as many of one: one request of 32768 tokens 15.8 -> 14.0.
+// Runs in all, where requests and heads leave them: as many workgroups of a CU as waves of a SIMD that the registers are cut
+// for (bf16 rows of 64 would leave room for four).  Measured, us, half as many / these: 32 requests of up to 131072 tokens
+// 90 / 73, one of 262144 of d 256 66 / 62, 8 of 60000 of d 64 29 / 26; twice as many: 90, 80, 24.  Fewer runs
+// of two rounds before as many of one: one request of 32768 tokens 15.8 -> 14.0.
 static int q4_runs(int esize, int64_t head_dim, int64_t group, int blocks) {
   return 256 * q4_waves(esize, (int)head_dim, (int)group, blocks);
 }

@@ -172,7 +172,8 @@ def paged_q4_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, page
     ``cos`` and ``sin`` [rows, r] (float32) are whole tables, ``positions`` (int64 [N]) picks their rows; elements
     from ``r`` on are not rotated.  q, k and v may be column ranges of one fused projection.  Every row of q is computed,
     in 32 bits and rounded once; k is computed in 64 bits up to its codes, which so do not depend on the order of a sum.
-    A position outside the tables gives NaN.  head_dim 64, 128 or 256, ``r`` a multiple of 16."""
+    (Rows that come normed and rotated in bfloat16, as a prompt's do through :func:`paged_q4_append`, have been rounded once
+    before that.)  A position outside the tables gives NaN.  head_dim 64, 128 or 256, ``r`` a multiple of 16."""
     dev = _device_of(q)
     if not slots.get_device() == positions.get_device() == cos.get_device() == sin.get_device() == dev:
         _other_device()
@@ -259,11 +260,11 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
 
     Returns ``out`` [B, Hq, 1, d], with ``return_stats`` the stream ``(out, l, m)`` of ``swa_stream_attention``.  A request
     without tokens gives zeros and the empty stream ``(0, 0, -1e30)``; a length beyond its table row, or a page id outside
-    the pages among those that are read, gives NaN for that request, and so do infinities and NaN in its queries or
-    scales (in v's scales: in that group).  Rows of a page that the request does not see are never part of the result, whatever
-    they hold.  Queries of
-    2^110 and more, or of 2^107 and more times the size of ``scale``, and scales of v of 2^80 and more, may give infinities
-    or NaN."""
+    the pages among those that are read, gives NaN for that request.  An infinity or NaN in a query gives NaN for its head, a
+    NaN in k's scales for its kv head's, in v's in that group.  (An infinity in a scale or bias, which rows into pages never
+    leave there, gives infinities or NaN, or takes its key's weight.)  Rows of a page that the request does not see are never
+    part of the result, whatever they hold.  Queries of 2^110 and more, or of 2^107 and more times the size of ``scale``, and
+    scales of v of 2^80 and more, may give infinities or NaN."""
     dev = _device_of(q)
     if not block_table.get_device() == lengths.get_device() == dev:
         _other_device()
