@@ -264,7 +264,8 @@ def paged_q4_attention(q: torch.Tensor, pages: Q4Pages, block_table: torch.Tenso
     NaN in k's scales for its kv head's, in v's in that group.  (An infinity in a scale or bias, which rows into pages never
     leave there, gives infinities or NaN, or takes its key's weight.)  Rows of a page that the request does not see are never
     part of the result, whatever they hold.  Queries of 2^110 and more, or of 2^107 and more times the size of ``scale``, and
-    scales of v of 2^80 and more, may give infinities or NaN."""
+    scales of v of 2^80 and more, may give infinities or NaN; values whose weighted sum passes 2^124 give infinities (sums keep
+    a reference while weights are at most 2^4, and are divided by ``l`` at the end)."""
     dev = _device_of(q)
     if not block_table.get_device() == lengths.get_device() == dev:
         _other_device()

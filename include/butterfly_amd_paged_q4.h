@@ -101,7 +101,7 @@ int bfly_paged_q4_read(const bfly_paged_q4_read_args_t* args, hipStream_t stream
  * Device: one new token of every request over its pages: bfly_paged_attention (butterfly_amd_paged.h) with
  * q and out in `dtype` (fp32 or bf16) and the keys and values as the codes stand for.
  * Queries of 2^110 and more, or of 2^107 and more times |scale|, and scales of v of 2^80 and more, may give
- * infinities or NaN.
+ * infinities or NaN; values whose weighted sum passes 2^124 may give infinities.
  * workspace: bfly_paged_q4_attention_workspace_bytes bytes, 16-byte aligned (it need not be cleared; calls
  * that overlap need one each).
  */

@@ -28,3 +28,21 @@ def test_large_queries_under_a_scale_that_does_not_shrink_them(dtype, d, group, 
     out, l, m = bf.paged_q4_attention(q, pages, table, _i32(lens), scale=scale, return_stats=True)
     assert bool(out.isfinite().all())
     _check(out, q, pages, table, _i32(lens), (l, m), scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 64), (256, 64)])
+def test_large_values_under_their_limits(dtype, d, group):
+    """Scales of v just below 2^80, and biases whose sum over 500 keys of weight 2^4 at most stays below 2^124."""
+    lens = [500, 33, 200]
+    pages = _pages(30, 2, 32, d, group)
+    table = _table(lens, 32, 30)
+    q = torch.randn(3, 8, 1, d, generator=_gen(1), device="cuda").to(dtype)
+    for scales, biases in ((80, 80), (0, 108)):
+        big = bf.Q4Pages(*(t.clone() for t in pages))
+        assert float(big.v_scales[..., 0].max()) < 1 and float(big.v_scales[..., 1].abs().max()) < 8
+        big.v_scales[..., 0].mul_(2.0 ** scales)
+        big.v_scales[..., 1].mul_(2.0 ** biases)
+        out = bf.paged_q4_attention(q, big, table, _i32(lens))
+        assert bool(out.isfinite().all())
+        _check(out, q, big, table, _i32(lens))
